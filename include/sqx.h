@@ -39,6 +39,12 @@ enum {
   SQX_FP4_SCALE_NV_E4M3 = 3, /* NVFP4 scales as E4M3 bytes [rows, cols/16] (sqx_nvfp4_ceil_quantize's) */
 };
 
+/* code formats of the block-scaled KV cache (sqx_kvblock_*) */
+enum {
+  SQX_KV_INT8 = 0, /* int8 codes in [-127, 127] */
+  SQX_KV_E4M3 = 1, /* E4M3 codes */
+};
+
 /* status codes */
 enum {
   SQX_OK = 0,
@@ -819,6 +825,80 @@ int sqx_argmax(const void* logits, int64_t B, int64_t V, int* next_tok, void* ws
 /* SlotKVCache.advance(1) (kv_cache.py:207-213): lengths[b] += 1 where active[b] != 0 (every row when
  * active is NULL). */
 int sqx_advance(int* lengths, const uint8_t* active, int64_t B, sqx_stream_t stream);
+
+/* ============================================================================================
+ * Serving over an 8-bit KV cache with one scale per block of tokens and head. No counterpart in the
+ * reference's quant modules: its FP8 cache keeps one scale per head (fp8_kv_per_head.py:120-223), its
+ * RoPE the interleaved full-head form (model.py:185-224), its sampler one token (sampling.py:80-86).
+ *
+ * The cache of a layer is paged. A page holds `block` tokens (16, 32, 64 or 128) of every kv head:
+ * k_codes [pages, Hkv, block, hd] and v_codes [pages, Hkv, hd, block] (one byte each, SQX_KV_*),
+ * k_scale and v_scale fp32 [pages, Hkv]; a code c stands for c * scale. table int32 [B, width]: the
+ * page of a row's positions block i .. block (i + 1) - 1. A page id outside [0, pages) is never
+ * followed. hd is 64, 128 or 256; positions stay below 2^30.
+ * ============================================================================================ */
+
+/* Rotary positions: out[n, h] is x[n, h] [heads, d] with its first rot columns rotated by the angles of
+ * row min(max(positions[n], 0), table_rows - 1) of cos_t / sin_t fp32 [table_rows, rot / 2] and the
+ * others copied. Pair i is columns (2i, 2i + 1) (interleaved) or (i, i + rot / 2):
+ *   y_a = x_a cos_i - x_b sin_i,  y_b = x_a sin_i + x_b cos_i
+ * each product and sum rounded to fp32, the result once to dtype (F32 / BF16 / F16). Strides in elements, of tokens and
+ * heads; columns are consecutive. out may be x. */
+int sqx_rope(const void* x, int dtype, int64_t n, int64_t heads, int64_t d, int64_t x_stride_n, int64_t x_stride_h,
+             const int* positions, const float* cos_t, const float* sin_t, int64_t table_rows, int64_t rot,
+             int interleaved, void* out, int64_t out_stride_n, int64_t out_stride_h, sqx_stream_t stream);
+
+/* Store the keys and values of counts[b] (NULL: T) new tokens of every row at positions starts[b] .. : k, v [B, T, Hkv,
+ * hd] of dtype, given by the strides of row, token and head (multiples of 8 elements; rows 16-byte aligned). With
+ * tables, keys are rotated first, by position, as sqx_rope rotates them (rot a multiple of 16), and rounded to dtype; q
+ * [B, T, H, hd], when given, is rotated into q_out (contiguous) for all T tokens of every row.
+ *   A block whose first token is written: s = max(fl(amax / qmax), 1e-12), qmax 127 or 448, amax over its finite new
+ *   values. A block that keeps earlier tokens: s 2^k with the least k >= 0 for which fl(amax / qmax) <= s 2^k, and its
+ *   codes become rne(c 2^-k).
+ *   code = clamp(rint(fl(x / s)), -127, 127), NaN 0; or the saturating E4M3 cast of fl(x / s).
+ * Nothing is stored for a negative start, outside the table, or where it names no page. The rows of one call must not
+ * write the same page. */
+int sqx_kvblock_write(const void* k, const void* v, int dtype, int64_t k_sb, int64_t k_st, int64_t k_sh, int64_t v_sb,
+                      int64_t v_st, int64_t v_sh, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, void* q_out,
+                      const float* cos_t, const float* sin_t, int64_t rope_rows, int64_t rot, int interleaved, int fmt,
+                      void* k_codes, void* v_codes, float* k_scale, float* v_scale, const int* table, const int* starts,
+                      const int* counts, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
+                      int64_t pages, int64_t width, sqx_stream_t stream);
+
+/* fp32(code) * scale, rounded once to dtype (F32 / BF16 / F16), of positions starts[b] .. starts[b] + T - 1 of every row:
+ * k_out, v_out [B, T, Hkv, hd]. Zeros from counts[b] (NULL: T) on, for a negative start, outside the table and where it
+ * names no page. */
+int sqx_kvblock_read(int fmt, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                     const int* table, const int* starts, const int* counts, int64_t B, int64_t T, int64_t Hkv,
+                     int64_t hd, int64_t block, int64_t pages, int64_t width, int dtype, void* k_out, void* v_out,
+                     sqx_stream_t stream);
+
+/* Causal attention of T new tokens a row over the cache, which already holds their keys and values:
+ *   out[b, t, h] = softmax_j(scale q[b, t, h] . k[b, j, h / G]) v[b, j, h / G],  j <= starts[b] + t,  G = H / Hkv
+ * for t < counts[b] (NULL: T); other tokens of out are left as they were. q BF16 or F16 [B, T, H, hd] by strides (as in
+ * sqx_kvblock_write), out contiguous of the same type. A token with no key (a negative position) gets zeros; one that
+ * attends a position without a page gets NaN. ws: sqx_kvblock_attention_workspace_bytes, 16-byte aligned (0: none). */
+int64_t sqx_kvblock_attention_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
+                                              int64_t width);
+int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int64_t q_st, int64_t q_sh, int fmt,
+                          const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                          const int* table, const int* starts, const int* counts, int64_t B, int64_t T, int64_t H,
+                          int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width, float scale, void* out,
+                          void* ws, int64_t ws_bytes, sqx_stream_t stream);
+
+/* Check counts[b] (NULL: T; T <= 63) drafted tokens of every row against the target's logits [B, T + 1, V] (F32 / BF16 /
+ * F16), from given random numbers. p_t = softmax(logits[b, t] / temperature), in double; q_t = probs[b, t] (F32 / BF16 /
+ * F16), or certainty for the drafted token (probs NULL).
+ *   Draft t is accepted while u[b, t] q_t(x_t) < p_t(x_t); n_accepted[b] is their number n.
+ *   The next token is the least i with cumsum(w)_i > r[b] sum(w): w = max(p_n - q_n, 0) after a rejection (p_n if that is
+ *   zero everywhere; a NaN of q takes the token out), p_n after none.
+ * temperature 0: accepted while x_t is the first maximum of its row (NaN counts as the maximum), then that maximum; u, r
+ * and probs are not read. tokens [B, T + 1]: the accepted drafts, the next token, then -1. An id outside [0, V) is
+ * rejected. A row that is no distribution (a NaN, +inf, or -inf everywhere) rejects its draft and its next token is -1. */
+int64_t sqx_verify_draft_workspace_bytes(int64_t B, int64_t T, int64_t V);
+int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int* counts, const void* probs,
+                     int probs_dtype, const float* u, const float* r, double temperature, int64_t B, int64_t T, int64_t V,
+                     int* n_accepted, int* tokens, void* ws, int64_t ws_bytes, sqx_stream_t stream);
 
 #ifdef __cplusplus
 }

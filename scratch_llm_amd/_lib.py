@@ -27,6 +27,8 @@ FP4_SCALE_MX_F32 = 0
 FP4_SCALE_MX_E8M0 = 1
 FP4_SCALE_NV_F32 = 2
 FP4_SCALE_NV_E4M3 = 3
+KV_INT8 = 0
+KV_E4M3 = 1
 GEMM_WEIGHTS = ("int4", "mxfp4", "nvfp4", "int8", "fp8")  # SQX_GEMM_* by index
 
 _TORCH_TO_SQX = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
@@ -233,6 +235,34 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sqx_argmax_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
     "sqx_argmax": (_c_i, [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p]),
     "sqx_advance": (_c_i, [_c_p, _c_p, _c_i64, _c_p]),
+    "sqx_rope": (
+        _c_i,
+        [_c_p, _c_i, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i, _c_p,
+         _c_i64, _c_i64, _c_p],
+    ),
+    "sqx_kvblock_write": (
+        _c_i,
+        [_c_p, _c_p, _c_i, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p,
+         _c_p, _c_p, _c_i64, _c_i64, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p],
+    ),
+    "sqx_kvblock_read": (
+        _c_i,
+        [_c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i, _c_p, _c_p, _c_p],
+    ),
+    "sqx_kvblock_attention_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "sqx_kvblock_attention": (
+        _c_i,
+        [_c_p, _c_i, _c_i64, _c_i64, _c_i64, _c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_i64, _c_p],
+    ),
+    "sqx_verify_draft_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "sqx_verify_draft": (
+        _c_i,
+        [_c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, ctypes.c_double, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
+         _c_p, _c_i64, _c_p],
+    ),
 }
 
 _lock = threading.Lock()

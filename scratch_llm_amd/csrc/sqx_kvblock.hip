@@ -1,0 +1,324 @@
+// The block-scaled 8-bit KV cache: writing new tokens (quantized as they are written, rotary positions included) and
+// reading values back. Layout and code formats: sqx_kvblock.h.
+//
+// A block's scale. A block whose first token is part of the write takes s = max(fl(amax / qmax), 1e-12) over the tokens
+// written (qmax 127 or 448). A block that already holds tokens keeps its scale, doubled k times, the least k with
+// fl(amax / qmax) <= s 2^k, and its codes become rne(c 2^-k). With growth in powers of two every later rescale at least
+// doubles the step, so what the rescales add to a token's error is at most s/2 (1 + 1/2 + 1/4 + ...) < s of the final
+// scale, however often the block grows; growing to each token's own amax would add s/2 at every token.
+// amax is taken over finite magnitudes: infinities saturate to the largest code, a NaN is a NaN in E4M3 and 0 in int8.
+#include "sqx_kvblock.h"
+
+namespace sqx {
+
+struct KvWriteArgs {
+  const void *k, *v, *q;  // q: NULL where none is rotated
+  void* q_out;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh, q_sb, q_st, q_sh;  // strides in elements: row, token, head
+  uint8_t *kc, *vc;
+  float *ks, *vs;
+  const int *table, *starts, *counts;  // counts: NULL means T everywhere
+  const float *cos_t, *sin_t;          // NULL: nothing is rotated
+  int rope_rows, rot, inter;
+  int T, H, Hkv, width, pages, block, shift;
+};
+
+constexpr int kQHeads = 8;  // query heads per workgroup of the rotary part
+
+// Workgroup (j, y, b): block j of the blocks that row b's tokens touch. y < Hkv: the keys of head y; then the values;
+// then groups of kQHeads query heads, whose rotation needs no block.
+template <int DT, int D, bool E4M3>
+__global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
+  using Code = KvCode<E4M3>;
+  constexpr int C = D / 8;                 // 8-element groups per token
+  constexpr int TP = 256 / C;              // tokens per pass
+  constexpr int NP = 128 / TP;             // passes of the largest block
+  constexpr int kPitch = 128 + 16;         // LDS pitch of a value column: a block's codes, 16-byte aligned
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[D * kPitch];
+  const int j = blockIdx.x, y = blockIdx.y, b = blockIdx.z;
+  const int start = a.starts[b];
+  const int off = start & (a.block - 1);
+  const int tid = threadIdx.x, c = tid % C, tl = tid / C;
+  auto table_row = [&](int t) {
+    const int64_t p = static_cast<int64_t>(start) + t;
+    return static_cast<int64_t>(p < 0 ? 0 : (p < a.rope_rows ? p : a.rope_rows - 1)) * (a.rot / 2);
+  };
+
+  if (y >= 2 * a.Hkv) {  // query heads: every token of the row, whatever its count
+    const int h0 = (y - 2 * a.Hkv) * kQHeads, nh = min(kQHeads, a.H - h0);
+    const int ta = max(0, j * a.block - off), tb = min(a.T, (j + 1) * a.block - off);
+    for (int i = tl; i < (tb - ta) * nh; i += TP) {
+      const int t = ta + i / nh, h = h0 + i % nh;
+      const int64_t row = b * a.q_sb + t * a.q_st + h * a.q_sh;
+      Row8<DT> x;
+      x.load(a.q, row + 8 * c);
+      const int64_t tr = table_row(t);
+      rope_row8<DT>(x, c, a.rot, a.inter, a.cos_t + tr, a.sin_t + tr, [&](int g) {
+        Row8<DT> o;
+        o.load(a.q, row + 8 * g);
+        return o;
+      });
+      x.store(a.q_out, ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * D + 8 * c);
+    }
+    return;
+  }
+
+  if (start < 0) return;
+  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  const int lo = j == 0 ? off : 0, hi = min(a.block, off + count - j * a.block);
+  const int blk = (start >> a.shift) + j;
+  if (hi <= lo || blk >= a.width) return;
+  const int page = a.table[static_cast<int64_t>(b) * a.width + blk];
+  if (page < 0 || page >= a.pages) return;  // no such page: the tokens are not stored
+  const bool is_v = y >= a.Hkv;
+  const int h = is_v ? y - a.Hkv : y;
+  const int64_t ph = static_cast<int64_t>(page) * a.Hkv + h;
+  float* const sp = (is_v ? a.vs : a.ks) + ph;
+  uint8_t* const codes = (is_v ? a.vc : a.kc) + ph * a.block * D;
+  const float had = lo > 0 ? fmaxf(*sp, kKvMinScale) : 0.0f;
+
+  Row8<DT> x[NP];
+  float most = 0.0f;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int slot = lo + p * TP + tl;
+    if (slot < hi) {
+      const int t = slot - off + j * a.block;
+      const void* src = is_v ? a.v : a.k;
+      const int64_t row = is_v ? b * a.v_sb + t * a.v_st + h * a.v_sh : b * a.k_sb + t * a.k_st + h * a.k_sh;
+      x[p].load(src, row + 8 * c);
+      if (!is_v && a.cos_t != nullptr) {
+        const int64_t tr = table_row(t);
+        rope_row8<DT>(x[p], c, a.rot, a.inter, a.cos_t + tr, a.sin_t + tr, [&](int g) {
+          Row8<DT> o;
+          o.load(src, row + 8 * g);
+          return o;
+        });
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float m = fabsf(x[p].get(e));
+        most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float s = fmaxf(__fdiv_rn(most, Code::kMax), kKvMinScale);
+  float down = 1.0f;  // 2^-k
+  if (lo > 0) {
+    int en, eh;
+    const float mn = frexpf(s, &en), mh = frexpf(had, &eh);
+    const int k = max(en - eh + (mn > mh ? 1 : 0), 0);
+    s = ldexpf(had, k);
+    down = ldexpf(1.0f, -k);
+  }
+  if (tid == 0) *sp = s;
+  const SharedDiv sd = shared_div(s);
+
+  if (!is_v) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int slot = lo + p * TP + tl;
+      if (slot < hi) {
+        u32x2v_t w = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= Code::encode(sd, x[p].get(e)) << (8 * (e & 3));
+        *reinterpret_cast<u32x2v_t*>(codes + slot * D + 8 * c) = w;
+      }
+    }
+    if (down != 1.0f) {
+      for (int i = tid; i < lo * (D / 4); i += 256) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(codes) + i;
+        *w = Code::shrink4(*w, down);
+      }
+    }
+    return;
+  }
+  // values: transposed through LDS, then 16 tokens of a column at a time, merged with the codes that stay
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int slot = lo + p * TP + tl;
+    if (slot < hi) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        tile[(8 * c + e) * kPitch + slot] = static_cast<uint8_t>(Code::encode(sd, x[p].get(e)));
+    }
+  }
+  __syncthreads();
+  const int nch = a.block >> 4;
+  for (int i = tid; i < D * nch; i += 256) {
+    const int d = i / nch, s0 = (i % nch) * 16;
+    if (s0 >= hi || (s0 + 16 <= lo && down == 1.0f)) continue;
+    u32x4_t* g = reinterpret_cast<u32x4_t*>(codes + d * a.block + s0);
+    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(tile + d * kPitch + s0);
+    u32x4_t w;
+    if (s0 >= lo && s0 + 16 <= hi) {
+      w = n;
+    } else {
+      w = *g;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t r = w[q];
+        const uint32_t nw = n[q];
+        const int s4 = s0 + 4 * q;
+        const uint32_t less = down != 1.0f && s4 < lo ? Code::shrink4(r, down) : r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t byte = 0xffu << (8 * e);
+          if (s4 + e < lo) r = (r & ~byte) | (less & byte);
+          else if (s4 + e < hi) r = (r & ~byte) | (nw & byte);
+        }
+        w[q] = r;
+      }
+    }
+    *g = w;
+  }
+}
+
+// Values of positions starts[b] .. + tokens - 1 of every row: fp32(code) * scale, rounded once; zeros from counts[b] on,
+// outside the table and where it names no page.
+template <int DT, int D, bool E4M3>
+__global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                      const float* __restrict__ ks, const float* __restrict__ vs,
+                                                      const int* __restrict__ table, const int* __restrict__ starts,
+                                                      const int* __restrict__ counts, int T, int Hkv, int width,
+                                                      int pages, int block, int shift, void* k_out, void* v_out) {
+  using Code = KvCode<E4M3>;
+  constexpr int C = D / 8, TP = 256 / C, kPitch = 128 + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[D * kPitch];
+  const int j = blockIdx.x, y = blockIdx.y, b = blockIdx.z;
+  const bool is_v = y >= Hkv;
+  const int h = is_v ? y - Hkv : y;
+  const int start = starts[b], off = start & (block - 1);
+  const int count = counts != nullptr ? min(max(counts[b], 0), T) : T;
+  const int lo = j == 0 ? off : 0, hi = min(block, off + T - j * block);
+  const int tid = threadIdx.x, c = tid % C, tl = tid / C;
+  if (hi <= lo) return;
+  const int64_t blk = (static_cast<int64_t>(start) >> shift) + j;
+  int page = -1;
+  if (start >= 0 && blk < width) page = table[static_cast<int64_t>(b) * width + blk];
+  const bool some = page >= 0 && page < pages;
+  const int64_t ph = some ? static_cast<int64_t>(page) * Hkv + h : 0;
+  const float s = some ? (is_v ? vs : ks)[ph] : 0.0f;
+  const uint8_t* codes = (is_v ? vc : kc) + ph * block * D;
+  if (is_v && some) {
+    const int nch = block >> 4;
+    for (int i = tid; i < D * nch; i += 256) {
+      const int d = i / nch, s0 = (i % nch) * 16;
+      *reinterpret_cast<u32x4_t*>(tile + d * kPitch + s0) = *reinterpret_cast<const u32x4_t*>(codes + d * block + s0);
+    }
+    __syncthreads();
+  }
+  for (int slot = lo + tl; slot < hi; slot += TP) {
+    const int t = slot - off + j * block;
+    const bool have = some && t < count;
+    u32x2v_t w = {0u, 0u};
+    if (have && !is_v) w = *reinterpret_cast<const u32x2v_t*>(codes + slot * D + 8 * c);
+    Row8<DT> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q = 2 * i + e;
+        const uint32_t byte = is_v ? (have ? tile[(8 * c + q) * kPitch + slot] : 0u) : (w[q >> 2] >> (8 * (q & 3))) & 0xffu;
+        f[e] = have ? Code::decode(byte) * s : 0.0f;
+      }
+      r.set_pair(i, f[0], f[1]);
+    }
+    r.store(is_v ? v_out : k_out, ((static_cast<int64_t>(b) * T + t) * Hkv + h) * D + 8 * c);
+  }
+}
+
+}  // namespace sqx
+
+using namespace sqx;
+
+extern "C" int sqx_kvblock_write(const void* k, const void* v, int dtype, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                                 int64_t v_sb, int64_t v_st, int64_t v_sh, const void* q, int64_t q_sb, int64_t q_st,
+                                 int64_t q_sh, void* q_out, const float* cos_t, const float* sin_t, int64_t rope_rows,
+                                 int64_t rot, int interleaved, int fmt, void* k_codes, void* v_codes, float* k_scale,
+                                 float* v_scale, const int* table, const int* starts, const int* counts, int64_t B,
+                                 int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block, int64_t pages,
+                                 int64_t width, sqx_stream_t stream) {
+  const char* fn = "sqx_kvblock_write";
+  KV_SHAPE(fn);
+  SQX_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), SQX_E_ARG, "%s: give both tables or neither", fn);
+  SQX_REQUIRE(q == nullptr || cos_t != nullptr, SQX_E_ARG, "%s: queries are only rotated here: give the tables", fn);
+  SQX_REQUIRE((q == nullptr) == (q_out == nullptr), SQX_E_ARG, "%s: q and q_out go together", fn);
+  SQX_REQUIRE(q == nullptr || (H >= 1 && H <= 8192), SQX_E_ARG, "%s: H=%lld (1 to 8192)", fn, (long long)H);
+  SQX_REQUIRE(cos_t == nullptr || (rot >= 16 && rot % 16 == 0 && rot <= hd && rope_rows >= 1 &&
+                                   rope_rows < (int64_t(1) << 31)),
+              SQX_E_ARG, "%s: rot=%lld must be a multiple of 16 up to head_dim, and the table not empty", fn, (long long)rot);
+  SQX_REQUIRE(k_sb >= 0 && k_st >= 0 && k_sh >= 0 && v_sb >= 0 && v_st >= 0 && v_sh >= 0 && q_sb >= 0 && q_st >= 0 &&
+                  q_sh >= 0,
+              SQX_E_ARG, "%s: negative stride", fn);
+  SQX_REQUIRE((k_sb | k_st | k_sh | v_sb | v_st | v_sh | q_sb | q_st | q_sh) % 8 == 0, SQX_E_ARG,
+              "%s: strides must be multiples of 8 elements", fn);
+  if (B == 0 || T == 0) return SQX_OK;
+  SQX_REQUIRE(k && v && k_codes && v_codes && k_scale && v_scale && table && starts, SQX_E_ARG, "%s: null pointer", fn);
+  SQX_REQUIRE(al16(k) && al16(v) && al16(q) && al16(q_out) && al16(k_codes) && al16(v_codes) && al16(cos_t) && al16(sin_t),
+              SQX_E_ARG, "%s: rows, codes and tables must be 16-byte aligned", fn);
+  KvWriteArgs a{};
+  a.k = k; a.v = v; a.q = q; a.q_out = q_out;
+  a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
+  a.v_sb = v_sb; a.v_st = v_st; a.v_sh = v_sh;
+  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.kc = static_cast<uint8_t*>(k_codes); a.vc = static_cast<uint8_t*>(v_codes);
+  a.ks = k_scale; a.vs = v_scale;
+  a.table = table; a.starts = starts; a.counts = counts;
+  a.cos_t = cos_t; a.sin_t = sin_t;
+  a.rope_rows = static_cast<int>(cos_t ? rope_rows : 1); a.rot = static_cast<int>(cos_t ? rot : 0); a.inter = interleaved;
+  a.T = static_cast<int>(T); a.H = static_cast<int>(H); a.Hkv = static_cast<int>(Hkv); a.width = static_cast<int>(width);
+  a.pages = static_cast<int>(pages); a.block = static_cast<int>(block);
+  a.shift = kv_shift(block);
+  const dim3 grid(static_cast<unsigned>((T + 2 * block - 2) / block),
+                  static_cast<unsigned>(2 * Hkv + (q ? ceil_div(H, kQHeads) : 0)), static_cast<unsigned>(B));
+  with_dtype(dtype, [&](auto dt) {
+    with_head(hd, [&](auto dd) {
+      if (fmt == SQX_KV_E4M3)
+        hipLaunchKernelGGL((kv_write_kernel<decltype(dt)::value, decltype(dd)::value, true>), grid, dim3(256), 0,
+                           as_stream(stream), a);
+      else
+        hipLaunchKernelGGL((kv_write_kernel<decltype(dt)::value, decltype(dd)::value, false>), grid, dim3(256), 0,
+                           as_stream(stream), a);
+    });
+  });
+  SQX_LAUNCH_CHECK(fn);
+  return SQX_OK;
+}
+
+extern "C" int sqx_kvblock_read(int fmt, const void* k_codes, const void* v_codes, const float* k_scale,
+                                const float* v_scale, const int* table, const int* starts, const int* counts, int64_t B,
+                                int64_t T, int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width,
+                                int dtype, void* k_out, void* v_out, sqx_stream_t stream) {
+  const char* fn = "sqx_kvblock_read";
+  KV_SHAPE(fn);
+  if (B == 0 || T == 0) return SQX_OK;
+  SQX_REQUIRE(k_codes && v_codes && k_scale && v_scale && table && starts && k_out && v_out, SQX_E_ARG, "%s: null pointer",
+              fn);
+  SQX_REQUIRE(al16(k_codes) && al16(v_codes) && al16(k_out) && al16(v_out), SQX_E_ARG,
+              "%s: codes and outputs must be 16-byte aligned", fn);
+  const int shift = kv_shift(block);
+  const dim3 grid(static_cast<unsigned>((T + 2 * block - 2) / block), static_cast<unsigned>(2 * Hkv),
+                  static_cast<unsigned>(B));
+  with_dtype(dtype, [&](auto dt) {
+    with_head(hd, [&](auto dd) {
+      auto go = [&](auto e4) {
+        hipLaunchKernelGGL((kv_read_kernel<decltype(dt)::value, decltype(dd)::value, decltype(e4)::value>), grid, dim3(256), 0,
+                           as_stream(stream), static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes),
+                           k_scale, v_scale, table, starts, counts, static_cast<int>(T), static_cast<int>(Hkv),
+                           static_cast<int>(width), static_cast<int>(pages), static_cast<int>(block), shift, k_out, v_out);
+      };
+      if (fmt == SQX_KV_E4M3) go(std::true_type{});
+      else go(std::false_type{});
+    });
+  });
+  SQX_LAUNCH_CHECK(fn);
+  return SQX_OK;
+}

@@ -1,0 +1,450 @@
+// Verification of drafted tokens against the target model's logits, from given random numbers (speculative sampling), and
+// the sampling of the token that follows.
+//
+// With p_t = softmax(logits_t / temperature) and q_t the draft's probabilities, draft t is accepted while
+// u_t q_t(x_t) < p_t(x_t). After the first rejection the token is drawn from max(p - q, 0) of that row, after none from p
+// of the row behind the drafts: the least i whose cumulative weight exceeds r times the total, so the kept tokens are
+// distributed as the target's own. Temperature 0: accept while x_t is the row's argmax, then take the argmax.
+//
+// Probabilities, totals and cumulative sums are double: the pick falls between two neighbours of a cumulative sum over a
+// whole vocabulary, and in fp32 about one pick in a hundred would depend on the order of the sums. The exponential costs a
+// dozen double operations (below), so a row is still bound by reading it once.
+//
+// Three launches (two at temperature 0): statistics of every slice of every row; the residual's sum of every slice of the
+// one row per sequence that needs it; the pick. The decision is a few operations on the slices' statistics, so the second
+// and third repeat it in every workgroup instead of waiting for one.
+#include <type_traits>
+
+#include "sqx_common.h"
+
+namespace sqx {
+
+constexpr int kSlice = 8192;                // elements of a workgroup's slice
+constexpr int kPer = 8;                     // consecutive elements of a thread, a pass
+constexpr int kPass = 256 * kPer;           // elements of a pass
+constexpr int kPasses = kSlice / kPass;
+constexpr int kMaxDrafts = 63;              // a lane each, and one for the row behind them
+
+struct VerifyArgs {
+  const void* logits;  // [B, T + 1, V]
+  const int* draft;    // [B, T]
+  const int* counts;   // NULL: T drafts in every row
+  const void* probs;   // [B, T, V], or NULL: each draft was certain
+  const float *u, *r;
+  int T, V, S;
+  double k;  // log2(e) / temperature
+  double* sums;  // [B, T + 1, S]
+  double* rest;  // [B, S]
+  float* maxs;   // [B, T + 1, S]
+  int* args;     // [B, T + 1, S], temperature 0
+  int *n_acc, *tokens;
+};
+
+// 2^y for y <= 0: y = n / 32 + f, |f| <= 1/64; 2^(n / 32) from a table of 32 powers and an exponent, 2^f from its Taylor
+// polynomial of degree 5 in f ln 2 (the term left out is below 3e-15).
+__device__ inline double exp2_neg(double y, const double* pow32) {
+  y = y < -1100.0 ? -1100.0 : y;  // NaN stays
+  const double n = __builtin_rint(y * 32.0);
+  const double x = fma(n, -0.03125, y) * 0.693147180559945309417;
+  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(p, x, 1.0 / 6.0);
+  p = fma(p, x, 0.5);
+  p = fma(p, x, 1.0);
+  p = fma(p, x, 1.0);
+  const int i = static_cast<int>(n);
+  return ldexp(p * pow32[i & 31], i >> 5);
+}
+__device__ inline void fill_pow32(double* pow32) {
+  if (threadIdx.x < 32) pow32[threadIdx.x] = exp2(threadIdx.x * 0.03125);
+}
+
+// Elements base .. base + 7 of a row of V as fp32; past the end `fill`.
+template <int DT, bool VEC>
+__device__ inline void load_row8(const void* p, int64_t row0, int base, int V, float fill, float (&v)[kPer]) {
+  if (VEC && base + kPer <= V) {
+    if constexpr (DT == SQX_DTYPE_F32) {
+      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + row0 + base);
+      const f32x4_t a = q[0], b = q[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    } else {
+      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + row0 + base);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = a[e];
+        v[2 * e] = DT == SQX_DTYPE_BF16 ? bf16_lo(w) : f16_bits_to_f32(static_cast<uint16_t>(w));
+        v[2 * e + 1] = DT == SQX_DTYPE_BF16 ? bf16_hi(w) : f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) v[e] = base + e < V ? load_as_f32(p, DT, row0 + base + e) : fill;
+}
+
+__device__ inline double wave_sum_f64(double v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// The sum over the workgroup, in every thread; `red` holds one value per wave and is free again after the call.
+__device__ inline double block_sum_f64(double v, double* red) {
+  v = wave_sum_f64(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = (red[0] + red[1]) + (red[2] + red[3]);
+  __syncthreads();
+  return v;
+}
+
+// Slice s of row (b, t): its maximum and the sum of 2^(k (x - maximum)); temperature 0: the maximum's first index
+// (NaN counts as the maximum).
+template <int DT, bool VEC, bool GREEDY>
+__global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
+  __shared__ double pow32[32], red[4];
+  __shared__ float redm[4];
+  __shared__ int redi[4];
+  const int s = blockIdx.x, row = blockIdx.y, b = row / (a.T + 1), t = row % (a.T + 1);
+  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  if (t > count) return;
+  if constexpr (!GREEDY) fill_pow32(pow32);
+  const int64_t row0 = static_cast<int64_t>(row) * a.V;
+  const int at = s * kSlice + threadIdx.x * kPer;
+  float v[kPasses][kPer];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) load_row8<DT, VEC>(a.logits, row0, at + p * kPass, a.V, -INFINITY, v[p]);
+  const int64_t out = static_cast<int64_t>(row) * a.S + s;
+  if constexpr (GREEDY) {
+    float best = -INFINITY;
+    int arg = 0x7fffffff;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int i = at + p * kPass + e;
+        const bool nan = v[p][e] != v[p][e], bn = best != best;
+        if (i < a.V && !bn && (nan || v[p][e] > best || arg == 0x7fffffff)) {
+          best = v[p][e];
+          arg = i;
+        }
+      }
+    auto join = [&](float ob, int oa) {
+      const bool on = ob != ob, bn = best != best;
+      const bool take = oa != 0x7fffffff &&
+                        (arg == 0x7fffffff || (on && !bn) || (on == bn && ((on || ob == best) ? oa < arg : ob > best)));
+      if (take) {
+        best = ob;
+        arg = oa;
+      }
+    };
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const float ob = __shfl_xor(best, o, 64);
+      const int oa = __shfl_xor(arg, o, 64);
+      join(ob, oa);
+    }
+    if ((threadIdx.x & 63) == 0) {
+      redm[threadIdx.x >> 6] = best;
+      redi[threadIdx.x >> 6] = arg;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 4; ++w) join(redm[w], redi[w]);
+      a.maxs[out] = best;
+      a.args[out] = arg;
+    }
+  } else {
+    float m = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) m = fmaxf(m, v[p][e]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) redm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
+    const double md = m == -INFINITY ? 0.0 : static_cast<double>(m);  // all masked: every term is zero
+    double sum = 0.0;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const double y = (static_cast<double>(v[p][e]) - md) * a.k;
+        sum += v[p][e] == -INFINITY ? 0.0 : exp2_neg(y, pow32);
+      }
+    sum = block_sum_f64(sum, red);
+    if (threadIdx.x == 0) {
+      a.maxs[out] = m;
+      a.sums[out] = sum;
+    }
+  }
+}
+
+struct Verdict {
+  int n, count;   // accepted, drafted
+  double m, inv;  // of row n: maximum, 1 / sum (NaN where the row has no distribution)
+};
+
+// Lane t of a wave judges draft t (and lane `count` the row behind the drafts); the same in every wave that calls it.
+template <int DT>
+__device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const double* pow32) {
+  const int lane = threadIdx.x & 63;
+  Verdict r;
+  r.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  double m = 0.0, z = 0.0, inv = 0.0;
+  bool good = false;
+  if (lane <= r.count) {
+    const int64_t at = (static_cast<int64_t>(b) * (a.T + 1) + lane) * a.S;
+    float mx = -INFINITY;
+    for (int s = 0; s < a.S; ++s) mx = fmaxf(mx, a.maxs[at + s]);
+    m = mx == -INFINITY ? 0.0 : static_cast<double>(mx);
+    for (int s = 0; s < a.S; ++s) {
+      const float ms = a.maxs[at + s];
+      if (ms != -INFINITY) z += a.sums[at + s] * exp2_neg((static_cast<double>(ms) - m) * a.k, pow32);
+    }
+    inv = 1.0 / z;  // of a sum of zero infinite, of NaN NaN
+    if (!(z > 0.0 && inv > 0.0)) inv = __builtin_nan("");
+    if (lane < r.count) {
+      const int x = a.draft[static_cast<int64_t>(b) * a.T + lane];
+      if (x >= 0 && x < a.V) {
+        const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + lane, prow = static_cast<int64_t>(b) * a.T + lane;
+        const float lx = load_as_f32(a.logits, DT, row * a.V + x);
+        const double px = lx == -INFINITY ? 0.0 * inv : exp2_neg((static_cast<double>(lx) - m) * a.k, pow32) * inv;
+        const double qx = a.probs != nullptr ? static_cast<double>(load_as_f32(a.probs, pdt, prow * a.V + x)) : 1.0;
+        good = static_cast<double>(a.u[prow]) * qx < px;
+      }
+    }
+  }
+  const uint64_t bad = ~__ballot(good);
+  r.n = min(static_cast<int>(__builtin_ctzll(bad | (uint64_t(1) << 63))), r.count);
+  r.m = __shfl(m, r.n, 64);
+  r.inv = __shfl(inv, r.n, 64);
+  return r;
+}
+
+// Weights of elements base .. base + 7 of the row that the pick is drawn from.
+template <int DT, bool VEC>
+__device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, int base, int pdt, bool residual, int x,
+                                const double* pow32, double (&w)[kPer]) {
+  const int64_t row0 = (static_cast<int64_t>(b) * (a.T + 1) + v.n) * a.V;
+  float l[kPer], q[kPer];
+  load_row8<DT, VEC>(a.logits, row0, base, a.V, -INFINITY, l);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) q[e] = 0.0f;
+  if (residual && a.probs != nullptr) {
+    const int64_t p0 = (static_cast<int64_t>(b) * a.T + v.n) * a.V;
+    if (pdt == SQX_DTYPE_F32) load_row8<SQX_DTYPE_F32, VEC>(a.probs, p0, base, a.V, 0.0f, q);
+    else if (pdt == SQX_DTYPE_BF16) load_row8<SQX_DTYPE_BF16, VEC>(a.probs, p0, base, a.V, 0.0f, q);
+    else load_row8<SQX_DTYPE_F16, VEC>(a.probs, p0, base, a.V, 0.0f, q);
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const double p = l[e] == -INFINITY ? 0.0 : exp2_neg((static_cast<double>(l[e]) - v.m) * a.k, pow32) * v.inv;
+    const double qe = residual && a.probs == nullptr ? (base + e == x ? 1.0 : 0.0) : static_cast<double>(q[e]);
+    w[e] = residual ? (p > qe ? p - qe : 0.0) : p;
+  }
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, int pdt) {
+  __shared__ double pow32[32], red[4];
+  fill_pow32(pow32);
+  __syncthreads();
+  const int s = blockIdx.x, b = blockIdx.y;
+  const Verdict v = judge<DT>(a, b, pdt, pow32);
+  if (v.n == v.count) return;  // nothing was rejected: the row's own statistics serve
+  const int x = a.draft[static_cast<int64_t>(b) * a.T + v.n];
+  double sum = 0.0;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    double w[kPer];
+    weights8<DT, VEC>(a, v, b, s * kSlice + p * kPass + threadIdx.x * kPer, pdt, true, x, pow32, w);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += w[e];
+  }
+  sum = block_sum_f64(sum, red);
+  if (threadIdx.x == 0) a.rest[static_cast<int64_t>(b) * a.S + s] = sum;
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a, int pdt) {
+  __shared__ double pow32[32], wsum[4];
+  __shared__ int found, last;
+  fill_pow32(pow32);
+  if (threadIdx.x == 0) {
+    found = 0x7fffffff;
+    last = -1;
+  }
+  __syncthreads();
+  const int b = blockIdx.x;
+  const Verdict v = judge<DT>(a, b, pdt, pow32);
+  const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
+  bool residual = v.n < v.count;
+  double total = 0.0;
+  if (residual) {
+    for (int s = 0; s < a.S; ++s) total += a.rest[static_cast<int64_t>(b) * a.S + s];
+    residual = !(total <= 0.0);  // p nowhere above q: drawn from p (a NaN goes on as one)
+  }
+  auto slice_sum = [&](int s) -> double {
+    if (residual) return a.rest[static_cast<int64_t>(b) * a.S + s];
+    const float ms = a.maxs[row * a.S + s];
+    return ms == -INFINITY ? 0.0 : a.sums[row * a.S + s] * exp2_neg((static_cast<double>(ms) - v.m) * a.k, pow32) * v.inv;
+  };
+  if (!residual) {
+    total = 0.0;
+    for (int s = 0; s < a.S; ++s) total += slice_sum(s);
+  }
+  int pick = -1;
+  if (total > 0.0) {  // false for a row without a distribution
+    const double theta = static_cast<double>(a.r[b]) * total;
+    int hit = -1, fallback = 0;
+    double before = 0.0, sum = 0.0;
+    for (int s = 0; s < a.S; ++s) {
+      const double w = slice_sum(s);
+      if (w > 0.0) fallback = s;
+      if (hit < 0 && sum + w > theta) {
+        hit = s;
+        before = sum;
+      }
+      sum += w;
+    }
+    const bool none = hit < 0;  // r next to 1 and a rounding: the last token that has a weight
+    if (none) hit = fallback;
+    const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
+    for (int p = 0; p < kPasses; ++p) {
+      const int at = hit * kSlice + p * kPass + threadIdx.x * kPer;
+      double w[kPer], mine = 0.0;
+      weights8<DT, VEC>(a, v, b, at, pdt, residual, x, pow32, w);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) mine += w[e];
+      double inc = mine;  // inclusive scan over the wave, then over the waves
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(inc, o, 64);
+        if ((threadIdx.x & 63) >= o) inc += u;
+      }
+      if ((threadIdx.x & 63) == 63) wsum[threadIdx.x >> 6] = inc;
+      __syncthreads();
+      double c = before;
+      for (int i = 0; i < static_cast<int>(threadIdx.x >> 6); ++i) c += wsum[i];
+      c += inc - mine;
+      int first = 0x7fffffff, end = -1;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        c += w[e];
+        if (w[e] > 0.0) end = at + e;
+        if (first == 0x7fffffff && w[e] > 0.0 && c > theta) first = at + e;
+      }
+      if (!none && first != 0x7fffffff) atomicMin(&found, first);
+      if (end >= 0) atomicMax(&last, end);
+      before += (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+      __syncthreads();
+      if (found != 0x7fffffff) break;
+      __syncthreads();
+    }
+    pick = found != 0x7fffffff ? found : last;
+  }
+  if (threadIdx.x == 0) a.n_acc[b] = v.n;
+  if (static_cast<int>(threadIdx.x) <= a.T) {
+    const int t = threadIdx.x;
+    a.tokens[static_cast<int64_t>(b) * (a.T + 1) + t] = t < v.n ? a.draft[static_cast<int64_t>(b) * a.T + t] : t == v.n ? pick : -1;
+  }
+}
+
+__global__ __launch_bounds__(64) void verify_greedy_kernel(const VerifyArgs a) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  int arg = 0x7fffffff;
+  float best = -INFINITY;
+  bool good = false;
+  if (lane <= count) {
+    const int64_t at = (static_cast<int64_t>(b) * (a.T + 1) + lane) * a.S;
+    for (int s = 0; s < a.S; ++s) {  // slices are in order: a later one has to be above
+      const float ob = a.maxs[at + s];
+      if (arg == 0x7fffffff || (best == best && (ob != ob || ob > best))) {
+        best = ob;
+        arg = a.args[at + s];
+      }
+    }
+    good = lane < count && a.draft[static_cast<int64_t>(b) * a.T + lane] == arg;
+  }
+  const uint64_t bad = ~__ballot(good);
+  const int n = min(static_cast<int>(__builtin_ctzll(bad | (uint64_t(1) << 63))), count);
+  const int pick = __shfl(arg, n, 64);
+  if (lane == 0) a.n_acc[b] = n;
+  if (lane <= a.T)
+    a.tokens[static_cast<int64_t>(b) * (a.T + 1) + lane] = lane < n ? a.draft[static_cast<int64_t>(b) * a.T + lane] : lane == n ? pick : -1;
+}
+
+}  // namespace sqx
+
+using namespace sqx;
+
+extern "C" int64_t sqx_verify_draft_workspace_bytes(int64_t B, int64_t T, int64_t V) {
+  if (B <= 0 || T < 0 || V <= 0) return 0;
+  const int64_t S = ceil_div(V, kSlice);
+  return B * (T + 1) * S * 16 + B * S * 8;
+}
+
+extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int* counts, const void* probs,
+                                int probs_dtype, const float* u, const float* r, double temperature, int64_t B, int64_t T,
+                                int64_t V, int* n_accepted, int* tokens, void* ws, int64_t ws_bytes, sqx_stream_t stream) {
+  const char* fn = "sqx_verify_draft";
+  SQX_REQUIRE(dtype == SQX_DTYPE_F32 || dtype == SQX_DTYPE_BF16 || dtype == SQX_DTYPE_F16, SQX_E_ARG,
+              "%s: logits must be F32, BF16 or F16", fn);
+  SQX_REQUIRE(probs == nullptr || probs_dtype == SQX_DTYPE_F32 || probs_dtype == SQX_DTYPE_BF16 || probs_dtype == SQX_DTYPE_F16,
+              SQX_E_ARG, "%s: probs must be F32, BF16 or F16", fn);
+  SQX_REQUIRE(B >= 0 && T >= 0 && T <= kMaxDrafts && B * (T + 1) < 65536, SQX_E_ARG,
+              "%s: bad shape (B=%lld, T=%lld up to %d, B (T + 1) below 65536)", fn, (long long)B, (long long)T, kMaxDrafts);
+  SQX_REQUIRE(V >= 1 && V < (int64_t(1) << 30), SQX_E_ARG, "%s: V=%lld", fn, (long long)V);
+  SQX_REQUIRE(temperature == 0.0 || (temperature >= 1e-4 && temperature <= 1e4), SQX_E_ARG,
+              "%s: temperature must be 0 or within 1e-4 .. 1e4", fn);
+  if (B == 0) return SQX_OK;
+  const bool greedy = temperature == 0.0;
+  SQX_REQUIRE(logits && n_accepted && tokens && ws && (T == 0 || draft) && (greedy || (r && (T == 0 || u))), SQX_E_ARG,
+              "%s: null pointer", fn);
+  const int64_t need = sqx_verify_draft_workspace_bytes(B, T, V);
+  SQX_REQUIRE(ws_bytes >= need, SQX_E_SPACE, "%s: workspace of %lld bytes, %lld needed", fn, (long long)ws_bytes,
+              (long long)need);
+  SQX_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 8 == 0, SQX_E_ARG, "%s: workspace must be 8-byte aligned", fn);
+  VerifyArgs a{};
+  a.logits = logits; a.draft = draft; a.counts = counts; a.probs = probs; a.u = u; a.r = r;
+  a.T = static_cast<int>(T); a.V = static_cast<int>(V); a.S = static_cast<int>(ceil_div(V, kSlice));
+  a.k = greedy ? 0.0 : 1.4426950408889634074 / temperature;
+  const int64_t rows = B * (T + 1) * a.S;
+  a.sums = static_cast<double*>(ws);
+  a.rest = a.sums + rows;
+  a.maxs = reinterpret_cast<float*>(a.rest + B * a.S);
+  a.args = reinterpret_cast<int*>(a.maxs + rows);
+  a.n_acc = n_accepted; a.tokens = tokens;
+  auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool vec = V % 8 == 0 && aligned(logits) && aligned(probs);
+  const hipStream_t s = as_stream(stream);
+  const dim3 all(static_cast<unsigned>(a.S), static_cast<unsigned>(B * (T + 1)));
+  const dim3 one(static_cast<unsigned>(a.S), static_cast<unsigned>(B)), seqs(static_cast<unsigned>(B));
+  auto go = [&](auto dt, auto vv) {
+    constexpr int DT = decltype(dt)::value;
+    constexpr bool VEC = decltype(vv)::value;
+    if (greedy) {
+      hipLaunchKernelGGL((verify_stats_kernel<DT, VEC, true>), all, dim3(256), 0, s, a);
+      hipLaunchKernelGGL(verify_greedy_kernel, seqs, dim3(64), 0, s, a);
+      return;
+    }
+    hipLaunchKernelGGL((verify_stats_kernel<DT, VEC, false>), all, dim3(256), 0, s, a);
+    if (T > 0) hipLaunchKernelGGL((verify_rest_kernel<DT, VEC>), one, dim3(256), 0, s, a, probs_dtype);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, VEC>), seqs, dim3(256), 0, s, a, probs_dtype);
+  };
+  auto with_vec = [&](auto dt) {
+    if (vec) go(dt, std::true_type{});
+    else go(dt, std::false_type{});
+  };
+  if (dtype == SQX_DTYPE_F32) with_vec(std::integral_constant<int, SQX_DTYPE_F32>{});
+  else if (dtype == SQX_DTYPE_BF16) with_vec(std::integral_constant<int, SQX_DTYPE_BF16>{});
+  else with_vec(std::integral_constant<int, SQX_DTYPE_F16>{});
+  SQX_LAUNCH_CHECK(fn);
+  return SQX_OK;
+}

@@ -1,0 +1,77 @@
+"""Verification of drafted tokens on MI355X: speculative sampling's accept and resample step, and its last sample.
+
+The reference samples one token from one row of logits (src/scratch_llm/sampling.py:80-86). Here a target
+model has scored several drafted tokens of every row in one pass (:meth:`Int4DecodeLM.extend`), and
+:func:`verify_draft` says how many of them to keep and which token follows, such that the kept tokens
+are distributed as the target's own. Random numbers are inputs, so a run can be repeated.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from scratch_llm_amd import _lib
+
+__all__ = ["MAX_DRAFTS", "verify_draft"]
+
+MAX_DRAFTS = 63  # drafted tokens per row of one call
+
+
+def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | None, *, draft_probs: Tensor | None = None,
+                 counts: Tensor | None = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
+    """Check ``draft [B, T]`` (int32 ids) against ``logits [B, T + 1, V]``: row t scores the token after t drafts.
+
+    With ``p_t = softmax(logits[:, t] / temperature)`` and ``q_t = draft_probs[:, t]`` (``[B, T, V]``; None: the
+    draft was certain of its token), draft t is accepted while ``u[b, t] * q_t(x_t) < p_t(x_t)``. The token that
+    follows is drawn from ``max(p - q, 0)`` of the first rejected row, or from ``p`` of the row behind the
+    drafts: the least id whose cumulative weight exceeds ``r[b]`` times the total. Probabilities and sums are
+    float64. ``temperature=0`` accepts while the draft is its row's argmax and then takes the argmax (``u``, ``r``
+    and ``draft_probs`` may be None). ``counts`` (int32 ``[B]``) says how many drafts a row has (default T).
+
+    ``u [B, T]`` and ``r [B]`` are float32 in [0, 1). Returns ``(n_accepted int32 [B], tokens int32 [B, T + 1])``:
+    the accepted drafts, the next token, then -1. An id outside the vocabulary is rejected; a row that is no
+    distribution (NaN, +inf, or -inf everywhere) rejects its draft and gives -1."""
+    fn = "verify_draft"
+    if logits.ndim != 3 or draft.ndim != 2:
+        raise ValueError(f"{fn}: logits must be [B, T + 1, V] and draft [B, T], got {tuple(logits.shape)}, {tuple(draft.shape)}")
+    b, t1, v = logits.shape
+    t = t1 - 1
+    if tuple(draft.shape) != (b, t):
+        raise ValueError(f"{fn}: draft must be {(b, t)} for logits {tuple(logits.shape)}, got {tuple(draft.shape)}")
+    if t > MAX_DRAFTS:
+        raise ValueError(f"{fn}: {t} drafted tokens, at most {MAX_DRAFTS}")
+    if v < 1:
+        raise ValueError(f"{fn}: empty vocabulary")
+    temperature = float(temperature)
+    if not (temperature == 0.0 or 1e-4 <= temperature <= 1e4):
+        raise ValueError(f"{fn}: temperature must be 0 or within 1e-4 .. 1e4, got {temperature}")
+    dt = _lib.sqx_dtype(logits.dtype)
+    if temperature == 0.0:
+        u = r = draft_probs = None
+    else:
+        for name, x, shape in (("u", u, (b, t)), ("r", r, (b,))):
+            if x is None or tuple(x.shape) != shape or x.dtype != torch.float32:
+                raise ValueError(f"{fn}: {name} must be float32 {shape}")
+        if draft_probs is not None and tuple(draft_probs.shape) != (b, t, v):
+            raise ValueError(f"{fn}: draft_probs must be {(b, t, v)}, got {tuple(draft_probs.shape)}")
+    for name, x in (("draft", draft), ("counts", counts)):
+        if x is not None and x.dtype != torch.int32:
+            raise TypeError(f"{fn}: {name} must be int32, got {x.dtype}")
+    if counts is not None and tuple(counts.shape) != (b,):
+        raise ValueError(f"{fn}: counts must be {(b,)}, got {tuple(counts.shape)}")
+    pdt = _lib.DTYPE_F32 if draft_probs is None else _lib.sqx_dtype(draft_probs.dtype)
+    dev = _lib.require_device(logits, draft, u, r, draft_probs, counts, fn=fn)
+    logits, draft = logits.contiguous(), draft.contiguous()
+    u, r, draft_probs, counts = (None if x is None else x.contiguous() for x in (u, r, draft_probs, counts))
+    lib = _lib.load()
+    n = torch.empty(b, dtype=torch.int32, device=dev)
+    tokens = torch.empty(b, t1, dtype=torch.int32, device=dev)
+    nb = lib.sqx_verify_draft_workspace_bytes(b, t, v)
+    ws = torch.empty(max(nb // 8, 1), dtype=torch.float64, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.sqx_verify_draft(
+            logits.data_ptr(), dt, draft.data_ptr(), _lib.ptr(counts), _lib.ptr(draft_probs), pdt, _lib.ptr(u), _lib.ptr(r),
+            temperature, b, t, v, n.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel() * 8, _lib.stream_ptr(dev))
+    _lib.check(rc, fn)
+    return n, tokens
