@@ -852,9 +852,9 @@ int sqx_rope(const void* x, int dtype, int64_t n, int64_t heads, int64_t d, int6
  * hd] of dtype, given by the strides of row, token and head (multiples of 8 elements; rows 16-byte aligned). With
  * tables, keys are rotated first, by position, as sqx_rope rotates them (rot a multiple of 16), and rounded to dtype; q
  * [B, T, H, hd], when given, is rotated into q_out (contiguous) for all T tokens of every row.
- *   A block whose first token is written: s = max(fl(amax / qmax), 1e-12), qmax 127 or 448, amax over its finite new
- *   values. A block that keeps earlier tokens: s 2^k with the least k >= 0 for which fl(amax / qmax) <= s 2^k, and its
- *   codes become rne(c 2^-k).
+ *   A block whose first token is written: s = max(a, 1e-12) with a = fl(amax fl(1 / qmax)), qmax 127 or 448, amax over its
+ *   finite new values. A block that keeps earlier tokens: s 2^k with the least k >= 0 for which a <= s 2^k, and its codes
+ *   become rne(c 2^-k).
  *   code = clamp(rint(fl(x / s)), -127, 127), NaN 0; or the saturating E4M3 cast of fl(x / s).
  * Nothing is stored for a negative start, outside the table, or where it names no page. The rows of one call must not
  * write the same page. */

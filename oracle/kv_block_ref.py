@@ -76,7 +76,7 @@ def write(k, v, kc, vc, ks, vs, table, starts, counts, fmt: str) -> None:
                         new = x[b, t:t + m, h].astype(F32)
                         a = np.abs(new[np.isfinite(new)])
                         most = a.max() if a.size else F32(0)
-                        s = max(F32(most / QMAX[fmt]), MIN_SCALE)
+                        s = max(F32(most * (F32(1) / QMAX[fmt])), MIN_SCALE)
                         if lo:
                             had = max(scale[page, h], MIN_SCALE)
                             e = 0

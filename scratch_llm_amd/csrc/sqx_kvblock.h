@@ -112,7 +112,7 @@ __device__ inline void rope_row8(Row8<DT>& x, int c, int rot, bool inter, const 
 // Codes.
 template <bool E4M3>
 struct KvCode {
-  static constexpr float kMax = E4M3 ? 448.0f : 127.0f;
+  static constexpr float kInvMax = 1.0f / (E4M3 ? 448.0f : 127.0f);  // the largest code may be passed by an ulp: it clamps
   __device__ static inline uint32_t encode(const SharedDiv& d, float v) {
     const float y = div_by(d, v);
     if constexpr (E4M3) return e4m3_encode_sat(y);

@@ -2,8 +2,8 @@
 // reading values back. Layout and code formats: sqx_kvblock.h.
 //
 // A block's scale. A block whose first token is part of the write takes s = max(fl(amax / qmax), 1e-12) over the tokens
-// written (qmax 127 or 448). A block that already holds tokens keeps its scale, doubled k times, the least k with
-// fl(amax / qmax) <= s 2^k, and its codes become rne(c 2^-k). With growth in powers of two every later rescale at least
+// written (the product with fl(1 / qmax), qmax 127 or 448). A block that already holds tokens keeps its scale, doubled k
+// times, the least k with fl(amax / qmax) <= s 2^k, and its codes become rne(c 2^-k). With growth in powers of two every later rescale at least
 // doubles the step, so what the rescales add to a token's error is at most s/2 (1 + 1/2 + 1/4 + ...) < s of the final
 // scale, however often the block grows; growing to each token's own amax would add s/2 at every token.
 // amax is taken over finite magnitudes: infinities saturate to the largest code, a NaN is a NaN in E4M3 and 0 in int8.
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
   if ((tid & 63) == 0) red[tid >> 6] = most;
   __syncthreads();
   most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float s = fmaxf(__fdiv_rn(most, Code::kMax), kKvMinScale);
+  float s = fmaxf(most * Code::kInvMax, kKvMinScale);
   float down = 1.0f;  // 2^-k
   if (lo > 0) {
     int en, eh;
