@@ -62,50 +62,44 @@ __device__ inline void rope_pair(float a, float b, float c, float s, float& ya, 
   yb = as + bc;
 }
 
-// Rotates the 8 elements at column 8 c of a row whose first `rot` columns are rotated (rot % 16 == 0), in the
-// interleaved layout (pairs 2i, 2i + 1) or in halves (pairs i, i + rot / 2; `load_other` fetches the 8 elements of
-// the other half). cos_r, sin_r: the position's table row.
-template <int DT, typename F>
-__device__ inline void rope_row8(Row8<DT>& x, int c, int rot, bool inter, const float* cos_r, const float* sin_r,
-                                 const F& load_other) {
-  if (8 * c >= rot) return;
-  if (inter) {
-    const f32x4_t cs = *reinterpret_cast<const f32x4_t*>(cos_r + 4 * c);
-    const f32x4_t sn = *reinterpret_cast<const f32x4_t*>(sin_r + 4 * c);
+// The angles of the 8 columns from column 8 c of a head whose first `rot` columns are rotated (rot % 16 == 0): interleaved
+// pairs 2i, 2i + 1 take four of them, halves (pairs i, i + rot / 2) eight. cos_r, sin_r: the position's table row.
+struct Angles8 {
+  float c[8], s[8];
+  __device__ inline void load(int col8, int rot, bool inter, const float* cos_r, const float* sin_r) {
+    if (8 * col8 >= rot) return;
+    const int at = inter ? 4 * col8 : 8 * (col8 < rot / 16 ? col8 : col8 - rot / 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float ya, yb;
-      rope_pair(x.get(2 * i), x.get(2 * i + 1), cs[i], sn[i], ya, yb);
-      x.set_pair(i, ya, yb);
-    }
-    return;
-  }
-  const int half8 = rot / 16;  // 8-element groups per half
-  const bool second = c >= half8;
-  const int cc = second ? c - half8 : c;
-  const Row8<DT> o = load_other(second ? cc : cc + half8);
-  float cs[8], sn[8];
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && inter) break;
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(cos_r + at + 4 * h);
+      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(sin_r + at + 4 * h);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(cos_r + 8 * cc + 4 * h);
-    const f32x4_t b = *reinterpret_cast<const f32x4_t*>(sin_r + 8 * cc + 4 * h);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      cs[4 * h + j] = a[j];
-      sn[4 * h + j] = b[j];
+      for (int j = 0; j < 4; ++j) {
+        c[4 * h + j] = a[j];
+        s[4 * h + j] = b[j];
+      }
     }
   }
+};
+template <int DT>
+__device__ inline void rotate_pairs(Row8<DT>& x, const Angles8& g) {  // interleaved
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float y[2];
+    float ya, yb;
+    rope_pair(x.get(2 * i), x.get(2 * i + 1), g.c[i], g.s[i], ya, yb);
+    x.set_pair(i, ya, yb);
+  }
+}
+template <int DT>
+__device__ inline void rotate_halves(Row8<DT>& a, Row8<DT>& b, const Angles8& g) {  // a of the first half, b of the second
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = 2 * i + e;
-      float ya, yb;
-      rope_pair(second ? o.get(k) : x.get(k), second ? x.get(k) : o.get(k), cs[k], sn[k], ya, yb);
-      y[e] = second ? yb : ya;
-    }
-    x.set_pair(i, y[0], y[1]);
+  for (int i = 0; i < 4; ++i) {
+    float ya[2], yb[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) rope_pair(a.get(2 * i + e), b.get(2 * i + e), g.c[2 * i + e], g.s[2 * i + e], ya[e], yb[e]);
+    a.set_pair(i, ya[0], ya[1]);
+    b.set_pair(i, yb[0], yb[1]);
   }
 }
 
@@ -118,6 +112,23 @@ struct KvCode {
     if constexpr (E4M3) return e4m3_encode_sat(y);
     const float r = y != y ? 0.0f : fminf(fmaxf(rintf(y), -127.0f), 127.0f);  // int8 has no NaN: it stores zero
     return static_cast<uint32_t>(static_cast<int>(r)) & 0xffu;
+  }
+  // Four codes where every value is finite and the shared division's fast form holds: the same bits as encode. The sum with
+  // 1.5 2^23 rounds to the nearest even integer and leaves it, as two's complement, in the low byte.
+  __device__ static inline uint32_t encode4(const SharedDiv& d, float v0, float v1, float v2, float v3) {
+    const float v[4] = {v0, v1, v2, v3};
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(quick_div(d, v[i]), E4M3 ? -448.0f : -127.0f, E4M3 ? 448.0f : 127.0f);
+    if constexpr (E4M3) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true));
+    }
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = __builtin_bit_cast(uint32_t, y[i] + 12582912.0f);
+    const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
+    return lo | hi;
   }
   __device__ static inline float decode(uint32_t byte) {
     if constexpr (E4M3) {

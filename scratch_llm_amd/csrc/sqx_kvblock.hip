@@ -23,43 +23,71 @@ struct KvWriteArgs {
   int T, H, Hkv, width, pages, block, shift;
 };
 
-constexpr int kQHeads = 8;  // query heads per workgroup of the rotary part
+constexpr int kQHeads = 8;     // query heads per workgroup of the rotary part
+constexpr int kHeadBatch = 4;  // of which a thread takes as many at once
+
+// The rotation of the rows x[0 .. NP) of one 8-column group. In halves the other half of a pair lies in the lane half8
+// further on or back, of the same token.
+template <int DT>
+__device__ inline void rotate_lane(Row8<DT>& x, int c, int rot, bool inter, const Angles8& g) {
+  if (inter) {
+    if (8 * c < rot) rotate_pairs<DT>(x, g);
+    return;
+  }
+  const int half8 = rot / 16, lane = threadIdx.x & 63;
+  const bool second = c >= half8;
+  const int from = 8 * c < rot ? (second ? lane - half8 : lane + half8) : lane;
+  Row8<DT> o;
+#pragma unroll
+  for (int i = 0; i < Row8<DT>::kWords; ++i) o.w[i] = __shfl(static_cast<int>(x.w[i]), from, 64);
+  if (8 * c >= rot) return;
+  if (second) {
+    rotate_halves<DT>(o, x, g);
+  } else {
+    rotate_halves<DT>(x, o, g);
+  }
+}
 
 // Workgroup (j, y, b): block j of the blocks that row b's tokens touch. y < Hkv: the keys of head y; then the values;
 // then groups of kQHeads query heads, whose rotation needs no block.
-template <int DT, int D, bool E4M3>
+//
+// A thread holds 8 columns of NP tokens: of a whole block, tokens NP tl .. NP tl + NP - 1, so that four codes of a value
+// column are one dword of the transposed tile; of at most 256 / C tokens (NP = 1), token tl of the write. Slots outside
+// the write read its nearest token, so that all loads are issued together, and are not stored.
+template <int DT, int D, bool E4M3, int NP>
 __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
   using Code = KvCode<E4M3>;
-  constexpr int C = D / 8;                 // 8-element groups per token
-  constexpr int TP = 256 / C;              // tokens per pass
-  constexpr int NP = 128 / TP;             // passes of the largest block
-  constexpr int kPitch = 128 + 16;         // LDS pitch of a value column: a block's codes, 16-byte aligned
+  constexpr int C = D / 8;                            // 8-column groups of a token
+  constexpr int TP = 256 / C;                         // tokens held by the workgroup, per NP
+  constexpr int kPitch = (NP == 1 ? 128 : NP * TP) + 16;  // LDS pitch of a value column
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[D * kPitch];
   const int j = blockIdx.x, y = blockIdx.y, b = blockIdx.z;
   const int start = a.starts[b];
   const int off = start & (a.block - 1);
   const int tid = threadIdx.x, c = tid % C, tl = tid / C;
-  auto table_row = [&](int t) {
+  auto angles = [&](Angles8& g, int t) {
     const int64_t p = static_cast<int64_t>(start) + t;
-    return static_cast<int64_t>(p < 0 ? 0 : (p < a.rope_rows ? p : a.rope_rows - 1)) * (a.rot / 2);
+    const int64_t at = static_cast<int64_t>(p < 0 ? 0 : (p < a.rope_rows ? p : a.rope_rows - 1)) * (a.rot / 2);
+    g.load(c, a.rot, a.inter, a.cos_t + at, a.sin_t + at);
   };
 
   if (y >= 2 * a.Hkv) {  // query heads: every token of the row, whatever its count
-    const int h0 = (y - 2 * a.Hkv) * kQHeads, nh = min(kQHeads, a.H - h0);
+    const int h0 = (y - 2 * a.Hkv) * kQHeads;
     const int ta = max(0, j * a.block - off), tb = min(a.T, (j + 1) * a.block - off);
-    for (int i = tl; i < (tb - ta) * nh; i += TP) {
-      const int t = ta + i / nh, h = h0 + i % nh;
-      const int64_t row = b * a.q_sb + t * a.q_st + h * a.q_sh;
-      Row8<DT> x;
-      x.load(a.q, row + 8 * c);
-      const int64_t tr = table_row(t);
-      rope_row8<DT>(x, c, a.rot, a.inter, a.cos_t + tr, a.sin_t + tr, [&](int g) {
-        Row8<DT> o;
-        o.load(a.q, row + 8 * g);
-        return o;
-      });
-      x.store(a.q_out, ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * D + 8 * c);
+    for (int i = tl; i < (tb - ta) * (kQHeads / kHeadBatch); i += TP) {
+      const int t = ta + i / (kQHeads / kHeadBatch), h = h0 + i % (kQHeads / kHeadBatch) * kHeadBatch;
+      Angles8 g;
+      angles(g, t);
+      Row8<DT> x[kHeadBatch];
+      const int64_t row = b * a.q_sb + t * a.q_st + 8 * c;
+#pragma unroll
+      for (int e = 0; e < kHeadBatch; ++e) x[e].load(a.q, row + min(h + e, a.H - 1) * a.q_sh);
+#pragma unroll
+      for (int e = 0; e < kHeadBatch; ++e) {
+        rotate_lane<DT>(x[e], c, a.rot, a.inter, g);
+        if (h + e < a.H) x[e].store(a.q_out, ((static_cast<int64_t>(b) * a.T + t) * a.H + h + e) * D + 8 * c);
+      }
     }
     return;
   }
@@ -78,30 +106,41 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
   uint8_t* const codes = (is_v ? a.vc : a.kc) + ph * a.block * D;
   const float had = lo > 0 ? fmaxf(*sp, kKvMinScale) : 0.0f;
 
+  const int slot0 = NP == 1 ? lo + tl : NP * tl;
   Row8<DT> x[NP];
-  float most = 0.0f;
+  {
+    const void* const src = is_v ? a.v : a.k;
+    const int64_t row = (is_v ? b * a.v_sb + h * a.v_sh : b * a.k_sb + h * a.k_sh) + 8 * c;
+    const int64_t st = is_v ? a.v_st : a.k_st;
 #pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const int slot = lo + p * TP + tl;
-    if (slot < hi) {
-      const int t = slot - off + j * a.block;
-      const void* src = is_v ? a.v : a.k;
-      const int64_t row = is_v ? b * a.v_sb + t * a.v_st + h * a.v_sh : b * a.k_sb + t * a.k_st + h * a.k_sh;
-      x[p].load(src, row + 8 * c);
-      if (!is_v && a.cos_t != nullptr) {
-        const int64_t tr = table_row(t);
-        rope_row8<DT>(x[p], c, a.rot, a.inter, a.cos_t + tr, a.sin_t + tr, [&](int g) {
-          Row8<DT> o;
-          o.load(src, row + 8 * g);
-          return o;
-        });
-      }
+    for (int p = 0; p < NP; ++p) x[p].load(src, row + (min(max(slot0 + p, lo), hi - 1) - off + j * a.block) * st);
+  }
+  if (!is_v && a.cos_t != nullptr) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      Angles8 g;
+      angles(g, min(max(slot0 + p, lo), hi - 1) - off + j * a.block);
+      rotate_lane<DT>(x[p], c, a.rot, a.inter, g);
+    }
+  }
+  float most = 0.0f, top = 0.0f;  // largest finite magnitude; largest of all, NaN where there is one
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float m = fabsf(x[p].get(e));
+      top = __builtin_elementwise_maximum(top, m);
+    }
+  most = top;
+  if (!(top <= 3.402823466e38f)) {
+    most = 0.0f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float m = fabsf(x[p].get(e));
         most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
       }
-    }
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
@@ -119,17 +158,19 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
   }
   if (tid == 0) *sp = s;
   const SharedDiv sd = shared_div(s);
+  const bool quick = sd.ok && __ballot(!fast_div(sd, top)) == 0;  // wave-uniform
+  auto encode4 = [&](float v0, float v1, float v2, float v3) -> uint32_t {
+    if (quick) return Code::encode4(sd, v0, v1, v2, v3);
+    return Code::encode(sd, v0) | (Code::encode(sd, v1) << 8) | (Code::encode(sd, v2) << 16) | (Code::encode(sd, v3) << 24);
+  };
 
   if (!is_v) {
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const int slot = lo + p * TP + tl;
-      if (slot < hi) {
-        u32x2v_t w = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= Code::encode(sd, x[p].get(e)) << (8 * (e & 3));
-        *reinterpret_cast<u32x2v_t*>(codes + slot * D + 8 * c) = w;
-      }
+      const int slot = slot0 + p;
+      const u32x2v_t w = {encode4(x[p].get(0), x[p].get(1), x[p].get(2), x[p].get(3)),
+                          encode4(x[p].get(4), x[p].get(5), x[p].get(6), x[p].get(7))};
+      if (slot >= lo && slot < hi) *reinterpret_cast<u32x2v_t*>(codes + slot * D + 8 * c) = w;
     }
     if (down != 1.0f) {
       for (int i = tid; i < lo * (D / 4); i += 256) {
@@ -139,23 +180,32 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
     }
     return;
   }
-  // values: transposed through LDS, then 16 tokens of a column at a time, merged with the codes that stay
+  // values: transposed through LDS, then 16 tokens of a column at a time, merged with the codes that stay. Column d lies at
+  // row (d % 8) C + d / 8: the lanes of a wave write rows kPitch apart, which spreads them over the banks.
 #pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const int slot = lo + p * TP + tl;
-    if (slot < hi) {
+  for (int e = 0; e < 8; ++e) {
+    uint8_t* const t = tile + (e * C + c) * kPitch;
+    if constexpr (NP >= 4) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        tile[(8 * c + e) * kPitch + slot] = static_cast<uint8_t>(Code::encode(sd, x[p].get(e)));
+      for (int p = 0; p < NP; p += 4)
+        *reinterpret_cast<uint32_t*>(t + slot0 + p) = encode4(x[p].get(e), x[p + 1].get(e), x[p + 2].get(e), x[p + 3].get(e));
+    } else if constexpr (NP == 2) {
+      *reinterpret_cast<uint16_t*>(t + slot0) = static_cast<uint16_t>(encode4(x[0].get(e), x[1].get(e), 0.0f, 0.0f));
+    } else if (e % 4 == 0) {
+      const uint32_t w = encode4(x[0].get(e), x[0].get(e + 1), x[0].get(e + 2), x[0].get(e + 3));
+      if (slot0 < hi) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t[q * C * kPitch + slot0] = static_cast<uint8_t>(w >> (8 * q));
+      }
     }
   }
   __syncthreads();
-  const int nch = a.block >> 4;
-  for (int i = tid; i < D * nch; i += 256) {
-    const int d = i / nch, s0 = (i % nch) * 16;
+  const int sh = a.shift - 4;  // 16-token pieces of a column: 1 << sh
+  for (int i = tid; i < D << sh; i += 256) {
+    const int d = i >> sh, s0 = (i & ((1 << sh) - 1)) * 16;
     if (s0 >= hi || (s0 + 16 <= lo && down == 1.0f)) continue;
     u32x4_t* g = reinterpret_cast<u32x4_t*>(codes + d * a.block + s0);
-    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(tile + d * kPitch + s0);
+    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(tile + ((d & 7) * C + (d >> 3)) * kPitch + s0);
     u32x4_t w;
     if (s0 >= lo && s0 + 16 <= hi) {
       w = n;
@@ -206,32 +256,50 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* __restrict_
   const int64_t ph = some ? static_cast<int64_t>(page) * Hkv + h : 0;
   const float s = some ? (is_v ? vs : ks)[ph] : 0.0f;
   const uint8_t* codes = (is_v ? vc : kc) + ph * block * D;
-  if (is_v && some) {
-    const int nch = block >> 4;
-    for (int i = tid; i < D * nch; i += 256) {
-      const int d = i / nch, s0 = (i % nch) * 16;
-      *reinterpret_cast<u32x4_t*>(tile + d * kPitch + s0) = *reinterpret_cast<const u32x4_t*>(codes + d * block + s0);
-    }
-    __syncthreads();
-  }
-  for (int slot = lo + tl; slot < hi; slot += TP) {
-    const int t = slot - off + j * block;
-    const bool have = some && t < count;
-    u32x2v_t w = {0u, 0u};
-    if (have && !is_v) w = *reinterpret_cast<const u32x2v_t*>(codes + slot * D + 8 * c);
+  void* const out = is_v ? v_out : k_out;
+  const int64_t row0 = static_cast<int64_t>(b) * T + (static_cast<int64_t>(j) * block - off);  // of slot 0
+  // eight codes of a token's columns 8 c .. as values, to its row of the output
+  auto put = [&](int slot, uint32_t w0, uint32_t w1) {
+    const bool have = some && slot - off + j * block < count;
     Row8<DT> r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float f[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int q = 2 * i + e;
-        const uint32_t byte = is_v ? (have ? tile[(8 * c + q) * kPitch + slot] : 0u) : (w[q >> 2] >> (8 * (q & 3))) & 0xffu;
-        f[e] = have ? Code::decode(byte) * s : 0.0f;
-      }
-      r.set_pair(i, f[0], f[1]);
+      const uint32_t w = i < 2 ? w0 : w1;
+      const float lo_v = Code::decode((w >> (16 * (i & 1))) & 0xffu) * s, hi_v = Code::decode((w >> (16 * (i & 1) + 8)) & 0xffu) * s;
+      r.set_pair(i, have ? lo_v : 0.0f, have ? hi_v : 0.0f);
     }
-    r.store(is_v ? v_out : k_out, ((static_cast<int64_t>(b) * T + t) * Hkv + h) * D + 8 * c);
+    r.store(out, ((row0 + slot) * Hkv + h) * D + 8 * c);
+  };
+  if (!is_v || !some) {
+#pragma unroll 4
+    for (int slot = lo + tl; slot < hi; slot += TP) {
+      u32x2v_t w = {0u, 0u};
+      if (some) w = *reinterpret_cast<const u32x2v_t*>(codes + slot * D + 8 * c);
+      put(slot, w[0], w[1]);
+    }
+    return;
+  }
+  // values: through LDS as in the write, four tokens of eight columns at a time
+  const int sh = shift - 4;
+#pragma unroll 4
+  for (int i = tid; i < D << sh; i += 256) {
+    const int d = i >> sh, s0 = (i & ((1 << sh) - 1)) * 16;
+    *reinterpret_cast<u32x4_t*>(tile + ((d & 7) * C + (d >> 3)) * kPitch + s0) = *reinterpret_cast<const u32x4_t*>(codes + d * block + s0);
+  }
+  __syncthreads();
+  for (int g = tl; g < block / 4; g += TP) {
+    if (4 * g + 4 <= lo || 4 * g >= hi) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = *reinterpret_cast<const uint32_t*>(tile + (e * C + c) * kPitch + 4 * g);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (4 * g + q < lo || 4 * g + q >= hi) continue;
+      const uint32_t sel = 0x0c0c0400u + 0x0101u * q;  // byte q of each of two dwords
+      const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], sel) | (__builtin_amdgcn_perm(w[3], w[2], sel) << 16);
+      const uint32_t z = __builtin_amdgcn_perm(w[5], w[4], sel) | (__builtin_amdgcn_perm(w[7], w[6], sel) << 16);
+      put(4 * g + q, a, z);
+    }
   }
 }
 
@@ -281,12 +349,23 @@ extern "C" int sqx_kvblock_write(const void* k, const void* v, int dtype, int64_
                   static_cast<unsigned>(2 * Hkv + (q ? ceil_div(H, kQHeads) : 0)), static_cast<unsigned>(B));
   with_dtype(dtype, [&](auto dt) {
     with_head(hd, [&](auto dd) {
-      if (fmt == SQX_KV_E4M3)
-        hipLaunchKernelGGL((kv_write_kernel<decltype(dt)::value, decltype(dd)::value, true>), grid, dim3(256), 0,
-                           as_stream(stream), a);
-      else
-        hipLaunchKernelGGL((kv_write_kernel<decltype(dt)::value, decltype(dd)::value, false>), grid, dim3(256), 0,
-                           as_stream(stream), a);
+      constexpr int DT = decltype(dt)::value, D = decltype(dd)::value, TP = 2048 / D;
+      auto go = [&](auto np) {
+        constexpr int NP = decltype(np)::value;
+        if (fmt == SQX_KV_E4M3)
+          hipLaunchKernelGGL((kv_write_kernel<DT, D, true, NP>), grid, dim3(256), 0, as_stream(stream), a);
+        else
+          hipLaunchKernelGGL((kv_write_kernel<DT, D, false, NP>), grid, dim3(256), 0, as_stream(stream), a);
+      };
+      // tokens per thread: one where those of a block fit the workgroup once, else a block's
+      const int64_t np = std::min(T, block) <= TP ? 1 : block / TP;
+      if (np == 1) go(std::integral_constant<int, 1>{});
+      else if (np == 2) go(std::integral_constant<int, 2>{});
+      else if (np == 4) go(std::integral_constant<int, 4>{});
+      else if constexpr (D > 64) {
+        if (np == 8) go(std::integral_constant<int, 8>{});
+        else if constexpr (D > 128) go(std::integral_constant<int, 16>{});
+      }
     });
   });
   SQX_LAUNCH_CHECK(fn);

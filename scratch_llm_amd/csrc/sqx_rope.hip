@@ -8,8 +8,35 @@
 
 namespace sqx {
 
-// One workgroup per token. A thread owns one group of 8 columns (the table row's part of it is read once) and walks the
-// heads; 256 threads cover 256 / (d / 8) heads at a time.
+// Eight columns of kRopeHeads heads of a row of heads: with halves the thread at a column of the first half takes both groups
+// of its pairs (rows may be rotated in place), and those of the second half are idle. All loads come before the first use.
+constexpr int kRopeHeads = 4;
+template <int DT>
+__device__ inline void rope_columns(const void* x, int64_t row, int64_t sh, void* out, int64_t orow, int64_t oh, int h0,
+                                    int hs, int heads, int c, int rot, bool inter, const Angles8& ang) {
+  const int half8 = inter ? 0 : rot / 16;
+  if (c >= half8 && c < 2 * half8) return;
+  Row8<DT> a[kRopeHeads], b[kRopeHeads];
+#pragma unroll
+  for (int i = 0; i < kRopeHeads; ++i) {
+    const int h = h0 + i * hs;
+    if (h >= heads) break;
+    a[i].load(x, row + h * sh + 8 * c);
+    if (c < half8) b[i].load(x, row + h * sh + 8 * (c + half8));
+  }
+#pragma unroll
+  for (int i = 0; i < kRopeHeads; ++i) {
+    const int h = h0 + i * hs;
+    if (h >= heads) break;
+    if (c < half8) rotate_halves<DT>(a[i], b[i], ang);
+    else if (inter && 8 * c < rot) rotate_pairs<DT>(a[i], ang);
+    a[i].store(out, orow + h * oh + 8 * c);
+    if (c < half8) b[i].store(out, orow + h * oh + 8 * (c + half8));
+  }
+}
+
+// One workgroup per token: a thread owns a group of 8 columns (its part of the table row is read once) and walks the heads,
+// 256 / (d / 8) heads apart, four at a time.
 template <int DT>
 __global__ __launch_bounds__(256) void rope_kernel(const void* x, int64_t sn, int64_t sh, const int* __restrict__ pos,
                                                    const float* __restrict__ cos_t, const float* __restrict__ sin_t,
@@ -19,28 +46,10 @@ __global__ __launch_bounds__(256) void rope_kernel(const void* x, int64_t sn, in
   const int c = threadIdx.x % d8, h0 = threadIdx.x / d8, hs = 256 / d8;
   if (h0 >= hs) return;
   const int p = min(max(pos[n], 0), rows - 1);
-  const float* cr = cos_t + static_cast<int64_t>(p) * (rot / 2);
-  const float* sr = sin_t + static_cast<int64_t>(p) * (rot / 2);
-  // in halves a thread takes both groups of its pairs, so that rows may be rotated in place
-  const int half8 = inter ? 0 : rot / 16;
-  if (!inter && c >= half8 && c < 2 * half8) return;
-  for (int h = h0; h < heads; h += hs) {
-    Row8<DT> a;
-    const int64_t row = n * sn + h * sh, orow = n * on + h * oh;
-    a.load(x, row + 8 * c);
-    if (c < half8) {
-      Row8<DT> b, a2 = a;
-      b.load(x, row + 8 * (c + half8));
-      Row8<DT> b2 = b;
-      rope_row8<DT>(a2, c, rot, false, cr, sr, [&](int) { return b; });
-      rope_row8<DT>(b2, c + half8, rot, false, cr, sr, [&](int) { return a; });
-      a2.store(out, orow + 8 * c);
-      b2.store(out, orow + 8 * (c + half8));
-      continue;
-    }
-    if (inter) rope_row8<DT>(a, c, rot, true, cr, sr, [&](int) { return a; });
-    a.store(out, orow + 8 * c);
-  }
+  Angles8 ang;
+  ang.load(c, rot, inter, cos_t + static_cast<int64_t>(p) * (rot / 2), sin_t + static_cast<int64_t>(p) * (rot / 2));
+  for (int h = h0; h < heads; h += kRopeHeads * hs)
+    rope_columns<DT>(x, n * sn, sh, out, n * on, oh, h, hs, heads, c, rot, inter, ang);
 }
 
 // Any even rot and any alignment: a thread per pair (or per column past the rotated ones).

@@ -32,7 +32,7 @@ struct VerifyArgs {
   const void* probs;   // [B, T, V], or NULL: each draft was certain
   const float *u, *r;
   int T, V, S;
-  double k;  // log2(e) / temperature
+  double k;  // 64 log2(e) / temperature
   double* sums;  // [B, T + 1, S]
   double* rest;  // [B, S]
   float* maxs;   // [B, T + 1, S]
@@ -40,22 +40,26 @@ struct VerifyArgs {
   int *n_acc, *tokens;
 };
 
-// 2^y for y <= 0: y = n / 32 + f, |f| <= 1/64; 2^(n / 32) from a table of 32 powers and an exponent, 2^f from its Taylor
-// polynomial of degree 5 in f ln 2 (the term left out is below 3e-15).
-__device__ inline double exp2_neg(double y, const double* pow32) {
-  y = y < -1100.0 ? -1100.0 : y;  // NaN stays
-  const double n = __builtin_rint(y * 32.0);
-  const double x = fma(n, -0.03125, y) * 0.693147180559945309417;
-  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(p, x, 1.0 / 6.0);
-  p = fma(p, x, 0.5);
-  p = fma(p, x, 1.0);
-  p = fma(p, x, 1.0);
-  const int i = static_cast<int>(n);
-  return ldexp(p * pow32[i & 31], i >> 5);
+// 2^(y / 64) for y <= 0: y = n + f with n the nearest integer and |f| <= 1/2; 2^(n / 64) from a table of 64 powers (64 lanes
+// reading 8-byte entries at random meet few bank conflicts) and an exponent, e^(f ln 2 / 64) from its Taylor polynomial with
+// the fourth power replaced by its Chebyshev economization over |x| <= h = ln 2 / 128: x^4 ~ h^2 x^2 - h^4 / 8, which
+// leaves an error of h^4 / 192 = 5e-12. A probability of 5e-12 moved anywhere in a vocabulary of 128256 changes a pick with a chance of about 1e-6 at the
+// worst; the order of the double sums has a millionth of that.
+constexpr double kLn2_64 = 0.693147180559945309417 / 64.0;
+constexpr double kH2 = (kLn2_64 / 2) * (kLn2_64 / 2);
+__device__ inline double exp2_64th(double y, const double* pow64) {
+  y = fmax(y, -64000.0);  // 2^-1000: nothing next to a sum that holds a 1. Drops a NaN: callers look for those in fp32
+  const double t = y + 0x1.8p52;  // the nearest integer in the low bits of the mantissa
+  const int n = __double2loint(t);
+  const double f = y - (t - 0x1.8p52);
+  double p = fma(f, kLn2_64 * kLn2_64 * kLn2_64 / 6.0, kLn2_64 * kLn2_64 * (0.5 + kH2 / 24.0));
+  p = fma(p, f, kLn2_64);
+  p = fma(p, f, 1.0 - kH2 * kH2 / 192.0);
+  const double w = pow64[n & 63];  // in [1, 2): the exponent n >> 6 is added to its bits
+  return p * __hiloint2double(__double2hiint(w) + ((n & ~63) << 14), __double2loint(w));
 }
-__device__ inline void fill_pow32(double* pow32) {
-  if (threadIdx.x < 32) pow32[threadIdx.x] = exp2(threadIdx.x * 0.03125);
+__device__ inline void fill_pow64(double* pow64) {
+  if (threadIdx.x < 64) pow64[threadIdx.x] = exp2(threadIdx.x / 64.0);
 }
 
 // Elements base .. base + 7 of a row of V as fp32; past the end `fill`.
@@ -104,13 +108,13 @@ __device__ inline double block_sum_f64(double v, double* red) {
 // (NaN counts as the maximum).
 template <int DT, bool VEC, bool GREEDY>
 __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
-  __shared__ double pow32[32], red[4];
+  __shared__ double pow64[64], red[4];
   __shared__ float redm[4];
   __shared__ int redi[4];
   const int s = blockIdx.x, row = blockIdx.y, b = row / (a.T + 1), t = row % (a.T + 1);
   const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   if (t > count) return;
-  if constexpr (!GREEDY) fill_pow32(pow32);
+  if constexpr (!GREEDY) fill_pow64(pow64);
   const int64_t row0 = static_cast<int64_t>(row) * a.V;
   const int at = s * kSlice + threadIdx.x * kPer;
   float v[kPasses][kPer];
@@ -157,79 +161,103 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
       a.args[out] = arg;
     }
   } else {
-    float m = -INFINITY;
+    float m = -INFINITY;  // the maximum that keeps a NaN
 #pragma unroll
     for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) m = fmaxf(m, v[p][e]);
+      for (int e = 0; e < kPer; ++e) m = __builtin_elementwise_maximum(m, v[p][e]);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    for (int o = 1; o < 64; o <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o, 64));
     if ((threadIdx.x & 63) == 0) redm[threadIdx.x >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
-    const double md = m == -INFINITY ? 0.0 : static_cast<double>(m);  // all masked: every term is zero
+    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(redm[0], redm[1]),
+                                      __builtin_elementwise_maximum(redm[2], redm[3]));
     double sum = 0.0;
+    if (m > -INFINITY && m < INFINITY) {  // the same in every thread; a masked element adds 2^-1000
+      const double off = -static_cast<double>(m) * a.k;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p)
+      for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const double y = (static_cast<double>(v[p][e]) - md) * a.k;
-        sum += v[p][e] == -INFINITY ? 0.0 : exp2_neg(y, pow32);
-      }
-    sum = block_sum_f64(sum, red);
+        for (int e = 0; e < kPer; ++e) sum += exp2_64th(fma(static_cast<double>(v[p][e]), a.k, off), pow64);
+      sum = block_sum_f64(sum, red);
+    }
     if (threadIdx.x == 0) {
-      a.maxs[out] = m;
+      a.maxs[out] = m;  // NaN or infinite: the row is no distribution; -infinite: the slice is all masked
       a.sums[out] = sum;
     }
   }
 }
 
+// e^((x - m) / temperature) / sum; 0 for a masked x.
+__device__ inline double prob(float x, double off, double k, double inv, const double* pow64) {
+  const double e = exp2_64th(fma(static_cast<double>(x), k, off), pow64) * inv;
+  return x == -INFINITY ? 0.0 : e;
+}
+
 struct Verdict {
-  int n, count;   // accepted, drafted
-  double m, inv;  // of row n: maximum, 1 / sum (NaN where the row has no distribution)
+  int n, count;     // accepted, drafted
+  double off, inv;  // of row n: -maximum k and 1 / sum; inv is NaN where the row has no distribution
 };
 
-// Lane t of a wave judges draft t (and lane `count` the row behind the drafts); the same in every wave that calls it.
+// Judges the drafts of row b: thread (t, part) joins every fourth slice of row t, lane by lane of a quad. The same in every
+// wave; up to 16 rows at a time (a wave holds 16 quads), so that the loads of a row's slices run side by side.
 template <int DT>
-__device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const double* pow32) {
-  const int lane = threadIdx.x & 63;
+__device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const double* pow64) {
+  const int lane = threadIdx.x & 63, part = lane & 3;
   Verdict r;
   r.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
-  double m = 0.0, z = 0.0, inv = 0.0;
-  bool good = false;
-  if (lane <= r.count) {
-    const int64_t at = (static_cast<int64_t>(b) * (a.T + 1) + lane) * a.S;
-    float mx = -INFINITY;
-    for (int s = 0; s < a.S; ++s) mx = fmaxf(mx, a.maxs[at + s]);
-    m = mx == -INFINITY ? 0.0 : static_cast<double>(mx);
-    for (int s = 0; s < a.S; ++s) {
-      const float ms = a.maxs[at + s];
-      if (ms != -INFINITY) z += a.sums[at + s] * exp2_neg((static_cast<double>(ms) - m) * a.k, pow32);
-    }
-    inv = 1.0 / z;  // of a sum of zero infinite, of NaN NaN
-    if (!(z > 0.0 && inv > 0.0)) inv = __builtin_nan("");
-    if (lane < r.count) {
-      const int x = a.draft[static_cast<int64_t>(b) * a.T + lane];
+  for (int t0 = 0;; t0 += 16) {
+    const int t = t0 + (lane >> 2);
+    const bool mine = t <= r.count;
+    const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + t, prow = static_cast<int64_t>(b) * a.T + t;
+    const int64_t at = row * a.S;
+    int x = -1;
+    float lx = 0.0f;
+    double qx = 1.0, ux = 0.0;
+    if (mine && t < r.count) {
+      x = a.draft[prow];
+      ux = static_cast<double>(a.u[prow]);
       if (x >= 0 && x < a.V) {
-        const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + lane, prow = static_cast<int64_t>(b) * a.T + lane;
-        const float lx = load_as_f32(a.logits, DT, row * a.V + x);
-        const double px = lx == -INFINITY ? 0.0 * inv : exp2_neg((static_cast<double>(lx) - m) * a.k, pow32) * inv;
-        const double qx = a.probs != nullptr ? static_cast<double>(load_as_f32(a.probs, pdt, prow * a.V + x)) : 1.0;
-        good = static_cast<double>(a.u[prow]) * qx < px;
+        lx = load_as_f32(a.logits, DT, row * a.V + x);
+        if (a.probs != nullptr) qx = static_cast<double>(load_as_f32(a.probs, pdt, prow * a.V + x));
       }
     }
+    float mx = -INFINITY;
+    if (mine) {
+#pragma unroll 4
+      for (int s = part; s < a.S; s += 4) mx = __builtin_elementwise_maximum(mx, a.maxs[at + s]);
+    }
+    mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 1, 64));
+    mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 2, 64));
+    const bool fine = mx > -INFINITY && mx < INFINITY;
+    const double off = fine ? -static_cast<double>(mx) * a.k : 0.0;
+    double z = 0.0;
+    if (mine && fine) {
+#pragma unroll 4
+      for (int s = part; s < a.S; s += 4) {
+        const float ms = a.maxs[at + s];
+        z += prob(ms, off, a.k, 1.0, pow64) * a.sums[at + s];
+      }
+    }
+    z += __shfl_xor(z, 1, 64);
+    z += __shfl_xor(z, 2, 64);
+    const double inv = fine ? 1.0 / z : __builtin_nan("");
+    const bool good = mine && t < r.count && x >= 0 && x < a.V && ux * qx < prob(lx, off, a.k, inv, pow64);
+    const uint64_t bad = ~__ballot(good || t >= r.count) & 0x1111111111111111ull;
+    const int stop = bad != 0 ? t0 + (static_cast<int>(__builtin_ctzll(bad)) >> 2) : r.count;
+    if (stop < t0 + 16 || r.count < t0 + 16) {
+      r.n = min(stop, r.count);
+      r.off = __shfl(off, (r.n - t0) * 4, 64);
+      r.inv = __shfl(inv, (r.n - t0) * 4, 64);
+      return r;
+    }
   }
-  const uint64_t bad = ~__ballot(good);
-  r.n = min(static_cast<int>(__builtin_ctzll(bad | (uint64_t(1) << 63))), r.count);
-  r.m = __shfl(m, r.n, 64);
-  r.inv = __shfl(inv, r.n, 64);
-  return r;
 }
 
 // Weights of elements base .. base + 7 of the row that the pick is drawn from.
 template <int DT, bool VEC>
 __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, int base, int pdt, bool residual, int x,
-                                const double* pow32, double (&w)[kPer]) {
+                                const double* pow64, double (&w)[kPer]) {
   const int64_t row0 = (static_cast<int64_t>(b) * (a.T + 1) + v.n) * a.V;
   float l[kPer], q[kPer];
   load_row8<DT, VEC>(a.logits, row0, base, a.V, -INFINITY, l);
@@ -243,7 +271,7 @@ __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, in
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    const double p = l[e] == -INFINITY ? 0.0 : exp2_neg((static_cast<double>(l[e]) - v.m) * a.k, pow32) * v.inv;
+    const double p = prob(l[e], v.off, a.k, v.inv, pow64);
     const double qe = residual && a.probs == nullptr ? (base + e == x ? 1.0 : 0.0) : static_cast<double>(q[e]);
     w[e] = residual ? (p > qe ? p - qe : 0.0) : p;
   }
@@ -251,18 +279,18 @@ __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, in
 
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, int pdt) {
-  __shared__ double pow32[32], red[4];
-  fill_pow32(pow32);
+  __shared__ double pow64[64], red[4];
+  fill_pow64(pow64);
   __syncthreads();
   const int s = blockIdx.x, b = blockIdx.y;
-  const Verdict v = judge<DT>(a, b, pdt, pow32);
+  const Verdict v = judge<DT>(a, b, pdt, pow64);
   if (v.n == v.count) return;  // nothing was rejected: the row's own statistics serve
   const int x = a.draft[static_cast<int64_t>(b) * a.T + v.n];
   double sum = 0.0;
-#pragma unroll
+#pragma unroll 2
   for (int p = 0; p < kPasses; ++p) {
     double w[kPer];
-    weights8<DT, VEC>(a, v, b, s * kSlice + p * kPass + threadIdx.x * kPer, pdt, true, x, pow32, w);
+    weights8<DT, VEC>(a, v, b, s * kSlice + p * kPass + threadIdx.x * kPer, pdt, true, x, pow64, w);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum += w[e];
   }
@@ -270,87 +298,100 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
   if (threadIdx.x == 0) a.rest[static_cast<int64_t>(b) * a.S + s] = sum;
 }
 
+// The pick: the slice in which the cumulative sum passes the threshold, then the element in it.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a, int pdt) {
-  __shared__ double pow32[32], wsum[4];
+  __shared__ double pow64[64], wsum[kPasses][4], part[256], red[4];
   __shared__ int found, last;
-  fill_pow32(pow32);
+  fill_pow64(pow64);
   if (threadIdx.x == 0) {
     found = 0x7fffffff;
     last = -1;
   }
   __syncthreads();
   const int b = blockIdx.x;
-  const Verdict v = judge<DT>(a, b, pdt, pow32);
+  const Verdict v = judge<DT>(a, b, pdt, pow64);
   const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
   bool residual = v.n < v.count;
-  double total = 0.0;
-  if (residual) {
-    for (int s = 0; s < a.S; ++s) total += a.rest[static_cast<int64_t>(b) * a.S + s];
-    residual = !(total <= 0.0);  // p nowhere above q: drawn from p (a NaN goes on as one)
-  }
   auto slice_sum = [&](int s) -> double {
     if (residual) return a.rest[static_cast<int64_t>(b) * a.S + s];
-    const float ms = a.maxs[row * a.S + s];
-    return ms == -INFINITY ? 0.0 : a.sums[row * a.S + s] * exp2_neg((static_cast<double>(ms) - v.m) * a.k, pow32) * v.inv;
+    return prob(a.maxs[row * a.S + s], v.off, a.k, v.inv, pow64) * a.sums[row * a.S + s];
   };
-  if (!residual) {
-    total = 0.0;
-    for (int s = 0; s < a.S; ++s) total += slice_sum(s);
+  double total = 0.0;
+  if (residual) {
+    double mine = 0.0;
+    for (int s = threadIdx.x; s < a.S; s += 256) mine += slice_sum(s);
+    total = block_sum_f64(mine, red);
+    residual = !(total <= 0.0);  // p nowhere above q: drawn from p (a NaN goes on as one)
   }
-  int pick = -1;
+  if (!residual) {
+    double mine = 0.0;
+    for (int s = threadIdx.x; s < a.S; s += 256) mine += slice_sum(s);
+    total = block_sum_f64(mine, red);
+  }
   if (total > 0.0) {  // false for a row without a distribution
     const double theta = static_cast<double>(a.r[b]) * total;
     int hit = -1, fallback = 0;
     double before = 0.0, sum = 0.0;
-    for (int s = 0; s < a.S; ++s) {
-      const double w = slice_sum(s);
-      if (w > 0.0) fallback = s;
-      if (hit < 0 && sum + w > theta) {
-        hit = s;
-        before = sum;
+    for (int s0 = 0; s0 < a.S && hit < 0; s0 += 256) {
+      if (s0 + static_cast<int>(threadIdx.x) < a.S) part[threadIdx.x] = slice_sum(s0 + threadIdx.x);
+      __syncthreads();
+      for (int s = s0; s < min(a.S, s0 + 256); ++s) {
+        const double w = part[s - s0];
+        if (w > 0.0) fallback = s;
+        if (hit < 0 && sum + w > theta) {
+          hit = s;
+          before = sum;
+        }
+        sum += w;
       }
-      sum += w;
+      __syncthreads();
     }
     const bool none = hit < 0;  // r next to 1 and a rounding: the last token that has a weight
     if (none) hit = fallback;
     const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
-    for (int p = 0; p < kPasses; ++p) {
-      const int at = hit * kSlice + p * kPass + threadIdx.x * kPer;
-      double w[kPer], mine = 0.0;
-      weights8<DT, VEC>(a, v, b, at, pdt, residual, x, pow32, w);
+    double w[kPasses][kPer], mine[kPasses], inc[kPasses];
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) mine += w[e];
-      double inc = mine;  // inclusive scan over the wave, then over the waves
+    for (int p = 0; p < kPasses; ++p) {
+      weights8<DT, VEC>(a, v, b, hit * kSlice + p * kPass + threadIdx.x * kPer, pdt, residual, x, pow64, w[p]);
+      mine[p] = 0.0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) mine[p] += w[p][e];
+      inc[p] = mine[p];  // inclusive scan over the wave, then over the waves
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(inc, o, 64);
-        if ((threadIdx.x & 63) >= o) inc += u;
+        const double u = __shfl_up(inc[p], o, 64);
+        if ((threadIdx.x & 63) >= o) inc[p] += u;
       }
-      if ((threadIdx.x & 63) == 63) wsum[threadIdx.x >> 6] = inc;
-      __syncthreads();
-      double c = before;
-      for (int i = 0; i < static_cast<int>(threadIdx.x >> 6); ++i) c += wsum[i];
-      c += inc - mine;
-      int first = 0x7fffffff, end = -1;
+      if ((threadIdx.x & 63) == 63) wsum[p][threadIdx.x >> 6] = inc[p];
+    }
+    __syncthreads();
+    double c0 = before;
+    int first = 0x7fffffff, end = -1;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      double c = c0;
+      for (int i = 0; i < 4; ++i) {
+        if (i < static_cast<int>(threadIdx.x >> 6)) c += wsum[p][i];
+        c0 += wsum[p][i];
+      }
+      c += inc[p] - mine[p];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        c += w[e];
-        if (w[e] > 0.0) end = at + e;
-        if (first == 0x7fffffff && w[e] > 0.0 && c > theta) first = at + e;
+        const int at = hit * kSlice + p * kPass + threadIdx.x * kPer + e;
+        c += w[p][e];
+        if (w[p][e] > 0.0) end = at;
+        if (first == 0x7fffffff && w[p][e] > 0.0 && c > theta) first = at;
       }
-      if (!none && first != 0x7fffffff) atomicMin(&found, first);
-      if (end >= 0) atomicMax(&last, end);
-      before += (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
-      __syncthreads();
-      if (found != 0x7fffffff) break;
-      __syncthreads();
     }
-    pick = found != 0x7fffffff ? found : last;
+    if (!none && first != 0x7fffffff) atomicMin(&found, first);  // of whole numbers: their order changes nothing
+    if (end >= 0) atomicMax(&last, end);
+    __syncthreads();
   }
   if (threadIdx.x == 0) a.n_acc[b] = v.n;
   if (static_cast<int>(threadIdx.x) <= a.T) {
     const int t = threadIdx.x;
+    const int pick = found != 0x7fffffff ? found : last;
     a.tokens[static_cast<int64_t>(b) * (a.T + 1) + t] = t < v.n ? a.draft[static_cast<int64_t>(b) * a.T + t] : t == v.n ? pick : -1;
   }
 }
@@ -414,7 +455,7 @@ extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft,
   VerifyArgs a{};
   a.logits = logits; a.draft = draft; a.counts = counts; a.probs = probs; a.u = u; a.r = r;
   a.T = static_cast<int>(T); a.V = static_cast<int>(V); a.S = static_cast<int>(ceil_div(V, kSlice));
-  a.k = greedy ? 0.0 : 1.4426950408889634074 / temperature;
+  a.k = greedy ? 0.0 : 64.0 * 1.4426950408889634074 / temperature;
   const int64_t rows = B * (T + 1) * a.S;
   a.sums = static_cast<double*>(ws);
   a.rest = a.sums + rows;

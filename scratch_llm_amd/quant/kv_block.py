@@ -32,6 +32,7 @@ __all__ = ["BLOCKS", "HEAD_DIMS", "attend_kv_blocks", "new_kv_blocks", "read_kv_
 
 BLOCKS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
+_F32, _I32 = torch.float32, torch.int32
 _FMT = {torch.int8: _lib.KV_INT8, FP8_DTYPE: _lib.KV_E4M3}
 
 
@@ -60,30 +61,40 @@ def _check_sizes(head_dim: int, block: int, dtype: torch.dtype, fn: str) -> None
 def _check_cache(kc: Tensor, vc: Tensor, ks: Tensor, vs: Tensor, table: Tensor, starts: Tensor, counts: Tensor | None,
                  batch: int, fn: str) -> tuple[int, int, int, int, int]:
     """Checks the cache, its table and the rows' positions; returns (pages, Hkv, block, D, format)."""
-    if kc.ndim != 4 or vc.ndim != 4:
-        raise ValueError(f"{fn}: k_codes must be [pages, Hkv, block, D], got {tuple(kc.shape)} and {tuple(vc.shape)}")
-    pages, hkv, block, d = kc.shape
-    _check_sizes(d, block, kc.dtype, fn)
-    if vc.shape != (pages, hkv, d, block) or vc.dtype != kc.dtype:
-        raise ValueError(f"{fn}: v_codes must be {(pages, hkv, d, block)} of {kc.dtype}, got {tuple(vc.shape)} of {vc.dtype}")
-    if ks.shape != (pages, hkv) or vs.shape != (pages, hkv) or ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise ValueError(f"{fn}: scales must be float32 {(pages, hkv)}, got {tuple(ks.shape)} and {tuple(vs.shape)}")
-    if table.ndim != 2 or table.shape[0] != batch or table.shape[1] < 1 or table.dtype != torch.int32:
-        raise ValueError(f"{fn}: block_table must be int32 [{batch}, width], got {tuple(table.shape)} of {table.dtype}")
-    if starts.shape != (batch,) or starts.dtype != torch.int32:
+    shape = kc.shape
+    if len(shape) != 4:
+        raise ValueError(f"{fn}: k_codes must be [pages, Hkv, block, D], got {tuple(shape)}")
+    pages, hkv, block, d = shape
+    dtype = kc.dtype
+    fmt = _FMT.get(dtype)
+    if fmt is None or d not in HEAD_DIMS or block not in BLOCKS:
+        _check_sizes(d, block, dtype, fn)
+    if vc.shape != (pages, hkv, d, block) or vc.dtype != dtype:
+        raise ValueError(f"{fn}: v_codes must be {(pages, hkv, d, block)} of {dtype}, got {tuple(vc.shape)} of {vc.dtype}")
+    one = (pages, hkv)
+    if ks.shape != one or vs.shape != one or ks.dtype != _F32 or vs.dtype != _F32:
+        raise ValueError(f"{fn}: scales must be float32 {one}, got {tuple(ks.shape)} and {tuple(vs.shape)}")
+    width = table.shape
+    if len(width) != 2 or width[0] != batch or width[1] < 1 or table.dtype != _I32:
+        raise ValueError(f"{fn}: block_table must be int32 [{batch}, width], got {tuple(width)} of {table.dtype}")
+    rows = (batch,)
+    if starts.shape != rows or starts.dtype != _I32:
         raise ValueError(f"{fn}: starts must be int32 [{batch}], got {tuple(starts.shape)} of {starts.dtype}")
-    if counts is not None and (counts.shape != (batch,) or counts.dtype != torch.int32):
+    if counts is not None and (counts.shape != rows or counts.dtype != _I32):
         raise ValueError(f"{fn}: counts must be int32 [{batch}], got {tuple(counts.shape)} of {counts.dtype}")
     if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()
             and starts.is_contiguous() and (counts is None or counts.is_contiguous())):
         raise ValueError(f"{fn}: codes, scales, block_table, starts and counts must be contiguous")
-    return pages, hkv, block, d, _FMT[kc.dtype]
+    return pages, hkv, block, d, fmt
 
 
-def _rows(x: Tensor) -> Tensor:
-    """x itself where the kernels can take its strides, else a contiguous copy."""
+def _rows(x: Tensor) -> tuple[Tensor, int, int, int]:
+    """x and its strides of row, token and head where the kernels can take them, else those of a contiguous copy."""
     sb, st, sh, sd = x.stride()
-    return x if sd == 1 and (sb | st | sh) & 7 == 0 and x.data_ptr() & 15 == 0 else x.contiguous()
+    if sd == 1 and (sb | st | sh) & 7 == 0 and x.data_ptr() & 15 == 0:
+        return x, sb, st, sh
+    x = x.contiguous()
+    return x, *x.stride()[:3]
 
 
 def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale: Tensor,
@@ -111,7 +122,7 @@ def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_sc
     if (hkv, d) != (hc, dc):
         raise ValueError(f"{fn}: k has {hkv} heads of {d}, the cache {hc} heads of {dc}")
     dt = _lib.sqx_dtype(k.dtype)
-    cos = sin = q_out = None
+    cos = sin = None
     rot = heads = 0
     if rope is not None:
         cos, sin = rope
@@ -123,20 +134,22 @@ def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_sc
             raise ValueError(f"{fn}: q is only rotated here: give rope")
         if q.ndim != 4 or q.shape[0] != b or q.shape[1] != t or q.shape[3] != d or q.dtype != k.dtype:
             raise ValueError(f"{fn}: q must be [{b}, {t}, H, {d}] of {k.dtype}, got {tuple(q.shape)} of {q.dtype}")
-    dev = _lib.require_device(k, v, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, q, cos, sin, fn=fn)
-    k, v = _rows(k), _rows(v)
-    qs = (0, 0, 0, 0)
+    index = _lib.device_index(fn, k, v, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, q, cos, sin)
+    k, k_sb, k_st, k_sh = _rows(k)
+    v, v_sb, v_st, v_sh = _rows(v)
+    qp = q_out = qo = cp = sp = None
+    q_sb = q_st = q_sh = rope_rows = 0
+    if rope is not None:
+        cp, sp, rope_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
     if q is not None:
-        q = _rows(q)
-        heads, qs = q.shape[2], q.stride()
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.load().sqx_kvblock_write(
-            k.data_ptr(), v.data_ptr(), dt, *k.stride()[:3], *v.stride()[:3], _lib.ptr(q), *qs[:3], _lib.ptr(q_out),
-            _lib.ptr(cos), _lib.ptr(sin), 0 if cos is None else cos.shape[0], rot, int(interleaved), fmt, k_codes.data_ptr(),
-            v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
-            _lib.ptr(counts), b, t, heads, hkv, d, block, pages, block_table.shape[1], _lib.stream_ptr(dev))
-    _lib.check(rc, fn)
+        heads = q.shape[2]
+        q, q_sb, q_st, q_sh = _rows(q)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
+    _lib.launch(index, fn, _lib.load().sqx_kvblock_write, k.data_ptr(), v.data_ptr(), dt, k_sb, k_st, k_sh, v_sb, v_st, v_sh,
+                qp, q_sb, q_st, q_sh, qo, cp, sp, rope_rows, rot, interleaved, fmt, k_codes.data_ptr(), v_codes.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(), _lib.ptr(counts), b, t,
+                heads, hkv, d, block, pages, block_table.shape[1])
     return q_out
 
 
@@ -152,14 +165,11 @@ def read_kv_blocks(k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale: T
     if tokens < 0:
         raise ValueError(f"{fn}: tokens must not be negative, got {tokens}")
     dt = _lib.sqx_dtype(dtype)
-    dev = _lib.require_device(k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, fn=fn)
-    k, v = (torch.empty(b, tokens, hkv, d, dtype=dtype, device=dev) for _ in range(2))
-    with torch.cuda.device(dev):
-        rc = _lib.load().sqx_kvblock_read(
-            fmt, k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
-            starts.data_ptr(), _lib.ptr(counts), b, tokens, hkv, d, block, pages, block_table.shape[1], dt, k.data_ptr(),
-            v.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc, fn)
+    index = _lib.device_index(fn, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts)
+    k, v = (torch.empty(b, tokens, hkv, d, dtype=dtype, device=k_codes.device) for _ in range(2))
+    _lib.launch(index, fn, _lib.load().sqx_kvblock_read, fmt, k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(), _lib.ptr(counts), b, tokens, hkv, d, block,
+                pages, block_table.shape[1], dt, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -184,24 +194,23 @@ def attend_kv_blocks(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Tenso
     pages, hkv, block, dc, fmt = _check_cache(k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, b, fn)
     if d != dc or h % hkv != 0:
         raise ValueError(f"{fn}: q has {h} heads of {d}, the cache {hkv} heads of {dc}")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    dt = _lib.sqx_dtype(q.dtype)
+    if dt == _lib.DTYPE_F32:
         raise TypeError(f"{fn}: q must be bfloat16 or float16, got {q.dtype}")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     elif not (0.0 < scale < 3.0e38):
         raise ValueError(f"{fn}: scale must be positive and finite, got {scale}")
-    dev = _lib.require_device(q, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, out, fn=fn)
-    q = _rows(q)
+    index = _lib.device_index(fn, q, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, out)
+    q, q_sb, q_st, q_sh = _rows(q)
     if out is None:
-        out = (torch.empty if counts is None else torch.zeros)(b, t, h, d, dtype=q.dtype, device=dev)
+        out = (torch.empty if counts is None else torch.zeros)(b, t, h, d, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"{fn}: out must be contiguous {tuple(q.shape)} of {q.dtype}")
-    nb = _attention_workspace(b, t, h, hkv, d, block, block_table.shape[1])
-    ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
-    with torch.cuda.device(dev):
-        rc = _lib.load().sqx_kvblock_attention(
-            q.data_ptr(), _lib.sqx_dtype(q.dtype), *q.stride()[:3], fmt, k_codes.data_ptr(), v_codes.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(), _lib.ptr(counts), b, t, h, hkv,
-            d, block, pages, block_table.shape[1], scale, out.data_ptr(), _lib.ptr(ws), nb, _lib.stream_ptr(dev))
-    _lib.check(rc, fn)
+    width = block_table.shape[1]
+    nb = _attention_workspace(b, t, h, hkv, d, block, width)
+    ws = torch.empty(nb // 4, dtype=_F32, device=q.device) if nb else None
+    _lib.launch(index, fn, _lib.load().sqx_kvblock_attention, q.data_ptr(), dt, q_sb, q_st, q_sh, fmt, k_codes.data_ptr(),
+                v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
+                _lib.ptr(counts), b, t, h, hkv, d, block, pages, width, scale, out.data_ptr(), _lib.ptr(ws), nb)
     return out

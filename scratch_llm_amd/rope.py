@@ -96,13 +96,14 @@ def rope_table(rot_dim: int, max_seq_len: int, theta: float = 10000.0, scaling: 
 
 def check_table(cos: Tensor, sin: Tensor, head_dim: int, fn: str) -> int:
     """The rotated columns that a table covers; raises where it is no table for such heads."""
-    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[0] < 1 or cos.shape[1] < 1:
-        raise ValueError(f"{fn}: cos and sin must be [positions, rot / 2] alike, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    shape = cos.shape
+    if len(shape) != 2 or shape != sin.shape or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"{fn}: cos and sin must be [positions, rot / 2] alike, got {tuple(shape)} and {tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise TypeError(f"{fn}: cos and sin must be float32, got {cos.dtype} and {sin.dtype}")
     if not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"{fn}: cos and sin must be contiguous")
-    rot = 2 * cos.shape[1]
+    rot = 2 * shape[1]
     if rot > head_dim:
         raise ValueError(f"{fn}: the table rotates {rot} columns of heads of {head_dim}")
     return rot
@@ -117,34 +118,36 @@ def apply_rope(x: Tensor, positions: Tensor, cos: Tensor, sin: Tensor, *, interl
     rounded once to ``x``'s type (float32, bfloat16 or float16). Positions outside the table take its first
     or last row. ``out`` may be ``x``."""
     fn = "apply_rope"
-    if x.ndim < 2:
-        raise ValueError(f"{fn}: x must be [..., heads, d], got {tuple(x.shape)}")
-    if positions.shape != x.shape[:-2]:
-        raise ValueError(f"{fn}: positions {tuple(positions.shape)} do not match x {tuple(x.shape)}")
-    rot = check_table(cos, sin, x.shape[-1], fn)
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{fn}: x must be [..., heads, d], got {tuple(shape)}")
+    if positions.shape != shape[:-2]:
+        raise ValueError(f"{fn}: positions {tuple(positions.shape)} do not match x {tuple(shape)}")
+    heads, d = shape[-2], shape[-1]
+    rot = check_table(cos, sin, d, fn)
     dt = _lib.sqx_dtype(x.dtype)
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype != torch.int32 and positions.dtype != torch.int64:
         raise TypeError(f"{fn}: positions must be int32 or int64, got {positions.dtype}")
-    dev = _lib.require_device(x, positions, cos, sin, out, fn=fn)
+    index = _lib.device_index(fn, x, positions, cos, sin, out)
     if x.stride(-1) != 1:
         x = x.contiguous()
-    heads, d = x.shape[-2], x.shape[-1]
-    rows = x.reshape(-1, heads, d)  # a copy where the leading strides do not combine
+    rows = x if len(shape) == 3 else x.reshape(-1, heads, d)  # a copy where the leading strides do not combine
     if positions.dtype == torch.int64:
         positions = positions.clamp(0, cos.shape[0] - 1).to(torch.int32)
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
-        raise ValueError(f"{fn}: out must be {tuple(x.shape)} of {x.dtype} with consecutive columns")
-    try:
-        to = out.view(-1, heads, d)
-    except RuntimeError:
-        raise ValueError(f"{fn}: the leading strides of out {out.stride()} do not combine") from None
-    with torch.cuda.device(dev):
-        rc = _lib.load().sqx_rope(
-            rows.data_ptr(), dt, rows.shape[0], heads, d, rows.stride(0), rows.stride(1), positions.data_ptr(),
-            cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot, int(interleaved), to.data_ptr(), to.stride(0), to.stride(1),
-            _lib.stream_ptr(dev))
-    _lib.check(rc, fn)
+        out = to = torch.empty(shape, dtype=x.dtype, device=x.device)
+        on, oh = heads * d, d
+    else:
+        if out.shape != shape or out.dtype != x.dtype or out.stride(-1) != 1:
+            raise ValueError(f"{fn}: out must be {tuple(shape)} of {x.dtype} with consecutive columns")
+        try:
+            to = out if len(shape) == 3 else out.view(-1, heads, d)
+        except RuntimeError:
+            raise ValueError(f"{fn}: the leading strides of out {out.stride()} do not combine") from None
+        on, oh, _ = to.stride()
+    xn, xh, _ = rows.stride()
+    _lib.launch(index, fn, _lib.load().sqx_rope, rows.data_ptr(), dt, rows.shape[0], heads, d, xn, xh, positions.data_ptr(),
+                cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot, interleaved, to.data_ptr(), on, oh)
     return out

@@ -61,17 +61,16 @@ def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | No
     if counts is not None and tuple(counts.shape) != (b,):
         raise ValueError(f"{fn}: counts must be {(b,)}, got {tuple(counts.shape)}")
     pdt = _lib.DTYPE_F32 if draft_probs is None else _lib.sqx_dtype(draft_probs.dtype)
-    dev = _lib.require_device(logits, draft, u, r, draft_probs, counts, fn=fn)
-    logits, draft = logits.contiguous(), draft.contiguous()
-    u, r, draft_probs, counts = (None if x is None else x.contiguous() for x in (u, r, draft_probs, counts))
+    index = _lib.device_index(fn, logits, draft, u, r, draft_probs, counts)
+    logits, draft, u, r, draft_probs, counts = (
+        x if x is None or x.is_contiguous() else x.contiguous() for x in (logits, draft, u, r, draft_probs, counts))
     lib = _lib.load()
+    dev = logits.device
     n = torch.empty(b, dtype=torch.int32, device=dev)
     tokens = torch.empty(b, t1, dtype=torch.int32, device=dev)
     nb = lib.sqx_verify_draft_workspace_bytes(b, t, v)
     ws = torch.empty(max(nb // 8, 1), dtype=torch.float64, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.sqx_verify_draft(
-            logits.data_ptr(), dt, draft.data_ptr(), _lib.ptr(counts), _lib.ptr(draft_probs), pdt, _lib.ptr(u), _lib.ptr(r),
-            temperature, b, t, v, n.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel() * 8, _lib.stream_ptr(dev))
-    _lib.check(rc, fn)
+    _lib.launch(index, fn, lib.sqx_verify_draft, logits.data_ptr(), dt, draft.data_ptr(), _lib.ptr(counts),
+                _lib.ptr(draft_probs), pdt, _lib.ptr(u), _lib.ptr(r), temperature, b, t, v, n.data_ptr(), tokens.data_ptr(),
+                ws.data_ptr(), nb)
     return n, tokens
