@@ -10,10 +10,11 @@
 //    the order in which it must hold P for the second product: the probabilities never leave their lane.
 //  - Values are stored [D, block], so a lane's part of V^T is 16 consecutive bytes, the same 16 keys.
 //  - A page holds at least 16 tokens, so a lane's 16 keys share one key scale and one value scale. With x the raw
-//    product, u = x (ks scale log2 e) + log2 vs; the running maximum is that of u, p = 2^(u - max + 15), O sums p c and
-//    the softmax's denominator sums p / vs. Probabilities thus carry their value scale, and the largest term of the
-//    output is near 2^15 whatever the scales: fp16 keeps 11 bits of every p down to 2^-29 of it. Sums, maxima and the
-//    denominator are fp32.
+//    product, u = x (ks scale log2 e) + log2 vs; with m a maximum of u, p = 2^(u - m + 7), O sums p c and the softmax's
+//    denominator sums p / vs. Probabilities thus carry their value scale, and the largest terms of the output are near
+//    2^7 whatever the scales. m follows the running maximum only where that has grown by more than 8: p stays below
+//    2^15, and a prompt rescales O in a few of its first steps only. fp16 rounds p by 2^-11 of itself, or by 2^-25
+//    (2^-32 of the largest) where it is subnormal, which the matrix unit keeps. Sums, m and the denominator are fp32.
 #include "sqx_kvblock.h"
 
 namespace sqx {
@@ -30,11 +31,10 @@ struct KvAttnArgs {
   float qscale;  // scale * log2(e)
 };
 
-typedef _Float16 f16x4_t __attribute__((__vector_size__(4 * sizeof(_Float16))));
-
 constexpr int kStepKeys = 64;
 constexpr int kAttnWaves = 4;
-constexpr float kPOffset = 15.0f;     // p reaches 2^15
+constexpr float kPOffset = 7.0f;      // p of the maximum that m stands for
+constexpr float kPGrowth = 8.0f;      // m stays while the maximum is within this: p is below 2^15
 constexpr float kTinyScale = 1e-30f;  // stands in for a scale of zero (a page never written)
 
 // Four codes of a dword as fp16 pairs (elements 0, 1 and 2, 3), exact.
@@ -65,10 +65,146 @@ __device__ inline u32x4_t codes8(uint32_t w0, uint32_t w1) {
 // Bytes of w that are E4M3 NaNs, as 0x80 in their place.
 __device__ inline uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// Workgroup (h, s * tiles + tile, b): kv head h, the 16 R (token, head) rows of a tile, part s of nsplit of its keys.
-// The four waves take alternate 64-key steps.
+// One 64-key step of the softmax for 16 query rows: lane (g, r) holds the raw scores of keys 16 g + 4 t + j of row r in
+// sc[t][j]; f and lvs bring them to u, ivs is 1 / vs. Updates m, l and O^T's columns, leaves p as the operand pf.
+template <int VD>
+__device__ inline void softmax_step(f32x4_t (&sc)[4], bool masked, int behind, float f, float lvs, float ivs, float& m,
+                                    float& l, f32x4_t (&o)[VD], u32x4_t (&pf)[2]) {
+  if (masked) {  // wave-uniform; keys of the lane from `behind` on are not attended
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * t + j >= behind) sc[t][j] = -INFINITY;
+  }
+  float mx = sc[0][0];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, sc[t][j]);
+  mx = fmaf(mx, f, lvs);  // f > 0: the maximum of u
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  if (__ballot(mx > m + kPGrowth) != 0) {  // wave-uniform; also from -infinity
+    const float mn = fmaxf(m, mx);
+    const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= al;
+#pragma unroll
+    for (int c = 0; c < VD; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[c][j] *= al;
+    m = mn;
+  }
+  const float base = lvs - (m == -INFINITY ? 0.0f : m) + kPOffset;
+  float p[16], sum = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(sc[t][j], f, base));
+      if (masked) p[4 * t + j] = sc[t][j] == -INFINITY ? 0.0f : p[4 * t + j];  // whatever its page's scales are
+      sum += p[4 * t + j];
+    }
+  l = sum == 0.0f ? l : fmaf(sum, ivs, l);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    pf[t >> 1][2 * (t & 1)] = ActF16::pack_rne(p[4 * t], p[4 * t + 1]);
+    pf[t >> 1][2 * (t & 1) + 1] = ActF16::pack_rne(p[4 * t + 2], p[4 * t + 3]);
+  }
+}
+
+// 1.0 for the lane's keys below `behind`, 0 from there on, in the order of softmax_step's pf.
+__device__ inline void attended(int behind, u32x4_t (&am)[2]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    am[i >> 2][i & 3] = (2 * i < behind ? 0x3c00u : 0u) | (2 * i + 1 < behind ? 0x3c000000u : 0u);
+}
+
+// The 8 KD dims of query row `src` that a lane holds (64 i + 16 g + 8 half ..), as fp16, and the factor that brings a raw
+// score to u. bf16 rows are scaled by a power of two; the row's four lanes share it.
+template <int KD, bool BF16>
+__device__ inline float load_query(const uint16_t* src, bool ok, int g, float qscale, u32x4_t (&qf)[2 * KD]) {
+#pragma unroll
+  for (int k = 0; k < 2 * KD; ++k) {
+    qf[k] = u32x4_t{0u, 0u, 0u, 0u};
+    if (ok) qf[k] = *reinterpret_cast<const u32x4_t*>(src + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+  }
+  if constexpr (!BF16) return qscale;
+  float most = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 2 * KD; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = qf[k][e];
+      most = fmaxf(most, fmaxf(fabsf(bf16_lo(w)), fabsf(bf16_hi(w))));
+    }
+  most = fmaxf(most, __shfl_xor(most, 16, 64));
+  most = fmaxf(most, __shfl_xor(most, 32, 64));
+  float up = 1.0f;
+  if (most > 0.0f && most <= 3.402823466e38f) {
+    int e;
+    frexpf(most, &e);
+    up = ldexpf(1.0f, 15 - max(e, -100));
+  }
+#pragma unroll
+  for (int k = 0; k < 2 * KD; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = qf[k][e];
+      qf[k][e] = ActF16::pack_rne(bf16_lo(w) * up, bf16_hi(w) * up);
+    }
+  return qscale * (1.0f / up);
+}
+
+// The rows and keys of a tile of `span` rows from row0: token `last` is its last one below the count, keys below `keys` are
+// attended by some row of it, keys up to `first` by every row.
+struct KvSpan {
+  int count, start, first, keys;
+};
+__device__ inline bool kv_span(const KvAttnArgs& a, int b, int row0, int span, KvSpan& s) {
+  s.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  if (row0 / a.G >= s.count) return false;  // rows from the count on are left as they are
+  s.start = a.starts[b];
+  const int last = min((row0 + span - 1) / a.G, s.count - 1);
+  const int64_t end = static_cast<int64_t>(s.start) + last + 1, most = static_cast<int64_t>(a.width) * a.block;
+  s.keys = static_cast<int>(end < 0 ? 0 : (end < most ? end : most));
+  s.first = s.start + row0 / a.G;
+  return true;
+}
+
+// Eight (D / 16) output dims of a joined row: to the workspace as they are, or divided and rounded to the output.
+template <int D, bool BF16, int DT>
+__device__ inline void put_row(const KvAttnArgs& a, int b, int h, int split, int row, int jd, float M, float sum,
+                               const float (&acc)[DT]) {
+  const int rows = a.T * a.G;
+  if (a.nsplit > 1) {
+    const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + h) * a.nsplit + split) * rows + row;
+    if (jd == 0) {
+      a.pml[2 * at] = M;
+      a.pml[2 * at + 1] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d += 4)
+      *reinterpret_cast<f32x4_t*>(a.po + at * D + jd + d) = f32x4_t{acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: zeros
+  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D + jd;
+#pragma unroll
+  for (int d = 0; d < DT; d += 4) {
+    const uint32_t w0 = BF16 ? ActBF16::pack_rne(acc[d] * inv, acc[d + 1] * inv) : ActF16::pack_rne(acc[d] * inv, acc[d + 1] * inv);
+    const uint32_t w1 = BF16 ? ActBF16::pack_rne(acc[d + 2] * inv, acc[d + 3] * inv) : ActF16::pack_rne(acc[d + 2] * inv, acc[d + 3] * inv);
+    *reinterpret_cast<u32x2v_t*>(dst + d) = u32x2v_t{w0, w1};
+  }
+}
+
+__device__ inline float scale_or_tiny(float s) { return fmaxf(s, kTinyScale) + (s - s); }  // a NaN or infinity gives NaN
+
+// Workgroup (h, s * tiles + tile, b): kv head h, the 16 R (token, head) rows of a tile, part s of nsplit of its keys. For few
+// rows, where reading the cache once is the bound: the four waves take alternate 64-key steps straight from memory into
+// registers and share nothing until the end.
 template <int D, int R, bool E4M3, bool BF16>
-__global__ __launch_bounds__(256) void kv_attn_kernel(const KvAttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const KvAttnArgs a) {
   constexpr int KD = D / 64;  // 16-byte pieces of a key per lane
   constexpr int VD = D / 16;  // 16-dim tiles of the output
   const int h = blockIdx.x, b = blockIdx.z;
@@ -77,73 +213,13 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(const KvAttnArgs a) {
   const int tile = blockIdx.y % tiles, split = blockIdx.y / tiles;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, r = lane & 15;
-  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   const int row0 = tile * 16 * R;
-  if (row0 / a.G >= count) return;  // rows from the count on are left as they are
-  const int start = a.starts[b];
-  const int last = min((row0 + 16 * R - 1) / a.G, count - 1);  // last token of the tile
-  // keys below L are attended by some row of the tile; keys up to `first` by every row
-  const int64_t end = static_cast<int64_t>(start) + last + 1;
-  const int L = static_cast<int>(end < 0 ? 0 : (end < static_cast<int64_t>(a.width) * a.block ? end : static_cast<int64_t>(a.width) * a.block));
-  const int first = start + row0 / a.G;
+  KvSpan sp;
+  if (!kv_span(a, b, row0, 16 * R, sp)) return;
+  const int L = sp.keys;
   const int steps = (L + kStepKeys - 1) / kStepKeys;
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / a.nsplit);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / a.nsplit);
-
-  // queries: dims 64 i + 16 g + 8 half .. of row r, scaled by a power of two
-  u32x4_t qf[R][2 * KD];
-  float qs[R];
-  int pos[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int row = row0 + 16 * i + r;
-    const int t = row / a.G;
-    const bool ok = row < rows && t < count;
-    pos[i] = ok ? start + t : -1;
-    const uint16_t* src = a.q + b * a.q_sb + (ok ? t * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0);
-#pragma unroll
-    for (int k = 0; k < 2 * KD; ++k) {
-      qf[i][k] = u32x4_t{0u, 0u, 0u, 0u};
-      if (ok) qf[i][k] = *reinterpret_cast<const u32x4_t*>(src + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
-    }
-    qs[i] = a.qscale;
-    if constexpr (BF16) {
-      float most = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 2 * KD; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t w = qf[i][k][e];
-          most = fmaxf(most, fmaxf(fabsf(bf16_lo(w)), fabsf(bf16_hi(w))));
-        }
-      most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(most, __shfl_xor(most, 32, 64));
-      int e = 0;
-      if (most > 0.0f && most <= 3.402823466e38f) {
-        frexpf(most, &e);
-        e = max(e, -100);
-      }
-      const float up = most > 0.0f && most <= 3.402823466e38f ? ldexpf(1.0f, 15 - e) : 1.0f;
-      qs[i] = a.qscale * (1.0f / up);
-#pragma unroll
-      for (int k = 0; k < 2 * KD; ++k)
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) {
-          const uint32_t w = qf[i][k][e2];
-          qf[i][k][e2] = ActF16::pack_rne(bf16_lo(w) * up, bf16_hi(w) * up);
-        }
-    }
-  }
-
-  f32x4_t o[R][VD];
-  float m[R], l[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < VD; ++c) o[i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
 
   const int64_t pstride = static_cast<int64_t>(a.Hkv) * a.block * D;
   const uint8_t* const kb = a.kc + static_cast<int64_t>(h) * a.block * D;
@@ -161,141 +237,121 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(const KvAttnArgs a) {
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int i = 0; i < KD; ++i) kr[t][i] = *reinterpret_cast<const u32x4_t*>(p + 4 * t * D + 64 * i);
-    const int64_t sp = static_cast<int64_t>(sane(pv)) * a.Hkv + h;
-    ks = a.ks[sp];
-    vs = a.vs[sp];
+    const int64_t at = static_cast<int64_t>(sane(pv)) * a.Hkv + h;
+    ks = a.ks[at];
+    vs = a.vs[at];
     if (pv < 0 || pv >= a.pages) ks = __builtin_nanf("");  // no such page: whoever attends it gets NaN
   };
-
   int step = s0 + wave;
+  int pk = 0, pv = 0, pk2 = 0, pv2 = 0;
   if (step < s1) {
-    int pk = page_of(step * kStepKeys + 16 * gk), pv = page_of(step * kStepKeys + 16 * g);
+    pk = page_of(step * kStepKeys + 16 * gk);
+    pv = page_of(step * kStepKeys + 16 * g);
+    pk2 = page_of((step + kAttnWaves) * kStepKeys + 16 * gk);
+    pv2 = page_of((step + kAttnWaves) * kStepKeys + 16 * g);
     load_k(step * kStepKeys, pk, pv);
-    int pk2 = page_of((step + kAttnWaves) * kStepKeys + 16 * gk), pv2 = page_of((step + kAttnWaves) * kStepKeys + 16 * g);
-    for (; step < s1; step += kAttnWaves) {
-      const int k0 = step * kStepKeys;
-      {
-        const uint8_t* p = vb + sane(pv) * pstride + r * a.block + ((k0 + 16 * g) & (a.block - 1));
-#pragma unroll
-        for (int c = 0; c < VD; ++c) vr[c] = *reinterpret_cast<const u32x4_t*>(p + 16 * c * a.block);
-      }
-      f32x4_t sc[R][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < KD; ++k) {
-          const u32x4_t w = kr[t][k];
-          const u32x4_t k0f = codes8<E4M3>(w[0], w[1]), k1f = codes8<E4M3>(w[2], w[3]);
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-            sc[i][t] = ActF16::mfma(k0f, qf[i][2 * k], sc[i][t]);
-            sc[i][t] = ActF16::mfma(k1f, qf[i][2 * k + 1], sc[i][t]);
-          }
-        }
-      }
-      const float kscale = fmaxf(ks, kTinyScale) + (ks - ks);  // a NaN stays one
-      const float vscale = fmaxf(vs, kTinyScale) + (vs - vs);
-      const float lvs = __log2f(vscale), ivs = 1.0f / vscale;
-      // the next step's keys, and the pages of the one after it
-      pv = pv2;
-      load_k(k0 + kAttnWaves * kStepKeys, pk2, pv2);
-      pk2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * gk);
-      pv2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * g);
+  }
 
-      const bool masked = k0 + kStepKeys - 1 > first;  // wave-uniform
-      u32x4_t pf[R][2];
+  u32x4_t qf[R][2 * KD];
+  float qs[R];
+  int pos[R];
+  f32x4_t o[R][VD];
+  float m[R], l[R];
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (masked) {
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + 16 * i + r;
+    const int t = row / a.G;
+    const bool ok = row < rows && t < sp.count;
+    pos[i] = ok ? sp.start + t : -1;
+    qs[i] = load_query<KD, BF16>(a.q + b * a.q_sb + (ok ? t * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, g, a.qscale, qf[i]);
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
+    for (int c = 0; c < VD; ++c) o[i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  for (; step < s1; step += kAttnWaves) {
+    const int k0 = step * kStepKeys;
+    {
+      const uint8_t* p = vb + sane(pv) * pstride + r * a.block + ((k0 + 16 * g) & (a.block - 1));
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (k0 + 16 * g + 4 * t + j > pos[i]) sc[i][t][j] = -INFINITY;
+      for (int c = 0; c < VD; ++c) vr[c] = *reinterpret_cast<const u32x4_t*>(p + 16 * c * a.block);
+    }
+    f32x4_t sc[R][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KD; ++k) {
+        const u32x4_t w = kr[t][k];
+        const u32x4_t k0f = codes8<E4M3>(w[0], w[1]), k1f = codes8<E4M3>(w[2], w[3]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          sc[i][t] = ActF16::mfma(k0f, qf[i][2 * k], sc[i][t]);
+          sc[i][t] = ActF16::mfma(k1f, qf[i][2 * k + 1], sc[i][t]);
         }
-        const float f = qs[i] * kscale;
-        float mx = sc[i][0][0];
+      }
+    }
+    const float kscale = scale_or_tiny(ks), vscale = scale_or_tiny(vs);
+    const float lvs = __log2f(vscale), ivs = 1.0f / vscale;
+    // the next step's keys, and the pages of the one after it
+    pv = pv2;
+    load_k(k0 + kAttnWaves * kStepKeys, pk2, pv2);
+    pk2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * gk);
+    pv2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * g);
+
+    const bool masked = k0 + kStepKeys - 1 > sp.first;  // wave-uniform
+    u32x4_t pf[R][2];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < R; ++i)
+      softmax_step<VD>(sc[i], masked, pos[i] + 1 - (k0 + 16 * g), qs[i] * kscale, lvs, ivs, m[i], l[i], o[i], pf[i]);
+    // E4M3 values may be NaN where some row must not see them (a later token, a slot never written), and 0 NaN is NaN: in
+    // masked steps NaN codes are taken out, and put back where a product of their indicator with that of the keys attended
+    // is not zero (p itself may round to zero).
+    if constexpr (E4M3) {
+      if (masked) {
+        uint32_t bad = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mx = fmaxf(mx, sc[i][t][j]);
-        mx = fmaf(mx, f, lvs);  // f > 0: the maximum of u
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[i], mx);
-        if (__ballot(mn > m[i]) != 0) {  // wave-uniform
-          const float al = m[i] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[i] - mn);
-          l[i] *= al;
+        for (int c = 0; c < VD; ++c)
 #pragma unroll
-          for (int c = 0; c < VD; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][c][j] *= al;
-          m[i] = mn;
-        }
-        const float base = lvs - (mn == -INFINITY ? 0.0f : mn) + kPOffset;
-        float p[16], sum = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][t][j], f, base));
-            if (masked) p[4 * t + j] = sc[i][t][j] == -INFINITY ? 0.0f : p[4 * t + j];  // whatever its page's scales are
-            sum += p[4 * t + j];
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = vr[c][e];
+            bad |= nan_bytes(w);
           }
-        l[i] = sum == 0.0f ? l[i] : fmaf(sum, ivs, l[i]);
+        if (__ballot(bad != 0) != 0) {  // wave-uniform
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          pf[i][t >> 1][2 * (t & 1)] = ActF16::pack_rne(p[4 * t], p[4 * t + 1]);
-          pf[i][t >> 1][2 * (t & 1) + 1] = ActF16::pack_rne(p[4 * t + 2], p[4 * t + 3]);
-        }
-      }
-      // E4M3 values may be NaN where some row must not see them (a later token, a slot never written), and 0 NaN is
-      // NaN: in masked steps NaN codes are taken out and put back through a product of their indicator.
-      bool any_nan = false;
-      if constexpr (E4M3) {
-        if (masked) {
-          uint32_t bad = 0;
-#pragma unroll
-          for (int c = 0; c < VD; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t w = vr[c][e];
-              bad |= nan_bytes(w);
-            }
-          any_nan = __ballot(bad != 0) != 0;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < VD; ++c) {
-        u32x4_t w = vr[c];
-        if constexpr (E4M3) {
-          if (any_nan) {  // wave-uniform
+          for (int c = 0; c < VD; ++c) {
             u32x4_t one;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t x = w[e], nb = nan_bytes(x);
-              one[e] = (nb >> 7) * 0x38u;  // 1.0
-              w[e] = x & ~((nb >> 7) * 0xffu);
+              const uint32_t w = vr[c][e], nb = nan_bytes(w) >> 7;
+              one[e] = nb * 0x38u;  // 1.0
+              vr[c][e] = w & ~(nb * 0xffu);
             }
 #pragma unroll
             for (int i = 0; i < R; ++i) {
+              u32x4_t am[2];
+              attended(pos[i] + 1 - (k0 + 16 * g), am);
               f32x4_t hit{0.0f, 0.0f, 0.0f, 0.0f};
-              hit = ActF16::mfma(codes8<true>(one[0], one[1]), pf[i][0], hit);
-              hit = ActF16::mfma(codes8<true>(one[2], one[3]), pf[i][1], hit);
+              hit = ActF16::mfma(codes8<true>(one[0], one[1]), am[0], hit);
+              hit = ActF16::mfma(codes8<true>(one[2], one[3]), am[1], hit);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 if (hit[j] > 0.0f) o[i][c][j] = __builtin_nanf("");
             }
           }
         }
-        const u32x4_t v0 = codes8<E4M3>(w[0], w[1]), v1 = codes8<E4M3>(w[2], w[3]);
+      }
+    }
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-          o[i][c] = ActF16::mfma(v0, pf[i][0], o[i][c]);
-          o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
-        }
+    for (int c = 0; c < VD; ++c) {
+      const u32x4_t w = vr[c];
+      const u32x4_t v0 = codes8<E4M3>(w[0], w[1]), v1 = codes8<E4M3>(w[2], w[3]);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        o[i][c] = ActF16::mfma(v0, pf[i][0], o[i][c]);
+        o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
       }
     }
   }
@@ -319,8 +375,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(const KvAttnArgs a) {
     for (int c = 0; c < VD; ++c) *reinterpret_cast<f32x4_t*>(&so[wave][r][16 * c + 4 * g]) = o[i][c];
     __syncthreads();
     const int row = row0 + 16 * i + jr;
-    const int t = row / a.G;
-    if (row < rows && t < count) {
+    if (row < rows && row / a.G < sp.count) {
       float M = sm[0][jr];
 #pragma unroll
       for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, sm[w][jr]);
@@ -334,30 +389,249 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(const KvAttnArgs a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] = fmaf(so[w][jr][jd + d], wt, acc[d]);
       }
-      if (a.nsplit > 1) {
-        const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + h) * a.nsplit + split) * rows + row;
-        if (jd == 0) {
-          a.pml[2 * at] = M;
-          a.pml[2 * at + 1] = sum;
+      put_row<D, BF16, DT>(a, b, h, split, row, jd, M, sum, acc);
+    }
+  }
+}
+
+// f16 pairs with NaNs replaced by zero; `one` gets 1.0 in their place.
+__device__ inline uint32_t drop_nan16(uint32_t w, uint32_t& one) {
+  const uint32_t lo = (w & 0x7fffu) > 0x7c00u ? 0xffffu : 0u, hi = (w & 0x7fff0000u) > 0x7c000000u ? 0xffff0000u : 0u;
+  one = (lo | hi) & 0x3c003c00u;
+  return w & ~(lo | hi);
+}
+
+// For many rows (prompts), where the matrix and vector units are the bound: workgroup (h, s * tiles + tile, b) takes 256
+// rows, 32 in each of eight waves (heads of 256: 128 rows, four waves with twice the registers), and all waves work on
+// the same keys. A 64-key piece of the cache is read once, turned
+// to fp16 once (its conversion would cost a wave of its own two thirds of its softmax) and kept in LDS as the operands
+// that the lanes want, so writes and reads are consecutive. Two tiles in LDS and one in registers: while a tile is worked
+// on, the next is converted behind one barrier a tile and the one after it is on its way.
+constexpr int tile_waves(int d) { return d == 256 ? 4 : 8; }
+constexpr int tile_rows(int d) { return 32 * tile_waves(d); }
+template <int D, bool E4M3, bool BF16>
+__global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_tile_kernel(const KvAttnArgs a) {
+  constexpr int kWaves = tile_waves(D), kTileRows = tile_rows(D);
+  constexpr int KD = D / 64, VD = D / 16, R = 2;
+  constexpr int NS = D == 64 ? 2 : 1;            // 64-key pieces of a tile
+  constexpr int U = 4 * KD * NS / kWaves;        // 16-byte units of keys, and of values, per thread
+  constexpr int kTileKeys = 64 * NS;
+  // operands of a tile: keys [piece][t][2 KD][lane], values [piece][c][2][lane], 16 bytes each
+  __shared__ u32x4_t lk[2][NS * 4 * 2 * KD * 64], lv[2][NS * VD * 2 * 64];
+  __shared__ float lf[2][NS * 4], lg[2][NS * 4], li[2][NS * 4];  // per 16 keys: key scale, log2 and inverse of the value scale
+  __shared__ int lnan[3];  // tile i holds a NaN value: slot i % 3, cleared while tile i - 2 is worked on
+  const int h = blockIdx.x, b = blockIdx.z;
+  const int rows = a.T * a.G;
+  const int tiles = (rows + kTileRows - 1) / kTileRows;
+  const int tile = tiles - 1 - blockIdx.y % tiles, split = blockIdx.y / tiles;  // the longest first
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, r = lane & 15;
+  const int row0 = tile * kTileRows;
+  KvSpan sp;
+  if (!kv_span(a, b, row0, kTileRows, sp)) return;
+  const int L = sp.keys;
+  const int steps = (L + kTileKeys - 1) / kTileKeys;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / a.nsplit);
+  const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / a.nsplit);
+
+  // loads: unit u of a thread is key piece (t, i) and value tile c of its lane, as the direct kernel's lanes hold them
+  const int64_t pstride = static_cast<int64_t>(a.Hkv) * a.block * D;
+  const uint8_t* const kb = a.kc + static_cast<int64_t>(h) * a.block * D;
+  const uint8_t* const vb = a.vc + static_cast<int64_t>(h) * a.block * D;
+  const int* const trow = a.table + static_cast<int64_t>(b) * a.width;
+  const int gk = (lane >> 2) & 3;
+  constexpr int kWavesPerPiece = kWaves / NS;  // waves that load one 64-key piece
+  const int piece = wave / kWavesPerPiece, pw = wave % kWavesPerPiece;
+  auto sane = [&](int p) { return p >= 0 && p < a.pages ? p : 0; };
+  auto page_of = [&](int key) { return trow[min(key, L - 1) >> a.shift]; };
+  u32x4_t kreg[U], vreg[U];
+  float ks = 0.0f, vs = 0.0f;
+  int pk = 0, pv = 0;
+  auto load_pages = [&](int step) {
+    const int k0 = step * kTileKeys + 64 * piece;
+    pk = page_of(k0 + 16 * gk);
+    pv = page_of(k0 + 16 * g);
+  };
+  auto load_tile = [&](int step) {
+    const int k0 = step * kTileKeys + 64 * piece;
+    const uint8_t* p = kb + sane(pk) * pstride + (((k0 + 16 * gk) & (a.block - 1)) + (lane & 3)) * D + 16 * g;
+    const uint8_t* q = vb + sane(pv) * pstride + r * a.block + ((k0 + 16 * g) & (a.block - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int w = pw + kWavesPerPiece * u;  // (t, i) of the keys, c of the values
+      kreg[u] = *reinterpret_cast<const u32x4_t*>(p + 4 * (w / KD) * D + 64 * (w % KD));
+      vreg[u] = *reinterpret_cast<const u32x4_t*>(q + 16 * w * a.block);
+    }
+    if (pw == 0) {
+      const int64_t at = static_cast<int64_t>(sane(pv)) * a.Hkv + h;
+      ks = a.ks[at];
+      vs = a.vs[at];
+      if (pv < 0 || pv >= a.pages) ks = __builtin_nanf("");
+    }
+  };
+  auto store_tile = [&](int to) {
+    const int buf = to & 1;
+    [[maybe_unused]] const int slot = to % 3;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int w = pw + kWavesPerPiece * u;
+      const u32x4_t k = kreg[u], v = vreg[u];
+      u32x4_t* dk = &lk[buf][((piece * 4 * KD + w) * 2) * 64 + lane];
+      u32x4_t* dv = &lv[buf][((piece * VD + w) * 2) * 64 + lane];
+      dk[0] = codes8<E4M3>(k[0], k[1]);
+      dk[64] = codes8<E4M3>(k[2], k[3]);
+      dv[0] = codes8<E4M3>(v[0], v[1]);
+      dv[64] = codes8<E4M3>(v[2], v[3]);
+      if constexpr (E4M3) bad |= nan_bytes(v[0]) | nan_bytes(v[1]) | nan_bytes(v[2]) | nan_bytes(v[3]);
+    }
+    if (pw == 0 && r == 0) {
+      const float vscale = scale_or_tiny(vs);
+      lf[buf][4 * piece + g] = scale_or_tiny(ks);
+      lg[buf][4 * piece + g] = __log2f(vscale);
+      li[buf][4 * piece + g] = 1.0f / vscale;
+    }
+    if constexpr (E4M3) {
+      if (bad != 0) lnan[slot] = 1;
+    }
+  };
+
+  u32x4_t qf[R][2 * KD];
+  float qs[R];
+  int pos[R];
+  f32x4_t o[R][VD];
+  float m[R], l[R];
+  const int wrow = row0 + 16 * R * wave;
+  int last = -1;  // the wave's last position
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = wrow + 16 * i + r;
+    const int t = row / a.G;
+    const bool ok = row < rows && t < sp.count;
+    pos[i] = ok ? sp.start + t : -1;
+    qs[i] = load_query<KD, BF16>(a.q + b * a.q_sb + (ok ? t * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, g, a.qscale, qf[i]);
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < VD; ++c) o[i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  {
+    const int end = min(min(wrow + 16 * R, rows), sp.count * a.G);  // rows of the wave below the count
+    if (end > wrow) last = sp.start + (end - 1) / a.G;
+  }
+  const int first = sp.start + wrow / a.G;
+
+  if (threadIdx.x < 3) lnan[threadIdx.x] = 0;
+  if (s0 < s1) {
+    load_pages(s0);
+    load_tile(s0);
+    load_pages(s0 + 1);
+  }
+  __syncthreads();  // lnan is clear
+  if (s0 < s1) {
+    store_tile(s0);
+    load_tile(s0 + 1);  // past the end: the last page again, not used
+    load_pages(s0 + 2);
+  }
+  for (int step = s0; step < s1; ++step) {
+    const int buf = step & 1;
+    __syncthreads();  // tile `step` is in LDS, the other buffer is free
+    if constexpr (E4M3) {
+      if (threadIdx.x == 0) lnan[(step + 2) % 3] = 0;  // read by nobody since this barrier, set after the next
+    }
+    if (step + 1 < s1) {
+      store_tile(step + 1);
+      load_tile(step + 2);
+      load_pages(step + 3);
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const int k0 = step * kTileKeys + 64 * n;
+      if (k0 > last) continue;  // wave-uniform: nothing here for its rows
+      const bool masked = k0 + kStepKeys - 1 > first;
+      f32x4_t sc[R][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2 * KD; ++k) {
+          const u32x4_t w = lk[buf][((n * 4 + t) * 2 * KD + k) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < R; ++i) sc[i][t] = ActF16::mfma(w, qf[i][k], sc[i][t]);
         }
+      }
+      const float kscale = lf[buf][4 * n + g], lvs = lg[buf][4 * n + g], ivs = li[buf][4 * n + g];
+      u32x4_t pf[R][2];
 #pragma unroll
-        for (int d = 0; d < DT; d += 4)
-          *reinterpret_cast<f32x4_t*>(a.po + at * D + jd + d) = f32x4_t{acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
-      } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: zeros
-        uint32_t w[DT / 2];
+      for (int i = 0; i < R; ++i)
+        softmax_step<VD>(sc[i], masked, pos[i] + 1 - (k0 + 16 * g), qs[i] * kscale, lvs, ivs, m[i], l[i], o[i], pf[i]);
+      if (E4M3 && masked && lnan[step % 3] != 0) {  // as in the direct kernel
+#pragma unroll 1
+        for (int c = 0; c < VD; ++c) {
+          u32x4_t* const at = &lv[buf][((n * VD + c) * 2) * 64 + lane];
+          u32x4_t one[2], w[2];
 #pragma unroll
-        for (int d = 0; d < DT; d += 2)
-          w[d / 2] = BF16 ? ActBF16::pack_rne(acc[d] * inv, acc[d + 1] * inv) : ActF16::pack_rne(acc[d] * inv, acc[d + 1] * inv);
-        uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h * a.G + row % a.G) * D + jd;
+          for (int x = 0; x < 2; ++x) {
+            w[x] = at[64 * x];
 #pragma unroll
-        for (int d = 0; d < DT / 2; d += 2) *reinterpret_cast<u32x2v_t*>(dst + 2 * d) = u32x2v_t{w[d], w[d + 1]};
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t q = w[x][e];
+              uint32_t z;
+              w[x][e] = drop_nan16(q, z);
+              one[x][e] = z;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            u32x4_t am[2];
+            attended(pos[i] + 1 - (k0 + 16 * g), am);
+            f32x4_t hit{0.0f, 0.0f, 0.0f, 0.0f};
+            hit = ActF16::mfma(one[0], am[0], hit);
+            hit = ActF16::mfma(one[1], am[1], hit);
+#pragma unroll
+            for (int cc = 0; cc < VD; ++cc) {
+              if (cc != c) continue;
+              o[i][cc] = ActF16::mfma(w[0], pf[i][0], o[i][cc]);
+              o[i][cc] = ActF16::mfma(w[1], pf[i][1], o[i][cc]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (hit[j] > 0.0f) o[i][cc][j] = __builtin_nanf("");
+            }
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < VD; ++c) {
+        const u32x4_t v0 = lv[buf][((n * VD + c) * 2) * 64 + lane], v1 = lv[buf][((n * VD + c) * 2 + 1) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          o[i][c] = ActF16::mfma(v0, pf[i][0], o[i][c]);
+          o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
+        }
+      }
+    }
+  }
+
+  // each wave has its rows whole: lane (g, r) holds dims 16 c + 4 g + j of row r
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    float ls = l[i];
+    ls += __shfl_xor(ls, 16, 64);
+    ls += __shfl_xor(ls, 32, 64);
+    const int row = wrow + 16 * i + r;
+    if (row < rows && row / a.G < sp.count) {
+#pragma unroll
+      for (int c = 0; c < VD; ++c) {
+        const float acc[4] = {o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]};
+        put_row<D, BF16, 4>(a, b, h, split, row, 16 * c + 4 * g, m[i], ls, acc);
       }
     }
   }
 }
 
-// Joins the nsplit parts of every (token, head) row: one wave per row.
+// Joins the nsplit (at most 64) parts of every (token, head) row: one wave per row, lane s holding part s's statistics.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, int64_t total) {
   constexpr int E = D / 64;
@@ -368,35 +642,52 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, i
   const int row = static_cast<int>(id % rows);
   const int64_t bh = id / rows;
   const int b = static_cast<int>(bh / a.Hkv), h = static_cast<int>(bh % a.Hkv);
-  const int t = row / a.G;
   const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
-  if (t >= count) return;
-  float M = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.pml[2 * ((bh * a.nsplit + s) * rows + row)]);
-  float sum = 0.0f, acc[E];
+  if (row / a.G >= count) return;
+  float ms = -INFINITY, ls = 0.0f;
+  if (lane < a.nsplit) {
+    const int64_t at = 2 * ((bh * a.nsplit + lane) * rows + row);
+    ms = a.pml[at];
+    ls = a.pml[at + 1];
+  }
+  float M = ms;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float wt = attn_chunk_weight(ms, M);
+  float sum = ls * wt, acc[E];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+  const float* src = a.po + (bh * a.nsplit * rows + row) * D + E * lane;
+  const int64_t next = static_cast<int64_t>(rows) * D;
+#pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) {
-    const int64_t at = (bh * a.nsplit + s) * rows + row;
-    const float wt = attn_chunk_weight(a.pml[2 * at], M);
-    sum = fmaf(a.pml[2 * at + 1], wt, sum);
-    const float* src = a.po + at * D + E * lane;
+    const float w = __shfl(wt, s, 64);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], wt, acc[e]);
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[s * next + e], w, acc[e]);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h * a.G + row % a.G) * D + E * lane;
+  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D + E * lane;
 #pragma unroll
   for (int e = 0; e < E; ++e) dst[e] = BF16 ? f32_to_bf16_bits(acc[e] * inv) : f32_to_f16_bits(acc[e] * inv);
 }
 
-// 16-row tiles of a workgroup, and the parts that its keys are cut into.
-inline int kv_attn_tiles(int64_t rows, int64_t hd) { return rows <= 16 ? 1 : (rows <= 32 || hd == 256) ? 2 : 4; }
-inline int kv_attn_splits(int64_t B, int64_t rows, int64_t Hkv, int64_t hd, int64_t keys) {
-  const int64_t groups = B * Hkv * ceil_div(rows, 16 * kv_attn_tiles(rows, hd));
-  const int64_t steps = ceil_div(keys, kStepKeys);
-  const int64_t want = ceil_div(512, groups);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(steps, kAttnWaves), 64})));
+// How a call is laid out: 16-row tiles of a workgroup of the direct kernel (0: the tile kernel), its tiles of rows, and
+// the parts that its keys are cut into.
+struct KvAttnPlan {
+  int R, tiles, splits;
+};
+inline KvAttnPlan kv_attn_plan(int64_t B, int64_t rows, int64_t Hkv, int64_t hd, int64_t keys) {
+  KvAttnPlan p;
+  p.R = rows > 64 ? 0 : rows <= 16 ? 1 : 2;
+  const int64_t span = p.R == 0 ? tile_rows(static_cast<int>(hd)) : 16 * p.R;
+  p.tiles = static_cast<int>(std::min<int64_t>(ceil_div(rows, span), 1 << 30));
+  const int64_t groups = B * Hkv * p.tiles, steps = ceil_div(keys, kStepKeys);
+  // two workgroups of the direct kernel a CU, one of the tile kernel; no further round for a few
+  const int64_t want = std::max<int64_t>(1, (p.R == 0 ? 256 : 512) / groups);
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(steps, kAttnWaves), 64})));
+  return p;
 }
 
 }  // namespace sqx
@@ -409,7 +700,7 @@ extern "C" int64_t sqx_kvblock_attention_workspace_bytes(int64_t B, int64_t T, i
       !kv_block_ok(block) || width <= 0)
     return 0;
   const int64_t rows = T * (H / Hkv);
-  const int ns = kv_attn_splits(B, rows, Hkv, hd, width * block);
+  const int ns = kv_attn_plan(B, rows, Hkv, hd, width * block).splits;
   return ns == 1 ? 0 : B * Hkv * ns * rows * (hd + 2) * 4;
 }
 
@@ -433,9 +724,9 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
               "%s: q, codes and out must be 16-byte aligned", fn);
   const int64_t G = H / Hkv, rows = T * G;
   SQX_REQUIRE(rows < (int64_t(1) << 28), SQX_E_ARG, "%s: %lld tokens of %lld heads per kv head", fn, (long long)T, (long long)G);
-  const int R = kv_attn_tiles(rows, hd);
-  const int64_t tiles = ceil_div(rows, 16 * R);
-  const int ns = kv_attn_splits(B, rows, Hkv, hd, width * block);
+  const KvAttnPlan plan = kv_attn_plan(B, rows, Hkv, hd, width * block);
+  const int64_t tiles = plan.tiles;
+  const int ns = plan.splits;
   const int64_t need = sqx_kvblock_attention_workspace_bytes(B, T, H, Hkv, hd, block, width);
   SQX_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need && al16(ws)), SQX_E_SPACE,
               "%s: %lld bytes of 16-byte aligned workspace needed, %lld given", fn, (long long)need, (long long)ws_bytes);
@@ -455,21 +746,20 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
   a.qscale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   const dim3 grid(static_cast<unsigned>(Hkv), static_cast<unsigned>(tiles * ns), static_cast<unsigned>(B));
   const hipStream_t s = as_stream(stream);
-  auto go = [&](auto dd, auto rr) {
-    constexpr int D = decltype(dd)::value, RR = decltype(rr)::value;
-    const bool bf = dtype == SQX_DTYPE_BF16;
-    if (fmt == SQX_KV_E4M3) {
-      if (bf) hipLaunchKernelGGL((kv_attn_kernel<D, RR, true, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((kv_attn_kernel<D, RR, true, false>), grid, dim3(256), 0, s, a);
-    } else {
-      if (bf) hipLaunchKernelGGL((kv_attn_kernel<D, RR, false, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((kv_attn_kernel<D, RR, false, false>), grid, dim3(256), 0, s, a);
-    }
-  };
   with_head(hd, [&](auto dd) {
-    if (R == 1) go(dd, std::integral_constant<int, 1>{});
-    else if (R == 2) go(dd, std::integral_constant<int, 2>{});
-    else if constexpr (decltype(dd)::value != 256) go(dd, std::integral_constant<int, 4>{});
+    constexpr int D = decltype(dd)::value;
+    auto go = [&](auto e4, auto bf) {
+      constexpr bool E = decltype(e4)::value, BF = decltype(bf)::value;
+      if (plan.R == 1) hipLaunchKernelGGL((kv_attn_kernel<D, 1, E, BF>), grid, dim3(256), 0, s, a);
+      else if (plan.R == 2) hipLaunchKernelGGL((kv_attn_kernel<D, 2, E, BF>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF>), grid, dim3(64 * tile_waves(D)), 0, s, a);
+    };
+    auto with_type = [&](auto e4) {
+      if (dtype == SQX_DTYPE_BF16) go(e4, std::true_type{});
+      else go(e4, std::false_type{});
+    };
+    if (fmt == SQX_KV_E4M3) with_type(std::true_type{});
+    else with_type(std::false_type{});
   });
   SQX_LAUNCH_CHECK(fn);
   if (ns > 1) {

@@ -11,8 +11,8 @@
 // dozen double operations (below), so a row is still bound by reading it once.
 //
 // Three launches (two at temperature 0): statistics of every slice of every row; the residual's sum of every slice of the
-// one row per sequence that needs it; the pick. The decision is a few operations on the slices' statistics, so the second
-// and third repeat it in every workgroup instead of waiting for one.
+// one row per sequence that needs it; the pick. The decision is a few operations on the slices' statistics, so every
+// workgroup of the second repeats it instead of waiting for one.
 #include <type_traits>
 
 #include "sqx_common.h"
@@ -35,6 +35,7 @@ struct VerifyArgs {
   double k;  // 64 log2(e) / temperature
   double* sums;  // [B, T + 1, S]
   double* rest;  // [B, S]
+  double* verdict;  // [B, 3]: accepted, then of the row behind them -maximum k and 1 / sum
   float* maxs;   // [B, T + 1, S]
   int* args;     // [B, T + 1, S], temperature 0
   int *n_acc, *tokens;
@@ -58,8 +59,26 @@ __device__ inline double exp2_64th(double y, const double* pow64) {
   const double w = pow64[n & 63];  // in [1, 2): the exponent n >> 6 is added to its bits
   return p * __hiloint2double(__double2hiint(w) + ((n & ~63) << 14), __double2loint(w));
 }
+static __device__ const double kPow64[64] = {  // 2^(i / 64)
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+};
 __device__ inline void fill_pow64(double* pow64) {
-  if (threadIdx.x < 64) pow64[threadIdx.x] = exp2(threadIdx.x / 64.0);
+  if (threadIdx.x < 64) pow64[threadIdx.x] = kPow64[threadIdx.x];
 }
 
 // Elements base .. base + 7 of a row of V as fp32; past the end `fill`.
@@ -284,6 +303,11 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
   __syncthreads();
   const int s = blockIdx.x, b = blockIdx.y;
   const Verdict v = judge<DT>(a, b, pdt, pow64);
+  if (s == 0 && threadIdx.x == 0) {
+    a.verdict[3 * b] = v.n;
+    a.verdict[3 * b + 1] = v.off;
+    a.verdict[3 * b + 2] = v.inv;
+  }
   if (v.n == v.count) return;  // nothing was rejected: the row's own statistics serve
   const int x = a.draft[static_cast<int64_t>(b) * a.T + v.n];
   double sum = 0.0;
@@ -310,7 +334,11 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a, in
   }
   __syncthreads();
   const int b = blockIdx.x;
-  const Verdict v = judge<DT>(a, b, pdt, pow64);
+  Verdict v;
+  v.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
+  v.n = static_cast<int>(a.verdict[3 * b]);
+  v.off = a.verdict[3 * b + 1];
+  v.inv = a.verdict[3 * b + 2];
   const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
   bool residual = v.n < v.count;
   auto slice_sum = [&](int s) -> double {
@@ -428,7 +456,7 @@ using namespace sqx;
 extern "C" int64_t sqx_verify_draft_workspace_bytes(int64_t B, int64_t T, int64_t V) {
   if (B <= 0 || T < 0 || V <= 0) return 0;
   const int64_t S = ceil_div(V, kSlice);
-  return B * (T + 1) * S * 16 + B * S * 8;
+  return B * (T + 1) * S * 16 + B * (S + 3) * 8;
 }
 
 extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int* counts, const void* probs,
@@ -459,7 +487,8 @@ extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft,
   const int64_t rows = B * (T + 1) * a.S;
   a.sums = static_cast<double*>(ws);
   a.rest = a.sums + rows;
-  a.maxs = reinterpret_cast<float*>(a.rest + B * a.S);
+  a.verdict = a.rest + B * a.S;
+  a.maxs = reinterpret_cast<float*>(a.verdict + 3 * B);
   a.args = reinterpret_cast<int*>(a.maxs + rows);
   a.n_acc = n_accepted; a.tokens = tokens;
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -476,7 +505,7 @@ extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft,
       return;
     }
     hipLaunchKernelGGL((verify_stats_kernel<DT, VEC, false>), all, dim3(256), 0, s, a);
-    if (T > 0) hipLaunchKernelGGL((verify_rest_kernel<DT, VEC>), one, dim3(256), 0, s, a, probs_dtype);
+    hipLaunchKernelGGL((verify_rest_kernel<DT, VEC>), one, dim3(256), 0, s, a, probs_dtype);
     hipLaunchKernelGGL((verify_pick_kernel<DT, VEC>), seqs, dim3(256), 0, s, a, probs_dtype);
   };
   auto with_vec = [&](auto dt) {

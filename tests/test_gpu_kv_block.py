@@ -313,7 +313,7 @@ def test_attention_over_scales_far_apart(kv, fmt):
     check_attention(kv, cache, fmt, q, table, [190], None)
 
 
-@pytest.mark.parametrize("t", [1, 9])
+@pytest.mark.parametrize("t", [1, 9, 40])
 def test_attention_long_and_strided(kv, t):
     """A context that is split over workgroups, queries as a strided view, a scale of the caller's."""
     block, d, hkv, h = 64, 64, 1, 4
