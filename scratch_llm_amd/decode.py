@@ -14,24 +14,32 @@ is ``w4a16_linear`` (int4_group.py:148-164). This module is that step on the lib
 A step allocates nothing: :class:`DecodeState` holds the cache and every buffer for one batch
 size, so :meth:`Int4DecodeLM.capture` can record the whole step in a HIP graph whose replays
 decode token after token (the pick of one replay is the input of the next).
+
+On the block-scaled 8-bit cache (``kv_dtype="int8_block"`` or ``"fp8_block"``,
+:mod:`scratch_llm_amd.quant.kv_block`) the model also takes several tokens a row: a chunk of a prompt
+(:meth:`Int4DecodeLM.extend`) and drafted tokens with their verification (:meth:`Int4DecodeLM.verify`).
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Callable
 
 import torch
 from torch import Tensor
 
-from scratch_llm_amd import _lib
+from scratch_llm_amd import _lib, speculative
 from scratch_llm_amd.quant import int4_group as i4
+from scratch_llm_amd.quant import kv_block
+from scratch_llm_amd.quant.fp8_weights import FP8_DTYPE
 
 __all__ = ["DecodeConfig", "DecodeState", "Int4DecodeLM", "LLAMA3_8B", "rope_tables"]
 
 # Batches of 2..64 rows run the linears through sqx_int4_skinny's shape choice (the GEMV or a
 # decode-regime kernel, K split into the state's workspace); larger batches run the prefill GEMM.
 _SKINNY_MAX_M = i4.GEMM_MIN_M - 1
+_BLOCK_KV = {"int8_block": torch.int8, "fp8_block": FP8_DTYPE}
 
 
 @dataclass(frozen=True)
@@ -95,26 +103,41 @@ class DecodeState:
     ``k``/``v``: ``[n_layers, B, Hkv, max_ctx, hd]``, bf16, or with ``kv_dtype="fp8"`` E4M3 codes (uint8)
     with fp32 per-(layer, kv head) scales ``k_scale``/``v_scale`` ``[n_layers, Hkv]`` (the per-head FP8
     cache of fp8_kv_per_head.py; set them with :meth:`set_kv_scales` before decoding, static after).
+    With ``kv_dtype="int8_block"`` or ``"fp8_block"`` it is the paged block-scaled cache of
+    :mod:`~scratch_llm_amd.quant.kv_block`: ``k`` ``[n_layers, pages, Hkv, kv_block, hd]`` and ``v``
+    ``[n_layers, pages, Hkv, hd, kv_block]`` int8 or E4M3 codes, ``k_scale``/``v_scale`` ``[n_layers, pages, Hkv]``, and
+    ``block_table`` int32 ``[B, ceil(max_ctx / kv_block)]``, at first row after row (a server may point it elsewhere).
+    Nothing is calibrated. Rows that are not active store nothing, and tokens past a row's table are not stored.
     ``lengths`` int32 ``[B]`` (valid positions before the next write); ``active`` uint8 ``[B]`` (rows that
     ``advance`` bumps); ``tokens`` int32 ``[B]``: the step's input ids, overwritten by its greedy picks;
     ``logits`` bf16 ``[B, vocab]``.
     """
 
-    def __init__(self, model: "Int4DecodeLM", batch: int, max_ctx: int, kv_dtype: str = "bf16") -> None:
+    def __init__(self, model: "Int4DecodeLM", batch: int, max_ctx: int, kv_dtype: str = "bf16", kv_block_size: int = 64) -> None:
         cfg, dev = model.cfg, model.device
         if batch < 1 or max_ctx < 1:
             raise ValueError("batch and max_ctx must be >= 1")
         if max_ctx > cfg.context_length:
             raise ValueError(f"max_ctx={max_ctx} exceeds context_length={cfg.context_length}")
-        if kv_dtype not in ("bf16", "fp8"):
-            raise ValueError(f"kv_dtype must be 'bf16' or 'fp8', got {kv_dtype!r}")
+        if kv_dtype not in ("bf16", "fp8", *_BLOCK_KV):
+            raise ValueError(f"kv_dtype must be 'bf16', 'fp8', 'int8_block' or 'fp8_block', got {kv_dtype!r}")
         self.batch, self.max_ctx, self.kv_dtype = batch, max_ctx, kv_dtype
         hkv, hd, d = cfg.n_kv_heads, cfg.head_dim, cfg.d_model
-        shape = (cfg.n_layers, batch, hkv, max_ctx, hd)
-        kvt = torch.bfloat16 if kv_dtype == "bf16" else torch.uint8
-        self.k = torch.zeros(shape, dtype=kvt, device=dev)
-        self.v = torch.zeros(shape, dtype=kvt, device=dev)
-        self.k_scale = self.v_scale = None
+        self.k_scale = self.v_scale = self.block_table = self.counts = None
+        self.block_kv = kv_dtype in _BLOCK_KV
+        if self.block_kv:
+            width = -(-max_ctx // kv_block_size)
+            layer = kv_block.new_kv_blocks(cfg.n_layers * batch * width, hkv, hd, block=kv_block_size, dtype=_BLOCK_KV[kv_dtype],
+                                           device=dev)
+            self.k, self.v, self.k_scale, self.v_scale = (t.view(cfg.n_layers, batch * width, *t.shape[1:]) for t in layer)
+            self.block_table = torch.arange(batch * width, dtype=torch.int32, device=dev).view(batch, width)
+            self.counts = torch.ones(batch, dtype=torch.int32, device=dev)  # tokens that a step stores: `active` as int32
+            self._kv = [(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]) for i in range(cfg.n_layers)]
+        else:
+            shape = (cfg.n_layers, batch, hkv, max_ctx, hd)
+            kvt = torch.bfloat16 if kv_dtype == "bf16" else torch.uint8
+            self.k = torch.zeros(shape, dtype=kvt, device=dev)
+            self.v = torch.zeros(shape, dtype=kvt, device=dev)
         if kv_dtype == "fp8":
             self.k_scale = torch.ones(cfg.n_layers, hkv, dtype=torch.float32, device=dev)
             self.v_scale = torch.ones(cfg.n_layers, hkv, dtype=torch.float32, device=dev)
@@ -131,13 +154,16 @@ class DecodeState:
         self.ss = torch.empty(batch, self.nss, dtype=torch.float32, device=dev)
         self.qkv = torch.empty(batch, (cfg.n_heads + 2 * hkv) * hd, **bf)
         self.q = torch.empty(batch, cfg.n_heads * hd, **bf)  # rotated q (one-row steps: the qkv epilogue's)
-        self.attn = torch.empty(batch, cfg.n_heads * hd, **bf)
+        self.attn = torch.zeros(batch, cfg.n_heads * hd, **bf)
         self.gu = torch.empty(batch, 2 * cfg.d_ff, **bf)
         self.act = torch.empty(batch, cfg.d_ff, **bf)
         self.logits = torch.empty(batch, cfg.vocab_size, **bf)
         lib = _lib.load()
         nb = max(int(lib.sqx_attn_workspace_bytes(batch, cfg.n_heads, hkv, max_ctx)),
                  int(lib.sqx_attn_partials_workspace_bytes(batch, cfg.n_heads, max_ctx)))
+        if self.block_kv:
+            nb = int(lib.sqx_kvblock_attention_workspace_bytes(batch, 1, cfg.n_heads, hkv, hd, kv_block_size,
+                                                               self.block_table.shape[1]))
         self.attn_ws = torch.empty(max(nb // 4, 4), dtype=torch.float32, device=dev)
         nb = int(lib.sqx_argmax_workspace_bytes(batch, cfg.vocab_size))
         self.argmax_ws = torch.empty(max(nb // 4, 4), dtype=torch.float32, device=dev)
@@ -161,10 +187,15 @@ class DecodeState:
 
     def write_kv(self, layer: int, k: Tensor, v: Tensor, start: int = 0) -> None:
         """Store a block ``[B, Hkv, T, hd]`` of keys and values at positions ``start..start+T`` of every slot
-        (a prefill's output): copied for a bf16 cache, quantized with the layer's scales for an fp8 one."""
+        (a prefill's output, keys rotated): copied for a bf16 cache, quantized with the layer's scales for an fp8 one,
+        block by block for a block-scaled one (whose blocks before ``start`` have to be written first)."""
         t = k.shape[2]
         if k.shape != v.shape or k.shape[0] != self.batch or start < 0 or start + t > self.max_ctx:
             raise ValueError(f"block {tuple(k.shape)} does not fit the cache at {start}")
+        if self.block_kv:
+            starts = torch.full((self.batch,), start, dtype=torch.int32, device=k.device)
+            kv_block.write_kv_blocks(k.transpose(1, 2), v.transpose(1, 2), *self.kv_layer(layer), self.block_table, starts)
+            return
         if self.kv_dtype == "bf16":
             self.k[layer, :, :, start:start + t].copy_(k)
             self.v[layer, :, :, start:start + t].copy_(v)
@@ -175,6 +206,12 @@ class DecodeState:
         vs = self.v_scale[layer].view(1, -1, 1, 1)
         self.k[layer, :, :, start:start + t].copy_(kv8.quantize_per_head(k, ks).view(torch.uint8))
         self.v[layer, :, :, start:start + t].copy_(kv8.quantize_per_head(v, vs).view(torch.uint8))
+
+    def kv_layer(self, layer: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+        """A layer of the block-scaled cache as the functions of :mod:`~scratch_llm_amd.quant.kv_block` take it."""
+        if not self.block_kv:
+            raise ValueError(f"a {self.kv_dtype} cache has no blocks")
+        return self._kv[layer]
 
     def set_lengths(self, lengths) -> None:
         """Set every slot's valid length (a host list or tensor), e.g. after filling the cache."""
@@ -190,6 +227,32 @@ class DecodeState:
         if t.device.type == "cpu" and (bool((t < 0).any()) or bool((t >= vocab_size).any())):
             raise IndexError(f"token id out of range [0, {vocab_size})")
         self.tokens.copy_(t.to(torch.int32))
+
+
+class _Rows:
+    """The buffers of one pass over ``rows`` token rows (those of a :class:`DecodeState` that do not depend on its cache),
+    allocated on the current stream by the pass itself."""
+
+    def __init__(self, model: "Int4DecodeLM", rows: int, head_only: bool = False) -> None:
+        cfg, lib = model.cfg, _lib.load()
+        bf = dict(dtype=torch.bfloat16, device=model.device)
+        d, hd = cfg.d_model, cfg.head_dim
+        self.batch = rows
+        self.h = torch.empty(rows, d, **bf)
+        used = [model.lm_head]
+        if not head_only:
+            used = model.linears()
+            self.x = [torch.empty(rows, d, **bf), torch.empty(rows, d, **bf)]
+            self.delta = torch.empty(rows, d, **bf)
+            self.qkv = torch.empty(rows, (cfg.n_heads + 2 * cfg.n_kv_heads) * hd, **bf)
+            self.q = torch.empty(rows, cfg.n_heads * hd, **bf)
+            self.attn = torch.zeros(rows, cfg.n_heads * hd, **bf)  # rows past their count are not written
+            self.gu = torch.empty(rows, 2 * cfg.d_ff, **bf)
+            self.act = torch.empty(rows, cfg.d_ff, **bf)
+        query = lib.sqx_int4_skinny_workspace_bytes if rows <= _SKINNY_MAX_M else lib.sqx_gemm_workspace_bytes
+        tail = (0,) if rows <= _SKINNY_MAX_M else ()
+        gw = max(int(query(rows, *shape, *tail)) for shape in {(tw.rows, tw.cols) for tw in used}) if rows > 1 else 0
+        self.gemm_ws = torch.empty(gw // 4, dtype=torch.float32, device=model.device) if gw > 0 else None
 
 
 class Int4DecodeLM:
@@ -312,8 +375,8 @@ class Int4DecodeLM:
             ly.attn_norm.numel() * 2 + ly.ffn_norm.numel() * 2 for ly in self.layers
         ) + self.final_norm.numel() * 2
 
-    def new_state(self, batch: int, max_ctx: int | None = None, kv_dtype: str = "bf16") -> DecodeState:
-        return DecodeState(self, batch, self.cfg.context_length if max_ctx is None else max_ctx, kv_dtype)
+    def new_state(self, batch: int, max_ctx: int | None = None, kv_dtype: str = "bf16", kv_block_size: int = 64) -> DecodeState:
+        return DecodeState(self, batch, self.cfg.context_length if max_ctx is None else max_ctx, kv_dtype, kv_block_size)
 
     # ------------------------------------------------------------------ the step
     def _linear(self, st: DecodeState, tw: i4.Int4Tiled, x: Tensor, y: Tensor, stream: int) -> None:
@@ -447,14 +510,16 @@ class Int4DecodeLM:
         # one row: the attention combine runs in the o projection's activation load (two 128-column
         # k-blocks per wave)
         kb_o = d // 128
-        merge = (self.fuse_attn_merge and sums and B == 1 and d % 256 == 0 and kb_o // 2 <= 16 and H * hd == d)
+        merge = (self.fuse_attn_merge and sums and B == 1 and not st.block_kv and d % 256 == 0 and kb_o // 2 <= 16 and H * hd == d)
         # a K-split q|k|v projection (the general step, B >= 48 at Llama-3-8B shapes) leaves its fp32
         # partials and the attention kernel adds them as the projection's reduce would (no reduce launch)
         qkv_split = 0
-        if not sums and self.fuse_qkv_parts and 2 <= B <= _SKINNY_MAX_M:
+        if not sums and self.fuse_qkv_parts and not st.block_kv and 2 <= B <= _SKINNY_MAX_M:
             S = lib.sqx_int4_skinny_default_splits(B, qkv_rows, d)
             qkv_split = S if S >= 2 else 0
         with torch.cuda.device(self.device):
+            if st.block_kv and go("attention"):
+                st.counts.copy_(st.active)  # the flags may change between replays of a captured step
             if go("other"):
                 ck(lib.sqx_embed(self.embed.data_ptr(), cfg.vocab_size, st.tokens.data_ptr(), B, d,
                                  st.x[0].data_ptr(), s), "embed")
@@ -483,6 +548,8 @@ class Int4DecodeLM:
                 # ---- attention over the cache
                 if not go("attention"):
                     pass
+                elif st.block_kv:
+                    self._block_attention(st, li, st.qkv, st.q, st.attn, B, 1, st.counts, st.attn_ws, s)
                 elif merge:  # the partials only; the o projection merges them
                     fp8 = st.kv_dtype == "fp8"
                     ck(lib.sqx_decode_attention_partials(
@@ -562,6 +629,112 @@ class Int4DecodeLM:
                                   st.argmax_ws.data_ptr(), st.argmax_ws.numel() * 4, s), "argmax")
                 ck(lib.sqx_advance(st.lengths.data_ptr(), st.active.data_ptr(), B, s), "advance")
         return st.tokens
+
+    def _block_attention(self, st: DecodeState, li: int, qkv: Tensor, q: Tensor, attn: Tensor, batch: int, t: int,
+                         counts: Tensor, ws: Tensor, stream: int) -> None:
+        """RoPE, the cache write and attention of ``t`` tokens a row over layer ``li`` of a block-scaled cache: ``qkv``
+        [batch * t, (H + 2 Hkv) hd] as the fused projection leaves it, ``q`` the rotated queries, ``attn`` the output (rows
+        past their count stay as they are)."""
+        cfg, lib = self.cfg, _lib.load()
+        H, Hkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        row = (H + 2 * Hkv) * hd
+        at = qkv.data_ptr()
+        k, v, ks, vs = st.kv_layer(li)
+        fmt = _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_E4M3
+        pages, _, block, _ = k.shape
+        width = st.block_table.shape[1]
+        cache = (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), st.block_table.data_ptr(), st.lengths.data_ptr(),
+                 counts.data_ptr(), batch, t, H, Hkv, hd, block, pages, width)
+        _lib.check(lib.sqx_kvblock_write(
+            at + 2 * H * hd, at + 2 * (H + Hkv) * hd, _lib.DTYPE_BF16, t * row, row, hd, t * row, row, hd, at, t * row, row, hd,
+            q.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), cfg.context_length, hd, 1, fmt, *cache, stream),
+            "rope + cache write")
+        _lib.check(lib.sqx_kvblock_attention(
+            q.data_ptr(), _lib.DTYPE_BF16, t * H * hd, H * hd, hd, fmt, *cache, 1.0 / math.sqrt(hd), attn.data_ptr(),
+            ws.data_ptr(), ws.numel() * 4, stream), "attention")
+
+    # ------------------------------------------------------------------ several tokens a row
+    @torch.no_grad()
+    def extend(self, st: DecodeState, tokens: Tensor, counts: Tensor | None = None, *, last_only: bool = False,
+               advance: bool = True) -> Tensor:
+        """Score ``tokens`` [B, T] (int32, on the device) of every row after its ``st.lengths`` tokens, on a block-scaled
+        cache: their keys and values are stored, and bf16 logits [B, T, vocab] come back; ``last_only``: [B, vocab] of each
+        row's last token. ``counts`` (int32 [B]; default T) is how many of a row's tokens are real; logits past them
+        mean nothing (for a count of 0 none do). Rows that are not active store nothing. ``advance`` adds the counts
+        of active rows to ``st.lengths``. Chunks of any size follow one another; T = 1 is a decode step without the
+        pick. Only device work is issued."""
+        cfg, lib = self.cfg, _lib.load()
+        if not st.block_kv:
+            raise ValueError(f"extend needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
+        if tokens.ndim != 2 or tokens.shape[0] != st.batch or tokens.shape[1] < 1 or tokens.dtype != torch.int32:
+            raise ValueError(f"tokens must be int32 [{st.batch}, T], got {tuple(tokens.shape)} of {tokens.dtype}")
+        if counts is not None and (tuple(counts.shape) != (st.batch,) or counts.dtype != torch.int32):
+            raise ValueError(f"counts must be int32 [{st.batch}], got {tuple(counts.shape)} of {counts.dtype}")
+        dev = _lib.require_device(tokens, counts, self.embed, fn="Int4DecodeLM.extend")
+        B, T = tokens.shape
+        d, H, Hkv, hd = cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        tokens = tokens.contiguous()
+        stored = torch.full((B,), T, dtype=torch.int32, device=dev) if counts is None else counts.clamp(0, T)
+        stored = stored * st.active
+        rows = _Rows(self, B * T)
+        nb = int(lib.sqx_kvblock_attention_workspace_bytes(B, T, H, Hkv, hd, st.k.shape[3], st.block_table.shape[1]))
+        ws = torch.empty(max(nb // 4, 4), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            s = _lib.stream_ptr(dev)
+            _lib.check(lib.sqx_embed(self.embed.data_ptr(), cfg.vocab_size, tokens.data_ptr(), B * T, d,
+                                     rows.x[0].data_ptr(), s), "embed")
+            cur, delta, dsplit = 0, None, 0
+            for li, ly in enumerate(self.layers):
+                cur = self._norm_linear(rows, cur, delta, ly.attn_norm, ly.wqkv, rows.qkv, s, dsplit)
+                self._block_attention(st, li, rows.qkv, rows.q, rows.attn, B, T, stored, ws, s)
+                delta, dsplit = self._delta_linear(rows, ly.wo, rows.attn, s)
+                cur = self._norm_linear(rows, cur, delta, ly.ffn_norm, ly.w13, rows.act, s, dsplit, swiglu=True)
+                delta, dsplit = self._delta_linear(rows, ly.w2, rows.act, s)
+            if last_only:
+                # the final norm of all rows (it also adds the last delta), then the head of each row's last token
+                self._final_norm(rows, cur, delta, dsplit, s)
+                at = torch.arange(B, device=dev) * T + (stored.long() - 1).clamp_min(0)
+                last = _Rows(self, B, head_only=True)
+                last.h.copy_(rows.h[at])
+                logits = torch.empty(B, cfg.vocab_size, dtype=torch.bfloat16, device=dev)
+                self._linear(last, self.lm_head, last.h, logits, s)
+            else:
+                logits = torch.empty(B, T, cfg.vocab_size, dtype=torch.bfloat16, device=dev)
+                self._norm_linear(rows, cur, delta, self.final_norm, self.lm_head, logits, s, dsplit)
+            if advance:
+                st.lengths.add_(stored)
+        return logits
+
+    def _final_norm(self, rows: "_Rows", cur: int, delta: int | None, splits: int, stream: int) -> None:
+        cfg, lib = self.cfg, _lib.load()
+        a = (self.final_norm.data_ptr(), cfg.norm_eps, rows.batch, cfg.d_model, rows.x[1 - cur].data_ptr(), rows.h.data_ptr(), stream)
+        if splits >= 2:
+            _lib.check(lib.sqx_rmsnorm_partials(rows.x[cur].data_ptr(), delta, splits, *a), "rmsnorm (partials)")
+        else:
+            _lib.check(lib.sqx_rmsnorm(rows.x[cur].data_ptr(), delta, *a), "rmsnorm")
+
+    @torch.no_grad()
+    def verify(self, st: DecodeState, draft: Tensor, u: Tensor | None, r: Tensor | None, *, draft_probs: Tensor | None = None,
+               counts: Tensor | None = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
+        """One step of speculative decoding: score ``st.tokens`` and the drafted tokens ``draft`` [B, T] behind them in one
+        pass, keep what :func:`scratch_llm_amd.speculative.verify_draft` accepts, and continue from there. Returns its
+        ``(n_accepted, tokens)``; ``st.lengths`` grows by the accepted tokens and one, and ``st.tokens`` becomes the token
+        that follows them (rows that are not active keep both, and give what the arguments say without meaning).
+        ``counts`` is how many drafts a row has (default T). What rejected drafts left in the cache lies behind the new
+        length and is written over; a block's scale that one of them raised stays raised until the block is begun anew."""
+        if draft.ndim != 2 or draft.shape[0] != st.batch or draft.dtype != torch.int32:
+            raise ValueError(f"draft must be int32 [{st.batch}, T], got {tuple(draft.shape)} of {draft.dtype}")
+        t = draft.shape[1]
+        if t > speculative.MAX_DRAFTS:
+            raise ValueError(f"{t} drafted tokens, at most {speculative.MAX_DRAFTS}")
+        logits = self.extend(st, torch.cat((st.tokens[:, None], draft), 1),
+                             None if counts is None else counts.clamp(0, t) + 1, advance=False)
+        n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)
+        live = st.active != 0
+        st.lengths.add_((n + 1) * st.active)
+        nxt = tokens.gather(1, n.long()[:, None])[:, 0]
+        st.tokens.copy_(torch.where(live, nxt, st.tokens))
+        return n, tokens
 
     def _delta_plan(self, st: DecodeState, tw: i4.Int4Tiled) -> tuple[int, int]:
         """What :meth:`_delta_linear` would return for ``tw``, without launching it."""
