@@ -65,51 +65,77 @@ __device__ inline u32x4_t codes8(uint32_t w0, uint32_t w1) {
 // Bytes of w that are E4M3 NaNs, as 0x80 in their place.
 __device__ inline uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// One 64-key step of the softmax for 16 query rows: lane (g, r) holds the raw scores of keys 16 g + 4 t + j of row r in
-// sc[t][j]; f and lvs bring them to u, ivs is 1 / vs. Updates m, l and O^T's columns, leaves p as the operand pf.
-template <int VD>
-__device__ inline void softmax_step(f32x4_t (&sc)[4], bool masked, int behind, float f, float lvs, float ivs, float& m,
-                                    float& l, f32x4_t (&o)[VD], u32x4_t (&pf)[2]) {
-  if (masked) {  // wave-uniform; keys of the lane from `behind` on are not attended
+// The maximum over the four lane groups, in all of them: two exchanges in registers.
+__device__ inline float groups_max(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t h0 = h[0], h1 = h[1];  // through scalars: hipcc's bit_cast of a vector element reads element 0
+  x = __builtin_elementwise_maximum(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+  u = __builtin_bit_cast(uint32_t, x);
+  const auto q = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t q0 = q[0], q1 = q[1];
+  return __builtin_elementwise_maximum(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
+}
+
+// One 64-key step of the softmax for R tiles of 16 query rows: lane (g, r) holds the raw scores of keys 16 g + 4 t + j of
+// row r in sc[.][t][j], of which those from behind[.] on are not attended (MASKED); f and lvs bring them to u, ivs is
+// 1 / vs. Updates m, l and O^T's columns, leaves p as the operands pf. A NaN score makes its row's l NaN: m takes no part.
+template <int R, int VD, bool MASKED>
+__device__ inline void softmax_step(f32x4_t (&sc)[R][4], const int (&behind)[R], const float (&f)[R], float lvs, float ivs,
+                                    float (&m)[R], float (&l)[R], f32x4_t (&o)[R][VD], u32x4_t (&pf)[R][2]) {
+  float mx[R];
+  bool grow = false;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[i][t][j] = 4 * t + j >= behind[i] ? -INFINITY : sc[i][t][j];
+    }
+    mx[i] = sc[i][0][0];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * t + j >= behind) sc[t][j] = -INFINITY;
+      for (int j = 0; j < 4; ++j) mx[i] = __builtin_elementwise_maximum(mx[i], sc[i][t][j]);
+    mx[i] = fmaf(mx[i], f[i], lvs);  // f > 0: the maximum of u
+    if constexpr (MASKED) mx[i] = behind[i] <= 0 ? -INFINITY : mx[i];  // a page that no key is attended on: any scale
+    mx[i] = groups_max(mx[i]);
+    grow = grow || mx[i] > m[i] + kPGrowth;
   }
-  float mx = sc[0][0];
+  if (__ballot(grow) != 0) {  // wave-uniform; also from -infinity
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < R; ++i) {
+      const float mn = fmaxf(m[i], mx[i]);  // not a NaN
+      const float al = m[i] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[i] - mn);
+      l[i] *= al;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, sc[t][j]);
-  mx = fmaf(mx, f, lvs);  // f > 0: the maximum of u
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  if (__ballot(mx > m + kPGrowth) != 0) {  // wave-uniform; also from -infinity
-    const float mn = fmaxf(m, mx);
-    const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    l *= al;
+      for (int c = 0; c < VD; ++c)
 #pragma unroll
-    for (int c = 0; c < VD; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[c][j] *= al;
-    m = mn;
-  }
-  const float base = lvs - (m == -INFINITY ? 0.0f : m) + kPOffset;
-  float p[16], sum = 0.0f;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      p[4 * t + j] = __builtin_amdgcn_exp2f(fmaf(sc[t][j], f, base));
-      if (masked) p[4 * t + j] = sc[t][j] == -INFINITY ? 0.0f : p[4 * t + j];  // whatever its page's scales are
-      sum += p[4 * t + j];
+        for (int j = 0; j < 4; ++j) o[i][c][j] *= al;
+      m[i] = mn;
     }
-  l = sum == 0.0f ? l : fmaf(sum, ivs, l);
+  }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    pf[t >> 1][2 * (t & 1)] = ActF16::pack_rne(p[4 * t], p[4 * t + 1]);
-    pf[t >> 1][2 * (t & 1) + 1] = ActF16::pack_rne(p[4 * t + 2], p[4 * t + 3]);
+  for (int i = 0; i < R; ++i) {
+    const float base = lvs - (m[i] == -INFINITY ? 0.0f : m[i]) + kPOffset;
+    float p[16], sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float& e = p[4 * t + j];
+        e = __builtin_amdgcn_exp2f(fmaf(sc[i][t][j], f[i], base));
+        if constexpr (MASKED) e = 4 * t + j >= behind[i] ? 0.0f : e;  // whatever its page's scales are
+        sum += e;
+      }
+    if constexpr (MASKED) l[i] = sum == 0.0f ? l[i] : fmaf(sum, ivs, l[i]);
+    else l[i] = fmaf(sum, ivs, l[i]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      pf[i][t >> 1][2 * (t & 1)] = ActF16::pack_rne(p[4 * t], p[4 * t + 1]);
+      pf[i][t >> 1][2 * (t & 1) + 1] = ActF16::pack_rne(p[4 * t + 2], p[4 * t + 3]);
+    }
   }
 }
 
@@ -303,9 +329,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
 
     const bool masked = k0 + kStepKeys - 1 > sp.first;  // wave-uniform
     u32x4_t pf[R][2];
+    int behind[R];
+    float f[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-      softmax_step<VD>(sc[i], masked, pos[i] + 1 - (k0 + 16 * g), qs[i] * kscale, lvs, ivs, m[i], l[i], o[i], pf[i]);
+    for (int i = 0; i < R; ++i) {
+      behind[i] = pos[i] + 1 - (k0 + 16 * g);
+      f[i] = qs[i] * kscale;
+    }
+    if (masked) softmax_step<R, VD, true>(sc, behind, f, lvs, ivs, m, l, o, pf);
+    else softmax_step<R, VD, false>(sc, behind, f, lvs, ivs, m, l, o, pf);
     // E4M3 values may be NaN where some row must not see them (a later token, a slot never written), and 0 NaN is NaN: in
     // masked steps NaN codes are taken out, and put back where a product of their indicator with that of the keys attended
     // is not zero (p itself may round to zero).
@@ -332,7 +364,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
 #pragma unroll
             for (int i = 0; i < R; ++i) {
               u32x4_t am[2];
-              attended(pos[i] + 1 - (k0 + 16 * g), am);
+              attended(behind[i], am);
               f32x4_t hit{0.0f, 0.0f, 0.0f, 0.0f};
               hit = ActF16::mfma(codes8<true>(one[0], one[1]), am[0], hit);
               hit = ActF16::mfma(codes8<true>(one[2], one[3]), am[1], hit);
@@ -392,6 +424,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
       put_row<D, BF16, DT>(a, b, h, split, row, jd, M, sum, acc);
     }
   }
+}
+
+// Orders a block of N operand reads from LDS, each used by R MFMAs: kLead reads ahead of the first use, then one per R
+// MFMAs. Left to itself the compiler waits for every read right before its use.
+template <int N, int R>
+__device__ inline void reads_ahead() {
+  constexpr int kLead = 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, kLead, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - kLead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, R, 0);  // MFMAs
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kLead * R, 0);
 }
 
 // f16 pairs with NaNs replaced by zero; `one` gets 1.0 in their place.
@@ -550,22 +596,31 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
       if (k0 > last) continue;  // wave-uniform: nothing here for its rows
       const bool masked = k0 + kStepKeys - 1 > first;
       f32x4_t sc[R][4];
+      const u32x4_t* const kt = &lk[buf][n * 4 * 2 * KD * 64 + lane];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int i = 0; i < R; ++i) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < 4; ++t) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < 2 * KD; ++k) {
-          const u32x4_t w = lk[buf][((n * 4 + t) * 2 * KD + k) * 64 + lane];
+      for (int k = 0; k < 2 * KD; ++k)  // 4 R chains of sums side by side
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4_t w = kt[(t * 2 * KD + k) * 64];
 #pragma unroll
           for (int i = 0; i < R; ++i) sc[i][t] = ActF16::mfma(w, qf[i][k], sc[i][t]);
         }
-      }
+      reads_ahead<8 * KD, R>();
       const float kscale = lf[buf][4 * n + g], lvs = lg[buf][4 * n + g], ivs = li[buf][4 * n + g];
       u32x4_t pf[R][2];
+      int behind[R];
+      float f[R];
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        softmax_step<VD>(sc[i], masked, pos[i] + 1 - (k0 + 16 * g), qs[i] * kscale, lvs, ivs, m[i], l[i], o[i], pf[i]);
+      for (int i = 0; i < R; ++i) {
+        behind[i] = pos[i] + 1 - (k0 + 16 * g);
+        f[i] = qs[i] * kscale;
+      }
+      if (masked) softmax_step<R, VD, true>(sc, behind, f, lvs, ivs, m, l, o, pf);
+      else softmax_step<R, VD, false>(sc, behind, f, lvs, ivs, m, l, o, pf);
       if (E4M3 && masked && lnan[step % 3] != 0) {  // as in the direct kernel
 #pragma unroll 1
         for (int c = 0; c < VD; ++c) {
@@ -585,7 +640,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
 #pragma unroll
           for (int i = 0; i < R; ++i) {
             u32x4_t am[2];
-            attended(pos[i] + 1 - (k0 + 16 * g), am);
+            attended(behind[i], am);
             f32x4_t hit{0.0f, 0.0f, 0.0f, 0.0f};
             hit = ActF16::mfma(one[0], am[0], hit);
             hit = ActF16::mfma(one[1], am[1], hit);
@@ -611,6 +666,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
           o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
         }
       }
+      reads_ahead<2 * VD, R>();
     }
   }
 
