@@ -146,26 +146,26 @@ __device__ inline void attended(int behind, u32x4_t (&am)[2]) {
     am[i >> 2][i & 3] = (2 * i < behind ? 0x3c00u : 0u) | (2 * i + 1 < behind ? 0x3c000000u : 0u);
 }
 
-// The 8 KD dims of query row `src` that a lane holds (64 i + 16 g + 8 half ..), as fp16, and the factor that brings a raw
-// score to u. bf16 rows are scaled by a power of two; the row's four lanes share it.
-template <int KD, bool BF16>
-__device__ inline float load_query(const uint16_t* src, bool ok, int g, float qscale, u32x4_t (&qf)[2 * KD]) {
+// The 8 N dims of query row `src` that a lane holds, 8 each from column `at(k)`, as fp16, and the factor that brings a raw
+// score to u. bf16 rows are scaled by a power of two; the lanes of a row, LANES apart, share it.
+template <int N, bool BF16, int LANES, typename F>
+__device__ inline float load_query_at(const uint16_t* src, bool ok, float qscale, u32x4_t (&qf)[N], const F& at) {
 #pragma unroll
-  for (int k = 0; k < 2 * KD; ++k) {
+  for (int k = 0; k < N; ++k) {
     qf[k] = u32x4_t{0u, 0u, 0u, 0u};
-    if (ok) qf[k] = *reinterpret_cast<const u32x4_t*>(src + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+    if (ok) qf[k] = *reinterpret_cast<const u32x4_t*>(src + at(k));
   }
   if constexpr (!BF16) return qscale;
   float most = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 2 * KD; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = qf[k][e];
       most = fmaxf(most, fmaxf(fabsf(bf16_lo(w)), fabsf(bf16_hi(w))));
     }
-  most = fmaxf(most, __shfl_xor(most, 16, 64));
-  most = fmaxf(most, __shfl_xor(most, 32, 64));
+#pragma unroll
+  for (int x = LANES; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x, 64));
   float up = 1.0f;
   if (most > 0.0f && most <= 3.402823466e38f) {
     int e;
@@ -173,13 +173,21 @@ __device__ inline float load_query(const uint16_t* src, bool ok, int g, float qs
     up = ldexpf(1.0f, 15 - max(e, -100));
   }
 #pragma unroll
-  for (int k = 0; k < 2 * KD; ++k)
+  for (int k = 0; k < N; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = qf[k][e];
       qf[k][e] = ActF16::pack_rne(bf16_lo(w) * up, bf16_hi(w) * up);
     }
   return qscale * (1.0f / up);
+}
+template <int KD, bool BF16>  // lane (g, r) of four groups: 64 i + 16 g + 8 half ..
+__device__ inline float load_query(const uint16_t* src, bool ok, int g, float qscale, u32x4_t (&qf)[2 * KD]) {
+  return load_query_at<2 * KD, BF16, 16>(src, ok, qscale, qf, [&](int k) { return 64 * (k >> 1) + 16 * g + 8 * (k & 1); });
+}
+template <int KD, bool BF16>  // lane (hi, r) of two: 32 i + 16 hi + 8 half ..
+__device__ inline float load_query32(const uint16_t* src, bool ok, int hi, float qscale, u32x4_t (&qf)[2 * KD]) {
+  return load_query_at<2 * KD, BF16, 32>(src, ok, qscale, qf, [&](int k) { return 32 * (k >> 1) + 16 * hi + 8 * (k & 1); });
 }
 
 // The rows and keys of a tile of `span` rows from row0: token `last` is its last one below the count, keys below `keys` are
@@ -426,18 +434,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
   }
 }
 
-// Orders a block of N operand reads from LDS, each used by R MFMAs: kLead reads ahead of the first use, then one per R
-// MFMAs. Left to itself the compiler waits for every read right before its use.
-template <int N, int R>
+typedef float f32x16_t __attribute__((__vector_size__(16 * sizeof(float))));
+
+__device__ inline f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Orders a block of N operand reads from LDS with an MFMA each: kLead reads ahead of the first use, then one per MFMA. Left
+// to itself the compiler waits for every read right before its use.
+template <int N>
 __device__ inline void reads_ahead() {
   constexpr int kLead = 4;
   __builtin_amdgcn_sched_group_barrier(0x100, kLead, 0);  // LDS reads
 #pragma unroll
   for (int i = 0; i < N - kLead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, R, 0);  // MFMAs
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMAs
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
   }
-  __builtin_amdgcn_sched_group_barrier(0x008, kLead * R, 0);
+  __builtin_amdgcn_sched_group_barrier(0x008, kLead, 0);
 }
 
 // f16 pairs with NaNs replaced by zero; `one` gets 1.0 in their place.
@@ -447,31 +461,95 @@ __device__ inline uint32_t drop_nan16(uint32_t w, uint32_t& one) {
   return w & ~(lo | hi);
 }
 
+// softmax_step for 32 query rows and N tiles of 32 keys: lane (hi, r), hi = lane / 32, holds the scores of the 16 keys
+// 32 t + 16 hi + e of row r in sc[t][e], attended below behind - 32 t. One m and l a lane.
+template <int N, int VD, bool MASKED>
+__device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, const float (&ks)[N], const float (&lvs)[N],
+                                      const float (&ivs)[N], float& m, float& l, f32x16_t (&o)[VD], u32x4_t (&pf)[N][2]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[t][e] = 32 * t + e >= behind ? -INFINITY : sc[t][e];
+    }
+    float mi = sc[t][0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mi = __builtin_elementwise_maximum(mi, sc[t][e]);
+    mi = fmaf(mi, qs * ks[t], lvs[t]);
+    if constexpr (MASKED) mi = behind <= 32 * t ? -INFINITY : mi;
+    mx = __builtin_elementwise_maximum(mx, mi);
+  }
+  {
+    const uint32_t u = __builtin_bit_cast(uint32_t, mx);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];
+    mx = __builtin_elementwise_maximum(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+  }
+  if (__ballot(mx > m + kPGrowth) != 0) {  // wave-uniform; also from -infinity
+    const float mn = fmaxf(m, mx);         // not a NaN
+    const float al = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= al;
+#pragma unroll
+    for (int c = 0; c < VD; ++c)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[c][e] *= al;
+    m = mn;
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    const float f = qs * ks[t], base = lvs[t] - (m == -INFINITY ? 0.0f : m) + kPOffset;
+    float p[16], sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(fmaf(sc[t][e], f, base));
+      if constexpr (MASKED) p[e] = 32 * t + e >= behind ? 0.0f : p[e];  // whatever its page's scales are
+      sum += p[e];
+    }
+    if constexpr (MASKED) l = sum == 0.0f ? l : fmaf(sum, ivs[t], l);
+    else l = fmaf(sum, ivs[t], l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pf[t][e >> 2][e & 3] = ActF16::pack_rne(p[2 * e], p[2 * e + 1]);
+  }
+}
+
 // For many rows (prompts), where the matrix and vector units are the bound: workgroup (h, s * tiles + tile, b) takes 256
 // rows, 32 in each of eight waves (heads of 256: 128 rows, four waves with twice the registers), and all waves work on
-// the same keys. A 64-key piece of the cache is read once, turned
-// to fp16 once (its conversion would cost a wave of its own two thirds of its softmax) and kept in LDS as the operands
-// that the lanes want, so writes and reads are consecutive. Two tiles in LDS and one in registers: while a tile is worked
-// on, the next is converted behind one barrier a tile and the one after it is on its way.
+// the same keys. A 64-key piece of the cache is read once, turned to fp16 once (its conversion would cost a wave of its
+// own two thirds of its softmax) and kept in LDS as the operands that the lanes want, so writes and reads are consecutive.
+// Two tiles in LDS and one in registers: while a tile is worked on, the next is converted behind one barrier a tile and the
+// one after it is on its way.
+//
+// The products are v_mfma_f32_32x32x16_f16, with the row order of the direct kernel carried over: row p of a 32-key tile is
+// key 16 ((p / 4) % 2) + 4 (p / 8) + p % 4, so that lane (hi, r) gets the scores of 16 hi .. 16 hi + 15.
+//
+// Bound by the vector and the matrix unit together: on this card two waves of a SIMD overlap little of them (an MFMA of 16
+// cycles hides two vector instructions; 16x16x32 with four vector instructions and an exponential takes 33.7 ns for two
+// waves where the parts take 16.3, 10.2 and 7.6, the 32x32x16 form 27.9). So vector instructions are what counts. Two groups
+// of waves half a tile apart (one in its products while the other is in its softmax), and products and softmax of
+// neighbouring tiles in one stream, took the same 290 us as this plain order.
+//
+// BIG: pages of 64 tokens or more, so a 64-key piece lies in one. Its page and scales are the same for all lanes and addresses
+// are scalar; the per-lane form costs 70 vector instructions a tile, a fifth of all.
 constexpr int tile_waves(int d) { return d == 256 ? 4 : 8; }
 constexpr int tile_rows(int d) { return 32 * tile_waves(d); }
-template <int D, bool E4M3, bool BF16>
+template <int D, bool E4M3, bool BF16, bool BIG>
 __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_tile_kernel(const KvAttnArgs a) {
   constexpr int kWaves = tile_waves(D), kTileRows = tile_rows(D);
-  constexpr int KD = D / 64, VD = D / 16, R = 2;
+  constexpr int KD = D / 32, VD = D / 32;        // 32-dim pieces of a key; of the output
   constexpr int NS = D == 64 ? 2 : 1;            // 64-key pieces of a tile
-  constexpr int U = 4 * KD * NS / kWaves;        // 16-byte units of keys, and of values, per thread
-  constexpr int kTileKeys = 64 * NS;
-  // operands of a tile: keys [piece][t][2 KD][lane], values [piece][c][2][lane], 16 bytes each
-  __shared__ u32x4_t lk[2][NS * 4 * 2 * KD * 64], lv[2][NS * VD * 2 * 64];
-  __shared__ float lf[2][NS * 4], lg[2][NS * 4], li[2][NS * 4];  // per 16 keys: key scale, log2 and inverse of the value scale
+  constexpr int U = 2 * KD * NS / kWaves;        // 16-byte units of keys, and of values, per thread
+  constexpr int kTileKeys = 64 * NS, NT = 2 * NS;  // 32-key tiles
+  // operands of a tile: keys [32-key tile][i][2][lane], values [32-key tile][c][2][lane], 16 bytes each
+  __shared__ u32x4_t lk[2][NT * KD * 2 * 64], lv[2][NT * VD * 2 * 64];
+  __shared__ float lf[2][2 * NT], lg[2][2 * NT], li[2][2 * NT];  // per 16 keys: key scale, log2 and inverse of the value scale
   __shared__ int lnan[3];  // tile i holds a NaN value: slot i % 3, cleared while tile i - 2 is worked on
   const int h = blockIdx.x, b = blockIdx.z;
   const int rows = a.T * a.G;
   const int tiles = (rows + kTileRows - 1) / kTileRows;
   const int tile = tiles - 1 - blockIdx.y % tiles, split = blockIdx.y / tiles;  // the longest first
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g = lane >> 4, r = lane & 15;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hi = lane >> 5, r = lane & 31;
   const int row0 = tile * kTileRows;
   KvSpan sp;
   if (!kv_span(a, b, row0, kTileRows, sp)) return;
@@ -480,38 +558,45 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / a.nsplit);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / a.nsplit);
 
-  // loads: unit u of a thread is key piece (t, i) and value tile c of its lane, as the direct kernel's lanes hold them
+  // loads: a thread's unit w is piece (t, i) of the keys and (t, c) of the values for its lane, t the 32-key tile
   const int64_t pstride = static_cast<int64_t>(a.Hkv) * a.block * D;
   const uint8_t* const kb = a.kc + static_cast<int64_t>(h) * a.block * D;
   const uint8_t* const vb = a.vc + static_cast<int64_t>(h) * a.block * D;
   const int* const trow = a.table + static_cast<int64_t>(b) * a.width;
-  const int gk = (lane >> 2) & 3;
-  constexpr int kWavesPerPiece = kWaves / NS;  // waves that load one 64-key piece
-  const int piece = wave / kWavesPerPiece, pw = wave % kWavesPerPiece;
+  constexpr int kWavesPerTile = kWaves / NT;  // waves that load one 32-key tile
+  const int lt = wave / kWavesPerTile, pw = wave % kWavesPerTile;
+  const int gk = (r >> 2) & 1;  // the 16-key half of the lane's key row; of its scores and values it is hi
   auto sane = [&](int p) { return p >= 0 && p < a.pages ? p : 0; };
-  auto page_of = [&](int key) { return trow[min(key, L - 1) >> a.shift]; };
+  // scalar loads: the table and the scales are constant while the kernel runs
+  auto constant = [](const auto* p) { return (const __attribute__((address_space(4))) std::decay_t<decltype(*p)>*)(uintptr_t)p; };
+  auto page_of = [&](int key) {
+    if constexpr (BIG) return constant(trow)[min(key, L - 1) >> a.shift];
+    else return trow[min(key, L - 1) >> a.shift];
+  };
   u32x4_t kreg[U], vreg[U];
   float ks = 0.0f, vs = 0.0f;
   int pk = 0, pv = 0;
+  const uint32_t klane = ((BIG ? 16 * gk : 0) + 4 * (r >> 3) + (r & 3)) * D + 16 * hi;
+  const uint32_t vlane = r * a.block + (BIG ? 16 * hi : 0);
   auto load_pages = [&](int step) {
-    const int k0 = step * kTileKeys + 64 * piece;
-    pk = page_of(k0 + 16 * gk);
-    pv = page_of(k0 + 16 * g);
+    const int k0 = step * kTileKeys + 32 * lt;
+    pk = page_of(k0 + (BIG ? 0 : 16 * gk));
+    pv = BIG ? pk : page_of(k0 + 16 * hi);
   };
-  auto load_tile = [&](int step) {
-    const int k0 = step * kTileKeys + 64 * piece;
-    const uint8_t* p = kb + sane(pk) * pstride + (((k0 + 16 * gk) & (a.block - 1)) + (lane & 3)) * D + 16 * g;
-    const uint8_t* q = vb + sane(pv) * pstride + r * a.block + ((k0 + 16 * g) & (a.block - 1));
+  auto load_tile = [&](int step) {  // past the end: the last page again, not used
+    const int k0 = step * kTileKeys + 32 * lt;
+    const uint8_t* p = kb + sane(pk) * pstride + ((k0 + (BIG ? 0 : 16 * gk)) & (a.block - 1)) * D;
+    const uint8_t* q = vb + sane(pv) * pstride + ((k0 + (BIG ? 0 : 16 * hi)) & (a.block - 1));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int w = pw + kWavesPerPiece * u;  // (t, i) of the keys, c of the values
-      kreg[u] = *reinterpret_cast<const u32x4_t*>(p + 4 * (w / KD) * D + 64 * (w % KD));
-      vreg[u] = *reinterpret_cast<const u32x4_t*>(q + 16 * w * a.block);
+      const int w = pw + kWavesPerTile * u;  // i of the keys, c of the values
+      kreg[u] = *reinterpret_cast<const u32x4_t*>(p + 32 * w + klane);
+      vreg[u] = *reinterpret_cast<const u32x4_t*>(q + 32 * w * a.block + vlane);
     }
     if (pw == 0) {
       const int64_t at = static_cast<int64_t>(sane(pv)) * a.Hkv + h;
-      ks = a.ks[at];
-      vs = a.vs[at];
+      ks = BIG ? constant(a.ks)[at] : a.ks[at];
+      vs = BIG ? constant(a.vs)[at] : a.vs[at];
       if (pv < 0 || pv >= a.pages) ks = __builtin_nanf("");
     }
   };
@@ -521,10 +606,10 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
     uint32_t bad = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int w = pw + kWavesPerPiece * u;
+      const int w = pw + kWavesPerTile * u;
       const u32x4_t k = kreg[u], v = vreg[u];
-      u32x4_t* dk = &lk[buf][((piece * 4 * KD + w) * 2) * 64 + lane];
-      u32x4_t* dv = &lv[buf][((piece * VD + w) * 2) * 64 + lane];
+      u32x4_t* dk = &lk[buf][((lt * KD + w) * 2) * 64 + lane];
+      u32x4_t* dv = &lv[buf][((lt * VD + w) * 2) * 64 + lane];
       dk[0] = codes8<E4M3>(k[0], k[1]);
       dk[64] = codes8<E4M3>(k[2], k[3]);
       dv[0] = codes8<E4M3>(v[0], v[1]);
@@ -533,157 +618,142 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
     }
     if (pw == 0 && r == 0) {
       const float vscale = scale_or_tiny(vs);
-      lf[buf][4 * piece + g] = scale_or_tiny(ks);
-      lg[buf][4 * piece + g] = __log2f(vscale);
-      li[buf][4 * piece + g] = 1.0f / vscale;
+      lf[buf][2 * lt + hi] = scale_or_tiny(ks);
+      lg[buf][2 * lt + hi] = __log2f(vscale);
+      li[buf][2 * lt + hi] = 1.0f / vscale;
     }
     if constexpr (E4M3) {
       if (bad != 0) lnan[slot] = 1;
     }
   };
 
-  u32x4_t qf[R][2 * KD];
-  float qs[R];
-  int pos[R];
-  f32x4_t o[R][VD];
-  float m[R], l[R];
-  const int wrow = row0 + 16 * R * wave;
-  int last = -1;  // the wave's last position
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int row = wrow + 16 * i + r;
-    const int t = row / a.G;
-    const bool ok = row < rows && t < sp.count;
-    pos[i] = ok ? sp.start + t : -1;
-    qs[i] = load_query<KD, BF16>(a.q + b * a.q_sb + (ok ? t * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, g, a.qscale, qf[i]);
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < VD; ++c) o[i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  {
-    const int end = min(min(wrow + 16 * R, rows), sp.count * a.G);  // rows of the wave below the count
-    if (end > wrow) last = sp.start + (end - 1) / a.G;
-  }
-  const int first = sp.start + wrow / a.G;
-
-  if (threadIdx.x < 3) lnan[threadIdx.x] = 0;
   if (s0 < s1) {
     load_pages(s0);
     load_tile(s0);
     load_pages(s0 + 1);
   }
-  __syncthreads();  // lnan is clear
+  u32x4_t qf[2 * KD];
+  const int wrow = row0 + 32 * wave, row = wrow + r, rt = row / a.G;
+  const bool ok = row < rows && rt < sp.count;
+  const int pos = ok ? sp.start + rt : -1;
+  const float qs = load_query32<KD, BF16>(a.q + b * a.q_sb + (ok ? rt * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, hi, a.qscale, qf);
+  float m = -INFINITY, l = 0.0f;
+  f32x16_t o[VD];
+#pragma unroll
+  for (int c = 0; c < VD; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
+  int last = -1;  // the wave's last position
+  {
+    const int end = min(min(wrow + 32, rows), sp.count * a.G);  // rows of the wave below the count
+    if (end > wrow) last = sp.start + (end - 1) / a.G;
+  }
+  const int first = sp.start + wrow / a.G;
+
+  if (threadIdx.x < 3) lnan[threadIdx.x] = 0;
+  __syncthreads();
   if (s0 < s1) {
     store_tile(s0);
-    load_tile(s0 + 1);  // past the end: the last page again, not used
+    load_tile(s0 + 1);
     load_pages(s0 + 2);
   }
-  for (int step = s0; step < s1; ++step) {
-    const int buf = step & 1;
-    __syncthreads();  // tile `step` is in LDS, the other buffer is free
+  auto work = [&](int step, auto masked) __attribute__((always_inline)) {
+    constexpr bool M = decltype(masked)::value;
+    const int buf = step & 1, k0 = step * kTileKeys;
+    f32x16_t sc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[t][e] = 0.0f;
+    const u32x4_t* const kt = &lk[buf][lane];
+#pragma unroll
+    for (int k = 0; k < 2 * KD; ++k)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sc[t] = mfma32(kt[(t * 2 * KD + k) * 64], qf[k], sc[t]);
+    reads_ahead<2 * KD * NT>();
+    float kscale[NT], lvs[NT], ivs[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      kscale[t] = lf[buf][2 * t + hi];
+      lvs[t] = lg[buf][2 * t + hi];
+      ivs[t] = li[buf][2 * t + hi];
+    }
+    u32x4_t pf[NT][2];
+    const int behind = pos + 1 - (k0 + 16 * hi);
+    softmax_step32<NT, VD, M>(sc, behind, qs, kscale, lvs, ivs, m, l, o, pf);
+    const u32x4_t* const vt = &lv[buf][lane];
+    if (E4M3 && M && lnan[step % 3] != 0) {  // as in the direct kernel
+#pragma unroll
+      for (int c = 0; c < VD; ++c)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          u32x4_t one[2], w[2], am[2];
+          attended(behind - 32 * t, am);
+          f32x16_t hit;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) hit[e] = 0.0f;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            w[y] = vt[((t * VD + c) * 2 + y) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t q = w[y][e];
+              uint32_t z;
+              w[y][e] = drop_nan16(q, z);
+              one[y][e] = z;
+            }
+            hit = mfma32(one[y], am[y], hit);
+            o[c] = mfma32(w[y], pf[t][y], o[c]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (hit[e] > 0.0f) o[c][e] = __builtin_nanf("");
+        }
+      return;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int c = 0; c < VD; ++c) o[c] = mfma32(vt[((t * VD + c) * 2 + y) * 64], pf[t][y], o[c]);
+    reads_ahead<2 * VD * NT>();
+  };
+  // tile `step` is in LDS behind this, the other buffer is free and takes the next one
+  auto next = [&](int step) __attribute__((always_inline)) {
+    __syncthreads();
     if constexpr (E4M3) {
       if (threadIdx.x == 0) lnan[(step + 2) % 3] = 0;  // read by nobody since this barrier, set after the next
     }
-    if (step + 1 < s1) {
-      store_tile(step + 1);
-      load_tile(step + 2);
-      load_pages(step + 3);
-    }
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const int k0 = step * kTileKeys + 64 * n;
-      if (k0 > last) continue;  // wave-uniform: nothing here for its rows
-      const bool masked = k0 + kStepKeys - 1 > first;
-      f32x4_t sc[R][4];
-      const u32x4_t* const kt = &lk[buf][n * 4 * 2 * KD * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) sc[i][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < 2 * KD; ++k)  // 4 R chains of sums side by side
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const u32x4_t w = kt[(t * 2 * KD + k) * 64];
-#pragma unroll
-          for (int i = 0; i < R; ++i) sc[i][t] = ActF16::mfma(w, qf[i][k], sc[i][t]);
-        }
-      reads_ahead<8 * KD, R>();
-      const float kscale = lf[buf][4 * n + g], lvs = lg[buf][4 * n + g], ivs = li[buf][4 * n + g];
-      u32x4_t pf[R][2];
-      int behind[R];
-      float f[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        behind[i] = pos[i] + 1 - (k0 + 16 * g);
-        f[i] = qs[i] * kscale;
-      }
-      if (masked) softmax_step<R, VD, true>(sc, behind, f, lvs, ivs, m, l, o, pf);
-      else softmax_step<R, VD, false>(sc, behind, f, lvs, ivs, m, l, o, pf);
-      if (E4M3 && masked && lnan[step % 3] != 0) {  // as in the direct kernel
-#pragma unroll 1
-        for (int c = 0; c < VD; ++c) {
-          u32x4_t* const at = &lv[buf][((n * VD + c) * 2) * 64 + lane];
-          u32x4_t one[2], w[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            w[x] = at[64 * x];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t q = w[x][e];
-              uint32_t z;
-              w[x][e] = drop_nan16(q, z);
-              one[x][e] = z;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-            u32x4_t am[2];
-            attended(behind[i], am);
-            f32x4_t hit{0.0f, 0.0f, 0.0f, 0.0f};
-            hit = ActF16::mfma(one[0], am[0], hit);
-            hit = ActF16::mfma(one[1], am[1], hit);
-#pragma unroll
-            for (int cc = 0; cc < VD; ++cc) {
-              if (cc != c) continue;
-              o[i][cc] = ActF16::mfma(w[0], pf[i][0], o[i][cc]);
-              o[i][cc] = ActF16::mfma(w[1], pf[i][1], o[i][cc]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (hit[j] > 0.0f) o[i][cc][j] = __builtin_nanf("");
-            }
-          }
-        }
-        continue;
-      }
-#pragma unroll
-      for (int c = 0; c < VD; ++c) {
-        const u32x4_t v0 = lv[buf][((n * VD + c) * 2) * 64 + lane], v1 = lv[buf][((n * VD + c) * 2 + 1) * 64 + lane];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          o[i][c] = ActF16::mfma(v0, pf[i][0], o[i][c]);
-          o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
-        }
-      }
-      reads_ahead<2 * VD, R>();
-    }
+    store_tile(step + 1);  // past the end: not used
+    load_tile(step + 2);
+    load_pages(step + 3);
+  };
+  // tiles that every row of the wave attends whole, tiles that some row does not, tiles past its last position
+  const int whole = min(max((first + 1) / kTileKeys, s0), s1);
+  const int some = max(whole, last < 0 ? s0 : min(max(last / kTileKeys + 1, s0), s1));
+  int step = s0;
+  for (; step < whole; ++step) {
+    next(step);
+    work(step, std::false_type{});
   }
+  for (; step < some; ++step) {
+    next(step);
+    work(step, std::true_type{});
+  }
+  for (; step < s1; ++step) next(step);
 
-  // each wave has its rows whole: lane (g, r) holds dims 16 c + 4 g + j of row r
+  // each wave has its rows whole: lane (hi, r) holds dims 32 c + 8 e + 4 hi + j of row r
+  float ls = l;
+  ls += __shfl_xor(ls, 32, 64);
+  if (ok) {
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    float ls = l[i];
-    ls += __shfl_xor(ls, 16, 64);
-    ls += __shfl_xor(ls, 32, 64);
-    const int row = wrow + 16 * i + r;
-    if (row < rows && row / a.G < sp.count) {
+    for (int c = 0; c < VD; ++c)
 #pragma unroll
-      for (int c = 0; c < VD; ++c) {
-        const float acc[4] = {o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]};
-        put_row<D, BF16, 4>(a, b, h, split, row, 16 * c + 4 * g, m[i], ls, acc);
+      for (int e = 0; e < 4; ++e) {
+        const float acc[4] = {o[c][4 * e], o[c][4 * e + 1], o[c][4 * e + 2], o[c][4 * e + 3]};
+        put_row<D, BF16, 4>(a, b, h, split, row, 32 * c + 8 * e + 4 * hi, m, ls, acc);
       }
-    }
   }
 }
 
@@ -808,7 +878,8 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
       constexpr bool E = decltype(e4)::value, BF = decltype(bf)::value;
       if (plan.R == 1) hipLaunchKernelGGL((kv_attn_kernel<D, 1, E, BF>), grid, dim3(256), 0, s, a);
       else if (plan.R == 2) hipLaunchKernelGGL((kv_attn_kernel<D, 2, E, BF>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF>), grid, dim3(64 * tile_waves(D)), 0, s, a);
+      else if (block >= kStepKeys) hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF, true>), grid, dim3(64 * tile_waves(D)), 0, s, a);
+      else hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF, false>), grid, dim3(64 * tile_waves(D)), 0, s, a);
     };
     auto with_type = [&](auto e4) {
       if (dtype == SQX_DTYPE_BF16) go(e4, std::true_type{});

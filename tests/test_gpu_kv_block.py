@@ -238,6 +238,10 @@ ATTENDS = [
     (1, 100, 6, 2, 64, 128, [0], None),
     (2, 70, 4, 1, 128, 16, [130, 0], [70, 1]),
     (1, 40, 2, 1, 256, 64, [50], None),
+    (2, 70, 8, 2, 64, 64, [186, 100], [70, 66]),
+    (1, 130, 4, 1, 64, 32, [700], None),
+    (1, 80, 4, 2, 256, 128, [600], None),
+    (1, 90, 4, 1, 128, 128, [1500], None),
 ]
 
 
