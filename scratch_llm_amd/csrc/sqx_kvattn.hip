@@ -127,15 +127,12 @@ __device__ inline void softmax_step(f32x4_t (&sc)[R][4], const int (&behind)[R],
         float& e = p[4 * t + j];
         e = __builtin_amdgcn_exp2f(fmaf(sc[i][t][j], f[i], base));
         if constexpr (MASKED) e = 4 * t + j >= behind[i] ? 0.0f : e;  // whatever its page's scales are
-        sum += e;
+        sum += e;  // in fp32, not of the rounded p: a p too small for fp16 may be a large p / vs
       }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pf[i][e >> 2][e & 3] = ActF16::pack_rne(p[2 * e], p[2 * e + 1]);
     if constexpr (MASKED) l[i] = sum == 0.0f ? l[i] : fmaf(sum, ivs, l[i]);
     else l[i] = fmaf(sum, ivs, l[i]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      pf[i][t >> 1][2 * (t & 1)] = ActF16::pack_rne(p[4 * t], p[4 * t + 1]);
-      pf[i][t >> 1][2 * (t & 1) + 1] = ActF16::pack_rne(p[4 * t + 2], p[4 * t + 3]);
-    }
   }
 }
 
@@ -304,7 +301,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
     for (int c = 0; c < VD; ++c) o[i][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  for (; step < s1; step += kAttnWaves) {
+  auto work = [&](auto is_masked) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(is_masked)::value;
     const int k0 = step * kStepKeys;
     {
       const uint8_t* p = vb + sane(pv) * pstride + r * a.block + ((k0 + 16 * g) & (a.block - 1));
@@ -335,7 +333,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
     pk2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * gk);
     pv2 = page_of(k0 + 2 * kAttnWaves * kStepKeys + 16 * g);
 
-    const bool masked = k0 + kStepKeys - 1 > sp.first;  // wave-uniform
     u32x4_t pf[R][2];
     int behind[R];
     float f[R];
@@ -344,13 +341,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
       behind[i] = pos[i] + 1 - (k0 + 16 * g);
       f[i] = qs[i] * kscale;
     }
-    if (masked) softmax_step<R, VD, true>(sc, behind, f, lvs, ivs, m, l, o, pf);
-    else softmax_step<R, VD, false>(sc, behind, f, lvs, ivs, m, l, o, pf);
+    softmax_step<R, VD, masked>(sc, behind, f, lvs, ivs, m, l, o, pf);
     // E4M3 values may be NaN where some row must not see them (a later token, a slot never written), and 0 NaN is NaN: in
     // masked steps NaN codes are taken out, and put back where a product of their indicator with that of the keys attended
     // is not zero (p itself may round to zero).
-    if constexpr (E4M3) {
-      if (masked) {
+    if constexpr (E4M3 && masked) {
+      {
         uint32_t bad = 0;
 #pragma unroll
         for (int c = 0; c < VD; ++c)
@@ -394,7 +390,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
         o[i][c] = ActF16::mfma(v1, pf[i][1], o[i][c]);
       }
     }
-  }
+  };
+  // steps whose keys every row attends, then those that some row does not
+  const int whole = min(max((sp.first + 1) / kStepKeys, 0), s1);
+  for (; step < whole; step += kAttnWaves) work(std::false_type{});
+  for (; step < s1; step += kAttnWaves) work(std::true_type{});
 
   // the waves' parts join through LDS, one 16-row tile at a time
   __shared__ float sm[kAttnWaves][16], sl[kAttnWaves][16];
@@ -506,10 +506,10 @@ __device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, c
       if constexpr (MASKED) p[e] = 32 * t + e >= behind ? 0.0f : p[e];  // whatever its page's scales are
       sum += p[e];
     }
-    if constexpr (MASKED) l = sum == 0.0f ? l : fmaf(sum, ivs[t], l);
-    else l = fmaf(sum, ivs[t], l);
 #pragma unroll
     for (int e = 0; e < 8; ++e) pf[t][e >> 2][e & 3] = ActF16::pack_rne(p[2 * e], p[2 * e + 1]);
+    if constexpr (MASKED) l = sum == 0.0f ? l : fmaf(sum, ivs[t], l);
+    else l = fmaf(sum, ivs[t], l);
   }
 }
 
