@@ -351,23 +351,23 @@ def require_device(*tensors: torch.Tensor | None, fn: str) -> torch.device:
 def device_index(fn: str, *tensors: torch.Tensor | None) -> int:
     """The index of the one ROCm device that all tensors live on; raises as :func:`require_device` does. Costs a sixth
     of it (0.1 us a tensor), for entry points of a dozen tensors whose kernels take a few microseconds."""
-    index = -1
+    index = None
     for t in tensors:
         if t is None:
             continue
         i = t.get_device()  # -1 for a CPU tensor
-        if i != index:
-            if i < 0 or index >= 0:
-                require_device(*tensors, fn=fn)
-            index = i
-    if index < 0:
-        require_device(*tensors, fn=fn)
+        if i < 0 or (index is not None and i != index):
+            require_device(*tensors, fn=fn)  # raises, and says what is where
+            raise RuntimeError(f"{fn}: tensors on different devices")
+        index = i
+    if index is None:
+        raise RuntimeError(f"{fn}: no tensor argument")
     return index
 
 
 def launch(index: int, what: str, entry, *args) -> None:
     """Call a C entry point with ``args`` and the current stream of device ``index``, made current if it is not."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

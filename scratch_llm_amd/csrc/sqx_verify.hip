@@ -322,95 +322,90 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
   if (threadIdx.x == 0) a.rest[static_cast<int64_t>(b) * a.S + s] = sum;
 }
 
-// The pick: the slice in which the cumulative sum passes the threshold, then the element in it.
+// The pick, by one workgroup of a thread per eight elements of a slice: the slice in which the cumulative sum passes the
+// threshold (every wave finds it from the slices' sums, a lane each), then the element in it.
+constexpr int kPickThreads = kSlice / kPer, kPickWaves = kPickThreads / 64;
 template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void verify_pick_kernel(const VerifyArgs a, int pdt) {
-  __shared__ double pow64[64], wsum[kPasses][4], part[256], red[4];
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a, int pdt) {
+  __shared__ double pow64[64], wsum[kPickWaves];
   __shared__ int found, last;
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   fill_pow64(pow64);
   if (threadIdx.x == 0) {
     found = 0x7fffffff;
     last = -1;
   }
-  __syncthreads();
-  const int b = blockIdx.x;
+  const double rest0 = lane < a.S ? a.rest[static_cast<int64_t>(b) * a.S + lane] : 0.0;  // on its way beside the verdict
   Verdict v;
   v.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   v.n = static_cast<int>(a.verdict[3 * b]);
   v.off = a.verdict[3 * b + 1];
   v.inv = a.verdict[3 * b + 2];
   const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
+  const double r = static_cast<double>(a.r[b]);
+  const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
+  __syncthreads();
   bool residual = v.n < v.count;
   auto slice_sum = [&](int s) -> double {
-    if (residual) return a.rest[static_cast<int64_t>(b) * a.S + s];
+    if (s >= a.S) return 0.0;
+    if (residual) return s < 64 ? rest0 : a.rest[static_cast<int64_t>(b) * a.S + s];
     return prob(a.maxs[row * a.S + s], v.off, a.k, v.inv, pow64) * a.sums[row * a.S + s];
   };
-  double total = 0.0;
-  if (residual) {
+  auto sum_all = [&]() {
     double mine = 0.0;
-    for (int s = threadIdx.x; s < a.S; s += 256) mine += slice_sum(s);
-    total = block_sum_f64(mine, red);
-    residual = !(total <= 0.0);  // p nowhere above q: drawn from p (a NaN goes on as one)
-  }
-  if (!residual) {
-    double mine = 0.0;
-    for (int s = threadIdx.x; s < a.S; s += 256) mine += slice_sum(s);
-    total = block_sum_f64(mine, red);
+    for (int s = lane; s < a.S; s += 64) mine += slice_sum(s);
+    return wave_sum_f64(mine);
+  };
+  auto scan = [&](double w) {  // inclusive, over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(w, o, 64);
+      if (lane >= o) w += u;
+    }
+    return w;
+  };
+  double total = sum_all();
+  if (residual && total <= 0.0) {  // p nowhere above q: drawn from p (a NaN goes on as one)
+    residual = false;
+    total = sum_all();
   }
   if (total > 0.0) {  // false for a row without a distribution
-    const double theta = static_cast<double>(a.r[b]) * total;
+    const double theta = r * total;
     int hit = -1, fallback = 0;
-    double before = 0.0, sum = 0.0;
-    for (int s0 = 0; s0 < a.S && hit < 0; s0 += 256) {
-      if (s0 + static_cast<int>(threadIdx.x) < a.S) part[threadIdx.x] = slice_sum(s0 + threadIdx.x);
-      __syncthreads();
-      for (int s = s0; s < min(a.S, s0 + 256); ++s) {
-        const double w = part[s - s0];
-        if (w > 0.0) fallback = s;
-        if (hit < 0 && sum + w > theta) {
-          hit = s;
-          before = sum;
-        }
-        sum += w;
+    double before = 0.0;
+    for (int s0 = 0; s0 < a.S && hit < 0; s0 += 64) {
+      const double w = slice_sum(s0 + lane), cum = before + scan(w);
+      const uint64_t over = __ballot(w > 0.0 && cum > theta), some = __ballot(w > 0.0);
+      if (some != 0) fallback = s0 + 63 - __builtin_clzll(some);
+      if (over != 0) {
+        const int first = __builtin_ctzll(over);
+        hit = s0 + first;
+        before = __shfl(cum - w, first, 64);
+      } else {
+        before = __shfl(cum, 63, 64);
       }
-      __syncthreads();
     }
     const bool none = hit < 0;  // r next to 1 and a rounding: the last token that has a weight
     if (none) hit = fallback;
-    const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
-    double w[kPasses][kPer], mine[kPasses], inc[kPasses];
+    const int at = hit * kSlice + threadIdx.x * kPer;
+    double w[kPer], mine = 0.0;
+    weights8<DT, VEC>(a, v, b, at, pdt, residual, x, pow64, w);
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      weights8<DT, VEC>(a, v, b, hit * kSlice + p * kPass + threadIdx.x * kPer, pdt, residual, x, pow64, w[p]);
-      mine[p] = 0.0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) mine[p] += w[p][e];
-      inc[p] = mine[p];  // inclusive scan over the wave, then over the waves
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(inc[p], o, 64);
-        if ((threadIdx.x & 63) >= o) inc[p] += u;
-      }
-      if ((threadIdx.x & 63) == 63) wsum[p][threadIdx.x >> 6] = inc[p];
-    }
+    for (int e = 0; e < kPer; ++e) mine += w[e];
+    const double inc = scan(mine);
+    if (lane == 63) wsum[wave] = inc;
     __syncthreads();
-    double c0 = before;
+    double c = before;
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i)
+      if (i < wave) c += wsum[i];
+    c += inc - mine;
     int first = 0x7fffffff, end = -1;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      double c = c0;
-      for (int i = 0; i < 4; ++i) {
-        if (i < static_cast<int>(threadIdx.x >> 6)) c += wsum[p][i];
-        c0 += wsum[p][i];
-      }
-      c += inc[p] - mine[p];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int at = hit * kSlice + p * kPass + threadIdx.x * kPer + e;
-        c += w[p][e];
-        if (w[p][e] > 0.0) end = at;
-        if (first == 0x7fffffff && w[p][e] > 0.0 && c > theta) first = at;
-      }
+    for (int e = 0; e < kPer; ++e) {
+      c += w[e];
+      if (w[e] > 0.0) end = at + e;
+      if (first == 0x7fffffff && w[e] > 0.0 && c > theta) first = at + e;
     }
     if (!none && first != 0x7fffffff) atomicMin(&found, first);  // of whole numbers: their order changes nothing
     if (end >= 0) atomicMax(&last, end);
@@ -506,7 +501,7 @@ extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft,
     }
     hipLaunchKernelGGL((verify_stats_kernel<DT, VEC, false>), all, dim3(256), 0, s, a);
     hipLaunchKernelGGL((verify_rest_kernel<DT, VEC>), one, dim3(256), 0, s, a, probs_dtype);
-    hipLaunchKernelGGL((verify_pick_kernel<DT, VEC>), seqs, dim3(256), 0, s, a, probs_dtype);
+    hipLaunchKernelGGL((verify_pick_kernel<DT, VEC>), seqs, dim3(kPickThreads), 0, s, a, probs_dtype);
   };
   auto with_vec = [&](auto dt) {
     if (vec) go(dt, std::true_type{});

@@ -144,7 +144,7 @@ def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_sc
     if q is not None:
         heads = q.shape[2]
         q, q_sb, q_st, q_sh = _rows(q)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty(b, t, heads, d, dtype=q.dtype, device=q.device)
         qp, qo = q.data_ptr(), q_out.data_ptr()
     _lib.launch(index, fn, _lib.load().sqx_kvblock_write, k.data_ptr(), v.data_ptr(), dt, k_sb, k_st, k_sh, v_sb, v_st, v_sh,
                 qp, q_sb, q_st, q_sh, qo, cp, sp, rope_rows, rot, interleaved, fmt, k_codes.data_ptr(), v_codes.data_ptr(),

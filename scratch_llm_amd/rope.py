@@ -137,7 +137,7 @@ def apply_rope(x: Tensor, positions: Tensor, cos: Tensor, sin: Tensor, *, interl
     if not positions.is_contiguous():
         positions = positions.contiguous()
     if out is None:
-        out = to = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = to = torch.empty(*shape, dtype=x.dtype, device=x.device)
         on, oh = heads * d, d
     else:
         if out.shape != shape or out.dtype != x.dtype or out.stride(-1) != 1:

@@ -404,3 +404,26 @@ def test_empty_calls(kv):
     assert kv.read_kv_blocks(*dev, i32([[0, 1]]), i32([0]), 0)[0].shape == (1, 0, 1, 64)
     z = torch.empty(1, 0, 1, 64, dtype=torch.bfloat16, device=DEV)
     assert kv.attend_kv_blocks(z, *dev, i32([[0, 1]]), i32([0])).shape == (1, 0, 1, 64)
+
+
+def test_a_cpu_tensor_among_device_tensors_is_refused(kv):
+    """Each tensor argument in turn on the CPU: an error before any launch."""
+    from scratch_llm_amd import rope, speculative
+
+    c = list(kv.new_kv_blocks(2, 1, 64, block=16, device=DEV))
+    x = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    cos, sin = rope.rope_table(64, 8, device=DEV)
+    tb, st = i32([[0, 1]]), i32([0])
+    lo, dr, u, r = torch.zeros(1, 2, 8, device=DEV), i32([[1]]), torch.zeros(1, 1, device=DEV), torch.zeros(1, device=DEV)
+    calls = [
+        (lambda *a: kv.write_kv_blocks(*a[:9], q=a[9], rope=(a[10], a[11])), [x, x, *c, tb, st, i32([1]), x, cos, sin]),
+        (lambda *a: kv.read_kv_blocks(*a[:6], 1, a[6]), [*c, tb, st, i32([1])]),
+        (lambda *a: kv.attend_kv_blocks(*a[:8], out=a[8]), [x, *c, tb, st, i32([1]), torch.zeros_like(x)]),
+        (lambda *a: rope.apply_rope(*a[:4], out=a[4]), [x[0], i32([0]), cos, sin, x[0].clone()]),
+        (lambda *a: speculative.verify_draft(*a[:4], draft_probs=a[4], counts=a[5]), [lo, dr, u, r, lo[:, :1].clone(), i32([1])]),
+    ]
+    for call, args in calls:
+        call(*args)
+        for i in range(len(args)):
+            with pytest.raises(RuntimeError, match="device tensors"):
+                call(*args[:i], args[i].cpu(), *args[i + 1:])

@@ -274,3 +274,28 @@ def test_oracle_verify_keeps_the_target_distribution():
     _, tok = R.verify(logits, draft, [1] * n, np.repeat(q[None, None], n, 0), g.random((n, 1)), g.random(n), 1.0)
     freq = np.bincount(tok[:, 0], minlength=v) / n
     assert np.abs(freq - p).max() < 5 * math.sqrt(0.25 / n)
+
+
+class _Fake:
+    """As much of a tensor as the device check reads."""
+
+    def __init__(self, index):
+        self.index = index
+        self.device = torch.device("cpu") if index < 0 else torch.device("cuda", index)
+
+    def get_device(self):
+        return self.index
+
+
+def test_device_index_takes_one_device_only():
+    a, b, c = _Fake(0), _Fake(1), _Fake(-1)
+    assert _lib.device_index("f", a, None, a) == 0 and _lib.device_index("f", b) == 1
+    for mixed in ((c, a), (a, c), (a, c, a), (c,)):
+        with pytest.raises(RuntimeError, match="device tensors"):
+            _lib.device_index("f", *mixed)
+    for mixed in ((a, b), (b, a, b)):
+        with pytest.raises(RuntimeError, match="different devices"):
+            _lib.device_index("f", *mixed)
+    for none in ((), (None,)):
+        with pytest.raises(RuntimeError, match="no tensor"):
+            _lib.device_index("f", *none)
