@@ -84,9 +84,10 @@ __device__ inline void fill_pow64(double* pow64) {
 // Elements base .. base + 7 of a row of V as fp32; past the end `fill`.
 template <int DT, bool VEC>
 __device__ inline void load_row8(const void* p, int64_t row0, int base, int V, float fill, float (&v)[kPer]) {
-  if (VEC && base + kPer <= V) {
+  if constexpr (VEC) {
+    const int64_t at = row0 + min(base, V - kPer);
     if constexpr (DT == SQX_DTYPE_F32) {
-      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + row0 + base);
+      const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + at);
       const f32x4_t a = q[0], b = q[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -94,7 +95,7 @@ __device__ inline void load_row8(const void* p, int64_t row0, int base, int V, f
         v[4 + e] = b[e];
       }
     } else {
-      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + row0 + base);
+      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t w = a[e];
@@ -102,10 +103,14 @@ __device__ inline void load_row8(const void* p, int64_t row0, int base, int V, f
         v[2 * e + 1] = DT == SQX_DTYPE_BF16 ? bf16_hi(w) : f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
       }
     }
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) v[e] = base + e < V ? load_as_f32(p, DT, row0 + base + e) : fill;
+    for (int e = 0; e < kPer; ++e) v[e] = load_as_f32(p, DT, row0 + min(base + e, V - 1));
+  }
+  if (base + kPer > V) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = base + e < V ? v[e] : fill;
+  }
 }
 
 __device__ inline double wave_sum_f64(double v) {
