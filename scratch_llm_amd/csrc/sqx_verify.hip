@@ -35,7 +35,7 @@ struct VerifyArgs {
   double k;  // 64 log2(e) / temperature
   double* sums;  // [B, T + 1, S]
   double* rest;  // [B, S]
-  double* verdict;  // [B, 3]: accepted, then of the row behind them -maximum k and 1 / sum
+  double* verdict;  // [B, 3]: accepted, then of the row behind them the maximum and 1 / sum
   float* maxs;   // [B, T + 1, S]
   int* args;     // [B, T + 1, S], temperature 0
   int *n_acc, *tokens;
@@ -198,11 +198,11 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
                                       __builtin_elementwise_maximum(redm[2], redm[3]));
     double sum = 0.0;
     if (m > -INFINITY && m < INFINITY) {  // the same in every thread; a masked element adds 2^-1000
-      const double off = -static_cast<double>(m) * a.k;
+      const double md = static_cast<double>(m);
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += exp2_64th(fma(static_cast<double>(v[p][e]), a.k, off), pow64);
+        for (int e = 0; e < kPer; ++e) sum += exp2_64th((static_cast<double>(v[p][e]) - md) * a.k, pow64);
       sum = block_sum_f64(sum, red);
     }
     if (threadIdx.x == 0) {
@@ -212,15 +212,16 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
   }
 }
 
-// e^((x - m) / temperature) / sum; 0 for a masked x.
-__device__ inline double prob(float x, double off, double k, double inv, const double* pow64) {
-  const double e = exp2_64th(fma(static_cast<double>(x), k, off), pow64) * inv;
+// e^((x - m) / temperature) / sum; 0 for a masked x. The difference comes before the factor: x k - m k, fused or not, would
+// leave the rounding of m k at x = m, which is many powers of two for an m of 1e20.
+__device__ inline double prob(float x, double m, double k, double inv, const double* pow64) {
+  const double e = exp2_64th((static_cast<double>(x) - m) * k, pow64) * inv;
   return x == -INFINITY ? 0.0 : e;
 }
 
 struct Verdict {
   int n, count;     // accepted, drafted
-  double off, inv;  // of row n: -maximum k and 1 / sum; inv is NaN where the row has no distribution
+  double m, inv;  // of row n: its maximum and 1 / sum; inv is NaN where the row has no distribution
 };
 
 // Judges the drafts of row b: thread (t, part) joins every fourth slice of row t, lane by lane of a quad. The same in every
@@ -254,24 +255,24 @@ __device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const doubl
     mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 1, 64));
     mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 2, 64));
     const bool fine = mx > -INFINITY && mx < INFINITY;
-    const double off = fine ? -static_cast<double>(mx) * a.k : 0.0;
+    const double m = fine ? static_cast<double>(mx) : 0.0;
     double z = 0.0;
     if (mine && fine) {
 #pragma unroll 4
       for (int s = part; s < a.S; s += 4) {
         const float ms = a.maxs[at + s];
-        z += prob(ms, off, a.k, 1.0, pow64) * a.sums[at + s];
+        z += prob(ms, m, a.k, 1.0, pow64) * a.sums[at + s];
       }
     }
     z += __shfl_xor(z, 1, 64);
     z += __shfl_xor(z, 2, 64);
     const double inv = fine ? 1.0 / z : __builtin_nan("");
-    const bool good = mine && t < r.count && x >= 0 && x < a.V && ux * qx < prob(lx, off, a.k, inv, pow64);
+    const bool good = mine && t < r.count && x >= 0 && x < a.V && ux * qx < prob(lx, m, a.k, inv, pow64);
     const uint64_t bad = ~__ballot(good || t >= r.count) & 0x1111111111111111ull;
     const int stop = bad != 0 ? t0 + (static_cast<int>(__builtin_ctzll(bad)) >> 2) : r.count;
     if (stop < t0 + 16 || r.count < t0 + 16) {
       r.n = min(stop, r.count);
-      r.off = __shfl(off, (r.n - t0) * 4, 64);
+      r.m = __shfl(m, (r.n - t0) * 4, 64);
       r.inv = __shfl(inv, (r.n - t0) * 4, 64);
       return r;
     }
@@ -295,7 +296,7 @@ __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, in
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    const double p = prob(l[e], v.off, a.k, v.inv, pow64);
+    const double p = prob(l[e], v.m, a.k, v.inv, pow64);
     const double qe = residual && a.probs == nullptr ? (base + e == x ? 1.0 : 0.0) : static_cast<double>(q[e]);
     w[e] = residual ? (p > qe ? p - qe : 0.0) : p;
   }
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
   const Verdict v = judge<DT>(a, b, pdt, pow64);
   if (s == 0 && threadIdx.x == 0) {
     a.verdict[3 * b] = v.n;
-    a.verdict[3 * b + 1] = v.off;
+    a.verdict[3 * b + 1] = v.m;
     a.verdict[3 * b + 2] = v.inv;
   }
   if (v.n == v.count) return;  // nothing was rejected: the row's own statistics serve
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   Verdict v;
   v.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   v.n = static_cast<int>(a.verdict[3 * b]);
-  v.off = a.verdict[3 * b + 1];
+  v.m = a.verdict[3 * b + 1];
   v.inv = a.verdict[3 * b + 2];
   const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
   const double r = static_cast<double>(a.r[b]);
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   auto slice_sum = [&](int s) -> double {
     if (s >= a.S) return 0.0;
     if (residual) return s < 64 ? rest0 : a.rest[static_cast<int64_t>(b) * a.S + s];
-    return prob(a.maxs[row * a.S + s], v.off, a.k, v.inv, pow64) * a.sums[row * a.S + s];
+    return prob(a.maxs[row * a.S + s], v.m, a.k, v.inv, pow64) * a.sums[row * a.S + s];
   };
   auto sum_all = [&]() {
     double mine = 0.0;

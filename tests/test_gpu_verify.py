@@ -89,6 +89,27 @@ def test_borders():
         run(logits, draft, None, u, r, counts, 1.0)
 
 
+@pytest.mark.parametrize("temp", [1.0, 1e-4, 1e4])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_large_logits(dtype, temp):
+    """Rows masked with the type's lowest value, all of a row too; logits up to the type's largest, equal ones among them."""
+    logits, draft, probs, u, r = make(12, 2, 9000, "fp32", "fp32", 16)
+    low = torch.finfo(DT[dtype]).min
+    top = torch.finfo(DT[dtype]).max
+    logits[0, :, 5000:] = low
+    logits[1] = low
+    logits[2, :, 1:] = low
+    logits[3] = top
+    logits[4] = torch.where(torch.rand(3, 9000, generator=torch.Generator().manual_seed(3)) < 0.5, top, low)
+    logits[5] = -1e4
+    logits[6] = torch.where(torch.rand(3, 9000, generator=torch.Generator().manual_seed(4)) < 0.01, 0.3 * top, 0.1 * top)
+    logits[7] = 0.77 * top
+    logits[8] = 0.77 * low
+    logits[9, :, ::2] = -math.inf
+    for p in (probs, None):
+        run(logits.to(DT[dtype]), draft, p, u, r, None, temp)
+
+
 def test_greedy_ties_and_nan():
     """Ties go to the lowest id within and across slices; a NaN is the maximum, the first one counts."""
     logits = torch.zeros(4, 2, 20000)
