@@ -188,18 +188,20 @@ __device__ inline float load_query32(const uint16_t* src, bool ok, int hi, float
 }
 
 // The rows and keys of a tile of `span` rows from row0: token `last` is its last one below the count, keys below `keys` are
-// attended by some row of it, keys up to `first` by every row.
+// attended by some row of it, keys up to `first` by every row. A token past the table attends what the table has.
 struct KvSpan {
-  int count, start, first, keys;
+  int count, start, most, first, keys;
+  __device__ int position(int t) const {  // without the sum's overflow
+    return static_cast<int>(min(static_cast<int64_t>(start) + t, static_cast<int64_t>(most) - 1));
+  }
 };
 __device__ inline bool kv_span(const KvAttnArgs& a, int b, int row0, int span, KvSpan& s) {
   s.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   if (row0 / a.G >= s.count) return false;  // rows from the count on are left as they are
   s.start = a.starts[b];
-  const int last = min((row0 + span - 1) / a.G, s.count - 1);
-  const int64_t end = static_cast<int64_t>(s.start) + last + 1, most = static_cast<int64_t>(a.width) * a.block;
-  s.keys = static_cast<int>(end < 0 ? 0 : (end < most ? end : most));
-  s.first = s.start + row0 / a.G;
+  s.most = a.width * a.block;  // below 2^30
+  s.keys = max(s.position(min((row0 + span - 1) / a.G, s.count - 1)) + 1, 0);
+  s.first = s.position(row0 / a.G);
   return true;
 }
 
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const Kv
     const int row = row0 + 16 * i + r;
     const int t = row / a.G;
     const bool ok = row < rows && t < sp.count;
-    pos[i] = ok ? sp.start + t : -1;
+    pos[i] = ok ? sp.position(t) : -1;
     qs[i] = load_query<KD, BF16>(a.q + b * a.q_sb + (ok ? t * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, g, a.qscale, qf[i]);
     m[i] = -INFINITY;
     l[i] = 0.0f;
@@ -635,7 +637,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
   u32x4_t qf[2 * KD];
   const int wrow = row0 + 32 * wave, row = wrow + r, rt = row / a.G;
   const bool ok = row < rows && rt < sp.count;
-  const int pos = ok ? sp.start + rt : -1;
+  const int pos = ok ? sp.position(rt) : -1;
   const float qs = load_query32<KD, BF16>(a.q + b * a.q_sb + (ok ? rt * a.q_st + (h * a.G + row % a.G) * a.q_sh : 0), ok, hi, a.qscale, qf);
   float m = -INFINITY, l = 0.0f;
   f32x16_t o[VD];
@@ -646,9 +648,9 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
   int last = -1;  // the wave's last position
   {
     const int end = min(min(wrow + 32, rows), sp.count * a.G);  // rows of the wave below the count
-    if (end > wrow) last = sp.start + (end - 1) / a.G;
+    if (end > wrow) last = sp.position((end - 1) / a.G);
   }
-  const int first = sp.start + wrow / a.G;
+  const int first = sp.position(wrow / a.G);
 
   if (threadIdx.x < 3) lnan[threadIdx.x] = 0;
   __syncthreads();
@@ -841,7 +843,7 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
   SQX_REQUIRE(dtype != SQX_DTYPE_F32, SQX_E_ARG, "%s: queries must be BF16 or F16", fn);
   SQX_REQUIRE(H >= 1 && H % Hkv == 0 && H <= 8192, SQX_E_ARG, "%s: H=%lld must be a multiple of Hkv=%lld, up to 8192", fn,
               (long long)H, (long long)Hkv);
-  SQX_REQUIRE(scale > 0.0f && scale <= 3.0e38f, SQX_E_ARG, "%s: scale must be positive and finite", fn);
+  SQX_REQUIRE(scale > 0.0f && scale <= 1.0e30f, SQX_E_ARG, "%s: scale must be positive and at most 1e30", fn);
   SQX_REQUIRE(q_sb >= 0 && q_st >= 0 && q_sh >= 0 && (q_sb | q_st | q_sh) % 8 == 0, SQX_E_ARG,
               "%s: strides must be multiples of 8 elements", fn);
   if (B == 0 || T == 0) return SQX_OK;

@@ -95,8 +95,8 @@ extern "C" int sqx_rope(const void* x, int dtype, int64_t n, int64_t heads, int6
   const char* fn = "sqx_rope";
   SQX_REQUIRE(dtype == SQX_DTYPE_F32 || dtype == SQX_DTYPE_BF16 || dtype == SQX_DTYPE_F16, SQX_E_ARG,
               "%s: x must be F32, BF16 or F16", fn);
-  SQX_REQUIRE(n >= 0 && n < (int64_t(1) << 31) && heads >= 1 && heads <= 65536 && d >= 1 && d <= 2048, SQX_E_ARG,
-              "%s: bad shape (n=%lld, heads=%lld up to 65536, d=%lld up to 2048)", fn, (long long)n, (long long)heads,
+  SQX_REQUIRE(n >= 0 && n < (int64_t(1) << 24) && heads >= 1 && heads <= 65536 && d >= 1 && d <= 2048, SQX_E_ARG,
+              "%s: bad shape (n=%lld below 2^24, heads=%lld up to 65536, d=%lld up to 2048)", fn, (long long)n, (long long)heads,
               (long long)d);
   SQX_REQUIRE(rot >= 2 && rot % 2 == 0 && rot <= d, SQX_E_ARG, "%s: rot=%lld must be even and within 2 .. d=%lld", fn,
               (long long)rot, (long long)d);

@@ -94,7 +94,10 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int, int]:
     if sd == 1 and (sb | st | sh) & 7 == 0 and x.data_ptr() & 15 == 0:
         return x, sb, st, sh
     x = x.contiguous()
-    return x, *x.stride()[:3]
+    if x.data_ptr() & 15:
+        x = x.clone()
+    _, t, h, d = x.shape  # not x.stride(): a dimension of one token or head keeps any
+    return x, t * h * d, h * d, d
 
 
 def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale: Tensor,
@@ -160,7 +163,7 @@ def read_kv_blocks(k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale: T
     ``fp32(code) * scale`` rounded once to ``dtype``. Zeros from ``counts[b]`` on, at a negative start, outside the
     table and on a page id outside the cache."""
     fn = "read_kv_blocks"
-    b = block_table.shape[0]
+    b = block_table.shape[0] if block_table.ndim else 0
     pages, hkv, block, d, fmt = _check_cache(k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, b, fn)
     if tokens < 0:
         raise ValueError(f"{fn}: tokens must not be negative, got {tokens}")
@@ -199,8 +202,8 @@ def attend_kv_blocks(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Tenso
         raise TypeError(f"{fn}: q must be bfloat16 or float16, got {q.dtype}")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    elif not (0.0 < scale < 3.0e38):
-        raise ValueError(f"{fn}: scale must be positive and finite, got {scale}")
+    elif not (0.0 < scale <= 1.0e30):
+        raise ValueError(f"{fn}: scale must be positive and at most 1e30, got {scale}")
     index = _lib.device_index(fn, q, k_codes, v_codes, k_scale, v_scale, block_table, starts, counts, out)
     q, q_sb, q_st, q_sh = _rows(q)
     if out is None:

@@ -291,6 +291,42 @@ def test_attention_ignores_what_it_must_not_see(kv, fmt, t):
         check_attention(kv, cache, fmt, q, table, starts, None)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("t,block,width", [(1, 16, 3), (6, 32, 1), (40, 16, 5), (90, 32, 3), (40, 64, 1)])
+def test_attention_past_the_table(kv, t, block, width, fmt):
+    """Tokens past the table's end, by a little, by a lot and up to the last int32: they attend all that the table has, which
+    is no whole number of 64-key steps; rows that begin inside it."""
+    print_case("kv attention past the table", t, block, width, fmt)
+    d, hkv, h, end = 128, 1, 4, width * block
+    starts = [end - 1, end + 100, (1 << 31) - 1, max(end - t, 0), 0]
+    b = len(starts)
+    cache = fill_valid(make_cache(kv, b * width + 1, hkv, d, block, fmt, t), fmt, 20 + t)
+    table = np.random.default_rng(t).permutation(b * width + 1)[:b * width].reshape(b, width).astype(np.int32)
+    q = torch.randn(b, t, h, d, generator=torch.Generator().manual_seed(t)).half()
+    check_attention(kv, cache, fmt, q, table, starts, None, dtype="fp16")
+
+
+def test_rows_that_need_a_copy(kv):
+    """Queries, keys and values off 16 bytes, with strides of no whole 16 bytes, and with any stride where there is one token
+    or one head: the same as of plain tensors."""
+    block, d = 16, 64
+    g = torch.Generator().manual_seed(11)
+    cache = fill_valid(make_cache(kv, 6, 1, d, block, "int8", 2), "int8", 3)
+    table, starts = i32([[1, 3, 5], [0, 2, 4]]), i32([20, 33])
+    x = torch.randn(2, 1, 1, d, generator=g).bfloat16().to(DEV)
+    want = to_dev(cache, "int8")
+    kv.write_kv_blocks(x, x, *want, table, starts)
+    plain = kv.attend_kv_blocks(x, *want, table, starts)
+    flat = torch.zeros(4 * d + 8, dtype=torch.bfloat16, device=DEV)
+    views = [flat[1:2 * d + 1].view(2, 1, 1, d), flat.as_strided((2, 1, 1, d), (d, 3, 5, 1)), flat.as_strided((2, 1, 1, d), (d + 1, 3, 5, 1))]
+    for i, y in enumerate(views):
+        y.copy_(x)
+        got = to_dev(cache, "int8")
+        kv.write_kv_blocks(y, y, *got, table, starts)
+        same_bytes(back(got), back(want), f"view {i}")
+        assert torch.equal(kv.attend_kv_blocks(y, *got, table, starts), plain), i
+
+
 def test_attention_on_a_bad_page_is_nan(kv):
     cache = fill_valid(make_cache(kv, 8, 1, 64, 16, "int8", 1), "int8", 2)
     table = np.array([[0, 1, 2, 3], [4, 8, 5, 6], [7, -1, 0, 0]], np.int32)

@@ -99,7 +99,8 @@ def test_attend_and_read_refuse():
     c = cache()
     q = torch.zeros(2, 1, 4, 64, dtype=BF)
     for change, what in ((dict(q=q[0]), "q must be"), (dict(q=q[:, :, :3]), "heads"), (dict(q=q[..., :32]), "heads"),
-                         (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=-1.0), "scale")):
+                         (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale"), (dict(scale=-1.0), "scale"),
+                         (dict(scale=1e31), "scale")):
         a = {**dict(q=q), **change}
         with pytest.raises(ValueError, match=what):
             kv.attend_kv_blocks(a.pop("q"), *c, t, s, **a)
@@ -173,7 +174,7 @@ def test_c_entries_refuse():
         return lib.sqx_kvblock_attention(a["q"], a["dt"], *a["qs"], a["fmt"], p, p, p, p, p, p, None, a["B"], a["T"], a["H"],
                                          a["Hkv"], a["hd"], a["block"], a["pages"], a["width"], a["scale"], a["out"], None, 0, None)
 
-    for bad in (dict(dt=0), dict(H=3, Hkv=2), dict(scale=0.0), dict(scale=float("nan")), dict(q=None), dict(out=ctypes.c_void_p(4)),
+    for bad in (dict(dt=0), dict(H=3, Hkv=2), dict(scale=0.0), dict(scale=float("nan")), dict(scale=2e30), dict(q=None), dict(out=ctypes.c_void_p(4)),
                 dict(qs=(64, 64, 4)), dict(hd=80), dict(T=(1 << 24) - 1, H=64)):
         assert attend(**bad) == -1, bad
     assert lib.sqx_kvblock_attention_workspace_bytes(1, 1, 32, 8, 128, 64, 4096) > 0
@@ -192,10 +193,11 @@ def test_c_entries_refuse():
         assert verify(**bad) == -1, bad
     assert verify(nb=8) == -3
     n = [3, 1, 8, 0]
-    for bad in (dict(dt=5), dict(rot=3), dict(rot=128), dict(rows=0), dict(x=None), dict(x=ctypes.c_void_p(3)), dict(d=0)):
-        a = dict(x=p, dt=1, d=64, rot=64, rows=4)
+    for bad in (dict(dt=5), dict(rot=3), dict(rot=128), dict(rows=0), dict(x=None), dict(x=ctypes.c_void_p(3)), dict(d=0),
+                dict(n=1 << 24), dict(h=0)):
+        a = dict(x=p, dt=1, d=64, rot=64, rows=4, n=n[0], h=n[1])
         a.update(bad)
-        assert lib.sqx_rope(a["x"], a["dt"], n[0], n[1], a["d"], 64, 64, p, p, p, a["rows"], a["rot"], 1, p, 64, 64, None) == -1, bad
+        assert lib.sqx_rope(a["x"], a["dt"], a["n"], a["h"], a["d"], 64, 64, p, p, p, a["rows"], a["rot"], 1, p, 64, 64, None) == -1, bad
 
 
 def test_rope_tables():
