@@ -759,46 +759,76 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
   }
 }
 
-// Joins the nsplit (at most 64) parts of every (token, head) row: one wave per row, lane s holding part s's statistics.
-template <int D, bool BF16>
+// Joins the nsplit parts of every (token, head) row. Bound by the latency of its loads, so PG threads share a part's place of
+// 16 bytes in the row: each takes every PG-th part, the first ones on their way while the maxima are compared.
+template <int D, bool BF16, int PG>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, int64_t total) {
-  constexpr int E = D / 64;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (id >= total) return;
-  const int lane = threadIdx.x & 63;
-  const int rows = a.T * a.G;
+  constexpr int C = D / 4, kRows = 256 / (PG * C), kAhead = 4;
+  __shared__ float rm[kRows][PG], rl[kRows][PG];
+  __shared__ f32x4_t ro[kRows][PG][C];
+  const int rr = threadIdx.x / (PG * C), p = threadIdx.x / C % PG, c = threadIdx.x % C;
+  const int64_t id = std::min<int64_t>(static_cast<int64_t>(blockIdx.x) * kRows + rr, total - 1);  // the last row again
+  const int rows = a.T * a.G, n = a.nsplit;
   const int row = static_cast<int>(id % rows);
   const int64_t bh = id / rows;
   const int b = static_cast<int>(bh / a.Hkv), h = static_cast<int>(bh % a.Hkv);
   const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
-  if (row / a.G >= count) return;
-  float ms = -INFINITY, ls = 0.0f;
-  if (lane < a.nsplit) {
-    const int64_t at = 2 * ((bh * a.nsplit + lane) * rows + row);
-    ms = a.pml[at];
-    ls = a.pml[at + 1];
+  const bool live = row / a.G < count;  // no part has been written of the others
+  const int mine = live ? n : 0;
+  auto at = [&](int s) { return (bh * n + s) * rows + row; };
+  f32x4_t x[kAhead];
+  float m[kAhead], l[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    x[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    m[u] = -INFINITY;
+    l[u] = 0.0f;
+    if (p + PG * u < mine) {
+      x[u] = *reinterpret_cast<const f32x4_t*>(a.po + at(p + PG * u) * D + 4 * c);
+      m[u] = a.pml[2 * at(p + PG * u)];
+      l[u] = a.pml[2 * at(p + PG * u) + 1];
+    }
   }
-  float M = ms;
+  float M = -INFINITY;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  const float wt = attn_chunk_weight(ms, M);
-  float sum = ls * wt, acc[E];
+  for (int u = 0; u < kAhead; ++u) M = fmaxf(M, m[u]);
+  for (int s = p + PG * kAhead; s < mine; s += PG) M = fmaxf(M, a.pml[2 * at(s)]);
+  if (c == 0) rm[rr][p] = M;
+  __syncthreads();
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  for (int i = 0; i < PG; ++i) M = fmaxf(M, rm[rr][i]);
+  float sum = 0.0f;
+  f32x4_t acc{0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](float ms, float ls, f32x4_t v) {
+    const float wt = attn_chunk_weight(ms, M);
+    sum = fmaf(ls, wt, sum);
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-  const float* src = a.po + (bh * a.nsplit * rows + row) * D + E * lane;
-  const int64_t next = static_cast<int64_t>(rows) * D;
-#pragma unroll 8
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float w = __shfl(wt, s, 64);
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(v[e], wt, acc[e]);
+  };
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[s * next + e], w, acc[e]);
+  for (int u = 0; u < kAhead; ++u)
+    if (p + PG * u < mine) add(m[u], l[u], x[u]);
+#pragma unroll 4
+  for (int s = p + PG * kAhead; s < mine; s += PG)
+    add(a.pml[2 * at(s)], a.pml[2 * at(s) + 1], *reinterpret_cast<const f32x4_t*>(a.po + at(s) * D + 4 * c));
+  ro[rr][p][c] = acc;
+  if (c == 0) rl[rr][p] = sum;
+  __syncthreads();
+  if (p != 0 || !live || static_cast<int64_t>(blockIdx.x) * kRows + rr >= total) return;
+  sum = 0.0f;
+  acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < PG; ++i) {
+    sum += rl[rr][i];
+    const f32x4_t v = ro[rr][i][c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += v[e];
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D + E * lane;
-#pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = BF16 ? f32_to_bf16_bits(acc[e] * inv) : f32_to_f16_bits(acc[e] * inv);
+  uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D + 4 * c;
+  const float o0 = acc[0] * inv, o1 = acc[1] * inv, o2 = acc[2] * inv, o3 = acc[3] * inv;
+  *reinterpret_cast<u32x2v_t*>(dst) = BF16 ? u32x2v_t{ActBF16::pack_rne(o0, o1), ActBF16::pack_rne(o2, o3)}
+                                           : u32x2v_t{ActF16::pack_rne(o0, o1), ActF16::pack_rne(o2, o3)};
 }
 
 // How a call is laid out: 16-row tiles of a workgroup of the direct kernel (0: the tile kernel), its tiles of rows, and
@@ -814,7 +844,7 @@ inline KvAttnPlan kv_attn_plan(int64_t B, int64_t rows, int64_t Hkv, int64_t hd,
   const int64_t groups = B * Hkv * p.tiles, steps = ceil_div(keys, kStepKeys);
   // two workgroups of the direct kernel a CU, one of the tile kernel; no further round for a few
   const int64_t want = std::max<int64_t>(1, (p.R == 0 ? 256 : 512) / groups);
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, ceil_div(steps, kAttnWaves), 64})));
+  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(steps, kAttnWaves))));
   return p;
 }
 
@@ -893,11 +923,19 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
   SQX_LAUNCH_CHECK(fn);
   if (ns > 1) {
     const int64_t total = B * Hkv * rows;
-    const dim3 jg(static_cast<unsigned>(ceil_div(total, 4)));
     with_head(hd, [&](auto dd) {
       constexpr int D = decltype(dd)::value;
-      if (dtype == SQX_DTYPE_BF16) hipLaunchKernelGGL((kv_attn_join_kernel<D, true>), jg, dim3(256), 0, s, a, total);
-      else hipLaunchKernelGGL((kv_attn_join_kernel<D, false>), jg, dim3(256), 0, s, a, total);
+      auto go = [&](auto bf, auto pg) {
+        constexpr int PG = decltype(pg)::value;
+        const dim3 jg(static_cast<unsigned>(ceil_div(total, 1024 / (PG * D))));
+        hipLaunchKernelGGL((kv_attn_join_kernel<D, decltype(bf)::value, PG>), jg, dim3(256), 0, s, a, total);
+      };
+      auto with_parts = [&](auto bf) {
+        if (ns > 4) go(bf, std::integral_constant<int, D == 256 ? 4 : 8>{});
+        else go(bf, std::integral_constant<int, 2>{});
+      };
+      if (dtype == SQX_DTYPE_BF16) with_parts(std::true_type{});
+      else with_parts(std::false_type{});
     });
     SQX_LAUNCH_CHECK(fn);
   }

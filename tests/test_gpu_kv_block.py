@@ -353,6 +353,24 @@ def test_attention_over_scales_far_apart(kv, fmt):
     check_attention(kv, cache, fmt, q, table, [190], None)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("t,h,hkv,d", [(1, 8, 2, 128), (6, 8, 2, 64), (5, 7, 1, 128), (3, 10, 1, 256)])
+def test_attention_of_uneven_rows(kv, t, h, hkv, d, fmt):
+    """Rows from nothing to thousands of keys in one call, idle ones between and at both ends: workgroups take parts that end
+    inside one row and begin inside another, hold several whole rows, or a piece of one."""
+    print_case("kv attention uneven", t, h, hkv, d, fmt)
+    block = 32
+    starts = [9, 4100, 0, 63, -1, 2500, 700, 1, 2, 1300, 64, 5]
+    counts = [0, t, t, t, t, t, 1, t, 0, max(t - 2, 1), t, 0]
+    b, width = len(starts), 4200 // block
+    cache = fill_valid(make_cache(kv, 300, hkv, d, block, fmt, t), fmt, t + 1)
+    table = np.random.default_rng(t).integers(0, 300, (b, width)).astype(np.int32)
+    q = torch.randn(b, t, h, d, generator=torch.Generator().manual_seed(t)).bfloat16()
+    check_attention(kv, cache, fmt, q, table, starts, counts)
+    check_attention(kv, cache, fmt, q, table, [0] * b, [0] * b)
+    check_attention(kv, cache, fmt, q[:2], table[:2], [3, 4000], [t, t])
+
+
 @pytest.mark.parametrize("t", [1, 9, 40])
 def test_attention_long_and_strided(kv, t):
     """A context that is split over workgroups, queries as a strided view, a scale of the caller's."""
