@@ -6,13 +6,17 @@
 // of the row behind the drafts: the least i whose cumulative weight exceeds r times the total, so the kept tokens are
 // distributed as the target's own. Temperature 0: accept while x_t is the row's argmax, then take the argmax.
 //
-// Probabilities, totals and cumulative sums are double: the pick falls between two neighbours of a cumulative sum over a
-// whole vocabulary, and in fp32 about one pick in a hundred would depend on the order of the sums. The exponential costs a
-// dozen double operations (below), so a row is still bound by reading it once.
+// What the pick is made from is double: it falls between two neighbours of a cumulative sum over a whole vocabulary, and in
+// fp32 about one pick in a hundred would depend on the order of the sums. That takes a dozen double operations an element
+// (below), for one row per sequence. The other rows are only compared with u: their sums are of fp32 exponentials, good to
+// 2^-18 (31 additions of at most 2^-24 each, exponentials to 2^-23, arguments to 2^-23 of at most 17 bits), which moves one
+// decision in a million or fewer. With every row in double, 64 x (5 + 1) x 128256 bf16 logits took 38 us, twice their reading.
 //
-// Three launches (two at temperature 0): statistics of every slice of every row; the residual's sum of every slice of the
-// one row per sequence that needs it; the pick. The decision is a few operations on the slices' statistics, so every
-// workgroup of the second repeats it instead of waiting for one.
+// Three launches (two at temperature 0): statistics of every slice of every row; the double sums of every slice of the one
+// row per sequence that is drawn from; the pick. The decision is a few operations on the slices' statistics, so every
+// workgroup of the second repeats it instead of waiting for one. The second does not know that row's total Z yet, only
+// its estimate 1 / inv: with e the exponentials and P the elements where e inv > q, its slices sum e, (e inv - q) over P
+// and e over P, and the third, which has Z, adds (1 / Z - inv) times the last. P misses only elements within 2^-18 of a tie.
 #include <type_traits>
 
 #include "sqx_common.h"
@@ -32,10 +36,11 @@ struct VerifyArgs {
   const void* probs;   // [B, T, V], or NULL: each draft was certain
   const float *u, *r;
   int T, V, S;
-  double k;  // 64 log2(e) / temperature
+  double k;   // 64 log2(e) / temperature
+  float k32;  // log2(e) / temperature
   double* sums;  // [B, T + 1, S]
-  double* rest;  // [B, S]
-  double* verdict;  // [B, 3]: accepted, then of the row behind them the maximum and 1 / sum
+  double* rest;  // [3, B, S]: of the row drawn from, the sums above
+  double* verdict;  // [B, 3]: accepted, then of the row behind them the maximum and 1 / sum as estimated
   float* maxs;   // [B, T + 1, S]
   int* args;     // [B, T + 1, S], temperature 0
   int *n_acc, *tokens;
@@ -118,27 +123,30 @@ __device__ inline double wave_sum_f64(double v) {
   for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// The sum over the workgroup, in every thread; `red` holds one value per wave and is free again after the call.
-__device__ inline double block_sum_f64(double v, double* red) {
-  v = wave_sum_f64(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+// The sums over the workgroup, in every thread.
+template <int N>
+__device__ inline void block_sums_f64(double (&v)[N], double (&red)[N][4]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum_f64(v[i]);
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i][threadIdx.x >> 6] = v[i];
+  }
   __syncthreads();
-  v = (red[0] + red[1]) + (red[2] + red[3]);
-  __syncthreads();
-  return v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (red[i][0] + red[i][1]) + (red[i][2] + red[i][3]);
 }
 
-// Slice s of row (b, t): its maximum and the sum of 2^(k (x - maximum)); temperature 0: the maximum's first index
+// Slice s of row (b, t): its maximum and the sum of 2^(k32 (x - maximum)); temperature 0: the maximum's first index
 // (NaN counts as the maximum).
 template <int DT, bool VEC, bool GREEDY>
 __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
-  __shared__ double pow64[64], red[4];
+  __shared__ double red[1][4];
   __shared__ float redm[4];
   __shared__ int redi[4];
   const int s = blockIdx.x, row = blockIdx.y, b = row / (a.T + 1), t = row % (a.T + 1);
   const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   if (t > count) return;
-  if constexpr (!GREEDY) fill_pow64(pow64);
   const int64_t row0 = static_cast<int64_t>(row) * a.V;
   const int at = s * kSlice + threadIdx.x * kPer;
   float v[kPasses][kPer];
@@ -196,18 +204,19 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(const VerifyArgs a) {
     __syncthreads();
     m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(redm[0], redm[1]),
                                       __builtin_elementwise_maximum(redm[2], redm[3]));
-    double sum = 0.0;
-    if (m > -INFINITY && m < INFINITY) {  // the same in every thread; a masked element adds 2^-1000
-      const double md = static_cast<double>(m);
+    double sum[1] = {0.0};
+    if (m > -INFINITY && m < INFINITY) {  // the same in every thread
+      float mine = 0.0f;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += exp2_64th((static_cast<double>(v[p][e]) - md) * a.k, pow64);
-      sum = block_sum_f64(sum, red);
+        for (int e = 0; e < kPer; ++e) mine += __builtin_amdgcn_exp2f((v[p][e] - m) * a.k32);
+      sum[0] = static_cast<double>(mine);
+      block_sums_f64(sum, red);
     }
     if (threadIdx.x == 0) {
       a.maxs[out] = m;  // NaN or infinite: the row is no distribution; -infinite: the slice is all masked
-      a.sums[out] = sum;
+      a.sums[out] = sum[0];
     }
   }
 }
@@ -279,10 +288,10 @@ __device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const doubl
   }
 }
 
-// Weights of elements base .. base + 7 of the row that the pick is drawn from.
+// Of elements base .. base + 7 of the row drawn from: e, and in w the weight by the estimated total, which is zero outside P.
 template <int DT, bool VEC>
 __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, int base, int pdt, bool residual, int x,
-                                const double* pow64, double (&w)[kPer]) {
+                                const double* pow64, double (&ex)[kPer], double (&w)[kPer]) {
   const int64_t row0 = (static_cast<int64_t>(b) * (a.T + 1) + v.n) * a.V;
   float l[kPer], q[kPer];
   load_row8<DT, VEC>(a.logits, row0, base, a.V, -INFINITY, l);
@@ -296,7 +305,8 @@ __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, in
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    const double p = prob(l[e], v.m, a.k, v.inv, pow64);
+    ex[e] = prob(l[e], v.m, a.k, 1.0, pow64);
+    const double p = ex[e] * v.inv;
     const double qe = residual && a.probs == nullptr ? (base + e == x ? 1.0 : 0.0) : static_cast<double>(q[e]);
     w[e] = residual ? (p > qe ? p - qe : 0.0) : p;
   }
@@ -304,7 +314,7 @@ __device__ inline void weights8(const VerifyArgs& a, const Verdict& v, int b, in
 
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, int pdt) {
-  __shared__ double pow64[64], red[4];
+  __shared__ double pow64[64], red[3][4];
   fill_pow64(pow64);
   __syncthreads();
   const int s = blockIdx.x, b = blockIdx.y;
@@ -314,18 +324,25 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
     a.verdict[3 * b + 1] = v.m;
     a.verdict[3 * b + 2] = v.inv;
   }
-  if (v.n == v.count) return;  // nothing was rejected: the row's own statistics serve
-  const int x = a.draft[static_cast<int64_t>(b) * a.T + v.n];
-  double sum = 0.0;
+  const bool residual = v.n < v.count;
+  const int x = residual ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
+  double sum[3] = {0.0, 0.0, 0.0};
 #pragma unroll 2
   for (int p = 0; p < kPasses; ++p) {
-    double w[kPer];
-    weights8<DT, VEC>(a, v, b, s * kSlice + p * kPass + threadIdx.x * kPer, pdt, true, x, pow64, w);
+    double ex[kPer], w[kPer];
+    weights8<DT, VEC>(a, v, b, s * kSlice + p * kPass + threadIdx.x * kPer, pdt, residual, x, pow64, ex, w);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) sum += w[e];
+    for (int e = 0; e < kPer; ++e) {
+      sum[0] += ex[e];
+      sum[1] += w[e];
+      sum[2] += w[e] > 0.0 ? ex[e] : 0.0;
+    }
   }
-  sum = block_sum_f64(sum, red);
-  if (threadIdx.x == 0) a.rest[static_cast<int64_t>(b) * a.S + s] = sum;
+  block_sums_f64(sum, red);
+  if (threadIdx.x < 3) {
+    const int64_t each = static_cast<int64_t>(gridDim.y) * a.S;
+    a.rest[threadIdx.x * each + static_cast<int64_t>(b) * a.S + s] = threadIdx.x == 0 ? sum[0] : threadIdx.x == 1 ? sum[1] : sum[2];
+  }
 }
 
 // The pick, by one workgroup of a thread per eight elements of a slice: the slice in which the cumulative sum passes the
@@ -341,22 +358,26 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     found = 0x7fffffff;
     last = -1;
   }
-  const double rest0 = lane < a.S ? a.rest[static_cast<int64_t>(b) * a.S + lane] : 0.0;  // on its way beside the verdict
+  const double* const rest = a.rest + static_cast<int64_t>(b) * a.S;
+  const int64_t each = static_cast<int64_t>(gridDim.x) * a.S;
+  double first[3];  // of slice `lane`, on their way beside the verdict
+#pragma unroll
+  for (int i = 0; i < 3; ++i) first[i] = lane < a.S ? rest[i * each + lane] : 0.0;
   Verdict v;
   v.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
   v.n = static_cast<int>(a.verdict[3 * b]);
   v.m = a.verdict[3 * b + 1];
   v.inv = a.verdict[3 * b + 2];
-  const int64_t row = static_cast<int64_t>(b) * (a.T + 1) + v.n;
   const double r = static_cast<double>(a.r[b]);
   const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
   __syncthreads();
   bool residual = v.n < v.count;
-  auto slice_sum = [&](int s) -> double {
-    if (s >= a.S) return 0.0;
-    if (residual) return s < 64 ? rest0 : a.rest[static_cast<int64_t>(b) * a.S + s];
-    return prob(a.maxs[row * a.S + s], v.m, a.k, v.inv, pow64) * a.sums[row * a.S + s];
-  };
+  auto sums = [&](int i, int s) -> double { return s >= a.S ? 0.0 : s < 64 ? first[i] : rest[i * each + s]; };
+  double all = 0.0;
+  for (int s = lane; s < a.S; s += 64) all += sums(0, s);
+  all = wave_sum_f64(all);
+  const double inv = v.inv == v.inv ? 1.0 / all : v.inv, more = inv - v.inv;
+  auto slice_sum = [&](int s) -> double { return residual ? fmax(sums(1, s) + sums(2, s) * more, 0.0) : sums(0, s) * inv; };
   auto sum_all = [&]() {
     double mine = 0.0;
     for (int s = lane; s < a.S; s += 64) mine += slice_sum(s);
@@ -371,7 +392,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     return w;
   };
   double total = sum_all();
-  if (residual && total <= 0.0) {  // p nowhere above q: drawn from p (a NaN goes on as one)
+  if (residual && v.inv == v.inv && total <= 0.0) {  // p nowhere above q: drawn from p
     residual = false;
     total = sum_all();
   }
@@ -394,10 +415,15 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     const bool none = hit < 0;  // r next to 1 and a rounding: the last token that has a weight
     if (none) hit = fallback;
     const int at = hit * kSlice + threadIdx.x * kPer;
-    double w[kPer], mine = 0.0;
-    weights8<DT, VEC>(a, v, b, at, pdt, residual, x, pow64, w);
+    double ex[kPer], w[kPer], mine = 0.0;
+    weights8<DT, VEC>(a, v, b, at, pdt, residual, x, pow64, ex, w);
+    int first = 0x7fffffff, end = -1;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) mine += w[e];
+    for (int e = 0; e < kPer; ++e) {
+      if (w[e] > 0.0) end = at + e;  // by the sums' own rule, so that a slice that has a sum has a last one
+      w[e] = w[e] > 0.0 ? fmax(w[e] + ex[e] * more, 0.0) : 0.0;
+      mine += w[e];
+    }
     const double inc = scan(mine);
     if (lane == 63) wsum[wave] = inc;
     __syncthreads();
@@ -406,11 +432,9 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
     for (int i = 0; i < kPickWaves; ++i)
       if (i < wave) c += wsum[i];
     c += inc - mine;
-    int first = 0x7fffffff, end = -1;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       c += w[e];
-      if (w[e] > 0.0) end = at + e;
       if (first == 0x7fffffff && w[e] > 0.0 && c > theta) first = at + e;
     }
     if (!none && first != 0x7fffffff) atomicMin(&found, first);  // of whole numbers: their order changes nothing
@@ -457,7 +481,7 @@ using namespace sqx;
 extern "C" int64_t sqx_verify_draft_workspace_bytes(int64_t B, int64_t T, int64_t V) {
   if (B <= 0 || T < 0 || V <= 0) return 0;
   const int64_t S = ceil_div(V, kSlice);
-  return B * (T + 1) * S * 16 + B * (S + 3) * 8;
+  return B * (T + 1) * S * 16 + B * (3 * S + 3) * 8;
 }
 
 extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int* counts, const void* probs,
@@ -485,10 +509,11 @@ extern "C" int sqx_verify_draft(const void* logits, int dtype, const int* draft,
   a.logits = logits; a.draft = draft; a.counts = counts; a.probs = probs; a.u = u; a.r = r;
   a.T = static_cast<int>(T); a.V = static_cast<int>(V); a.S = static_cast<int>(ceil_div(V, kSlice));
   a.k = greedy ? 0.0 : 64.0 * 1.4426950408889634074 / temperature;
+  a.k32 = static_cast<float>(a.k / 64.0);
   const int64_t rows = B * (T + 1) * a.S;
   a.sums = static_cast<double*>(ws);
   a.rest = a.sums + rows;
-  a.verdict = a.rest + B * a.S;
+  a.verdict = a.rest + 3 * B * a.S;
   a.maxs = reinterpret_cast<float*>(a.verdict + 3 * B);
   a.args = reinterpret_cast<int*>(a.maxs + rows);
   a.n_acc = n_accepted; a.tokens = tokens;

@@ -25,8 +25,8 @@ def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | No
     With ``p_t = softmax(logits[:, t] / temperature)`` and ``q_t = draft_probs[:, t]`` (``[B, T, V]``; None: the
     draft was certain of its token), draft t is accepted while ``u[b, t] * q_t(x_t) < p_t(x_t)``. The token that
     follows is drawn from ``max(p - q, 0)`` of the first rejected row, or from ``p`` of the row behind the
-    drafts: the least id whose cumulative weight exceeds ``r[b]`` times the total. Probabilities and sums are
-    float64. ``temperature=0`` accepts while the draft is its row's argmax and then takes the argmax (``u``, ``r``
+    drafts: the least id whose cumulative weight exceeds ``r[b]`` times the total. What the pick is made from is
+    float64; the ``p_t(x_t)`` that a draft is accepted by is within 2^-18 of itself. ``temperature=0`` accepts while the draft is its row's argmax and then takes the argmax (``u``, ``r``
     and ``draft_probs`` may be None). ``counts`` (int32 ``[B]``) says how many drafts a row has (default T).
 
     ``u [B, T]`` and ``r [B]`` are float32 in [0, 1). Returns ``(n_accepted int32 [B], tokens int32 [B, T + 1])``:

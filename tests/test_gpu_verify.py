@@ -1,7 +1,8 @@
 """verify_draft (scratch_llm_amd/speculative.py) on the GPU against oracle/kv_block_ref.py: whole numbers, compared exactly.
 
-Both sides work in float64: a pick can differ only where a cumulative sum lies within about 1e-12 of its threshold, which
-over a vocabulary of v tokens has a chance of about v 1e-12 a row."""
+Picks are made in float64 on both sides: one can differ only where a cumulative sum lies within about 1e-12 of its
+threshold, which over a vocabulary of v tokens has a chance of about v 1e-12 a row. A draft is judged by probabilities good
+to 2^-18, mostly to 2^-22: a decision can differ where u q is that near to p, about one in a million."""
 
 from __future__ import annotations
 
