@@ -875,7 +875,7 @@ int sqx_kvblock_read(int fmt, const void* k_codes, const void* v_codes, const fl
 
 /* Causal attention of T new tokens a row over the cache, which already holds their keys and values:
  *   out[b, t, h] = softmax_j(scale q[b, t, h] . k[b, j, h / G]) v[b, j, h / G],  j <= starts[b] + t,  G = H / Hkv
- * for t < counts[b] (NULL: T); other tokens of out are left as they were. q BF16 or F16 [B, T, H, hd] by strides (as in
+ * for t < counts[b] (NULL: T); other tokens of out are left as they were. Positions past the table do not exist. q BF16 or F16 [B, T, H, hd] by strides (as in
  * sqx_kvblock_write), out contiguous of the same type. A token with no key (a negative position) gets zeros; one that
  * attends a position without a page gets NaN. ws: sqx_kvblock_attention_workspace_bytes, 16-byte aligned (0: none). */
 int64_t sqx_kvblock_attention_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
@@ -887,11 +887,11 @@ int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int64_t q_st, 
                           void* ws, int64_t ws_bytes, sqx_stream_t stream);
 
 /* Check counts[b] (NULL: T; T <= 63) drafted tokens of every row against the target's logits [B, T + 1, V] (F32 / BF16 /
- * F16), from given random numbers. p_t = softmax(logits[b, t] / temperature), in double; q_t = probs[b, t] (F32 / BF16 /
- * F16), or certainty for the drafted token (probs NULL).
- *   Draft t is accepted while u[b, t] q_t(x_t) < p_t(x_t); n_accepted[b] is their number n.
+ * F16), from given random numbers. p_t = softmax(logits[b, t] / temperature); q_t = probs[b, t] (F32 / BF16 / F16), or
+ * certainty for the drafted token (probs NULL).
+ *   Draft t is accepted while u[b, t] q_t(x_t) < p_t(x_t), this p good to 2^-18; n_accepted[b] is their number n.
  *   The next token is the least i with cumsum(w)_i > r[b] sum(w): w = max(p_n - q_n, 0) after a rejection (p_n if that is
- *   zero everywhere; a NaN of q takes the token out), p_n after none.
+ *   zero everywhere; a NaN of q takes the token out), p_n after none; p, weights and sums in double.
  * temperature 0: accepted while x_t is the first maximum of its row (NaN counts as the maximum), then that maximum; u, r
  * and probs are not read. tokens [B, T + 1]: the accepted drafts, the next token, then -1. An id outside [0, V) is
  * rejected. A row that is no distribution (a NaN, +inf, or -inf everywhere) rejects its draft and its next token is -1. */
