@@ -32,9 +32,9 @@ struct Row8 {
       w[2 * pair] = __builtin_bit_cast(uint32_t, lo);
       w[2 * pair + 1] = __builtin_bit_cast(uint32_t, hi);
     } else if constexpr (DT == SQX_DTYPE_BF16) {
-      w[pair] = static_cast<uint32_t>(f32_to_bf16_bits(lo)) | (static_cast<uint32_t>(f32_to_bf16_bits(hi)) << 16);
+      w[pair] = ActBF16::pack_rne(lo, hi);
     } else {
-      w[pair] = static_cast<uint32_t>(f32_to_f16_bits(lo)) | (static_cast<uint32_t>(f32_to_f16_bits(hi)) << 16);
+      w[pair] = ActF16::pack_rne(lo, hi);
     }
   }
   __device__ inline void load(const void* base, int64_t elem) {  // elem a multiple of 8, base 16-byte aligned

@@ -23,8 +23,7 @@ struct KvWriteArgs {
   int T, H, Hkv, width, pages, block, shift;
 };
 
-constexpr int kQHeads = 8;     // query heads per workgroup of the rotary part
-constexpr int kHeadBatch = 4;  // of which a thread takes as many at once
+constexpr int kQHeads = 4;  // query heads per workgroup of the rotary part, all taken by a thread at once
 
 // The rotation of the rows x[0 .. NP) of one 8-column group. In halves the other half of a pair lies in the lane half8
 // further on or back, of the same token.
@@ -75,18 +74,17 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
   if (y >= 2 * a.Hkv) {  // query heads: every token of the row, whatever its count
     const int h0 = (y - 2 * a.Hkv) * kQHeads;
     const int ta = max(0, j * a.block - off), tb = min(a.T, (j + 1) * a.block - off);
-    for (int i = tl; i < (tb - ta) * (kQHeads / kHeadBatch); i += TP) {
-      const int t = ta + i / (kQHeads / kHeadBatch), h = h0 + i % (kQHeads / kHeadBatch) * kHeadBatch;
+    for (int t = ta + tl; t < tb; t += TP) {
       Angles8 g;
       angles(g, t);
-      Row8<DT> x[kHeadBatch];
+      Row8<DT> x[kQHeads];
       const int64_t row = b * a.q_sb + t * a.q_st + 8 * c;
 #pragma unroll
-      for (int e = 0; e < kHeadBatch; ++e) x[e].load(a.q, row + min(h + e, a.H - 1) * a.q_sh);
+      for (int e = 0; e < kQHeads; ++e) x[e].load(a.q, row + min(h0 + e, a.H - 1) * a.q_sh);
 #pragma unroll
-      for (int e = 0; e < kHeadBatch; ++e) {
+      for (int e = 0; e < kQHeads; ++e) {
         rotate_lane<DT>(x[e], c, a.rot, a.inter, g);
-        if (h + e < a.H) x[e].store(a.q_out, ((static_cast<int64_t>(b) * a.T + t) * a.H + h + e) * D + 8 * c);
+        if (h0 + e < a.H) x[e].store(a.q_out, ((static_cast<int64_t>(b) * a.T + t) * a.H + h0 + e) * D + 8 * c);
       }
     }
     return;
