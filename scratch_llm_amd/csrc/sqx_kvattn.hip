@@ -235,7 +235,12 @@ __device__ inline float scale_or_tiny(float s) { return fmaxf(s, kTinyScale) + (
 
 // Workgroup (h, s * tiles + tile, b): kv head h, the 16 R (token, head) rows of a tile, part s of nsplit of its keys. For few
 // rows, where reading the cache once is the bound: the four waves take alternate 64-key steps straight from memory into
-// registers and share nothing until the end.
+// registers and share nothing until the end. A step's keys are loaded while the step before is worked on.
+//
+// Measured with 32 heads over 8 kv heads of 128: one token in 64 rows of up to 8192 keys 150 us, 5.3 TB/s; in 3 rows of
+// 800000 keys 830 us, 5.9 TB/s; over 2048 keys 7 us, the latency of two steps a wave and the join through LDS. Five tokens in
+// 16 rows of E4M3 73 us where one row of 16000 keys stands beside others of half, 4.1 TB/s (62 us, 4.8 TB/s, with even
+// rows). Cutting all rows' steps laid end to end into equal parts, so that the workgroups end together, took 74 us there.
 template <int D, int R, bool E4M3, bool BF16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const KvAttnArgs a) {
   constexpr int KD = D / 64;  // 16-byte pieces of a key per lane
@@ -525,11 +530,14 @@ __device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, c
 // The products are v_mfma_f32_32x32x16_f16, with the row order of the direct kernel carried over: row p of a 32-key tile is
 // key 16 ((p / 4) % 2) + 4 (p / 8) + p % 4, so that lane (hi, r) gets the scores of 16 hi .. 16 hi + 15.
 //
-// Bound by the vector and the matrix unit together: on this card two waves of a SIMD overlap little of them (an MFMA of 16
+// 2 rows, 2048 tokens of 32 heads (8 kv heads) and up to 6000 keys: 245 us, 914 TFLOP/s; 4 even rows of as many tokens run at
+// 1005, a library product of 8192^3 in fp16 at 1101. Bound by the vector and the matrix unit together: on this card two waves of a SIMD overlap little of them (an MFMA of 16
 // cycles hides two vector instructions; 16x16x32 with four vector instructions and an exponential takes 33.7 ns for two
 // waves where the parts take 16.3, 10.2 and 7.6, the 32x32x16 form 27.9). So vector instructions are what counts. Two groups
 // of waves half a tile apart (one in its products while the other is in its softmax), and products and softmax of
-// neighbouring tiles in one stream, took the same 290 us as this plain order.
+// neighbouring tiles in one stream, took as long as this plain order (290 and 298 us against 287, before the 32x32x16
+// form); turning the order of the second half of the workgroups, so that the shortest share a CU with the longest, 309
+// against 278 under the profiler; 128 rows in four waves 366 against 338.
 //
 // BIG: pages of 64 tokens or more, so a 64-key piece lies in one. Its page and scales are the same for all lanes and addresses
 // are scalar; the per-lane form costs 70 vector instructions a tile, a fifth of all.
@@ -760,7 +768,9 @@ __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_attn_
 }
 
 // Joins the nsplit parts of every (token, head) row. Bound by the latency of its loads, so PG threads share a part's place of
-// 16 bytes in the row: each takes every PG-th part, the first ones on their way while the maxima are compared.
+// 16 bytes in the row: each takes every PG-th part, the first ones on their way while the maxima are compared. 96 rows of 21
+// parts take 4.4 us (12.5 with a wave a row), 32 of 8 parts 2.7; up to 4 parts, PG = 2 and more rows a workgroup: 2560 rows
+// of 4 parts 4.2 us, 5.5 with PG = 8 and 8 parts.
 template <int D, bool BF16, int PG>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, int64_t total) {
   constexpr int C = D / 4, kRows = 256 / (PG * C), kAhead = 4;
@@ -838,11 +848,16 @@ struct KvAttnPlan {
 };
 inline KvAttnPlan kv_attn_plan(int64_t B, int64_t rows, int64_t Hkv, int64_t hd, int64_t keys) {
   KvAttnPlan p;
-  p.R = rows > 64 ? 0 : rows <= 16 ? 1 : 2;
+  // The direct kernel reads the cache once for every 32 rows, the tile kernel for every 256 (128 with heads of 256) and keeps
+  // its matrix unit busier. us, direct and tile, 8 kv heads, int8, in 8 rows of 16000 keys and 1 of 2000:
+  //   heads of 128: 64 rows 65, 127 and 12, 17; 128 rows 112, 136 and 14, 19; 192 rows 185, 151 and 19, 21
+  //   heads of 256 (the direct kernel spills): 64 rows 187, 203 and 20, 26; 68 rows 314, 203 and 20, 26
+  p.R = rows > (hd == 256 ? 64 : 128) ? 0 : rows <= 16 ? 1 : 2;
   const int64_t span = p.R == 0 ? tile_rows(static_cast<int>(hd)) : 16 * p.R;
   p.tiles = static_cast<int>(std::min<int64_t>(ceil_div(rows, span), 1 << 30));
   const int64_t groups = B * Hkv * p.tiles, steps = ceil_div(keys, kStepKeys);
-  // two workgroups of the direct kernel a CU, one of the tile kernel; no further round for a few
+  // Two workgroups of the direct kernel a CU (twice as many: 28 -> 39 us for 2 rows of 60000 keys and 16 heads over one), one
+  // of the tile kernel (two: 30 -> 43 us for 128 rows over 16000 keys); no further round for a few.
   const int64_t want = std::max<int64_t>(1, (p.R == 0 ? 256 : 512) / groups);
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(steps, kAttnWaves))));
   return p;

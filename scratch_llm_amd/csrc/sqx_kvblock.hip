@@ -48,7 +48,12 @@ __device__ inline void rotate_lane(Row8<DT>& x, int c, int rot, bool inter, cons
 }
 
 // Workgroup (j, y, b): block j of the blocks that row b's tokens touch. y < Hkv: the keys of head y; then the values;
-// then groups of kQHeads query heads, whose rotation needs no block.
+// then groups of kQHeads query heads, whose rotation needs no block. A block's scale needs all of its new tokens before the
+// first code, so a workgroup holds a block of one head in registers and reads it once.
+//
+// Bound by HBM for prompts: 12977 tokens in 8 rows, 32 query and 8 kv heads of 128, bf16 to int8: 70 us, 4.2 TB/s (two
+// thirds of it queries; eight heads a workgroup took 81). One token in each of 8 rows takes 5.8 us: a launch and a chain of
+// table, scale and old codes.
 //
 // A thread holds 8 columns of NP tokens: of a whole block, tokens NP tl .. NP tl + NP - 1, so that four codes of a value
 // column are one dword of the transposed tile; of at most 256 / C tokens (NP = 1), token tl of the write. Slots outside
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
 }
 
 // Values of positions starts[b] .. + tokens - 1 of every row: fp32(code) * scale, rounded once; zeros from counts[b] on,
-// outside the table and where it names no page.
+// outside the table and where it names no page. 12977 tokens as bf16: 20 us, 3.9 TB/s, values through LDS.
 template <int DT, int D, bool E4M3>
 __global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                       const float* __restrict__ ks, const float* __restrict__ vs,

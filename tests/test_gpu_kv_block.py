@@ -242,6 +242,8 @@ ATTENDS = [
     (1, 130, 4, 1, 64, 32, [700], None),
     (1, 80, 4, 2, 256, 128, [600], None),
     (1, 90, 4, 1, 128, 128, [1500], None),
+    (2, 30, 4, 1, 128, 32, [333, 0], [30, 17]),
+    (1, 43, 6, 2, 64, 16, [90], None),
 ]
 
 
