@@ -229,7 +229,8 @@ __device__ inline double prob(float x, double m, double k, double inv, const dou
 }
 
 struct Verdict {
-  int n, count;     // accepted, drafted
+  int n, count;   // accepted, drafted
+  int x;          // the draft of row n, where n < count
   double m, inv;  // of row n: its maximum and 1 / sum; inv is NaN where the row has no distribution
 };
 
@@ -281,6 +282,7 @@ __device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const doubl
     const int stop = bad != 0 ? t0 + (static_cast<int>(__builtin_ctzll(bad)) >> 2) : r.count;
     if (stop < t0 + 16 || r.count < t0 + 16) {
       r.n = min(stop, r.count);
+      r.x = __shfl(x, (r.n - t0) * 4, 64);
       r.m = __shfl(m, (r.n - t0) * 4, 64);
       r.inv = __shfl(inv, (r.n - t0) * 4, 64);
       return r;
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
     a.verdict[3 * b + 2] = v.inv;
   }
   const bool residual = v.n < v.count;
-  const int x = residual ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
+  const int x = v.x;
   double sum[3] = {0.0, 0.0, 0.0};
 #pragma unroll 2
   for (int p = 0; p < kPasses; ++p) {
@@ -369,7 +371,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
   v.m = a.verdict[3 * b + 1];
   v.inv = a.verdict[3 * b + 2];
   const double r = static_cast<double>(a.r[b]);
-  const int x = v.n < v.count ? a.draft[static_cast<int64_t>(b) * a.T + v.n] : -1;
+  const int drafted = lane < a.T ? a.draft[static_cast<int64_t>(b) * a.T + lane] : -1;
+  const int x = __shfl(drafted, v.n, 64);
   __syncthreads();
   bool residual = v.n < v.count;
   auto sums = [&](int i, int s) -> double { return s >= a.S ? 0.0 : s < 64 ? first[i] : rest[i * each + s]; };
@@ -437,15 +440,17 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyA
       c += w[e];
       if (first == 0x7fffffff && w[e] > 0.0 && c > theta) first = at + e;
     }
-    if (!none && first != 0x7fffffff) atomicMin(&found, first);  // of whole numbers: their order changes nothing
-    if (end >= 0) atomicMax(&last, end);
+    // the wave's first and last, which lie in its first and last lane that has one; of whole numbers: any order of the waves
+    const uint64_t firsts = __ballot(!none && first != 0x7fffffff), ends = __ballot(end >= 0);
+    if (firsts != 0 && lane == static_cast<int>(__builtin_ctzll(firsts))) atomicMin(&found, first);
+    if (ends != 0 && lane == 63 - static_cast<int>(__builtin_clzll(ends))) atomicMax(&last, end);
     __syncthreads();
   }
   if (threadIdx.x == 0) a.n_acc[b] = v.n;
   if (static_cast<int>(threadIdx.x) <= a.T) {
     const int t = threadIdx.x;
     const int pick = found != 0x7fffffff ? found : last;
-    a.tokens[static_cast<int64_t>(b) * (a.T + 1) + t] = t < v.n ? a.draft[static_cast<int64_t>(b) * a.T + t] : t == v.n ? pick : -1;
+    a.tokens[static_cast<int64_t>(b) * (a.T + 1) + t] = t < v.n ? drafted : t == v.n ? pick : -1;  // t is the lane
   }
 }
 
