@@ -530,14 +530,14 @@ __device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, c
 // The products are v_mfma_f32_32x32x16_f16, with the row order of the direct kernel carried over: row p of a 32-key tile is
 // key 16 ((p / 4) % 2) + 4 (p / 8) + p % 4, so that lane (hi, r) gets the scores of 16 hi .. 16 hi + 15.
 //
-// 2 rows, 2048 tokens of 32 heads (8 kv heads) and up to 6000 keys: 245 us, 914 TFLOP/s; 4 even rows of as many tokens run at
-// 1005, a library product of 8192^3 in fp16 at 1101. Bound by the vector and the matrix unit together: on this card two waves of a SIMD overlap little of them (an MFMA of 16
-// cycles hides two vector instructions; 16x16x32 with four vector instructions and an exponential takes 33.7 ns for two
-// waves where the parts take 16.3, 10.2 and 7.6, the 32x32x16 form 27.9). So vector instructions are what counts. Two groups
-// of waves half a tile apart (one in its products while the other is in its softmax), and products and softmax of
-// neighbouring tiles in one stream, took as long as this plain order (290 and 298 us against 287, before the 32x32x16
-// form); turning the order of the second half of the workgroups, so that the shortest share a CU with the longest, 309
-// against 278 under the profiler; 128 rows in four waves 366 against 338.
+// 2 rows, 2048 tokens of 32 heads (8 kv heads) and up to 6000 keys: 247 us, 908 TFLOP/s; 4 even rows of as many tokens run at
+// 1005, a library product of 8192^3 in fp16 at 1101. Bound by the vector and the matrix unit together: on this card two waves
+// of a SIMD overlap little of them (an MFMA of 16 cycles hides two vector instructions; 16x16x32 with four vector
+// instructions and an exponential takes 33.7 ns for two waves where the parts take 16.3, 10.2 and 7.6, the 32x32x16 form
+// 27.9). So vector instructions are what counts. Two groups of waves half a tile apart (one in its products while the other
+// is in its softmax), and products and softmax of neighbouring tiles in one stream, took as long as this plain order (290
+// and 298 us against 287, before the 32x32x16 form); turning the order of the second half of the workgroups, so that the
+// shortest share a CU with the longest, 309 against 278 under the profiler; 128 rows in four waves 366 against 338.
 //
 // BIG: pages of 64 tokens or more, so a 64-key piece lies in one. Its page and scales are the same for all lanes and addresses
 // are scalar; the per-lane form costs 70 vector instructions a tile, a fifth of all.
