@@ -238,10 +238,10 @@ struct Verdict {
   double m, inv;  // of row n: its maximum and 1 / sum; inv is NaN where the row has no distribution
 };
 
-// Judges the drafts of row b: thread (t, part) joins every fourth slice of row t, lane by lane of a quad. The same in every
+// Decides on the drafts of row b: thread (t, part) joins every fourth slice of row t, lane by lane of a quad. The same in every
 // wave; up to 16 rows at a time (a wave holds 16 quads), so that the loads of a row's slices run side by side.
 template <int DT>
-__device__ inline Verdict judge(const VerifyArgs& a, int b, int pdt, const double* pow64) {
+__device__ inline Verdict decide(const VerifyArgs& a, int b, int pdt, const double* pow64) {
   const int lane = threadIdx.x & 63, part = lane & 3;
   Verdict r;
   r.count = a.counts != nullptr ? min(max(a.counts[b], 0), a.T) : a.T;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(const VerifyArgs a, in
   fill_pow64(pow64);
   __syncthreads();
   const int s = blockIdx.x, b = blockIdx.y;
-  const Verdict v = judge<DT>(a, b, pdt, pow64);
+  const Verdict v = decide<DT>(a, b, pdt, pow64);
   if (s == 0 && threadIdx.x == 0) {
     a.verdict[3 * b] = v.n;
     a.verdict[3 * b + 1] = v.m;
