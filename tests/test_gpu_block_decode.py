@@ -267,6 +267,46 @@ def test_verify_samples_with_given_numbers_and_skips_inactive_rows(small):
     assert int(st.tokens[2]) == 7 and int(st.tokens[0]) == int(wt[0, wn[0]])
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.9])
+def test_a_captured_chunk_and_verification_replay_as_eager(small, temperature):
+    """A chunk and a speculative step recorded in one graph and replayed with other tokens, drafts, numbers and counts: the
+    same logits, tokens and cache as the calls themselves, which run between the replays."""
+    model, _ = small
+    B, T = 3, 3
+    g = torch.Generator().manual_seed(8)
+    ids, draft = (torch.zeros(B, n, dtype=torch.int32, device=DEV) for n in (5, T))
+    counts = torch.zeros(B, dtype=torch.int32, device=DEV)
+    u, r, probs = torch.zeros(B, T, device=DEV), torch.zeros(B, device=DEV), torch.zeros(B, T, 1000, device=DEV)
+
+    def fresh():
+        for x in (ids, draft):
+            x.copy_(torch.randint(0, 1000, x.shape, generator=g, dtype=torch.int32))
+        counts.copy_(torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32))
+        u.copy_(torch.rand(B, T, generator=g))
+        r.copy_(torch.rand(B, generator=g))
+        probs.copy_(torch.softmax(2 * torch.randn(B, T, 1000, generator=g), -1))
+
+    def go(s):
+        return (model.extend(s, ids, last_only=True), *model.verify(s, draft, u, r, draft_probs=probs, counts=counts, temperature=temperature))
+
+    fresh()
+    st, eager = (model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=32) for _ in range(2))
+    go(model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=32))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = go(st)
+    for i in range(4):
+        fresh()
+        want = go(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y, name in zip(got, want, ("logits", "accepted", "tokens")):
+            assert torch.equal(x, y), f"replay {i}: {name}"
+        for name in ("k", "v", "k_scale", "v_scale", "lengths", "tokens"):
+            assert torch.equal(getattr(st, name), getattr(eager, name)), f"replay {i}: state's {name}"
+
+
 def test_refusals(small):
     model, _ = small
     st = model.new_state(2, 64, kv_dtype="int8_block")
