@@ -841,21 +841,27 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, i
                                            : u32x2v_t{ActF16::pack_rne(o0, o1), ActF16::pack_rne(o2, o3)};
 }
 
-// How a call is laid out: 16-row tiles of a workgroup of the direct kernel (0: the tile kernel), its tiles of rows, and
+// How a call is laid out: 16-row tiles of a workgroup of the direct kernel (0: the tile kernel), tiles of rows, and
 // the parts that its keys are cut into.
 struct KvAttnPlan {
   int R, tiles, splits;
 };
 inline KvAttnPlan kv_attn_plan(int64_t B, int64_t rows, int64_t Hkv, int64_t hd, int64_t keys) {
   KvAttnPlan p;
-  // The direct kernel reads the cache once for every 32 rows, the tile kernel for every 256 (128 with heads of 256) and keeps
-  // its matrix unit busier. us, direct and tile, 8 kv heads, int8, in 8 rows of 16000 keys and 1 of 2000:
-  //   heads of 128: 64 rows 65, 127 and 12, 17; 128 rows 112, 136 and 14, 19; 192 rows 185, 151 and 19, 21
-  //   heads of 256 (the direct kernel spills): 64 rows 187, 203 and 20, 26; 68 rows 314, 203 and 20, 26
-  p.R = rows > (hd == 256 ? 64 : 128) ? 0 : rows <= 16 ? 1 : 2;
+  const int64_t steps = ceil_div(keys, kStepKeys);
+  // The direct kernel reads the cache once for every 16 R rows, the tile kernel for every 256 (128 with heads of 256) and keeps
+  // its matrix unit busier. us, direct (R = 2) and tile, heads of 128, 8 kv heads, int8, in 8 rows of 16000 keys and 1 of 2000:
+  //   64 rows 65, 127 and 12, 17; 128 rows 112, 136 and 14, 19; 192 rows 185, 151 and 19, 21
+  // heads of 256, direct (R = 1) and tile: 64 rows 199, 203 and 16, 26; 68 rows 354, 204 and 24, 26.
+  // With R = 2 it needs registers that heads of 256 do not have (E4M3, 36 rows: 232 against 195, 20 against 14); smaller heads
+  // are better off with R = 1 while a call has at most 4096 steps, two for each of 512 x 4 waves, R = 2 and R = 1:
+  //   1 row of 2000 keys: 20 rows 11.4, 9.5, 64 rows 12.4, 10.4; of 16000 keys: 32 rows 20.1, 17.8, 64 rows 21.1, 22.7
+  //   8 rows of 16000 keys: 20 rows 51, 57, 36 rows 61, 99
+  const bool one = hd == 256 || rows <= 16 || (rows <= 64 && B * Hkv * ceil_div(rows, 16) * steps <= 4096);
+  p.R = rows > (hd == 256 ? 64 : 128) ? 0 : one ? 1 : 2;
   const int64_t span = p.R == 0 ? tile_rows(static_cast<int>(hd)) : 16 * p.R;
   p.tiles = static_cast<int>(std::min<int64_t>(ceil_div(rows, span), 1 << 30));
-  const int64_t groups = B * Hkv * p.tiles, steps = ceil_div(keys, kStepKeys);
+  const int64_t groups = B * Hkv * p.tiles;
   // Two workgroups of the direct kernel a CU (twice as many: 28 -> 39 us for 2 rows of 60000 keys and 16 heads over one), one
   // of the tile kernel (two: 30 -> 43 us for 128 rows over 16000 keys); no further round for a few.
   const int64_t want = std::max<int64_t>(1, (p.R == 0 ? 256 : 512) / groups);
@@ -924,8 +930,9 @@ extern "C" int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int
     auto go = [&](auto e4, auto bf) {
       constexpr bool E = decltype(e4)::value, BF = decltype(bf)::value;
       if (plan.R == 1) hipLaunchKernelGGL((kv_attn_kernel<D, 1, E, BF>), grid, dim3(256), 0, s, a);
-      else if (plan.R == 2) hipLaunchKernelGGL((kv_attn_kernel<D, 2, E, BF>), grid, dim3(256), 0, s, a);
-      else if (block >= kStepKeys) hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF, true>), grid, dim3(64 * tile_waves(D)), 0, s, a);
+      else if (plan.R == 2) {
+        if constexpr (D < 256) hipLaunchKernelGGL((kv_attn_kernel<D, 2, E, BF>), grid, dim3(256), 0, s, a);
+      } else if (block >= kStepKeys) hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF, true>), grid, dim3(64 * tile_waves(D)), 0, s, a);
       else hipLaunchKernelGGL((kv_attn_tile_kernel<D, E, BF, false>), grid, dim3(64 * tile_waves(D)), 0, s, a);
     };
     auto with_type = [&](auto e4) {

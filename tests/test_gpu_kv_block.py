@@ -244,6 +244,9 @@ ATTENDS = [
     (1, 90, 4, 1, 128, 128, [1500], None),
     (2, 30, 4, 1, 128, 32, [333, 0], [30, 17]),
     (1, 43, 6, 2, 64, 16, [90], None),
+    (3, 6, 16, 4, 128, 32, [9000, 4111, 6000], None),
+    (4, 13, 16, 4, 64, 128, [9000, 4111, 60, 0], [13, 13, 2, 12]),
+    (2, 15, 4, 1, 256, 64, [777, 63], None),
 ]
 
 
