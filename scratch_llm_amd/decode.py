@@ -213,6 +213,17 @@ class DecodeState:
             raise ValueError(f"a {self.kv_dtype} cache has no blocks")
         return self._kv[layer]
 
+    def check_rows(self, fn: str) -> None:
+        """Raises where ``block_table`` or ``lengths`` are not what the kernels of the block-scaled cache read by their bare
+        addresses: int32, one row a slot, without gaps, on the model's device. The table may have any width."""
+        table, n = self.block_table, self.lengths
+        if (table.ndim != 2 or table.shape[0] != self.batch or table.shape[1] < 1 or table.dtype != torch.int32
+                or not table.is_contiguous()):
+            raise ValueError(f"{fn}: block_table must be contiguous int32 [{self.batch}, width], got {tuple(table.shape)} of {table.dtype}")
+        if tuple(n.shape) != (self.batch,) or n.dtype != torch.int32 or not n.is_contiguous():
+            raise ValueError(f"{fn}: lengths must be contiguous int32 [{self.batch}], got {tuple(n.shape)} of {n.dtype}")
+        _lib.require_device(table, n, self.k, fn=fn)
+
     def set_lengths(self, lengths) -> None:
         """Set every slot's valid length (a host list or tensor), e.g. after filling the cache."""
         t = torch.as_tensor(lengths, dtype=torch.int32)
@@ -485,6 +496,8 @@ class Int4DecodeLM:
             raise ValueError(f"only must be one of {self.STEP_KINDS}, got {only!r}")
         if tokens is not None:
             st.set_tokens(tokens, cfg.vocab_size)
+        if st.block_kv:
+            st.check_rows("Int4DecodeLM.step")
         _lib.require_device(st.tokens, self.embed, fn="Int4DecodeLM.step")
         B, d, H, Hkv, hd, T = st.batch, cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, st.max_ctx
         s = _lib.stream_ptr(self.device)
@@ -670,7 +683,8 @@ class Int4DecodeLM:
             raise ValueError(f"tokens must be int32 [{st.batch}, T], got {tuple(tokens.shape)} of {tokens.dtype}")
         if counts is not None and (tuple(counts.shape) != (st.batch,) or counts.dtype != torch.int32):
             raise ValueError(f"counts must be int32 [{st.batch}], got {tuple(counts.shape)} of {counts.dtype}")
-        dev = _lib.require_device(tokens, counts, self.embed, fn="Int4DecodeLM.extend")
+        st.check_rows("Int4DecodeLM.extend")
+        dev = _lib.require_device(tokens, counts, self.embed, st.lengths, fn="Int4DecodeLM.extend")
         B, T = tokens.shape
         d, H, Hkv, hd = cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
         tokens = tokens.contiguous()
