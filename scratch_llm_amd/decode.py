@@ -126,6 +126,8 @@ class DecodeState:
         self.k_scale = self.v_scale = self.block_table = self.counts = None
         self.block_kv = kv_dtype in _BLOCK_KV
         if self.block_kv:
+            if kv_block_size not in kv_block.BLOCKS:
+                raise ValueError(f"kv_block_size: block must be one of {kv_block.BLOCKS}, got {kv_block_size}")
             width = -(-max_ctx // kv_block_size)
             layer = kv_block.new_kv_blocks(cfg.n_layers * batch * width, hkv, hd, block=kv_block_size, dtype=_BLOCK_KV[kv_dtype],
                                            device=dev)

@@ -24,6 +24,12 @@ def state(batch=2, block=16):
     return DecodeState(model(), batch, 64, "int8_block", block)
 
 
+@pytest.mark.parametrize("block", [0, 48, -16, 256])
+def test_block_sizes(block):
+    with pytest.raises(ValueError, match="block must be one of"):
+        state(block=block)
+
+
 TABLES = {
     "int64": lambda t: t.long(), "fewer rows": lambda t: t[:1], "more rows": lambda t: torch.cat((t, t)), "one row": lambda t: t[0],
     "no blocks": lambda t: t[:, :0], "transposed": lambda t: t.t().contiguous().t(), "every other": lambda t: t[:, ::2],
