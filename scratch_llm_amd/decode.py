@@ -691,7 +691,7 @@ class Int4DecodeLM:
         d, H, Hkv, hd = cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
         tokens = tokens.contiguous()
         stored = torch.full((B,), T, dtype=torch.int32, device=dev) if counts is None else counts.clamp(0, T)
-        stored = stored * st.active
+        stored = stored * (st.active != 0)
         rows = _Rows(self, B * T)
         nb = int(lib.sqx_kvblock_attention_workspace_bytes(B, T, H, Hkv, hd, st.k.shape[3], st.block_table.shape[1]))
         ws = torch.empty(max(nb // 4, 4), dtype=torch.float32, device=dev)
@@ -747,7 +747,7 @@ class Int4DecodeLM:
                              None if counts is None else counts.clamp(0, t) + 1, advance=False)
         n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)
         live = st.active != 0
-        st.lengths.add_((n + 1) * st.active)
+        st.lengths.add_((n + 1) * live)
         nxt = tokens.gather(1, n.long()[:, None])[:, 0]
         st.tokens.copy_(torch.where(live, nxt, st.tokens))
         return n, tokens

@@ -1,0 +1,60 @@
+"""What the decode model's passes over several tokens a row leave of a state on the block-scaled cache."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import decode_ref as D
+from tests.conftest import print_case
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SMALL = dict(vocab=512, d_model=512, n_layers=2, n_heads=4, n_kv_heads=2, d_ff=1024)
+CTX = 96
+LOUD, NAN = 500, 501  # a token whose keys and values are many times the others', and one that has none
+KV = ["int8_block", "fp8_block"]
+
+
+def build(p):
+    from scratch_llm_amd.decode import DecodeConfig, Int4DecodeLM
+
+    cfg = DecodeConfig(vocab_size=SMALL["vocab"], d_model=SMALL["d_model"], n_layers=SMALL["n_layers"], n_heads=SMALL["n_heads"],
+                       n_kv_heads=SMALL["n_kv_heads"], d_ff=SMALL["d_ff"], context_length=CTX)
+    return Int4DecodeLM.from_state_dict(cfg, lambda n: p[n], DEV)
+
+
+@pytest.fixture(scope="module")
+def model():
+    """Layer 0's keys and values depend on the embeddings alone, so its cache can be compared bit for bit. LOUD's embedding
+    points along one key row and one value row of each kv head."""
+    p = D.random_params(**SMALL, seed=21, std=0.05)
+    k, v = p["blocks.0.attn.k_proj.weight"], p["blocks.0.attn.v_proj.weight"]
+    e = sum(x / x.norm() for w in (k, v) for x in (w[5], w[128 + 9]))
+    p["token_emb.weight"][LOUD] = e * (SMALL["d_model"] ** 0.5 / e.norm())
+    p["token_emb.weight"][NAN] = float("nan")
+    return build(p)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def ids(shape, seed):
+    return torch.randint(0, LOUD, shape, generator=torch.Generator().manual_seed(seed), dtype=torch.int32).to(DEV)
+
+
+def test_any_flag_but_zero_is_active(model):
+    """`active` is read as the step's `advance` reads it: a row is active where its flag is not zero."""
+    B = 2
+    one, two = (model.new_state(B, CTX, kv_dtype="int8_block") for _ in range(2))
+    two.active.copy_(torch.tensor([2, 255], dtype=torch.uint8))
+    prompt, draft = ids((B, 9), 9), ids((B, 3), 10)
+    u, r = torch.full((B, 3), 0.5, device=DEV), torch.full((B,), 0.5, device=DEV)
+    for s in (one, two):
+        model.extend(s, prompt, i32([9, 4]))
+        s.tokens.copy_(i32([1, 2]))
+        model.step(s)
+        model.verify(s, draft, u, r)
+    assert torch.equal(one.lengths, two.lengths) and torch.equal(one.tokens, two.tokens)
+    assert torch.equal(one.k, two.k) and torch.equal(one.v_scale, two.v_scale)
