@@ -738,11 +738,16 @@ class Int4DecodeLM:
         that follows them (rows that are not active keep both, and give what the arguments say without meaning).
         ``counts`` is how many drafts a row has (default T). What rejected drafts left in the cache lies behind the new
         length and is written over; a block's scale that one of them raised stays raised until the block is begun anew."""
+        fn = "Int4DecodeLM.verify"
         if draft.ndim != 2 or draft.shape[0] != st.batch or draft.dtype != torch.int32:
             raise ValueError(f"draft must be int32 [{st.batch}, T], got {tuple(draft.shape)} of {draft.dtype}")
         t = draft.shape[1]
-        if t > speculative.MAX_DRAFTS:
-            raise ValueError(f"{t} drafted tokens, at most {speculative.MAX_DRAFTS}")
+        if st.block_kv:
+            st.check_rows(fn)
+        # all of it before the pass, which writes into the cache
+        temperature, u, r, draft_probs = speculative.check_arguments(fn, st.batch, t, self.cfg.vocab_size, draft, u, r, draft_probs,
+                                                                     counts, temperature)
+        _lib.require_device(draft, u, r, draft_probs, counts, self.embed, fn=fn)
         logits = self.extend(st, torch.cat((st.tokens[:, None], draft), 1),
                              None if counts is None else counts.clamp(0, t) + 1, advance=False)
         n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)

@@ -18,6 +18,39 @@ __all__ = ["MAX_DRAFTS", "verify_draft"]
 MAX_DRAFTS = 63  # drafted tokens per row of one call
 
 
+def check_arguments(fn: str, b: int, t: int, v: int, draft: Tensor, u: Tensor | None, r: Tensor | None, draft_probs: Tensor | None,
+                    counts: Tensor | None, temperature: float) -> tuple[float, Tensor | None, Tensor | None, Tensor | None]:
+    """Everything that :func:`verify_draft` refuses of its arguments beside logits [b, t + 1, v]. Returns ``(temperature, u,
+    r, draft_probs)`` as they are used: at temperature 0 the last three are not."""
+    if tuple(draft.shape) != (b, t):
+        raise ValueError(f"{fn}: draft must be {(b, t)} for logits {(b, t + 1, v)}, got {tuple(draft.shape)}")
+    if t > MAX_DRAFTS:
+        raise ValueError(f"{fn}: {t} drafted tokens, at most {MAX_DRAFTS}")
+    if b * (t + 1) >= 1 << 16:
+        raise ValueError(f"{fn}: {b} rows of {t} drafts and the token behind them, together at most {(1 << 16) - 1}")
+    if v < 1:
+        raise ValueError(f"{fn}: empty vocabulary")
+    temperature = float(temperature)
+    if not (temperature == 0.0 or 1e-4 <= temperature <= 1e4):
+        raise ValueError(f"{fn}: temperature must be 0 or within 1e-4 .. 1e4, got {temperature}")
+    if temperature == 0.0:
+        u = r = draft_probs = None
+    else:
+        for name, x, shape in (("u", u, (b, t)), ("r", r, (b,))):
+            if x is None or tuple(x.shape) != shape or x.dtype != torch.float32:
+                raise ValueError(f"{fn}: {name} must be float32 {shape}")
+        if draft_probs is not None:
+            if tuple(draft_probs.shape) != (b, t, v):
+                raise ValueError(f"{fn}: draft_probs must be {(b, t, v)}, got {tuple(draft_probs.shape)}")
+            _lib.sqx_dtype(draft_probs.dtype)
+    for name, x in (("draft", draft), ("counts", counts)):
+        if x is not None and x.dtype != torch.int32:
+            raise TypeError(f"{fn}: {name} must be int32, got {x.dtype}")
+    if counts is not None and tuple(counts.shape) != (b,):
+        raise ValueError(f"{fn}: counts must be {(b,)}, got {tuple(counts.shape)}")
+    return temperature, u, r, draft_probs
+
+
 def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | None, *, draft_probs: Tensor | None = None,
                  counts: Tensor | None = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
     """Check ``draft [B, T]`` (int32 ids) against ``logits [B, T + 1, V]``: row t scores the token after t drafts.
@@ -37,29 +70,8 @@ def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | No
         raise ValueError(f"{fn}: logits must be [B, T + 1, V] and draft [B, T], got {tuple(logits.shape)}, {tuple(draft.shape)}")
     b, t1, v = logits.shape
     t = t1 - 1
-    if tuple(draft.shape) != (b, t):
-        raise ValueError(f"{fn}: draft must be {(b, t)} for logits {tuple(logits.shape)}, got {tuple(draft.shape)}")
-    if t > MAX_DRAFTS:
-        raise ValueError(f"{fn}: {t} drafted tokens, at most {MAX_DRAFTS}")
-    if v < 1:
-        raise ValueError(f"{fn}: empty vocabulary")
-    temperature = float(temperature)
-    if not (temperature == 0.0 or 1e-4 <= temperature <= 1e4):
-        raise ValueError(f"{fn}: temperature must be 0 or within 1e-4 .. 1e4, got {temperature}")
+    temperature, u, r, draft_probs = check_arguments(fn, b, t, v, draft, u, r, draft_probs, counts, temperature)
     dt = _lib.sqx_dtype(logits.dtype)
-    if temperature == 0.0:
-        u = r = draft_probs = None
-    else:
-        for name, x, shape in (("u", u, (b, t)), ("r", r, (b,))):
-            if x is None or tuple(x.shape) != shape or x.dtype != torch.float32:
-                raise ValueError(f"{fn}: {name} must be float32 {shape}")
-        if draft_probs is not None and tuple(draft_probs.shape) != (b, t, v):
-            raise ValueError(f"{fn}: draft_probs must be {(b, t, v)}, got {tuple(draft_probs.shape)}")
-    for name, x in (("draft", draft), ("counts", counts)):
-        if x is not None and x.dtype != torch.int32:
-            raise TypeError(f"{fn}: {name} must be int32, got {x.dtype}")
-    if counts is not None and tuple(counts.shape) != (b,):
-        raise ValueError(f"{fn}: counts must be {(b,)}, got {tuple(counts.shape)}")
     pdt = _lib.DTYPE_F32 if draft_probs is None else _lib.sqx_dtype(draft_probs.dtype)
     index = _lib.device_index(fn, logits, draft, u, r, draft_probs, counts)
     logits, draft, u, r, draft_probs, counts = (

@@ -44,6 +44,14 @@ def ids(shape, seed):
     return torch.randint(0, LOUD, shape, generator=torch.Generator().manual_seed(seed), dtype=torch.int32).to(DEV)
 
 
+def raw(st):
+    return [x.view(torch.uint8).clone() if x.element_size() == 1 else x.clone() for x in (st.k, st.v, st.k_scale, st.v_scale)]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_any_flag_but_zero_is_active(model):
     """`active` is read as the step's `advance` reads it: a row is active where its flag is not zero."""
     B = 2
@@ -58,3 +66,22 @@ def test_any_flag_but_zero_is_active(model):
         model.verify(s, draft, u, r)
     assert torch.equal(one.lengths, two.lengths) and torch.equal(one.tokens, two.tokens)
     assert torch.equal(one.k, two.k) and torch.equal(one.v_scale, two.v_scale)
+
+
+def test_a_refused_verification_changes_nothing(model):
+    """Every argument that the verification refuses is refused before the pass writes into the cache."""
+    B, T = 2, 3
+    st = model.new_state(B, CTX, kv_dtype="int8_block")
+    model.extend(st, ids((B, 9), 11))
+    st.tokens.copy_(i32([1, 2]))
+    draft, u, r = ids((B, T), 12), torch.rand(B, T, device=DEV), torch.rand(B, device=DEV)
+    probs = torch.full((B, T, SMALL["vocab"]), 1.0 / SMALL["vocab"], device=DEV)
+    held = raw(st) + [st.lengths.clone(), st.tokens.clone()]
+    for change in (dict(temperature=-1.0), dict(u=None), dict(r=None), dict(u=u.double()), dict(u=u[:, :2]), dict(r=r[:1]),
+                   dict(draft_probs=probs[:, :2]), dict(draft_probs=probs.double()), dict(counts=i32([1])),
+                   dict(counts=torch.ones(B, device=DEV)), dict(u=u.cpu()), dict(draft_probs=probs.cpu()), dict(draft=draft.cpu())):
+        a = {**dict(draft=draft, u=u, r=r), **change}
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            model.verify(st, a.pop("draft"), a.pop("u"), a.pop("r"), **a)
+        torch.cuda.synchronize()
+        assert same(raw(st) + [st.lengths, st.tokens], held), f"{list(change)}: the state has changed"
