@@ -735,7 +735,10 @@ class Int4DecodeLM:
         """One step of speculative decoding: score ``st.tokens`` and the drafted tokens ``draft`` [B, T] behind them in one
         pass, keep what :func:`scratch_llm_amd.speculative.verify_draft` accepts, and continue from there. Returns its
         ``(n_accepted, tokens)``; ``st.lengths`` grows by the accepted tokens and one, and ``st.tokens`` becomes the token
-        that follows them (rows that are not active keep both, and give what the arguments say without meaning).
+        that follows them (rows that are not active keep both, and give what the arguments say without meaning). Where no
+        token follows, because the row of logits behind the kept ones is no distribution (-1 in ``tokens``), the row stays
+        before it: ``st.tokens`` is its last kept token and ``st.lengths`` grows by one less, so that the next pass scores
+        that token anew.
         ``counts`` is how many drafts a row has (default T). What rejected drafts left in the cache lies behind the new
         length and is written over; a block's scale that one of them raised stays raised until the block is begun anew."""
         fn = "Int4DecodeLM.verify"
@@ -748,13 +751,15 @@ class Int4DecodeLM:
         temperature, u, r, draft_probs = speculative.check_arguments(fn, st.batch, t, self.cfg.vocab_size, draft, u, r, draft_probs,
                                                                      counts, temperature)
         _lib.require_device(draft, u, r, draft_probs, counts, self.embed, fn=fn)
-        logits = self.extend(st, torch.cat((st.tokens[:, None], draft), 1),
-                             None if counts is None else counts.clamp(0, t) + 1, advance=False)
+        ids = torch.cat((st.tokens[:, None], draft), 1)
+        logits = self.extend(st, ids, None if counts is None else counts.clamp(0, t) + 1, advance=False)
         n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)
         live = st.active != 0
-        st.lengths.add_((n + 1) * live)
-        nxt = tokens.gather(1, n.long()[:, None])[:, 0]
-        st.tokens.copy_(torch.where(live, nxt, st.tokens))
+        at = n.long()[:, None]
+        nxt = tokens.gather(1, at)[:, 0]
+        nxt_ok = nxt >= 0
+        st.lengths.add_((n + nxt_ok) * live)
+        st.tokens.copy_(torch.where(live, torch.where(nxt_ok, nxt, ids.gather(1, at)[:, 0]), st.tokens))
         return n, tokens
 
     def _delta_plan(self, st: DecodeState, tw: i4.Int4Tiled) -> tuple[int, int]:

@@ -85,3 +85,20 @@ def test_a_refused_verification_changes_nothing(model):
             model.verify(st, a.pop("draft"), a.pop("u"), a.pop("r"), **a)
         torch.cuda.synchronize()
         assert same(raw(st) + [st.lengths, st.tokens], held), f"{list(change)}: the state has changed"
+
+
+@pytest.mark.parametrize("temperature", [0.9, 1.0])
+def test_a_row_without_a_next_token_stays_before_it(model, temperature):
+    """Behind a token of NaN every row of logits is no distribution: there is no next token (-1), the row's state stays at the
+    last kept token, which the next pass scores anew, and the other rows go on."""
+    B, T = 3, 3
+    st = model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=16)
+    model.extend(st, ids((B, 12), 7))
+    st.tokens.copy_(i32([5, NAN, 6]))
+    draft = ids((B, T), 8)
+    draft[0, 1] = NAN
+    n, tok = model.verify(st, draft, torch.zeros(B, T, device=DEV), torch.full((B,), 0.5, device=DEV), temperature=temperature)
+    assert n.tolist() == [2, 0, 3]
+    assert tok[0].tolist() == [int(draft[0, 0]), NAN, -1, -1] and tok[1].tolist() == [-1] * 4
+    assert st.lengths.tolist() == [14, 12, 16]
+    assert st.tokens.tolist() == [NAN, NAN, int(tok[2, 3])] and int(st.tokens[2]) >= 0
