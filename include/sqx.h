@@ -865,6 +865,17 @@ int sqx_kvblock_write(const void* k, const void* v, int dtype, int64_t k_sb, int
                       const int* counts, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
                       int64_t pages, int64_t width, sqx_stream_t stream);
 
+/* The open block of a row is the one that position starts[b] lies in behind earlier tokens; a write there may raise its scale
+ * and halve the earlier tokens' codes. back 0 copies every row's open block and scales of L layers into `saved`, back 1
+ * puts them back: for tokens that may have to be taken out again (rejected drafts). k_codes [L, pages, Hkv, block, hd] and so
+ * on: the layers' caches one behind the other, one table for all. Rows with rows[b] == 0 (NULL: none), a negative start, a
+ * start at a block's first slot or outside the table, or no page are left alone. saved: sqx_kvblock_open_bytes, 16-byte
+ * aligned; its contents are those of the rows that both calls take. Rows must not share the page of an open block. */
+int64_t sqx_kvblock_open_bytes(int64_t L, int64_t B, int64_t Hkv, int64_t hd, int64_t block);
+int sqx_kvblock_open(int back, void* k_codes, void* v_codes, float* k_scale, float* v_scale, const int* table,
+                     const int* starts, const int* rows, int64_t L, int64_t B, int64_t Hkv, int64_t hd, int64_t block,
+                     int64_t pages, int64_t width, void* saved, int64_t saved_bytes, sqx_stream_t stream);
+
 /* fp32(code) * scale, rounded once to dtype (F32 / BF16 / F16), of positions starts[b] .. starts[b] + T - 1 of every row:
  * k_out, v_out [B, T, Hkv, hd]. Zeros from counts[b] (NULL: T) on, for a negative start, outside the table and where it
  * names no page. */

@@ -246,6 +246,12 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_p, _c_p, _c_i64, _c_i64, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p],
     ),
+    "sqx_kvblock_open_bytes": (_c_i64, [_c_i64] * 5),
+    "sqx_kvblock_open": (
+        _c_i,
+        [_c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_p, _c_i64, _c_p],
+    ),
     "sqx_kvblock_read": (
         _c_i,
         [_c_i, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,

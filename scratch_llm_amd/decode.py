@@ -246,7 +246,7 @@ class _Rows:
     """The buffers of one pass over ``rows`` token rows (those of a :class:`DecodeState` that do not depend on its cache),
     allocated on the current stream by the pass itself."""
 
-    def __init__(self, model: "Int4DecodeLM", rows: int, head_only: bool = False) -> None:
+    def __init__(self, model: "Int4DecodeLM", rows: int, head_only: bool = False, each_qkv: bool = False) -> None:
         cfg, lib = model.cfg, _lib.load()
         bf = dict(dtype=torch.bfloat16, device=model.device)
         d, hd = cfg.d_model, cfg.head_dim
@@ -257,7 +257,8 @@ class _Rows:
             used = model.linears()
             self.x = [torch.empty(rows, d, **bf), torch.empty(rows, d, **bf)]
             self.delta = torch.empty(rows, d, **bf)
-            self.qkv = torch.empty(rows, (cfg.n_heads + 2 * cfg.n_kv_heads) * hd, **bf)
+            # of one layer after the other, or of every layer to keep
+            self.qkv = torch.empty(cfg.n_layers if each_qkv else 1, rows, (cfg.n_heads + 2 * cfg.n_kv_heads) * hd, **bf)
             self.q = torch.empty(rows, cfg.n_heads * hd, **bf)
             self.attn = torch.zeros(rows, cfg.n_heads * hd, **bf)  # rows past their count are not written
             self.gu = torch.empty(rows, 2 * cfg.d_ff, **bf)
@@ -678,7 +679,6 @@ class Int4DecodeLM:
         mean nothing (for a count of 0 none do). Rows that are not active store nothing. ``advance`` adds the counts
         of active rows to ``st.lengths``. Chunks of any size follow one another; T = 1 is a decode step without the
         pick. Only device work is issued."""
-        cfg, lib = self.cfg, _lib.load()
         if not st.block_kv:
             raise ValueError(f"extend needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         if tokens.ndim != 2 or tokens.shape[0] != st.batch or tokens.shape[1] < 1 or tokens.dtype != torch.int32:
@@ -686,23 +686,38 @@ class Int4DecodeLM:
         if counts is not None and (tuple(counts.shape) != (st.batch,) or counts.dtype != torch.int32):
             raise ValueError(f"counts must be int32 [{st.batch}], got {tuple(counts.shape)} of {counts.dtype}")
         st.check_rows("Int4DecodeLM.extend")
-        dev = _lib.require_device(tokens, counts, self.embed, st.lengths, fn="Int4DecodeLM.extend")
+        _lib.require_device(tokens, counts, self.embed, st.lengths, fn="Int4DecodeLM.extend")
+        stored = self._stored(st, tokens.shape[1], counts)
+        logits, _ = self._pass(st, tokens.contiguous(), stored, last_only)
+        if advance:
+            st.lengths.add_(stored)
+        return logits
+
+    @staticmethod
+    def _stored(st: DecodeState, t: int, counts: Tensor | None) -> Tensor:
+        """How many of its t tokens each row stores: its count, none where it is not active."""
+        n = torch.full((st.batch,), t, dtype=torch.int32, device=st.lengths.device) if counts is None else counts.clamp(0, t)
+        return n * (st.active != 0)
+
+    def _pass(self, st: DecodeState, tokens: Tensor, stored: Tensor, last_only: bool = False,
+              each_qkv: bool = False) -> tuple[Tensor, Tensor]:
+        """The layers over ``tokens`` [B, T], of which the cache keeps ``stored`` a row: the logits, and the fused projections
+        q|k|v [layers, B * T, (H + 2 Hkv) hd] of every layer (``each_qkv``), else the last one's."""
+        cfg, lib, dev = self.cfg, _lib.load(), st.lengths.device
         B, T = tokens.shape
-        d, H, Hkv, hd = cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
-        tokens = tokens.contiguous()
-        stored = torch.full((B,), T, dtype=torch.int32, device=dev) if counts is None else counts.clamp(0, T)
-        stored = stored * (st.active != 0)
-        rows = _Rows(self, B * T)
-        nb = int(lib.sqx_kvblock_attention_workspace_bytes(B, T, H, Hkv, hd, st.k.shape[3], st.block_table.shape[1]))
+        rows = _Rows(self, B * T, each_qkv=each_qkv)
+        nb = int(lib.sqx_kvblock_attention_workspace_bytes(B, T, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, st.k.shape[3],
+                                                           st.block_table.shape[1]))
         ws = torch.empty(max(nb // 4, 4), dtype=torch.float32, device=dev)
         with torch.cuda.device(dev):
             s = _lib.stream_ptr(dev)
-            _lib.check(lib.sqx_embed(self.embed.data_ptr(), cfg.vocab_size, tokens.data_ptr(), B * T, d,
+            _lib.check(lib.sqx_embed(self.embed.data_ptr(), cfg.vocab_size, tokens.data_ptr(), B * T, cfg.d_model,
                                      rows.x[0].data_ptr(), s), "embed")
             cur, delta, dsplit = 0, None, 0
             for li, ly in enumerate(self.layers):
-                cur = self._norm_linear(rows, cur, delta, ly.attn_norm, ly.wqkv, rows.qkv, s, dsplit)
-                self._block_attention(st, li, rows.qkv, rows.q, rows.attn, B, T, stored, ws, s)
+                qkv = rows.qkv[li if each_qkv else 0]
+                cur = self._norm_linear(rows, cur, delta, ly.attn_norm, ly.wqkv, qkv, s, dsplit)
+                self._block_attention(st, li, qkv, rows.q, rows.attn, B, T, stored, ws, s)
                 delta, dsplit = self._delta_linear(rows, ly.wo, rows.attn, s)
                 cur = self._norm_linear(rows, cur, delta, ly.ffn_norm, ly.w13, rows.act, s, dsplit, swiglu=True)
                 delta, dsplit = self._delta_linear(rows, ly.w2, rows.act, s)
@@ -717,9 +732,46 @@ class Int4DecodeLM:
             else:
                 logits = torch.empty(B, T, cfg.vocab_size, dtype=torch.bfloat16, device=dev)
                 self._norm_linear(rows, cur, delta, self.final_norm, self.lm_head, logits, s, dsplit)
-            if advance:
-                st.lengths.add_(stored)
-        return logits
+        return logits, rows.qkv
+
+    def _open_blocks(self, st: DecodeState, rows: Tensor, saved: Tensor | None = None) -> Tensor:
+        """A copy of the blocks that the rows with ``rows`` not zero are in the middle of, in all layers; with ``saved`` they
+        are put back from it."""
+        cfg, lib, dev = self.cfg, _lib.load(), st.lengths.device
+        hkv, hd, pages, block = cfg.n_kv_heads, cfg.head_dim, st.k.shape[1], st.k.shape[3]
+        back = saved is not None
+        if saved is None:
+            saved = torch.empty(int(lib.sqx_kvblock_open_bytes(cfg.n_layers, st.batch, hkv, hd, block)), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(lib.sqx_kvblock_open(
+                back, st.k.data_ptr(), st.v.data_ptr(), st.k_scale.data_ptr(), st.v_scale.data_ptr(), st.block_table.data_ptr(),
+                st.lengths.data_ptr(), rows.data_ptr(), cfg.n_layers, st.batch, hkv, hd, block, pages, st.block_table.shape[1],
+                saved.data_ptr(), saved.numel(), _lib.stream_ptr(dev)), "open blocks")
+        return saved
+
+    def _write_again(self, st: DecodeState, qkv: Tensor, t: int, counts: Tensor) -> None:
+        """Store the keys and values of ``counts`` of each row's t tokens in all layers from what a pass projected. The layers
+        are rows of one write: layer l's page p is page l * pages + p of the whole cache."""
+        cfg, lib, dev, B = self.cfg, _lib.load(), st.lengths.device, st.batch
+        H, hkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+        pages, block, width = st.k.shape[1], st.k.shape[3], st.block_table.shape[1]
+        fmt = _lib.KV_INT8 if st.k.dtype == torch.int8 else _lib.KV_E4M3
+        row = (H + 2 * hkv) * hd
+        on = (st.block_table >= 0) & (st.block_table < pages)
+        each = max(1, min(cfg.n_layers, 65535 // B))  # layers of a call: it takes fewer than 65536 rows
+        first = torch.arange(each, dtype=torch.int32, device=dev)[:, None, None] * pages
+        table = torch.where(on, st.block_table + first, -1)
+        starts, counts = st.lengths.repeat(each), counts.repeat(each)
+        with torch.cuda.device(dev):
+            s = _lib.stream_ptr(dev)
+            for l in range(0, cfg.n_layers, each):
+                n = min(each, cfg.n_layers - l)
+                at = qkv[l].data_ptr()
+                _lib.check(lib.sqx_kvblock_write(
+                    at + 2 * H * hd, at + 2 * (H + hkv) * hd, _lib.DTYPE_BF16, t * row, row, hd, t * row, row, hd, None, 0, 0, 0,
+                    None, self.cos.data_ptr(), self.sin.data_ptr(), cfg.context_length, hd, 1, fmt, st.k[l].data_ptr(),
+                    st.v[l].data_ptr(), st.k_scale[l].data_ptr(), st.v_scale[l].data_ptr(), table.data_ptr(), starts.data_ptr(),
+                    counts.data_ptr(), n * B, t, H, hkv, hd, block, n * pages, width, s), "cache write")
 
     def _final_norm(self, rows: "_Rows", cur: int, delta: int | None, splits: int, stream: int) -> None:
         cfg, lib = self.cfg, _lib.load()
@@ -739,26 +791,35 @@ class Int4DecodeLM:
         token follows, because the row of logits behind the kept ones is no distribution (-1 in ``tokens``), the row stays
         before it: ``st.tokens`` is its last kept token and ``st.lengths`` grows by one less, so that the next pass scores
         that token anew.
-        ``counts`` is how many drafts a row has (default T). What rejected drafts left in the cache lies behind the new
-        length and is written over; a block's scale that one of them raised stays raised until the block is begun anew."""
+        ``counts`` is how many drafts a row has (default T). Rejected drafts leave no trace before the new length: the blocks
+        that they shared with older or kept tokens are put back and the kept tokens stored again without them, as a chunk
+        of those alone would be."""
         fn = "Int4DecodeLM.verify"
         if draft.ndim != 2 or draft.shape[0] != st.batch or draft.dtype != torch.int32:
             raise ValueError(f"draft must be int32 [{st.batch}, T], got {tuple(draft.shape)} of {draft.dtype}")
         t = draft.shape[1]
-        if st.block_kv:
-            st.check_rows(fn)
+        if not st.block_kv:
+            raise ValueError(f"verify needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         # all of it before the pass, which writes into the cache
+        st.check_rows(fn)
         temperature, u, r, draft_probs = speculative.check_arguments(fn, st.batch, t, self.cfg.vocab_size, draft, u, r, draft_probs,
                                                                      counts, temperature)
-        _lib.require_device(draft, u, r, draft_probs, counts, self.embed, fn=fn)
+        _lib.require_device(draft, u, r, draft_probs, counts, self.embed, st.lengths, fn=fn)
         ids = torch.cat((st.tokens[:, None], draft), 1)
-        logits = self.extend(st, ids, None if counts is None else counts.clamp(0, t) + 1, advance=False)
+        stored = self._stored(st, t + 1, None if counts is None else counts.clamp(0, t) + 1)
+        saved = self._open_blocks(st, stored)
+        logits, qkv = self._pass(st, ids, stored, each_qkv=True)
         n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)
         live = st.active != 0
         at = n.long()[:, None]
         nxt = tokens.gather(1, at)[:, 0]
         nxt_ok = nxt >= 0
-        st.lengths.add_((n + nxt_ok) * live)
+        kept = (n + nxt_ok) * live
+        # rows that keep fewer tokens than the pass stored: as it was before, then the kept ones
+        less = (kept < stored).to(torch.int32)
+        self._open_blocks(st, less, saved)
+        self._write_again(st, qkv, t + 1, kept * less)
+        st.lengths.add_(kept)
         st.tokens.copy_(torch.where(live, torch.where(nxt_ok, nxt, ids.gather(1, at)[:, 0]), st.tokens))
         return n, tokens
 

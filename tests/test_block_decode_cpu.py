@@ -67,3 +67,29 @@ def test_tables_that_stay_allowed():
         for call in (lambda: m.step(st), lambda: m.extend(st, ids)):
             with pytest.raises(RuntimeError, match="device tensors"):
                 call()
+
+
+def test_open_blocks_refuse():
+    """Every check of sqx_kvblock_open, before anything reaches the GPU (a non-null pointer is never followed)."""
+    import ctypes
+
+    from scratch_llm_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(256)
+
+    def call(**c):
+        a = dict(kc=p, vc=p, ks=p, table=p, starts=p, L=2, B=3, Hkv=1, hd=64, block=16, pages=4, width=2, saved=p, nb=1 << 20)
+        a.update(c)
+        return lib.sqx_kvblock_open(0, a["kc"], a["vc"], a["ks"], p, a["table"], a["starts"], None, a["L"], a["B"], a["Hkv"], a["hd"],
+                                    a["block"], a["pages"], a["width"], a["saved"], a["nb"], None)
+
+    for bad in (dict(L=-1), dict(L=1 << 16), dict(B=1 << 16), dict(Hkv=0), dict(hd=96), dict(block=48), dict(pages=0), dict(width=0),
+                dict(kc=None), dict(ks=None), dict(table=None), dict(starts=None), dict(saved=None), dict(vc=ctypes.c_void_p(8)),
+                dict(saved=ctypes.c_void_p(24))):
+        assert call(**bad) == -1, bad
+        assert b"sqx_kvblock_open" in lib.sqx_last_error()
+    assert lib.sqx_kvblock_open_bytes(2, 3, 1, 64, 16) == 2 * 3 * 2 * (16 * 64 + 4)
+    assert call(nb=2 * 3 * 2 * (16 * 64 + 4) - 1) == -3
+    assert call(L=0) == 0 and call(B=0) == 0
+    for none in ((0, 3, 1, 64, 16), (2, 3, 1, 80, 16), (2, 3, 1, 64, 20), (2, 0, 1, 64, 16)):
+        assert lib.sqx_kvblock_open_bytes(*none) == 0

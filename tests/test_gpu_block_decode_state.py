@@ -52,6 +52,27 @@ def same(a, b):
     return all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def layer0(st, row, n):
+    """Values of a row's first n positions in layer 0, and the scales of their blocks."""
+    from scratch_llm_amd.quant import kv_block
+
+    block = st.k.shape[3]
+    k, v = kv_block.read_kv_blocks(*st.kv_layer(0), st.block_table[row:row + 1], i32([0]), n)
+    page = st.block_table[row, :-(-n // block)].long()
+    return k, v, st.k_scale[0, page], st.v_scale[0, page]
+
+
+# prompt lengths (blocks of 16), drafts that are kept, drafts a row has
+ROWS = [(10, 7, 8),   # kept tokens reach into a block that the pass begins; the loud rejected one lies behind them in it
+        (13, 8, 8),   # all kept, the loud one too
+        (10, 3, 8),   # not active; its table names row 0's pages
+        (16, 0, 8),   # at a block's first slot: nothing older is in the block
+        (9, 2, 8),    # the loud rejected one lies in the block that holds older tokens
+        (7, 0, 5),    # the same, nothing kept but the current token
+        (12, 1, 1),   # one draft, kept
+        (15, 0, 0)]   # none
+
+
 def test_any_flag_but_zero_is_active(model):
     """`active` is read as the step's `advance` reads it: a row is active where its flag is not zero."""
     B = 2
@@ -102,3 +123,137 @@ def test_a_row_without_a_next_token_stays_before_it(model, temperature):
     assert tok[0].tolist() == [int(draft[0, 0]), NAN, -1, -1] and tok[1].tolist() == [-1] * 4
     assert st.lengths.tolist() == [14, 12, 16]
     assert st.tokens.tolist() == [NAN, NAN, int(tok[2, 3])] and int(st.tokens[2]) >= 0
+
+
+@pytest.mark.parametrize("hkv,d,block", [(1, 64, 16), (3, 64, 32), (2, 256, 16), (8, 128, 64), (5, 128, 128)])
+def test_open_blocks_are_put_back(hkv, d, block):
+    """What sqx_kvblock_open saves of three layers it puts back whole, for the rows that are asked for and are in the middle of
+    a block on a page, and nothing else."""
+    from scratch_llm_amd import _lib
+
+    print_case("open blocks", hkv, d, block)
+    L, pages, width = 3, 9, 2
+    starts = [1, block - 1, block, 0, block + 3, 2 * block - 1, 2 * block + 1, -5, 3, 7]
+    rows = [1, 1, 1, 1, 5, 1, 1, 1, 0, 1]
+    B = len(starts)
+    table = torch.tensor([[0, 1], [2, 1], [1, 3], [3, 1], [1, 4], [1, 5], [6, 6], [6, 6], [7, 1], [9, 1]], dtype=torch.int32)
+    open_pages = [0, 2, 4, 5]
+    g = torch.Generator().manual_seed(block + d)
+    codes = [torch.randint(0, 256, (L, pages, hkv, block * d), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2)]
+    scales = [torch.rand(L, pages, hkv, generator=g).to(DEV) for _ in range(2)]
+    held = [x.clone() for x in codes + scales]
+    lib = _lib.load()
+    nb = lib.sqx_kvblock_open_bytes(L, B, hkv, d, block)
+    saved = torch.zeros(nb + 64, dtype=torch.uint8, device=DEV)
+    table, st, rw = table.to(DEV), i32(starts), i32(rows)
+
+    def go(back):
+        _lib.check(lib.sqx_kvblock_open(back, *(x.data_ptr() for x in codes + scales), table.data_ptr(), st.data_ptr(), rw.data_ptr(), L,
+                                        B, hkv, d, block, pages, width, saved.data_ptr(), nb,
+                                        torch.cuda.current_stream().cuda_stream), "open")
+
+    go(0)
+    assert all(torch.equal(x, y) for x, y in zip(codes + scales, held)) and int(saved[nb:].max()) == 0
+    other = [torch.randint(0, 256, x.shape, generator=g, dtype=torch.uint8).to(DEV) for x in codes]
+    other += [torch.rand(x.shape, generator=g).to(DEV) for x in scales]
+    for x, y in zip(codes + scales, other):
+        x.copy_(y)
+    go(1)
+    torch.cuda.synchronize()
+    for x, y, z in zip(codes + scales, held, other):
+        want = z.clone()
+        want[:, open_pages] = y[:, open_pages]
+        assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("replay", [False, True])
+@pytest.mark.parametrize("kv_dtype", KV)
+def test_rejected_drafts_leave_no_trace(model, kv_dtype, replay):
+    """After a verification the cache's first layer is, bit for bit, that of a pass over the kept tokens alone: neither the
+    older tokens' codes nor the scales nor the kept tokens' codes show what a rejected draft of many times their size did
+    to their blocks in between. Eager and as the second replay of a graph."""
+    print_case("verify leaves no trace", kv_dtype, replay)
+    B, T = len(ROWS), 8
+    start, kept, count = (list(x) for x in zip(*ROWS))
+    prompt = ids((B, 16), 1)
+    st, ref = (model.new_state(B, CTX, kv_dtype=kv_dtype, kv_block_size=16) for _ in range(2))
+    draft = ids((B, T), 2)
+    for b in range(B):
+        draft[b, min(kept[b], T - 1)] = LOUD
+    u = torch.full((B, T), 0.9999, device=DEV)
+    for b in range(B):
+        u[b, :kept[b]] = 0.0
+    r, counts = torch.full((B,), 0.3, device=DEV), i32(count)
+
+    def fill(s):
+        s.lengths.zero_()
+        s.active.fill_(1)
+        s.block_table.copy_(torch.arange(s.block_table.numel(), dtype=torch.int32, device=DEV).view_as(s.block_table))
+        for x in (s.k, s.v):
+            x.view(torch.uint8).zero_()
+        s.k_scale.zero_()
+        s.v_scale.zero_()
+        model.extend(s, prompt, i32(start))
+        s.tokens.copy_(ids((B,), 3))
+        s.active[2] = 0
+        s.block_table[2] = s.block_table[0]
+
+    go = lambda: model.verify(st, draft, u, r, counts=counts)
+    fill(st)
+    n, tok = go()
+    if replay:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            n, tok = go()
+        for _ in range(2):
+            fill(st)
+            graph.replay()
+    fill(ref)
+    before = ref.lengths.cpu().tolist()
+    tokens = torch.cat((ref.tokens[:, None], draft), 1)
+    model.extend(ref, tokens, i32([k + 1 for k in kept]))
+    live = [b for b in range(B) if b != 2]
+    assert [int(n[b]) for b in live] == [kept[b] for b in live]
+    assert [int(st.lengths[b]) for b in live] == [before[b] + kept[b] + 1 for b in live] and int(st.lengths[2]) == before[2]
+    for b in live:
+        for x, y, name in zip(layer0(st, b, int(st.lengths[b])), layer0(ref, b, int(ref.lengths[b])), ("keys", "values", "key scales", "value scales")):
+            assert torch.equal(x, y), f"row {b}: {name}"
+        assert int(st.tokens[b]) == int(tok[b, kept[b]])
+    # that the rejected drafts would have shown: written together with them, scales are larger
+    loud = model.new_state(B, CTX, kv_dtype=kv_dtype, kv_block_size=16)
+    fill(loud)
+    model.extend(loud, tokens, i32([c + 1 for c in count]), advance=False)
+    for b in (0, 4, 5):
+        page = int(st.block_table[b, (int(st.lengths[b]) - 1) // 16])
+        assert bool((loud.k_scale[0, page] > ref.k_scale[0, page]).all()) and bool((loud.v_scale[0, page] > ref.v_scale[0, page]).all())
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+def test_rejected_drafts_at_the_table(model, kv_dtype):
+    """Rows whose open block is on no page, past the table's end and at a negative length beside an ordinary one: nothing of
+    the other rows' pages changes but what the ordinary row's kept tokens change."""
+    print_case("verify at the table", kv_dtype)
+    B, T = 4, 5
+    st, ref = (model.new_state(B, 64, kv_dtype=kv_dtype, kv_block_size=32) for _ in range(2))
+    prompt, draft, cur = ids((B, 40), 4), ids((B, T), 5), ids((B,), 6)
+    draft[:, 2] = LOUD
+    u = torch.full((B, T), 0.9999, device=DEV)
+    u[:, :2] = 0.0
+    for s in (st, ref):
+        model.extend(s, prompt)
+        s.tokens.copy_(cur)
+        s.block_table[1, 1] = 1 << 20
+        s.lengths[2] = 70  # the table ends at 64
+        s.lengths[3] = -3
+    held = raw(st)
+    n, tok = model.verify(st, draft, u, torch.full((B,), 0.3, device=DEV))
+    model.extend(ref, torch.cat((cur[:, None], draft), 1), i32([3, 0, 0, 0]))
+    assert int(n[0]) == 2
+    for x, y in zip(layer0(st, 0, 43), layer0(ref, 0, 43)):
+        assert torch.equal(x, y)
+    mine = st.block_table[0].long()
+    for x, y in zip(raw(st), held):
+        keep = torch.ones(x.shape[1], dtype=torch.bool, device=DEV)
+        keep[mine] = False
+        assert torch.equal(x[:, keep], y[:, keep])
