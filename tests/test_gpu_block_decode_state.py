@@ -257,3 +257,66 @@ def test_rejected_drafts_at_the_table(model, kv_dtype):
         keep = torch.ones(x.shape[1], dtype=torch.bool, device=DEV)
         keep[mine] = False
         assert torch.equal(x[:, keep], y[:, keep])
+
+
+def test_scores_are_those_of_the_whole_chunk():
+    """A chunk is attended over a cache that holds all of it, so a loud token scales its block for the tokens before it in the
+    chunk as well: the scores are those of the reference over a cache written so, loud token or not."""
+    from tests.test_gpu_block_decode import BlockRefCache, check, ref_chunk
+    from tests.test_gpu_block_decode import CTX as REF_CTX
+
+    p = D.random_params(**SMALL, seed=21, std=0.05)
+    k, v = p["blocks.0.attn.k_proj.weight"], p["blocks.0.attn.v_proj.weight"]
+    e = sum(x / x.norm() for w in (k, v) for x in (w[5], w[128 + 9]))
+    p["token_emb.weight"][LOUD] = e * (SMALL["d_model"] ** 0.5 / e.norm())
+    model = build(p)
+    refs = {dt: D.int4_model(p, n_layers=SMALL["n_layers"], n_heads=SMALL["n_heads"], n_kv_heads=SMALL["n_kv_heads"],
+                             context_length=REF_CTX, dtype=dt) for dt in (torch.bfloat16, torch.float32)}
+    B = 2
+    st = model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=16)
+    caches = {dt: BlockRefCache.make(r, B, dt, "int8", 16) for dt, r in refs.items()}
+    prompt, chunk = ids((B, 10), 41).cpu(), ids((B, 4), 42).cpu()
+    chunk[0, 2] = LOUD
+    for x in (prompt, chunk):
+        got = model.extend(st, x.to(DEV))
+        l16, l32 = ref_chunk(refs, caches, x, [x.shape[1]] * B)
+        check(got, l16, l32, f"chunk of {x.shape[1]}")
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+def test_speculation_follows_a_clear_continuation(kv_dtype):
+    """A head whose row of the token that follows t is t's embedding, behind layers that add little: every pick is far ahead of
+    the next best, so counts and continuation hold without conditions. Rows: all kept; a wrong second draft; an id
+    outside the vocabulary first; fewer drafts than the others."""
+    p = D.random_params(**SMALL, seed=31, std=0.02)
+    follows = torch.randperm(SMALL["vocab"], generator=torch.Generator().manual_seed(32))
+    p["lm_head.weight"] = torch.zeros_like(p["lm_head.weight"])
+    p["lm_head.weight"][follows] = 0.05 * p["token_emb.weight"]
+    model = build(p)
+    B, T = 4, 4
+    plain, spec = (model.new_state(B, CTX, kv_dtype=kv_dtype, kv_block_size=16) for _ in range(2))
+    prompt = ids((B, 13), 33)
+    for s in (plain, spec):
+        s.tokens.copy_(model.extend(s, prompt, last_only=True).argmax(-1).to(torch.int32))
+    want = [spec.tokens.cpu()]
+    assert want[0].tolist() == follows[prompt[:, -1].long().cpu()].tolist()
+    for _ in range(20):
+        model.step(plain)
+        top = plain.logits.float().topk(2, -1).values
+        assert bool((top[:, 0] - top[:, 1] > 2.0**-3 * top[:, 0]).all())
+        want.append(plain.tokens.cpu().clone())
+        assert want[-1].tolist() == follows[want[-2].long()].tolist()
+    want = torch.stack(want, 1)
+    have = [[int(want[b, 0])] for b in range(B)]
+    for step in range(3):
+        draft = torch.zeros(B, T, dtype=torch.int32)
+        for b in range(B):
+            draft[b] = want[b, len(have[b]):len(have[b]) + T]
+        draft[1, 1] = (draft[1, 1] + 1) % SMALL["vocab"]
+        draft[2, 0] = SMALL["vocab"]
+        n, tok = model.verify(spec, draft.to(DEV), None, None, temperature=0.0, counts=i32([T, T, T, 2]))
+        assert n.tolist() == [T, 1, 0, 2], f"step {step}"
+        for b in range(B):
+            have[b] += tok[b, :int(n[b]) + 1].tolist()
+            assert have[b] == want[b, :len(have[b])].tolist(), f"row {b} step {step}"
+            assert int(spec.lengths[b]) == 13 + len(have[b]) - 1 and int(spec.tokens[b]) == have[b][-1]
