@@ -320,3 +320,24 @@ def test_speculation_follows_a_clear_continuation(kv_dtype):
             have[b] += tok[b, :int(n[b]) + 1].tolist()
             assert have[b] == want[b, :len(have[b])].tolist(), f"row {b} step {step}"
             assert int(spec.lengths[b]) == 13 + len(have[b]) - 1 and int(spec.tokens[b]) == have[b][-1]
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+def test_steps_of_a_wide_batch(kv_dtype):
+    """70 rows: the step's linears are the prompt GEMM."""
+    from tests.test_gpu_block_decode import CTX as REF_CTX
+    from tests.test_gpu_block_decode import FMT, BlockRefCache, check, ref_steps
+
+    print_case("block kv step of 70 rows", kv_dtype)
+    p = D.random_params(**SMALL, seed=51, std=0.05)
+    model = build(p)
+    refs = {dt: D.int4_model(p, n_layers=SMALL["n_layers"], n_heads=SMALL["n_heads"], n_kv_heads=SMALL["n_kv_heads"],
+                             context_length=REF_CTX, dtype=dt) for dt in (torch.bfloat16, torch.float32)}
+    B = 70
+    st = model.new_state(B, CTX, kv_dtype=kv_dtype, kv_block_size=32)
+    caches = {dt: BlockRefCache.make(r, B, dt, FMT[kv_dtype], 32) for dt, r in refs.items()}
+    for t in range(3):
+        tok = ids((B,), 52 + t).cpu()
+        model.step(st, tok)
+        l16, l32 = ref_steps(refs, caches, tok[:, None])
+        check(st.logits, l16[:, 0], l32[:, 0], f"step {t}")
