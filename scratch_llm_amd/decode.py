@@ -677,14 +677,15 @@ class Int4DecodeLM:
         cache: their keys and values are stored, and bf16 logits [B, T, vocab] come back; ``last_only``: [B, vocab] of each
         row's last token. ``counts`` (int32 [B]; default T) is how many of a row's tokens are real; logits past them
         mean nothing (for a count of 0 none do). Rows that are not active store nothing. ``advance`` adds the counts
-        of active rows to ``st.lengths``. Chunks of any size follow one another; T = 1 is a decode step without the
-        pick. Only device work is issued."""
+        of active rows to ``st.lengths``. Chunks follow one another, each of fewer than 2^30 / d_ff tokens over all rows; T = 1 is a
+        decode step without the pick. Only device work is issued."""
         if not st.block_kv:
             raise ValueError(f"extend needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         if tokens.ndim != 2 or tokens.shape[0] != st.batch or tokens.shape[1] < 1 or tokens.dtype != torch.int32:
             raise ValueError(f"tokens must be int32 [{st.batch}, T], got {tuple(tokens.shape)} of {tokens.dtype}")
         if counts is not None and (tuple(counts.shape) != (st.batch,) or counts.dtype != torch.int32):
             raise ValueError(f"counts must be int32 [{st.batch}], got {tuple(counts.shape)} of {counts.dtype}")
+        self._check_pass(*tokens.shape, "Int4DecodeLM.extend")
         st.check_rows("Int4DecodeLM.extend")
         _lib.require_device(tokens, counts, self.embed, st.lengths, fn="Int4DecodeLM.extend")
         stored = self._stored(st, tokens.shape[1], counts)
@@ -692,6 +693,16 @@ class Int4DecodeLM:
         if advance:
             st.lengths.add_(stored)
         return logits
+
+    def _check_pass(self, b: int, t: int, fn: str) -> None:
+        """Refuses a pass that a kernel would refuse behind others that have stored a layer's keys and values already."""
+        cfg = self.cfg
+        most = ((1 << 31) - 1) // (2 * max(cfg.d_model, cfg.n_heads * cfg.head_dim, cfg.d_ff))
+        if b * t > max(most, _SKINNY_MAX_M):
+            raise ValueError(f"{fn}: {b} rows of {t} tokens, at most {most} of this model in one pass (2 GiB of activations a linear): "
+                             "take smaller chunks")
+        if t >= 1 << 24 or -(-t * (cfg.n_heads // cfg.n_kv_heads) // 256) >= 1 << 16:
+            raise ValueError(f"{fn}: {t} tokens a row are too many for one pass: take smaller chunks")
 
     @staticmethod
     def _stored(st: DecodeState, t: int, counts: Tensor | None) -> Tensor:
@@ -802,6 +813,7 @@ class Int4DecodeLM:
             raise ValueError(f"verify needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         # all of it before the pass, which writes into the cache
         st.check_rows(fn)
+        self._check_pass(st.batch, t + 1, fn)
         temperature, u, r, draft_probs = speculative.check_arguments(fn, st.batch, t, self.cfg.vocab_size, draft, u, r, draft_probs,
                                                                      counts, temperature)
         _lib.require_device(draft, u, r, draft_probs, counts, self.embed, st.lengths, fn=fn)

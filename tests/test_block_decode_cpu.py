@@ -69,6 +69,20 @@ def test_tables_that_stay_allowed():
                 call()
 
 
+def test_a_pass_that_a_linear_cannot_take_is_refused():
+    """Rows of 256 columns of bf16 below 2 GiB: 2^22 - 1 of them. More are refused before anything is written."""
+    m, st = model(), state()
+    assert CFG.d_model == CFG.d_ff == 256
+    m._check_pass(2, (1 << 21) - 1, "f")
+    for t in (1 << 21, 1 << 23):
+        with pytest.raises(ValueError, match="smaller chunks"):
+            m.extend(st, torch.zeros(1, dtype=torch.int32).expand(2, t))
+    one = state(batch=1)
+    m._check_pass(1, (1 << 22) - 1, "f")
+    with pytest.raises(ValueError, match="smaller chunks"):
+        m.extend(one, torch.zeros(1, dtype=torch.int32).expand(1, 1 << 22))
+
+
 def test_open_blocks_refuse():
     """Every check of sqx_kvblock_open, before anything reaches the GPU (a non-null pointer is never followed)."""
     import ctypes
