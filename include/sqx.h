@@ -856,8 +856,8 @@ int sqx_rope(const void* x, int dtype, int64_t n, int64_t heads, int64_t d, int6
  *   finite new values. A block that keeps earlier tokens: s 2^k with the least k >= 0 for which a <= s 2^k, and its codes
  *   become rne(c 2^-k).
  *   code = clamp(rint(fl(x / s)), -127, 127), NaN 0; or the saturating E4M3 cast of fl(x / s).
- * Nothing is stored for a negative start, outside the table, or where it names no page. The rows of one call must not
- * write the same page. */
+ * Nothing is stored for a negative start, outside the table, or where it names no page. No page may be written twice by
+ * one call, by two rows or by two blocks of one. */
 int sqx_kvblock_write(const void* k, const void* v, int dtype, int64_t k_sb, int64_t k_st, int64_t k_sh, int64_t v_sb,
                       int64_t v_st, int64_t v_sh, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, void* q_out,
                       const float* cos_t, const float* sin_t, int64_t rope_rows, int64_t rot, int interleaved, int fmt,
@@ -905,7 +905,8 @@ int sqx_kvblock_attention(const void* q, int dtype, int64_t q_sb, int64_t q_st, 
  *   zero everywhere; a NaN of q takes the token out), p_n after none; p, weights and sums in double.
  * temperature 0: accepted while x_t is the first maximum of its row (NaN counts as the maximum), then that maximum; u, r
  * and probs are not read. tokens [B, T + 1]: the accepted drafts, the next token, then -1. An id outside [0, V) is
- * rejected. A row that is no distribution (a NaN, +inf, or -inf everywhere) rejects its draft and its next token is -1. */
+ * rejected. At other temperatures a row that is no distribution (a NaN, +inf, or -inf everywhere) rejects its draft and its
+ * next token is -1. */
 int64_t sqx_verify_draft_workspace_bytes(int64_t B, int64_t T, int64_t V);
 int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int* counts, const void* probs,
                      int probs_dtype, const float* u, const float* r, double temperature, int64_t B, int64_t T, int64_t V,

@@ -237,10 +237,11 @@ __device__ inline float scale_or_tiny(float s) { return fmaxf(s, kTinyScale) + (
 // rows, where reading the cache once is the bound: the four waves take alternate 64-key steps straight from memory into
 // registers and share nothing until the end. A step's keys are loaded while the step before is worked on.
 //
-// Measured with 32 heads over 8 kv heads of 128: one token in 64 rows of up to 8192 keys 150 us, 5.3 TB/s; in 3 rows of
-// 800000 keys 830 us, 5.9 TB/s; over 2048 keys 7 us, the latency of two steps a wave and the join through LDS. Five tokens in
-// 16 rows of E4M3 73 us where one row of 16000 keys stands beside others of half, 4.1 TB/s (62 us, 4.8 TB/s, with even
-// rows). Cutting all rows' steps laid end to end into equal parts, so that the workgroups end together, took 74 us there.
+// Measured with 32 heads over 8 kv heads of 128: one token in 64 rows of up to 8192 keys 151 us a call, 5.2 TB/s; in 3 rows of
+// 800000 keys 836 us, 5.8 TB/s; over 2048 keys 7 us, the latency of two steps a wave and the join through LDS. Five tokens in
+// 16 rows of E4M3 80 us a call where one row of 16000 keys stands beside others of half, 3.8 TB/s; int8 74. E4M3 with R = 2 and
+// heads of 128 spills 36 to 41 registers, which the NaNs' put-back below holds whether it runs or not. Cutting all rows' steps
+// laid end to end into equal parts, so that the workgroups end together, took 74 us in the kernel where this order took 73.
 template <int D, int R, bool E4M3, bool BF16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_kernel(const KvAttnArgs a) {
   constexpr int KD = D / 64;  // 16-byte pieces of a key per lane
@@ -530,8 +531,8 @@ __device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, c
 // The products are v_mfma_f32_32x32x16_f16, with the row order of the direct kernel carried over: row p of a 32-key tile is
 // key 16 ((p / 4) % 2) + 4 (p / 8) + p % 4, so that lane (hi, r) gets the scores of 16 hi .. 16 hi + 15.
 //
-// 2 rows, 2048 tokens of 32 heads (8 kv heads) and up to 6000 keys: 247 us, 908 TFLOP/s; 4 even rows of as many tokens run at
-// 1005, a library product of 8192^3 in fp16 at 1101. Bound by the vector and the matrix unit together: on this card two waves
+// 2 rows, 2048 tokens of 32 heads (8 kv heads) and up to 6000 keys: 247 us, 908 TFLOP/s (E4M3, whose forms all spill, 19 to 128
+// registers: 259); 4 even rows of as many tokens run at 1005, a library product of 8192^3 in fp16 at 1101. Bound by the vector and the matrix unit together: on this card two waves
 // of a SIMD overlap little of them (an MFMA of 16 cycles hides two vector instructions; 16x16x32 with four vector
 // instructions and an exponential takes 33.7 ns for two waves where the parts take 16.3, 10.2 and 7.6, the 32x32x16 form
 // 27.9). So vector instructions are what counts. Two groups of waves half a tile apart (one in its products while the other
@@ -540,7 +541,8 @@ __device__ inline void softmax_step32(f32x16_t (&sc)[N], int behind, float qs, c
 // shortest share a CU with the longest, 309 against 278 under the profiler; 128 rows in four waves 366 against 338.
 //
 // BIG: pages of 64 tokens or more, so a 64-key piece lies in one. Its page and scales are the same for all lanes and addresses
-// are scalar; the per-lane form costs 70 vector instructions a tile, a fifth of all.
+// are scalar; the per-lane form costs 70 vector instructions a tile, a fifth of all: 270 and 261 us with pages of 16 and 32
+// tokens where 64 take 247.
 constexpr int tile_waves(int d) { return d == 256 ? 4 : 8; }
 constexpr int tile_rows(int d) { return 32 * tile_waves(d); }
 template <int D, bool E4M3, bool BF16, bool BIG>
@@ -842,7 +844,8 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, i
 }
 
 // How a call is laid out: 16-row tiles of a workgroup of the direct kernel (0: the tile kernel), tiles of rows, and
-// the parts that its keys are cut into.
+// the parts that its keys are cut into. The host knows the table's width, not what the rows hold: one token over 2048 keys
+// takes 9.6 us behind a table of 2048 tokens and 11.5 behind one of 32768 to 524288, 16 rows of it 22.5 behind any.
 struct KvAttnPlan {
   int R, tiles, splits;
 };

@@ -1,9 +1,9 @@
 // The block-scaled 8-bit KV cache: writing new tokens (quantized as they are written, rotary positions included) and
 // reading values back. Layout and code formats: sqx_kvblock.h.
 //
-// A block's scale. A block whose first token is part of the write takes s = max(fl(amax / qmax), 1e-12) over the tokens
-// written (the product with fl(1 / qmax), qmax 127 or 448). A block that already holds tokens keeps its scale, doubled k
-// times, the least k with fl(amax / qmax) <= s 2^k, and its codes become rne(c 2^-k). With growth in powers of two every later rescale at least
+// A block's scale. A block whose first token is part of the write takes s = max(a, 1e-12), a = fl(amax fl(1 / qmax)) over the
+// tokens written, qmax 127 or 448. A block that already holds tokens keeps its scale, doubled k times, the least k with
+// a <= s 2^k, and its codes become rne(c 2^-k). With growth in powers of two every later rescale at least
 // doubles the step, so what the rescales add to a token's error is at most s/2 (1 + 1/2 + 1/4 + ...) < s of the final
 // scale, however often the block grows; growing to each token's own amax would add s/2 at every token.
 // amax is taken over finite magnitudes: infinities saturate to the largest code, a NaN is a NaN in E4M3 and 0 in int8.
@@ -51,9 +51,10 @@ __device__ inline void rotate_lane(Row8<DT>& x, int c, int rot, bool inter, cons
 // then groups of kQHeads query heads, whose rotation needs no block. A block's scale needs all of its new tokens before the
 // first code, so a workgroup holds a block of one head in registers and reads it once.
 //
-// Bound by HBM for prompts: 12977 tokens in 8 rows, 32 query and 8 kv heads of 128, bf16 to int8: 70 us, 4.2 TB/s (two
-// thirds of it queries; eight heads a workgroup took 81). One token in each of 8 rows takes 5.8 us: a launch and a chain of
-// table, scale and old codes.
+// Bound by HBM for prompts: 12977 tokens in 8 rows, 32 query and 8 kv heads of 128, bf16 to int8: 80 us, 3.7 TB/s (the least of
+// 27 passes 70, of the form with eight heads a workgroup 81). Two thirds of that are queries, which need no block: their
+// four rounds of load, rotate and store wait for one another. One token in each of 8 rows takes 5.8 us: a launch and a
+// chain of table, scale and old codes, behind which the rows and angles are loaded.
 //
 // A thread holds 8 columns of NP tokens: of a whole block, tokens NP tl .. NP tl + NP - 1, so that four codes of a value
 // column are one dword of the transposed tile; of at most 256 / C tokens (NP = 1), token tl of the write. Slots outside

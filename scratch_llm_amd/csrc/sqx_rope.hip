@@ -3,8 +3,9 @@
 //
 // y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos, in fp32 with every product and sum rounded on its own, rounded once
 // to x's type. Three flops per element against two memory passes over it: bound by HBM for prompts (8191 tokens of 40 heads
-// of 128 columns in fp16, half of them rotated: 27 us, 6.3 TB/s), by the launch for a few tokens (one: 2.2 us). Rounding
-// pairs by the packed conversions instead of one by one was worth 31 -> 27 us.
+// of 128 columns in fp16, half of them rotated: 28 us, 6.1 TB/s, of which the 84 MB written partly end in the last cache; a
+// call among others 31 us, 5.5 TB/s), by the launch for a few tokens (one: 2.2 us). Rounding pairs by the packed conversions
+// instead of one by one was worth 31 -> 27 us.
 #include "sqx_kvblock.h"
 
 namespace sqx {
@@ -53,7 +54,8 @@ __global__ __launch_bounds__(256) void rope_kernel(const void* x, int64_t sn, in
     rope_columns<DT>(x, n * sn, sh, out, n * on, oh, h, hs, heads, c, rot, inter, ang);
 }
 
-// Any even rot and any alignment: a thread per pair (or per column past the rotated ones), two bytes a load.
+// Any even rot and any alignment: a thread per pair (or per column past the rotated ones), two bytes a load: 91 us where the
+// form above takes 29 (8191 tokens of 40 heads of 128, 40 and 48 columns rotated).
 template <int DT>
 __global__ __launch_bounds__(256) void rope_pairs_kernel(const void* x, int64_t sn, int64_t sh,
                                                          const int* __restrict__ pos, const float* __restrict__ cos_t,

@@ -678,7 +678,9 @@ class Int4DecodeLM:
         row's last token. ``counts`` (int32 [B]; default T) is how many of a row's tokens are real; logits past them
         mean nothing (for a count of 0 none do). Rows that are not active store nothing. ``advance`` adds the counts
         of active rows to ``st.lengths``. Chunks follow one another, each of fewer than 2^30 / d_ff tokens over all rows; T = 1 is a
-        decode step without the pick. Only device work is issued."""
+        decode step without the pick. A chunk is attended over a cache that holds all of it, and a block's scale goes by all
+        of its tokens: scores depend on the later tokens of their blocks by that much, up to a step of the codes. Only
+        device work is issued."""
         if not st.block_kv:
             raise ValueError(f"extend needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         if tokens.ndim != 2 or tokens.shape[0] != st.batch or tokens.shape[1] < 1 or tokens.dtype != torch.int32:
@@ -804,7 +806,7 @@ class Int4DecodeLM:
         that token anew.
         ``counts`` is how many drafts a row has (default T). Rejected drafts leave no trace before the new length: the blocks
         that they shared with older or kept tokens are put back and the kept tokens stored again without them, as a chunk
-        of those alone would be."""
+        of those alone would be. Only the scores have seen them, as those of :meth:`extend` see a chunk."""
         fn = "Int4DecodeLM.verify"
         if draft.ndim != 2 or draft.shape[0] != st.batch or draft.dtype != torch.int32:
             raise ValueError(f"draft must be int32 [{st.batch}, T], got {tuple(draft.shape)} of {draft.dtype}")

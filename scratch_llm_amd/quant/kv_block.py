@@ -110,13 +110,16 @@ def write_kv_blocks(k: Tensor, v: Tensor, k_codes: Tensor, v_codes: Tensor, k_sc
     rounded to their type, and the rotated ``q [B, T, H, D]`` is returned, if given (all T tokens), as
     :func:`~scratch_llm_amd.rope.apply_rope` rotates it.
 
-    A block whose first token is written takes the scale ``amax / 127`` (int8) or ``amax / 448`` (E4M3) of the
-    tokens written, at least 1e-12. A block that keeps earlier tokens has its scale doubled until the new
+    A block whose first token is written takes the scale ``amax * fl(1 / 127)`` (int8) or ``amax * fl(1 / 448)`` (E4M3)
+    of the tokens written, an fp32 product, at least 1e-12. A block that keeps earlier tokens has its scale doubled until the new
     ones fit, and its codes halved with it: the rescales together cost a token less than one step of the
     block's final scale. Infinities saturate; a NaN is stored as NaN in E4M3 and as 0 in int8.
 
-    Tokens at a negative start, outside the table, or on a page id outside the cache are not stored. Rows of
-    one call must not write to the same page."""
+    So what a block's tokens lose depends on all that was ever written into it, tokens that are written over later
+    included. To take tokens out again, keep the open block's codes and scales beside and put them back.
+
+    Tokens at a negative start, outside the table, or on a page id outside the cache are not stored. No page may be
+    written twice by one call, by two rows or by two blocks of one."""
     fn = "write_kv_blocks"
     if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError(f"{fn}: k and v must be [B, T, Hkv, D] alike, got {tuple(k.shape)} of {k.dtype}, {tuple(v.shape)} of {v.dtype}")
@@ -189,7 +192,9 @@ def attend_kv_blocks(q: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Tenso
     Token t of row b stands at position ``starts[b] + t`` and attends every position at and before it, ``H / Hkv``
     query heads to a kv head; ``scale`` defaults to ``1 / sqrt(D)``. Tokens from ``counts[b]`` on are left as they are
     in ``out`` (in a new output they are zero). A token at a negative position attends nothing and gets zeros; one
-    that attends a position on a page id outside the cache gets NaN. Positions past the table do not exist."""
+    that attends a position on a page id outside the cache gets NaN. Positions past the table do not exist. The work is laid out
+    for the table's width, as the lengths are on the device: with one row and a few thousand keys a table many times as wide
+    costs a fifth."""
     fn = "attend_kv_blocks"
     if q.ndim != 4:
         raise ValueError(f"{fn}: q must be [B, T, H, D], got {tuple(q.shape)}")

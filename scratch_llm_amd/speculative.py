@@ -3,7 +3,10 @@
 The reference samples one token from one row of logits (src/scratch_llm/sampling.py:80-86). Here a target
 model has scored several drafted tokens of every row in one pass (:meth:`Int4DecodeLM.extend`), and
 :func:`verify_draft` says how many of them to keep and which token follows, such that the kept tokens
-are distributed as the target's own. Random numbers are inputs, so a run can be repeated.
+are distributed as the softmax of those logits says. The logits are the target's own as far as scoring several tokens
+at once leaves them so: over the block-scaled cache a chunk's tokens share their blocks' scales, later drafts' among
+them (:mod:`scratch_llm_amd.quant.kv_block`), and its linears round in another order than one token's. Random
+numbers are inputs, so a run can be repeated.
 """
 
 from __future__ import annotations
@@ -59,12 +62,13 @@ def verify_draft(logits: Tensor, draft: Tensor, u: Tensor | None, r: Tensor | No
     draft was certain of its token), draft t is accepted while ``u[b, t] * q_t(x_t) < p_t(x_t)``. The token that
     follows is drawn from ``max(p - q, 0)`` of the first rejected row, or from ``p`` of the row behind the
     drafts: the least id whose cumulative weight exceeds ``r[b]`` times the total. What the pick is made from is
-    float64; the ``p_t(x_t)`` that a draft is accepted by is within 2^-18 of itself. ``temperature=0`` accepts while the draft is its row's argmax and then takes the argmax (``u``, ``r``
+    float64; the ``p_t(x_t)`` that a draft is accepted by is within 2^-18 of itself. ``temperature=0`` accepts while the
+    draft is its row's argmax (the first of equals; a NaN counts as the maximum) and then takes the argmax (``u``, ``r``
     and ``draft_probs`` may be None). ``counts`` (int32 ``[B]``) says how many drafts a row has (default T).
 
     ``u [B, T]`` and ``r [B]`` are float32 in [0, 1). Returns ``(n_accepted int32 [B], tokens int32 [B, T + 1])``:
-    the accepted drafts, the next token, then -1. An id outside the vocabulary is rejected; a row that is no
-    distribution (NaN, +inf, or -inf everywhere) rejects its draft and gives -1."""
+    the accepted drafts, the next token, then -1. An id outside the vocabulary is rejected. At temperatures above 0 a row
+    that is no distribution (NaN, +inf, or -inf everywhere) rejects its draft and gives -1; at 0 every row has an argmax."""
     fn = "verify_draft"
     if logits.ndim != 3 or draft.ndim != 2:
         raise ValueError(f"{fn}: logits must be [B, T + 1, V] and draft [B, T], got {tuple(logits.shape)}, {tuple(draft.shape)}")
