@@ -39,6 +39,7 @@ __all__ = ["DecodeConfig", "DecodeState", "Int4DecodeLM", "LLAMA3_8B", "rope_tab
 # Batches of 2..64 rows run the linears through sqx_int4_skinny's shape choice (the GEMV or a
 # decode-regime kernel, K split into the state's workspace); larger batches run the prefill GEMM.
 _SKINNY_MAX_M = i4.GEMM_MIN_M - 1
+_WRITE_ROWS = (1 << 16) - 1  # rows that one write into the block-scaled cache takes
 _BLOCK_KV = {"int8_block": torch.int8, "fp8_block": FP8_DTYPE}
 
 
@@ -771,7 +772,7 @@ class Int4DecodeLM:
         fmt = _lib.KV_INT8 if st.k.dtype == torch.int8 else _lib.KV_E4M3
         row = (H + 2 * hkv) * hd
         on = (st.block_table >= 0) & (st.block_table < pages)
-        each = max(1, min(cfg.n_layers, 65535 // B))  # layers of a call: it takes fewer than 65536 rows
+        each = max(1, min(cfg.n_layers, _WRITE_ROWS // B))  # layers of a call
         first = torch.arange(each, dtype=torch.int32, device=dev)[:, None, None] * pages
         table = torch.where(on, st.block_table + first, -1)
         starts, counts = st.lengths.repeat(each), counts.repeat(each)

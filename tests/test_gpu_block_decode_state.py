@@ -229,6 +229,30 @@ def test_rejected_drafts_leave_no_trace(model, kv_dtype, replay):
         assert bool((loud.k_scale[0, page] > ref.k_scale[0, page]).all()) and bool((loud.v_scale[0, page] > ref.v_scale[0, page]).all())
 
 
+@pytest.mark.parametrize("most", [5, 9, 14])
+def test_the_kept_tokens_layers_in_several_writes(most, monkeypatch):
+    """Where all layers' rows are more than a write takes, they go layer by layer or a few at a time, the last ones fewer: the
+    cache is the same. Three layers of 5 rows."""
+    from scratch_llm_amd import decode
+
+    p = D.random_params(**{**SMALL, "n_layers": 3}, seed=22, std=0.05)
+    cfg = decode.DecodeConfig(vocab_size=SMALL["vocab"], d_model=SMALL["d_model"], n_layers=3, n_heads=SMALL["n_heads"],
+                              n_kv_heads=SMALL["n_kv_heads"], d_ff=SMALL["d_ff"], context_length=CTX)
+    model = decode.Int4DecodeLM.from_state_dict(cfg, lambda n: p[n], DEV)
+    B, T = 5, 4
+    draft, u = ids((B, T), 61), torch.full((B, T), 0.9999, device=DEV)
+    u[0], u[2, :2] = 0.0, 0.0
+    states = []
+    for limit in (1 << 16, most):
+        st = model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=16)
+        model.extend(st, ids((B, 13), 62), i32([13, 12, 9, 11, 0]))
+        monkeypatch.setattr(decode, "_WRITE_ROWS", limit)
+        n, _ = model.verify(st, draft, u, torch.full((B,), 0.3, device=DEV))
+        assert n.tolist() == [4, 0, 2, 0, 0]
+        states.append(raw(st))
+    assert same(*states)
+
+
 @pytest.mark.parametrize("kv_dtype", KV)
 def test_rejected_drafts_at_the_table(model, kv_dtype):
     """Rows whose open block is on no page, past the table's end and at a negative length beside an ordinary one: nothing of
@@ -341,3 +365,31 @@ def test_steps_of_a_wide_batch(kv_dtype):
         model.step(st, tok)
         l16, l32 = ref_steps(refs, caches, tok[:, None])
         check(st.logits, l16[:, 0], l32[:, 0], f"step {t}")
+
+
+def test_two_states_on_two_streams(model):
+    """Verifications of two states issued beside each other on streams of their own: each as alone."""
+    B, T = 3, 4
+    draft, u = ids((B, T), 71), torch.full((B, T), 0.9999, device=DEV)
+    u[0], u[1, :2] = 0.0, 0.0
+    r = torch.full((B,), 0.4, device=DEV)
+
+    def fresh(seed):
+        s = model.new_state(B, CTX, kv_dtype="int8_block", kv_block_size=16)
+        model.extend(s, ids((B, 11), seed))
+        s.tokens.copy_(i32([3, 4, 5]))
+        return s
+
+    alone, beside = [fresh(72 + i) for i in range(2)], [fresh(72 + i) for i in range(2)]
+    for s in alone:
+        for _ in range(3):
+            model.verify(s, draft, u, r)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for s, stream in zip(beside, streams):
+            with torch.cuda.stream(stream):
+                model.verify(s, draft, u, r)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, beside):
+        assert same(raw(a) + [a.lengths, a.tokens], raw(b) + [b.lengths, b.tokens])
