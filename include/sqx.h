@@ -912,6 +912,45 @@ int sqx_verify_draft(const void* logits, int dtype, const int* draft, const int*
                      int probs_dtype, const float* u, const float* r, double temperature, int64_t B, int64_t T, int64_t V,
                      int* n_accepted, int* tokens, void* ws, int64_t ws_bytes, sqx_stream_t stream);
 
+/* Pages of the block-scaled KV cache. The caches of L layers lie one behind the other: k_codes [L, pages, Hkv, block, hd], v_codes
+ * [L, pages, Hkv, hd, block] (either format), scales [L, pages, Hkv]; one table int32 [B, width] for all. refs int32 [pages]
+ * counts the table entries that name a page, 0: free. An entry outside [0, pages) names none. All arguments in device memory
+ * are read there: a call that hands out pages writes 1 to ok, or 0 where there are too few free ones and then changes
+ * nothing else. Free pages are taken from the lowest on, row after row. ws: 16-byte aligned. */
+
+/* Copy page src[i] to page dst[i] (n < 2^31), all layers. Ids outside the pool and pairs of one page are left out. No page may
+ * be written by two pairs, or written by one and read by another. */
+int sqx_kvpages_copy(const int* src, const int* dst, int64_t n, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                     int64_t L, int64_t Hkv, int64_t hd, int64_t block, int64_t pages, sqx_stream_t stream);
+
+/* Every row b goes on from row parents[b] as it was before the call. parents[b] == b: unchanged; outside [0, B): emptied. Else it
+ * takes the parent's length n (within the table) and its pages of blocks below n / block, entries behind are -1; if block does not
+ * divide n, the page of block n / block is copied to a free page, but for the first such row of a parent that does not go on from
+ * itself, which takes that page. What the rows held is released first. */
+int64_t sqx_kvpages_fork_workspace_bytes(int64_t B, int64_t width, int64_t pages);
+int sqx_kvpages_fork(const int* parents, void* k_codes, void* v_codes, float* k_scale, float* v_scale, int* table, int* lengths,
+                     int* refs, int64_t L, int64_t B, int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width,
+                     int* ok, void* ws, int64_t ws_bytes, sqx_stream_t stream);
+
+/* The blocks of positions starts[b] .. starts[b] + counts[b] - 1 (those within the table; none for a negative start) get a free
+ * page where they have none, and a copy on a free page where refs of theirs exceeds 1. */
+int64_t sqx_kvpages_reserve_workspace_bytes(int64_t B, int64_t width, int64_t pages);
+int sqx_kvpages_reserve(void* k_codes, void* v_codes, float* k_scale, float* v_scale, int* table, const int* starts,
+                        const int* counts, int* refs, int64_t L, int64_t B, int64_t Hkv, int64_t hd, int64_t block, int64_t pages,
+                        int64_t width, int* ok, void* ws, int64_t ws_bytes, sqx_stream_t stream);
+
+/* Release the pages of blocks from ceil(max(keep[b], 0) / block) on: refs down by one, entry -1. lengths[b] = min(lengths[b],
+ * max(keep[b], 0)). */
+int sqx_kvpages_free(const int* keep, int* table, int* lengths, int* refs, int64_t B, int64_t block, int64_t pages, int64_t width,
+                     sqx_stream_t stream);
+
+/* With live the number of pages whose refs exceed 0: those with ids from `live` on move to the free ids below it, both in ascending
+ * order; table and refs follow. moved [pages]: a page's new id, -1 for those not in use. */
+int64_t sqx_kvpages_compact_workspace_bytes(int64_t pages);
+int sqx_kvpages_compact(void* k_codes, void* v_codes, float* k_scale, float* v_scale, int* table, int* refs, int64_t L, int64_t B,
+                        int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width, int* live, int* moved, void* ws,
+                        int64_t ws_bytes, sqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -269,6 +269,14 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, ctypes.c_double, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
          _c_p, _c_i64, _c_p],
     ),
+    "sqx_kvpages_copy": (_c_i, [_c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, *[_c_i64] * 5, _c_p]),
+    "sqx_kvpages_fork_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "sqx_kvpages_fork": (_c_i, [*[_c_p] * 8, *[_c_i64] * 7, _c_p, _c_p, _c_i64, _c_p]),
+    "sqx_kvpages_reserve_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "sqx_kvpages_reserve": (_c_i, [*[_c_p] * 8, *[_c_i64] * 7, _c_p, _c_p, _c_i64, _c_p]),
+    "sqx_kvpages_free": (_c_i, [*[_c_p] * 4, *[_c_i64] * 4, _c_p]),
+    "sqx_kvpages_compact_workspace_bytes": (_c_i64, [_c_i64]),
+    "sqx_kvpages_compact": (_c_i, [*[_c_p] * 6, *[_c_i64] * 7, _c_p, _c_p, _c_p, _c_i64, _c_p]),
 }
 
 _lock = threading.Lock()
