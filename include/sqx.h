@@ -951,6 +951,19 @@ int sqx_kvpages_compact(void* k_codes, void* v_codes, float* k_scale, float* v_s
                         int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width, int* live, int* moved, void* ws,
                         int64_t ws_bytes, sqx_stream_t stream);
 
+/* The next token of every row of logits [B, V] (F32 / BF16 / F16, V <= 2^20) from u fp32 [B]. With m a row's maximum and w_i =
+ * exp((l_i - m) / temperature), tokens stand in the order of their logits, equal ones by their id. Kept of these: the first top_k
+ * (0: all); of these those with less than top_p of these's weight before them (1: all; always the first); of these those with
+ * w_i >= min_p. tokens[b] is the least i whose cumulative kept weight, ids ascending, exceeds u[b] times the whole. Weights and sums
+ * in double; a token with (m - l_i) / temperature of about 32 or more is not drawn. temperature 0: the first maximum, a NaN counts as one; else
+ * a row with a NaN or +inf, or of -inf only, gives -1. Each setting is a number, or per row where its pointer is not NULL
+ * (temperature not above 0: 0, else within 1e-4 .. 1e4; top_k below 1: 0; top_p not above 0: the first token; min_p above 1:
+ * 1; a limit of NaN: none). ws: 16-byte aligned. */
+int64_t sqx_sample_workspace_bytes(int64_t B, int64_t V);
+int sqx_sample(const void* logits, int dtype, const float* u, const float* temperature_t, double temperature, const int* top_k_t,
+               int64_t top_k, const float* top_p_t, double top_p, const float* min_p_t, double min_p, int64_t B, int64_t V,
+               int* tokens, void* ws, int64_t ws_bytes, sqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,233 @@
+"""Sampling (scratch_llm_amd/sampling.py) on the GPU against oracle/sample_ref.py: the same token for the same random number.
+
+Weights are good to 2^-48 of the row's largest, sums of up to 2^20 of them to 1e-9; a cut or a draw of the inputs here, which
+are fixed, would have to fall that near to a border to differ."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import sample_ref as R
+from tests.conftest import print_case
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+LARGEST_U = 1.0 - 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def draw():
+    from scratch_llm_amd.sampling import sample_tokens
+
+    return sample_tokens
+
+
+def logits_of(g, b, v, dtype, spread=2.0, peaks=20):
+    x = g.normal(0, spread, (b, v))
+    for row in x:
+        row[g.integers(0, v, min(peaks, v))] += 6.0
+    t = torch.from_numpy(x.astype(np.float32)).to(DT[dtype])
+    return t, t.float().numpy()
+
+
+def check(draw, t, x, u, **kw):
+    got = draw(t.to(DEV), torch.from_numpy(np.asarray(u, np.float32)).to(DEV), **kw)
+    assert got.dtype == torch.int32 and got.shape == (len(x),)
+    rows = [{k: (float(a[i]) if a.dtype.is_floating_point else int(a[i])) if isinstance(a, torch.Tensor) else a for k, a in kw.items()}
+            for i in range(len(x))]
+    want = [R.sample(row, np.float32(ui), **r) for row, ui, r in zip(x, u, rows)]
+    assert got.tolist() == want
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.7, top_k=1), dict(top_k=5), dict(top_k=40, temperature=1.3), dict(top_p=0.9),
+            dict(top_p=0.3, temperature=0.6), dict(min_p=0.05), dict(top_k=50, top_p=0.95, min_p=0.02, temperature=0.8),
+            dict(top_k=3000, top_p=0.99), dict(top_k=7, min_p=0.5), dict(top_p=0.999, min_p=1e-4)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("v", [1, 2, 7, 8, 63, 1000, 8191, 8192, 8193, 50257, 128256])
+def test_settings(draw, v, dtype):
+    g = np.random.default_rng(v)
+    b = 5 if v < 20000 else 3
+    t, x = logits_of(g, b, v, dtype)
+    for kw in SETTINGS:
+        print_case("sample", dtype, v, kw)
+        check(draw, t, x, np.float32(g.random(b)), **kw)
+
+
+def test_the_largest_vocabulary(draw):
+    g = np.random.default_rng(77)
+    t, x = logits_of(g, 2, 1 << 20, "bf16")
+    for kw in (dict(), dict(top_k=100, top_p=0.9), dict(top_p=0.95), dict(temperature=30.0, top_k=200000, top_p=0.9)):
+        check(draw, t, x, [0.3, 0.99], **kw)
+
+
+@pytest.mark.parametrize("u", [0.0, 2.0 ** -24, 0.5, LARGEST_U])
+def test_the_ends_of_u(draw, u):
+    g = np.random.default_rng(4)
+    for v in (3, 9000):
+        t, x = logits_of(g, 4, v, "fp32")
+        for kw in SETTINGS:
+            check(draw, t, x, [u] * 4, **kw)
+
+
+def test_u_outside_its_range(draw):
+    """The last kept token for 1 and above and for a NaN, the first for negative numbers."""
+    t = torch.zeros(5, 9001)
+    t[:, 7], t[:, 9000] = -math.inf, -math.inf
+    got = draw(t.to(DEV), torch.tensor([1.0, math.inf, math.nan, -1.0, -math.inf], device=DEV))
+    assert got.tolist() == [8999, 8999, 8999, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("v,levels", [(100, 3), (20000, 1), (20000, 2), (20000, 40), (60000, 5)])
+def test_ties(draw, v, levels, dtype):
+    """Equal logits go by id, in the sorted list and where more tokens than that holds are equal."""
+    g = np.random.default_rng(levels)
+    x = g.integers(0, levels, (4, v)).astype(np.float32)
+    t = torch.from_numpy(x).to(DT[dtype])
+    u = np.float32(g.random(4))
+    for kw in (dict(), dict(top_k=1), dict(top_k=v // 2), dict(top_k=v - 1), dict(top_k=4097), dict(top_p=0.5), dict(top_p=0.25, top_k=v // 2),
+               dict(top_p=0.75, min_p=0.3), dict(min_p=1.0), dict(min_p=0.2, top_k=v - 3), dict(top_p=1e-9), dict(temperature=0.0)):
+        print_case("ties", dtype, v, levels, kw)
+        check(draw, t, x, u, **kw)
+
+
+@pytest.mark.parametrize("temperature", [1e-4, 1e-2, 0.3, 20.0, 1e4])
+def test_temperatures(draw, temperature):
+    """Rows that are one token, and rows that are flat: more tokens than the sorted list holds end in a bin."""
+    g = np.random.default_rng(5)
+    for dtype, v in (("bf16", 128256), ("fp32", 40000), ("fp32", 300)):
+        t, x = logits_of(g, 3, v, dtype)
+        for kw in (dict(), dict(top_k=50), dict(top_k=v // 3, top_p=0.8), dict(top_p=0.7), dict(min_p=0.3), dict(min_p=0.9, top_p=0.99)):
+            print_case("temperature", temperature, dtype, v, kw)
+            check(draw, t, x, np.float32(g.random(3)), temperature=temperature, **kw)
+
+
+def test_masks(draw):
+    """-inf masks: all but some, all but one, whole slices, everything; limits that reach past what is left."""
+    g = np.random.default_rng(6)
+    v = 30000
+    t, x = logits_of(g, 6, v, "fp32")
+    x[1, g.random(v) < 0.999] = -np.inf
+    x[2] = -np.inf
+    x[2, 29999] = -5.0
+    x[3, :20000] = -np.inf
+    x[4] = -np.inf
+    x[5, 100:] = -np.inf
+    t = torch.from_numpy(x)
+    for kw in (dict(), dict(top_k=50), dict(top_k=20000, top_p=0.9), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=0.0), dict(temperature=0.1, top_k=200)):
+        check(draw, t, x, np.float32(g.random(6)), **kw)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("where", [0, 8191, 8192, 19999])
+def test_rows_that_are_no_distribution(draw, bad, where):
+    g = np.random.default_rng(7)
+    t, x = logits_of(g, 3, 20000, "fp32")
+    x[1, where] = bad
+    t = torch.from_numpy(x)
+    for kw in (dict(), dict(top_k=3, top_p=0.5), dict(min_p=0.1), dict(temperature=0.0)):
+        check(draw, t, x, [0.4] * 3, **kw)
+
+
+def test_large_numbers_and_zeros(draw):
+    g = np.random.default_rng(8)
+    x = g.normal(0, 1, (4, 9000)).astype(np.float32)
+    x[0] = np.float32(3e38) * np.sign(x[0])
+    x[1] = 1e30
+    x[1, ::3] = 1.0000001e30
+    x[2] = np.where(x[2] > 0, 0.0, -0.0)      # equal, whatever their sign
+    x[3] *= np.float32(1e-40)                  # subnormal: equal but for their order
+    t = torch.from_numpy(x)
+    for kw in (dict(), dict(top_k=100), dict(top_k=4500, top_p=0.5), dict(top_p=0.5), dict(min_p=1.0), dict(temperature=1e-4, top_k=5000)):
+        check(draw, t, x, np.float32(g.random(4)), **kw)
+
+
+def test_settings_of_each_row(draw):
+    g = np.random.default_rng(9)
+    b, v = 24, 12000
+    t, x = logits_of(g, b, v, "bf16")
+    temp = torch.tensor([0.0, 1.0, 0.5, -1.0, 1e-9, 1e9, 2.0, 0.8] * 3)
+    k = torch.tensor([0, 5, -3, 50, 100000, 1], dtype=torch.int32).repeat(4)
+    p = torch.tensor([1.0, 0.9, 2.0, 0.5, 0.0, -1.0, 0.1, 0.99] * 3)
+    m = torch.tensor([0.0, -1.0, 0.1, 5.0] * 6)
+    u = np.float32(g.random(b))
+    got = draw(t.to(DEV), torch.from_numpy(u).to(DEV), temperature=temp.to(DEV), top_k=k.to(DEV), top_p=p.to(DEV), min_p=m.to(DEV)).tolist()
+    want = [R.sample(x[i], u[i], float(temp[i]), int(k[i]), float(p[i]), float(m[i])) for i in range(b)]
+    assert got == want
+    # limits of NaN are none; a temperature of NaN is 0
+    nan = torch.full((b,), math.nan, device=DEV)
+    assert draw(t.to(DEV), torch.from_numpy(u).to(DEV), top_p=nan, min_p=nan).tolist() == [R.sample(x[i], u[i]) for i in range(b)]
+    assert draw(t.to(DEV), torch.from_numpy(u).to(DEV), temperature=nan).tolist() == x.argmax(1).tolist()
+
+
+def test_frequencies_are_the_probabilities(draw):
+    """Evenly spaced random numbers give every kept token its share of the draws, to one."""
+    g = np.random.default_rng(10)
+    n = 4000
+    t, x = logits_of(g, 1, 600, "fp32", spread=1.5, peaks=3)
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    for kw in (dict(), dict(temperature=0.7, top_k=30), dict(top_p=0.8), dict(min_p=0.1)):
+        got = draw(t.to(DEV).expand(n, 600), torch.from_numpy(u).to(DEV), **kw).cpu().numpy()
+        w = R.kept(x[0], kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), kw.get("min_p", 0.0))
+        assert np.abs(np.bincount(got, minlength=600) - n * w / w.sum()).max() <= 1.0 + n * 2.0 ** -23
+        assert not (np.bincount(got, minlength=600) > 0)[w == 0].any()
+
+
+def test_layouts_streams_and_repetition(draw):
+    g = np.random.default_rng(11)
+    t, x = logits_of(g, 6, 9999, "bf16")
+    u = np.float32(g.random(6))
+    kw = dict(top_k=200, top_p=0.9, min_p=0.01)
+    want = [R.sample(row, ui, **kw) for row, ui in zip(x, u)]
+    ud = torch.from_numpy(u).to(DEV)
+    wide = torch.zeros(6, 20000, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1:19998:2] = t.to(DEV)
+    flat = torch.zeros(6 * 9999 + 3, dtype=torch.bfloat16, device=DEV)
+    flat[3:] = t.to(DEV).flatten()
+    spread = torch.zeros(12, device=DEV)
+    spread[::2] = ud
+    out = torch.full((6,), -7, dtype=torch.int32, device=DEV)
+    for args in ((wide[:, 1:19998:2], ud), (flat[3:].view(6, 9999), ud), (t.to(DEV).t().contiguous().t(), spread[::2])):
+        for _ in range(3):
+            assert draw(*args, out=out, **kw) is out and out.tolist() == want
+    assert draw(torch.zeros(0, 5, device=DEV), torch.zeros(0, device=DEV)).shape == (0,)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    there = t.to(DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        first = draw(there, ud, **kw)
+    with torch.cuda.stream(b):
+        second = draw(there, ud, **kw)
+    torch.cuda.synchronize()
+    assert first.tolist() == second.tolist() == want
+
+
+def test_captured(draw):
+    g = np.random.default_rng(12)
+    sets = [logits_of(g, 4, 20011, "fp16") for _ in range(4)]
+    us = [np.float32(g.random(4)) for _ in range(4)]
+    x, u = sets[0][0].to(DEV), torch.from_numpy(us[0]).to(DEV)
+    temp, k = torch.full((4,), 0.9, device=DEV), torch.full((4,), 60, dtype=torch.int32, device=DEV)
+    draw(x, u, temperature=temp, top_k=k, top_p=0.9)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = draw(x, u, temperature=temp, top_k=k, top_p=0.9)
+    for i in (1, 2, 3, 1):
+        x.copy_(sets[i][0])
+        u.copy_(torch.from_numpy(us[i]))
+        temp.fill_(0.5 + 0.25 * i)
+        k.fill_(10 * i)
+        graph.replay()
+        torch.cuda.synchronize()
+        t32 = float(np.float32(0.5 + 0.25 * i))
+        assert got.tolist() == [R.sample(row, ui, t32, 10 * i, 0.9) for row, ui in zip(sets[i][1], us[i])]
+        torch.ones(1 << 18, device=DEV).sum().item()
