@@ -951,6 +951,23 @@ int sqx_kvpages_compact(void* k_codes, void* v_codes, float* k_scale, float* v_s
                         int64_t Hkv, int64_t hd, int64_t block, int64_t pages, int64_t width, int* live, int* moved, void* ws,
                         int64_t ws_bytes, sqx_stream_t stream);
 
+/* Attention of a batch whose rows share the first pages of their contexts. Rows with the same leaders[b] >= 0 make a group; what
+ * they share is the whole blocks in front that all of them name alike and that lie before every one's start. A plan is made
+ * for T tokens a row and these heads (B <= 4096); it holds while the groups' rows and the table entries of their shared blocks
+ * stay. A row whose start has fallen behind the shared blocks is attended for itself. sqx_kvshared_attention is
+ * sqx_kvblock_attention otherwise, the shared keys read once for a group (with T H / Hkv above 128, or 64 with heads of 256, it is
+ * that call). plan and ws: 16-byte aligned; calls that overlap need workspaces of their own and may share a plan. */
+int64_t sqx_kvshared_plan_bytes(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd);
+int sqx_kvshared_plan(const int* table, const int* starts, const int* leaders, int64_t B, int64_t T, int64_t H, int64_t Hkv,
+                      int64_t hd, int64_t block, int64_t width, void* plan, int64_t plan_bytes, sqx_stream_t stream);
+int64_t sqx_kvshared_attention_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
+                                               int64_t width);
+int sqx_kvshared_attention(const void* q, int dtype, int64_t q_sb, int64_t q_st, int64_t q_sh, int fmt, const void* k_codes,
+                           const void* v_codes, const float* k_scale, const float* v_scale, const int* table, const int* starts,
+                           const int* counts, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd, int64_t block,
+                           int64_t pages, int64_t width, float scale, const void* plan, int64_t plan_bytes, void* out, void* ws,
+                           int64_t ws_bytes, sqx_stream_t stream);
+
 /* The next token of every row of logits [B, V] (F32 / BF16 / F16, V <= 2^20) from u fp32 [B]. With m a row's maximum and w_i =
  * exp((l_i - m) / temperature), tokens stand in the order of their logits, equal ones by their id. Kept of these: the first top_k
  * (0: all); of these those with less than top_p of these's weight before them (1: all; always the first); of these those with

@@ -277,6 +277,14 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sqx_kvpages_free": (_c_i, [*[_c_p] * 4, *[_c_i64] * 4, _c_p]),
     "sqx_kvpages_compact_workspace_bytes": (_c_i64, [_c_i64]),
     "sqx_kvpages_compact": (_c_i, [*[_c_p] * 6, *[_c_i64] * 7, _c_p, _c_p, _c_p, _c_i64, _c_p]),
+    "sqx_kvshared_plan_bytes": (_c_i64, [_c_i64] * 5),
+    "sqx_kvshared_plan": (_c_i, [*[_c_p] * 3, *[_c_i64] * 7, _c_p, _c_i64, _c_p]),
+    "sqx_kvshared_attention_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "sqx_kvshared_attention": (
+        _c_i,
+        [_c_p, _c_i, _c_i64, _c_i64, _c_i64, _c_i, *[_c_p] * 7, *[_c_i64] * 8, ctypes.c_float, _c_p, _c_i64, _c_p, _c_p, _c_i64,
+         _c_p],
+    ),
     "sqx_sample_workspace_bytes": (_c_i64, [_c_i64] * 2),
     "sqx_sample": (_c_i, [_c_p, _c_i, _c_p, _c_p, ctypes.c_double, _c_p, _c_i64, _c_p, ctypes.c_double, _c_p, ctypes.c_double,
                           _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p]),
