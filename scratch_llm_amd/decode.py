@@ -17,7 +17,10 @@ decode token after token (the pick of one replay is the input of the next).
 
 On the block-scaled 8-bit cache (``kv_dtype="int8_block"`` or ``"fp8_block"``,
 :mod:`scratch_llm_amd.quant.kv_block`) the model also takes several tokens a row: a chunk of a prompt
-(:meth:`Int4DecodeLM.extend`) and drafted tokens with their verification (:meth:`Int4DecodeLM.verify`).
+(:meth:`Int4DecodeLM.extend`) and drafted tokens with their verification (:meth:`Int4DecodeLM.verify`). Its pages
+may come from a pool (``kv_pages``, :mod:`scratch_llm_amd.quant.kv_pages`), from which rows are forked, cut and freed; rows that
+share the front of their contexts may read it once (:meth:`DecodeState.share`); and a step may sample
+(:meth:`DecodeState.set_sampling`).
 """
 
 from __future__ import annotations
@@ -31,8 +34,9 @@ from torch import Tensor
 
 from scratch_llm_amd import _lib, speculative
 from scratch_llm_amd.quant import int4_group as i4
-from scratch_llm_amd.quant import kv_block
+from scratch_llm_amd.quant import kv_block, kv_pages, kv_shared
 from scratch_llm_amd.quant.fp8_weights import FP8_DTYPE
+from scratch_llm_amd.sampling import Sampling, sample_tokens
 
 __all__ = ["DecodeConfig", "DecodeState", "Int4DecodeLM", "LLAMA3_8B", "rope_tables"]
 
@@ -109,12 +113,16 @@ class DecodeState:
     ``[n_layers, pages, Hkv, hd, kv_block]`` int8 or E4M3 codes, ``k_scale``/``v_scale`` ``[n_layers, pages, Hkv]``, and
     ``block_table`` int32 ``[B, ceil(max_ctx / kv_block)]``, at first row after row (a server may point it elsewhere).
     Nothing is calibrated. Rows that are not active store nothing, and tokens past a row's table are not stored.
+    With ``kv_pages`` the block-scaled cache has that many pages, none of them handed out: ``block_table`` begins as -1 and ``refs``
+    int32 ``[kv_pages]`` counts who holds a page. :meth:`Int4DecodeLM.step`, ``extend`` and ``verify`` take the pages of their
+    tokens from the pool; where it is too small they change nothing of the state and set ``room`` (int32 ``[1]``, else 1) to 0.
     ``lengths`` int32 ``[B]`` (valid positions before the next write); ``active`` uint8 ``[B]`` (rows that
     ``advance`` bumps); ``tokens`` int32 ``[B]``: the step's input ids, overwritten by its greedy picks;
     ``logits`` bf16 ``[B, vocab]``.
     """
 
-    def __init__(self, model: "Int4DecodeLM", batch: int, max_ctx: int, kv_dtype: str = "bf16", kv_block_size: int = 64) -> None:
+    def __init__(self, model: "Int4DecodeLM", batch: int, max_ctx: int, kv_dtype: str = "bf16", kv_block_size: int = 64,
+                 kv_pages: int | None = None) -> None:
         cfg, dev = model.cfg, model.device
         if batch < 1 or max_ctx < 1:
             raise ValueError("batch and max_ctx must be >= 1")
@@ -124,16 +132,25 @@ class DecodeState:
             raise ValueError(f"kv_dtype must be 'bf16', 'fp8', 'int8_block' or 'fp8_block', got {kv_dtype!r}")
         self.batch, self.max_ctx, self.kv_dtype = batch, max_ctx, kv_dtype
         hkv, hd, d = cfg.n_kv_heads, cfg.head_dim, cfg.d_model
+        self.n_heads = cfg.n_heads
         self.k_scale = self.v_scale = self.block_table = self.counts = None
         self.block_kv = kv_dtype in _BLOCK_KV
+        self.refs = self.room = self.leaders = self.shared = self.sampling = None
+        if kv_pages is not None and (not self.block_kv or kv_pages < 1):
+            raise ValueError(f"kv_pages must be positive and belongs to a block-scaled cache, got {kv_pages} for {kv_dtype!r}")
         if self.block_kv:
             if kv_block_size not in kv_block.BLOCKS:
                 raise ValueError(f"kv_block_size: block must be one of {kv_block.BLOCKS}, got {kv_block_size}")
             width = -(-max_ctx // kv_block_size)
-            layer = kv_block.new_kv_blocks(cfg.n_layers * batch * width, hkv, hd, block=kv_block_size, dtype=_BLOCK_KV[kv_dtype],
-                                           device=dev)
-            self.k, self.v, self.k_scale, self.v_scale = (t.view(cfg.n_layers, batch * width, *t.shape[1:]) for t in layer)
-            self.block_table = torch.arange(batch * width, dtype=torch.int32, device=dev).view(batch, width)
+            pages = batch * width if kv_pages is None else kv_pages
+            layer = kv_block.new_kv_blocks(cfg.n_layers * pages, hkv, hd, block=kv_block_size, dtype=_BLOCK_KV[kv_dtype], device=dev)
+            self.k, self.v, self.k_scale, self.v_scale = (t.view(cfg.n_layers, pages, *t.shape[1:]) for t in layer)
+            if kv_pages is None:
+                self.block_table = torch.arange(batch * width, dtype=torch.int32, device=dev).view(batch, width)
+            else:
+                self.block_table = torch.full((batch, width), -1, dtype=torch.int32, device=dev)
+                self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+                self.room = torch.ones(1, dtype=torch.int32, device=dev)
             self.counts = torch.ones(batch, dtype=torch.int32, device=dev)  # tokens that a step stores: `active` as int32
             self._kv = [(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]) for i in range(cfg.n_layers)]
         else:
@@ -147,6 +164,11 @@ class DecodeState:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.active = torch.ones(batch, dtype=torch.uint8, device=dev)
         self.tokens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        # steps that sample or take pages: the pick, whether it counts, the rows that advance
+        self.u = torch.zeros(batch, dtype=torch.float32, device=dev)
+        self.pick = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.good = torch.zeros(batch, dtype=torch.bool, device=dev)
+        self.live = torch.zeros(batch, dtype=torch.uint8, device=dev)
         bf = dict(dtype=torch.bfloat16, device=dev)
         self.x = [torch.empty(batch, d, **bf), torch.empty(batch, d, **bf)]  # residual stream (ping-pong)
         self.h = torch.empty(batch, d, **bf)  # normalised input of the next projection
@@ -226,6 +248,72 @@ class DecodeState:
         if tuple(n.shape) != (self.batch,) or n.dtype != torch.int32 or not n.is_contiguous():
             raise ValueError(f"{fn}: lengths must be contiguous int32 [{self.batch}], got {tuple(n.shape)} of {n.dtype}")
         _lib.require_device(table, n, self.k, fn=fn)
+
+    # ------------------------------------------------------------------ pages of a pool
+    def _pool(self, fn: str) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+        if self.refs is None:
+            raise ValueError(f"{fn}: the state has no pool of pages (new_state(kv_pages=...))")
+        self.check_rows(fn)
+        return self.k, self.v, self.k_scale, self.v_scale
+
+    def reserve(self, counts: Tensor) -> Tensor:
+        """Pages for the next ``counts[b]`` tokens of every row (int32 ``[B]``) from the pool, copies of those that others hold
+        too (:func:`~scratch_llm_amd.quant.kv_pages.reserve_kv_pages`). Returns ``room``: 1, or 0 and nothing changed."""
+        pool = self._pool("DecodeState.reserve")
+        self.room.copy_(kv_pages.reserve_kv_pages(*pool, self.block_table, self.lengths, counts, self.refs))
+        return self.room
+
+    def free(self, keep: Tensor) -> None:
+        """Cut every row to its first ``keep[b]`` tokens (int32 ``[B]``; 0: all of it goes) and give the pages behind them back."""
+        self._pool("DecodeState.free")
+        kv_pages.free_kv_rows(keep, self.block_table, self.lengths, self.refs, block=self.k.shape[3])
+        self._replan()
+
+    def fork(self, parents: Tensor) -> Tensor:
+        """Let every row go on from row ``parents[b]`` (int32 ``[B]``): its pages, length and next input token
+        (:func:`~scratch_llm_amd.quant.kv_pages.fork_kv_rows`; the ``active`` flags stay). Returns ``room``: 1, or 0 and nothing changed."""
+        pool = self._pool("DecodeState.fork")
+        self.room.copy_(kv_pages.fork_kv_rows(parents, *pool, self.block_table, self.lengths, self.refs))
+        at = torch.where((parents >= 0) & (parents < self.batch), parents, 0).long()
+        self.tokens.copy_(torch.where(self.room > 0, self.tokens[at], self.tokens))
+        self._replan()
+        return self.room
+
+    def compact(self) -> Tensor:
+        """Move the pages in use to the front of the pool; returns their number, int32 ``[1]``."""
+        pool = self._pool("DecodeState.compact")
+        return kv_pages.compact_kv_pages(*pool, self.block_table, self.refs)[0]
+
+    def share(self, leaders: Tensor | None) -> None:
+        """Let steps read what the rows of a group share once (:func:`~scratch_llm_amd.quant.kv_shared.plan_shared_kv`): rows with the
+        same number in ``leaders`` (int32 ``[B]``, at least 0; kept, and read again by every :meth:`fork` and :meth:`free`) make
+        a group. None: every row for itself. Call it again after other changes of what the table's shared entries name. A step
+        captured while rows share uses the plan as it is when it is replayed; share first, then capture."""
+        if not self.block_kv:
+            raise ValueError(f"DecodeState.share needs a block-scaled cache, got {self.kv_dtype!r}")
+        self.check_rows("DecodeState.share")
+        if leaders is None:
+            self.leaders = self.shared = None
+            return
+        old = self.shared if self.shared is not None and self.shared.width == self.block_table.shape[1] else None
+        plan = self._plan(leaders, old)
+        self.leaders, self.shared = leaders, plan
+
+    def _plan(self, leaders: Tensor, out: "kv_shared.SharedKV | None") -> "kv_shared.SharedKV":
+        return kv_shared.plan_shared_kv(self.block_table, self.lengths, leaders, block=self.k.shape[3], tokens=1, heads=self.n_heads,
+                                        kv_heads=self.k.shape[2], head_dim=self.k.shape[4], out=out)
+
+    def _replan(self) -> None:
+        if self.shared is not None:
+            self._plan(self.leaders, self.shared)
+
+    def set_sampling(self, sampling: "Sampling | None") -> None:
+        """Let steps draw their tokens (:func:`~scratch_llm_amd.sampling.sample_tokens`) with the random numbers in ``u`` (float32 ``[B]``,
+        in [0, 1), to be set before every step); None: greedy picks. A row whose logits are no distribution keeps its token and
+        does not advance."""
+        if sampling is not None:
+            sampling.check(self.batch, "DecodeState.set_sampling")
+        self.sampling = sampling
 
     def set_lengths(self, lengths) -> None:
         """Set every slot's valid length (a host list or tensor), e.g. after filling the cache."""
@@ -390,8 +478,9 @@ class Int4DecodeLM:
             ly.attn_norm.numel() * 2 + ly.ffn_norm.numel() * 2 for ly in self.layers
         ) + self.final_norm.numel() * 2
 
-    def new_state(self, batch: int, max_ctx: int | None = None, kv_dtype: str = "bf16", kv_block_size: int = 64) -> DecodeState:
-        return DecodeState(self, batch, self.cfg.context_length if max_ctx is None else max_ctx, kv_dtype, kv_block_size)
+    def new_state(self, batch: int, max_ctx: int | None = None, kv_dtype: str = "bf16", kv_block_size: int = 64,
+                  kv_pages: int | None = None) -> DecodeState:
+        return DecodeState(self, batch, self.cfg.context_length if max_ctx is None else max_ctx, kv_dtype, kv_block_size, kv_pages)
 
     # ------------------------------------------------------------------ the step
     def _linear(self, st: DecodeState, tw: i4.Int4Tiled, x: Tensor, y: Tensor, stream: int) -> None:
@@ -489,8 +578,9 @@ class Int4DecodeLM:
 
     def step(self, st: DecodeState, tokens=None, only: str | None = None) -> Tensor:
         """Decode one token per row: logits of ``st.tokens`` (or ``tokens``) at each row's position,
-        written to ``st.logits``; the greedy picks replace ``st.tokens``; active rows advance. Returns
-        ``st.tokens``. Only device work is issued (no host synchronisation).
+        written to ``st.logits``; the greedy picks (or draws, :meth:`DecodeState.set_sampling`) replace ``st.tokens``; active
+        rows advance. Returns ``st.tokens``. Only device work is issued (no host synchronisation). On a pool of pages the
+        step takes those of its tokens first; with too few of them free it leaves tokens, lengths and cache as they are.
 
         ``only`` (one of ``STEP_KINDS``) issues just the launches of that kind, with the arguments the
         full step gives them, for timing each kind's share of the step; the results are then
@@ -502,6 +592,11 @@ class Int4DecodeLM:
             st.set_tokens(tokens, cfg.vocab_size)
         if st.block_kv:
             st.check_rows("Int4DecodeLM.step")
+            if st.shared is not None and st.shared.width != st.block_table.shape[1]:
+                raise ValueError(f"Int4DecodeLM.step: the rows share a table of {st.shared.width} blocks, block_table has "
+                                 f"{st.block_table.shape[1]}: call share again")
+        if st.sampling is not None and (tuple(st.u.shape) != (st.batch,) or st.u.dtype != torch.float32):
+            raise ValueError(f"Int4DecodeLM.step: u must be float32 [{st.batch}], got {tuple(st.u.shape)} of {st.u.dtype}")
         _lib.require_device(st.tokens, self.embed, fn="Int4DecodeLM.step")
         B, d, H, Hkv, hd, T = st.batch, cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, st.max_ctx
         s = _lib.stream_ptr(self.device)
@@ -537,10 +632,13 @@ class Int4DecodeLM:
         with torch.cuda.device(self.device):
             if st.block_kv and go("attention"):
                 st.counts.copy_(st.active)  # the flags may change between replays of a captured step
+                if st.refs is not None:
+                    st.counts.clamp_(max=1).mul_(st.reserve(st.counts))
             if go("other"):
                 ck(lib.sqx_embed(self.embed.data_ptr(), cfg.vocab_size, st.tokens.data_ptr(), B, d,
                                  st.x[0].data_ptr(), s), "embed")
             cur, delta, dsplit, have_ss = 0, None, 0, False
+            shared_ws = None if st.shared is None else self._shared_workspace(st)
             for li, ly in enumerate(self.layers):
                 # ---- q|k|v (with the attention norm)
                 if rope_in_qkv:
@@ -566,7 +664,8 @@ class Int4DecodeLM:
                 if not go("attention"):
                     pass
                 elif st.block_kv:
-                    self._block_attention(st, li, st.qkv, st.q, st.attn, B, 1, st.counts, st.attn_ws, s)
+                    self._block_attention(st, li, st.qkv, st.q, st.attn, B, 1, st.counts, st.attn_ws if shared_ws is None else shared_ws, s,
+                                          st.shared)
                 elif merge:  # the partials only; the o projection merges them
                     fp8 = st.kv_dtype == "fp8"
                     ck(lib.sqx_decode_attention_partials(
@@ -642,16 +741,33 @@ class Int4DecodeLM:
             else:
                 self._norm_linear(st, cur, delta, self.final_norm, self.lm_head, st.logits, s, dsplit)
             if go("other"):
-                ck(lib.sqx_argmax(st.logits.data_ptr(), B, cfg.vocab_size, st.tokens.data_ptr(),
-                                  st.argmax_ws.data_ptr(), st.argmax_ws.numel() * 4, s), "argmax")
-                ck(lib.sqx_advance(st.lengths.data_ptr(), st.active.data_ptr(), B, s), "advance")
+                plain = st.refs is None and st.sampling is None
+                if st.sampling is None:
+                    ck(lib.sqx_argmax(st.logits.data_ptr(), B, cfg.vocab_size, (st.tokens if plain else st.pick).data_ptr(),
+                                      st.argmax_ws.data_ptr(), st.argmax_ws.numel() * 4, s), "argmax")
+                else:
+                    x = st.sampling
+                    sample_tokens(st.logits, st.u, temperature=x.temperature, top_k=x.top_k, top_p=x.top_p, min_p=x.min_p, out=st.pick)
+                if not plain:
+                    torch.ge(st.pick, 0, out=st.good)
+                    if st.refs is not None:
+                        st.good.logical_and_(st.room)
+                    torch.where(st.good, st.pick, st.tokens, out=st.tokens)
+                    torch.mul(st.active, st.good, out=st.live)
+                ck(lib.sqx_advance(st.lengths.data_ptr(), (st.active if plain else st.live).data_ptr(), B, s), "advance")
         return st.tokens
 
+    def _shared_workspace(self, st: DecodeState) -> Tensor:
+        cfg = self.cfg
+        nb = int(_lib.load().sqx_kvshared_attention_workspace_bytes(st.batch, 1, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, st.k.shape[3],
+                                                                    st.block_table.shape[1]))
+        return torch.empty(max(nb // 4, 4), dtype=torch.float32, device=st.lengths.device)
+
     def _block_attention(self, st: DecodeState, li: int, qkv: Tensor, q: Tensor, attn: Tensor, batch: int, t: int,
-                         counts: Tensor, ws: Tensor, stream: int) -> None:
+                         counts: Tensor, ws: Tensor, stream: int, shared: "kv_shared.SharedKV | None" = None) -> None:
         """RoPE, the cache write and attention of ``t`` tokens a row over layer ``li`` of a block-scaled cache: ``qkv``
         [batch * t, (H + 2 Hkv) hd] as the fused projection leaves it, ``q`` the rotated queries, ``attn`` the output (rows
-        past their count stay as they are)."""
+        past their count stay as they are). ``shared``: what the rows read together."""
         cfg, lib = self.cfg, _lib.load()
         H, Hkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
         row = (H + 2 * Hkv) * hd
@@ -666,9 +782,12 @@ class Int4DecodeLM:
             at + 2 * H * hd, at + 2 * (H + Hkv) * hd, _lib.DTYPE_BF16, t * row, row, hd, t * row, row, hd, at, t * row, row, hd,
             q.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), cfg.context_length, hd, 1, fmt, *cache, stream),
             "rope + cache write")
-        _lib.check(lib.sqx_kvblock_attention(
-            q.data_ptr(), _lib.DTYPE_BF16, t * H * hd, H * hd, hd, fmt, *cache, 1.0 / math.sqrt(hd), attn.data_ptr(),
-            ws.data_ptr(), ws.numel() * 4, stream), "attention")
+        query = (q.data_ptr(), _lib.DTYPE_BF16, t * H * hd, H * hd, hd, fmt, *cache, 1.0 / math.sqrt(hd))
+        tail = (attn.data_ptr(), ws.data_ptr(), ws.numel() * 4, stream)
+        if shared is None:
+            _lib.check(lib.sqx_kvblock_attention(*query, *tail), "attention")
+        else:
+            _lib.check(lib.sqx_kvshared_attention(*query, shared.plan.data_ptr(), shared.plan.numel(), *tail), "attention")
 
     # ------------------------------------------------------------------ several tokens a row
     @torch.no_grad()
@@ -681,7 +800,8 @@ class Int4DecodeLM:
         of active rows to ``st.lengths``. Chunks follow one another, each of fewer than 2^30 / d_ff tokens over all rows; T = 1 is a
         decode step without the pick. A chunk is attended over a cache that holds all of it, and a block's scale goes by all
         of its tokens: scores depend on the later tokens of their blocks by that much, up to a step of the codes. Only
-        device work is issued."""
+        device work is issued. On a pool of pages the chunk's are taken first; with too few free nothing is stored, no length
+        grows and the logits mean nothing."""
         if not st.block_kv:
             raise ValueError(f"extend needs a block-scaled cache (kv_dtype 'int8_block' or 'fp8_block'), got {st.kv_dtype!r}")
         if tokens.ndim != 2 or tokens.shape[0] != st.batch or tokens.shape[1] < 1 or tokens.dtype != torch.int32:
@@ -692,6 +812,8 @@ class Int4DecodeLM:
         st.check_rows("Int4DecodeLM.extend")
         _lib.require_device(tokens, counts, self.embed, st.lengths, fn="Int4DecodeLM.extend")
         stored = self._stored(st, tokens.shape[1], counts)
+        if st.refs is not None:
+            stored = stored * st.reserve(stored)
         logits, _ = self._pass(st, tokens.contiguous(), stored, last_only)
         if advance:
             st.lengths.add_(stored)
@@ -807,7 +929,8 @@ class Int4DecodeLM:
         that token anew.
         ``counts`` is how many drafts a row has (default T). Rejected drafts leave no trace before the new length: the blocks
         that they shared with older or kept tokens are put back and the kept tokens stored again without them, as a chunk
-        of those alone would be. Only the scores have seen them, as those of :meth:`extend` see a chunk."""
+        of those alone would be. Only the scores have seen them, as those of :meth:`extend` see a chunk. On a pool of pages those
+        of all drafts are taken first; with too few free the state stays as it is and what is returned means nothing."""
         fn = "Int4DecodeLM.verify"
         if draft.ndim != 2 or draft.shape[0] != st.batch or draft.dtype != torch.int32:
             raise ValueError(f"draft must be int32 [{st.batch}, T], got {tuple(draft.shape)} of {draft.dtype}")
@@ -822,10 +945,13 @@ class Int4DecodeLM:
         _lib.require_device(draft, u, r, draft_probs, counts, self.embed, st.lengths, fn=fn)
         ids = torch.cat((st.tokens[:, None], draft), 1)
         stored = self._stored(st, t + 1, None if counts is None else counts.clamp(0, t) + 1)
+        live = st.active != 0
+        if st.refs is not None:
+            room = st.reserve(stored)
+            stored, live = stored * room, live & (room != 0)
         saved = self._open_blocks(st, stored)
         logits, qkv = self._pass(st, ids, stored, each_qkv=True)
         n, tokens = speculative.verify_draft(logits, draft, u, r, draft_probs=draft_probs, counts=counts, temperature=temperature)
-        live = st.active != 0
         at = n.long()[:, None]
         nxt = tokens.gather(1, at)[:, 0]
         nxt_ok = nxt >= 0
