@@ -32,6 +32,7 @@ constexpr int kSampleSlice = 8192;
 constexpr int kBins = 1024;
 constexpr int kPerT = 32;          // bins per unit of (m - l) / T
 constexpr int kCap = 4096;         // tokens that are sorted
+constexpr int kFew = 1024;         // up to this k all tokens that may stay are collected, and slices leave no weights
 constexpr int kMaxSlices = 128;    // 2^20 tokens
 constexpr int kHistThreads = 512, kPickThreads = 1024;
 constexpr double kFix = 0x1p48;
@@ -45,8 +46,8 @@ struct SampleArgs {
   int k, V, S;
   float* smax;                // [B, S]
   int* sarg;                  // [B, S]
-  unsigned long long* mass;   // [B, S, kBins]
-  unsigned* count;            // [B, S, kBins]
+  unsigned long long* mass;   // [B, S, kBins], summed from bin 0 on
+  unsigned* count;            // [B, S, kBins], likewise
   int* out;
 };
 
@@ -76,29 +77,33 @@ __device__ inline double row_temp(const SampleArgs& a, int b) {
   return t > 0.0 ? fmin(fmax(t, 1e-4), 1e4) : 0.0;
 }
 
+__device__ inline int row_k(const SampleArgs& a, int b) { return a.k_t != nullptr ? a.k_t[b] : a.k; }
+
+// Eight elements of a row of V in one load, at any multiple of an element: those from `at` on, or the row's last eight where it ends
+// within them. Element e is number first(at, V) + e, a thread's own if has(at, V, e).
 template <int DT>
-struct Loads8 {  // eight elements, at any multiple of an element
+struct Loads8 {
   static constexpr int kBytes = DT == SQX_DTYPE_F32 ? 4 : 2;
   struct __attribute__((packed, aligned(kBytes))) Raw { uint32_t w[2 * kBytes]; };
-  __device__ static inline void load(const void* p, int64_t row0, int at, int V, float (&v)[8]) {
-    if (at + 8 <= V) {
-      const Raw r = *reinterpret_cast<const Raw*>(static_cast<const char*>(p) + (row0 + at) * kBytes);
+  __device__ static inline int first(int at, int V) { return min(at, V - 8); }  // V >= 8
+  __device__ static inline bool has(int at, int V, int e) { return first(at, V) + e >= at; }
+  __device__ static inline Raw raw(const void* p, int64_t row0, int at, int V) {
+    return *reinterpret_cast<const Raw*>(static_cast<const char*>(p) + (row0 + first(at, V)) * kBytes);
+  }
+  __device__ static inline void floats(const Raw& r, float (&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (DT == SQX_DTYPE_F32) {
-          const uint32_t w = r.w[e];
-          v[e] = __builtin_bit_cast(float, w);
-        } else {
-          const uint32_t w = r.w[e >> 1];
-          const uint16_t h = static_cast<uint16_t>(e & 1 ? w >> 16 : w);
-          v[e] = DT == SQX_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-        }
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (DT == SQX_DTYPE_F32) {
+        const uint32_t w = r.w[e];
+        v[e] = __builtin_bit_cast(float, w);
+      } else {
+        const uint32_t w = r.w[e >> 1];
+        const uint16_t h = static_cast<uint16_t>(e & 1 ? w >> 16 : w);
+        v[e] = DT == SQX_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = at + e < V ? load_as_f32(p, DT, row0 + at + e) : -INFINITY;
     }
   }
+  __device__ static inline void load(const void* p, int64_t row0, int at, int V, float (&v)[8]) { floats(raw(p, row0, at, V), v); }
 };
 
 // Whether (ov, oi) comes before (cv, ci) as a greedy pick: the first maximum, a NaN counts as one.
@@ -116,6 +121,9 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(const SampleA
   __shared__ unsigned count[kBins];
   __shared__ float redv[W];
   __shared__ int redi[W];
+  __shared__ unsigned long long redm[W];
+  __shared__ unsigned redc[W];
+  static_assert(kBins == 2 * kHistThreads, "two bins a thread");
   const int s = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int base = s * kSampleSlice + 8 * tid;
   float v[G][8];
@@ -133,8 +141,8 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(const SampleA
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int i = base + g * 8 * kHistThreads + e;
-      if (i < a.V && greedy_takes(v[g][e], i, best, arg)) {
+      const int i = Loads8<DT>::first(base + g * 8 * kHistThreads, a.V) + e;
+      if (Loads8<DT>::has(base + g * 8 * kHistThreads, a.V, e) && greedy_takes(v[g][e], i, best, arg)) {
         best = v[g][e];
         arg = i;
       }
@@ -168,28 +176,64 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(const SampleA
   }
   const double T = row_temp(a, b);
   if (T == 0.0 || !(best < INFINITY)) return;  // greedy, or no distribution: no bin is read
+  const int want_k = row_k(a, b);
+  const bool few = want_k >= 1 && want_k <= kFew;
   const double inv = kPerT / T, k = 64.0 * 1.4426950408889634074 / T, m = static_cast<double>(best), top = floor(m * inv);
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int i = base + g * 8 * kHistThreads + e;
       const double l = static_cast<double>(v[g][e]);
       const double d = top - floor(l * inv);
-      if (i < a.V && d < kBins) {  // false of a NaN: a masked token of a slice that is all masked
+      if (Loads8<DT>::has(base + g * 8 * kHistThreads, a.V, e) && d < kBins) {  // false of a NaN: a masked token of a slice that is all masked
         const int bin = static_cast<int>(d);
-        atomicAdd(&count[bin], 1u);
-        atomicAdd(&mass[bin], to_fix(pow2_64th((l - m) * k, pow64)));
+        if (want_k >= 1) atomicAdd(&count[bin], 1u);
+        if (!few) atomicAdd(&mass[bin], to_fix(pow2_64th((l - m) * k, pow64)));
       }
     }
   __syncthreads();
-  for (int i = tid; i < kBins; i += kHistThreads) {
-    a.mass[at * kBins + i] = mass[i];
-    a.count[at * kBins + i] = count[i];
+  // sums from bin 0 on: two bins a thread, then over the workgroup
+  const int lane = tid & 63, wave = tid >> 6;
+  const unsigned long long m0 = mass[2 * tid], m1 = m0 + mass[2 * tid + 1];
+  const unsigned c0 = count[2 * tid], c1 = c0 + count[2 * tid + 1];
+  unsigned long long ms = m1;
+  unsigned cs = c1;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned long long y = __shfl_up(ms, o, 64);
+    const unsigned z = __shfl_up(cs, o, 64);
+    if (lane >= o) {
+      ms += y;
+      cs += z;
+    }
+  }
+  if (lane == 63) {
+    redm[wave] = ms;
+    redc[wave] = cs;
+  }
+  __syncthreads();
+  ms -= m1;
+  cs -= c1;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    ms += w < wave ? redm[w] : 0ull;
+    cs += w < wave ? redc[w] : 0u;
+  }
+  if (!few) {
+    ulonglong2 mo;
+    mo.x = ms + m0;
+    mo.y = ms + m1;
+    reinterpret_cast<ulonglong2*>(a.mass + at * kBins)[tid] = mo;
+  }
+  if (want_k >= 1) {
+    uint2 co;
+    co.x = cs + c0;
+    co.y = cs + c1;
+    reinterpret_cast<uint2*>(a.count + at * kBins)[tid] = co;
   }
 }
 
-// Inclusive sums over the workgroup of kPickThreads threads, of a double and of an int.
+// Inclusive sums over the workgroup of kPickThreads threads.
 __device__ inline double pick_scan(double x, double* red, double& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -210,25 +254,14 @@ __device__ inline double pick_scan(double x, double* red, double& total) {
   __syncthreads();
   return before + x;
 }
-__device__ inline int pick_scan(int x, int* red, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  if (lane == 63) red[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kPickThreads / 64; ++w) {
-    const int r = red[w];
-    if (w == wave) before = total;
-    total += r;
-  }
-  __syncthreads();
-  return before + x;
+// The largest, or the least, of the workgroup's values where `is`, into *to; values ascend with the lanes. One atomic a wave.
+__device__ inline void raise(int* to, bool is, int value) {
+  const unsigned long long b = __ballot(is);
+  if (b != 0 && (threadIdx.x & 63) == 63 - __clzll(b)) atomicMax(to, value);
+}
+__device__ inline void lower(int* to, bool is, int value) {
+  const unsigned long long b = __ballot(is);
+  if (b != 0 && (threadIdx.x & 63) == __ffsll(b) - 1) atomicMin(to, value);
 }
 
 // A token's place in the order: the larger the earlier. Zeros of either sign are equal.
@@ -243,13 +276,120 @@ __device__ inline float place_logit(unsigned long long q) {
   return __builtin_bit_cast(float, key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
+typedef __attribute__((address_space(3))) unsigned long long* lds_u64_t;
+// The value of lane ^ X, by moves between lanes' registers.
+template <int X>
+__device__ inline uint32_t lane_xor(uint32_t v) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);  // within four: 1 0 3 2
+  if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);  // 2 3 0 1
+  if constexpr (X == 4) return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true), 0x1b, 0xf, 0xf, true);  // eight reversed, fours reversed
+  if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // sixteen turned by eight
+  if constexpr (X == 16) {
+    const auto h = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];
+    return threadIdx.x & 16 ? h0 : h1;
+  }
+  const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t h0 = h[0], h1 = h[1];
+  return threadIdx.x & 32 ? h0 : h1;
+}
+// Bitonic steps over 64 E elements of a wave, element E lane + e in x[e]: all of them unrolled, as the instructions of loops over
+// strides would take several times those of the steps. `len` is the length of the runs that are made.
+template <int STRIDE, int E>
+__device__ inline void sort_step(unsigned long long (&x)[E], int len) {
+  auto keep = [](unsigned long long mine, unsigned long long other, bool larger) { return (mine > other) == larger ? mine : other; };
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool down = ((E * threadIdx.x + e) & len) == 0;
+    if constexpr (STRIDE < E) {
+      if ((e & STRIDE) == 0) {
+        const unsigned long long p = x[e], q = x[e | STRIDE];
+        x[e] = keep(p, q, down);
+        x[e | STRIDE] = keep(q, p, !down);
+      }
+    } else {
+      constexpr int X = STRIDE / E;
+      const unsigned long long y = (static_cast<unsigned long long>(lane_xor<X>(static_cast<uint32_t>(x[e] >> 32))) << 32) |
+                                   lane_xor<X>(static_cast<uint32_t>(x[e]));
+      x[e] = keep(x[e], y, ((threadIdx.x & X) == 0) == down);
+    }
+  }
+}
+template <int LEN, int E>
+__device__ inline void sort_merge(unsigned long long (&x)[E], int len) {  // strides LEN / 2 .. 1
+  if constexpr (LEN > 1) {
+    sort_step<LEN / 2>(x, len);
+    sort_merge<LEN / 2>(x, len);
+  }
+}
+template <int LEN, int E>
+__device__ inline void sort_wave(unsigned long long (&x)[E]) {  // runs of 2, 4 .. LEN
+  if constexpr (LEN > 2) sort_wave<LEN / 2>(x);
+  sort_merge<LEN>(x, LEN);
+}
+// Sorts list[0 .. n), n <= E kPickThreads, the largest first. Only strides of 64 E and more cross LDS behind barriers, and only
+// waves that hold some of the n (or are merged with such) take part.
+template <int E>
+__device__ inline void sort_places(lds_u64_t list, int n) {
+  constexpr int W = 64 * E;
+  const int tid = threadIdx.x, i0 = E * tid;
+  unsigned long long x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = i0 + e < n ? list[i0 + e] : 0ull;
+  if ((i0 & ~(W - 1)) < n) sort_wave<W>(x);
+  for (int len = 2 * W; len < 2 * n; len <<= 1) {  // up to the power of two that holds n
+    const bool in = (i0 & ~(len - 1)) < n;
+    for (int half = len >> 1; half >= W; half >>= 1) {
+      __syncthreads();
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) list[i0 + e] = x[e];
+      }
+      __syncthreads();
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const unsigned long long y = list[(i0 + e) ^ half];
+          const bool down = ((i0 + e) & len) == 0, low = (i0 & half) == 0;
+          x[e] = (x[e] > y) == (low == down) ? x[e] : y;
+        }
+      }
+    }
+    if (in) sort_merge<W>(x, len);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) list[i0 + e] = x[e];
+  __syncthreads();
+}
+__device__ inline void sort_list(lds_u64_t list, int n) {
+  __syncthreads();
+  if (n <= kPickThreads) sort_places<1>(list, n);
+  else sort_places<kCap / kPickThreads>(list, n);
+}
+
 // A row's bins and weights.
 struct RowBins {
   double inv, k, m, top;
   const double* pow64;
-  __device__ int bin(double l) const {  // kBins: none
+  __device__ int bin(double l) const {  // kBins: none. A number above the maximum (a limit's margin) counts as the maximum
     const double d = top - floor(l * inv);
-    return d < kBins ? static_cast<int>(d) : kBins;
+    return d < kBins ? static_cast<int>(fmax(d, 0.0)) : kBins;
+  }
+  // The least logit of bins up to b: the float next to the bin's end, or a neighbour of it.
+  __device__ float least(int b) const {
+    if (b < 0) return INFINITY;
+    float f = static_cast<float>((top - b) / inv);
+    if (f != f) f = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float lower = nextafterf(f, -INFINITY);
+      if (bin(static_cast<double>(lower)) <= b) f = lower;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (bin(static_cast<double>(f)) > b) f = nextafterf(f, INFINITY);
+    return f;
   }
   __device__ double weight(float l) const {
     const double w = pow2_64th((static_cast<double>(l) - m) * k, pow64);
@@ -259,31 +399,36 @@ struct RowBins {
   __device__ static int lift(int c) { return static_cast<int>((max(c, 1) - 1) * (1.4426950408889634 / kPerT)); }
 };
 
+// One workgroup a row.
 template <int DT>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleArgs a) {
+  constexpr int kAhead = DT == SQX_DTYPE_F32 ? 4 : 8, kWaves = kPickThreads / 64, E = kCap / kPickThreads;
   __shared__ double pow64[64];
-  __shared__ double redd[kPickThreads / 64], weight_to[kBins], slice_w[kMaxSlices], scale[kMaxSlices];
-  __shared__ int redi[kPickThreads / 64], shift[kMaxSlices];
+  __shared__ double redd[kWaves], weight_to[kBins], slice_w[kMaxSlices], scale[kMaxSlices];
+  __shared__ int shift[kMaxSlices], count_to[kBins];
   __shared__ float smax[kMaxSlices];
   __shared__ unsigned long long slice_fix[kMaxSlices];
   __shared__ unsigned long long list[kCap];
-  __shared__ double before[kCap + 1];  // weight of the list's tokens before each; the digits' counts and weights where it is not sorted
-  __shared__ int found, at_k, rank_k, in_k, at_p0, at_p1, pos_k, pos_p, pos_m, n_p, n_m, end_p, end_m, pick, last;
-  __shared__ double z0, z1;
+  __shared__ double before[kCap + 1];  // weight of the list's tokens before each; where there is no list, of a digit's tokens
+  __shared__ int found, at_k, at_p0, at_p1, begin[3], end[3], cut_p, cut_m, pick, last, digit_rank;
   __shared__ unsigned long long digit_place, dropped;
   __shared__ double digit_left;
-  __shared__ int digit_rank;
   const int b = blockIdx.x, tid = threadIdx.x, S = a.S;
   const int64_t at = static_cast<int64_t>(b) * S, row0 = static_cast<int64_t>(b) * a.V;
+  // the row's first slices are on their way while the histograms are joined
+  typename Loads8<DT>::Raw ahead[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) ahead[j] = Loads8<DT>::raw(a.logits, row0, j * kSampleSlice + 8 * tid, a.V);
   if (tid < S) smax[tid] = a.smax[at + tid];
   if (tid < kMaxSlices) slice_fix[tid] = 0;
   fill_pow64(pow64);
   if (tid == 0) {
-    found = at_k = at_p0 = at_p1 = pos_k = pos_p = pos_m = n_p = n_m = rank_k = in_k = 0;
-    end_p = pick = 0x7fffffff;
-    end_m = 0x7fffffff;
+    found = at_k = at_p0 = at_p1 = 0;
+    pick = cut_p = cut_m = 0x7fffffff;
     last = -1;
     dropped = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) begin[i] = end[i] = 0x7fffffff;
   }
   __syncthreads();
   float m = smax[0];
@@ -304,9 +449,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   r.m = static_cast<double>(m);
   r.top = floor(r.m * r.inv);
   r.pow64 = pow64;
-  const int want_k = a.k_t != nullptr ? a.k_t[b] : a.k;
-  const double p = a.p_t != nullptr ? static_cast<double>(a.p_t[b]) : a.p;
+  const int want_k = row_k(a, b);
+  const double p = a.p_t != nullptr ? static_cast<double>(a.p_t[b]) : a.p, u = static_cast<double>(a.u[b]);
   const double minp_in = a.minp_t != nullptr ? static_cast<double>(a.minp_t[b]) : a.minp, minp = minp_in > 0.0 ? fmin(minp_in, 1.0) : 0.0;
+  const bool few = want_k >= 1 && want_k <= kFew, by_p = p < 1.0, by_m = minp > 0.0;
 
   // ---- the row's histogram: thread i is bin i
   if (tid < S) {
@@ -314,74 +460,122 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     scale[tid] = smax[tid] == -INFINITY ? 0.0 : r.weight(smax[tid]) * (1.0 / kFix);
   }
   __syncthreads();
-  int c = 0;
-  double w = 0.0;
-  for (int s = 0; s < S; ++s) {
-    const int64_t h = (at + s) * kBins;
-    const int from = tid - shift[s];
-    if (from >= 0) {
-      c += a.count[h + from];
-      w = fma(static_cast<double>(a.mass[h + from]), scale[s], w);
+  int to = 0;
+  double w_to = 0.0;
+  auto join = [&](auto counts, auto weights) {
+#pragma unroll 8
+    for (int s = 0; s < S; ++s) {  // sums of monotone terms in one order: monotone
+      const int from = tid - shift[s];
+      const int64_t h = (at + s) * kBins + max(from, 0);
+      if constexpr (decltype(counts)::value) {
+        const unsigned cs = a.count[h];
+        to += from >= 0 ? cs : 0u;
+      }
+      if constexpr (decltype(weights)::value) {
+        const unsigned long long ws = a.mass[h];
+        w_to = fma(from >= 0 ? static_cast<double>(ws) : 0.0, scale[s], w_to);
+      }
     }
-  }
-  int all;
-  double total;
-  const int to = pick_scan(c, redi, all);
-  weight_to[tid] = pick_scan(w, redd, total);
+  };
+  if (few) join(std::true_type{}, std::false_type{});
+  else if (want_k >= 1) join(std::true_type{}, std::true_type{});
+  else join(std::false_type{}, std::true_type{});
+  weight_to[tid] = w_to;
+  count_to[tid] = to;
   __syncthreads();
-  const double w_before = tid > 0 ? weight_to[tid - 1] : 0.0;
-  const bool by_k = want_k >= 1 && want_k < all, by_p = p < 1.0, by_m = minp > 0.0;
+  const int all = count_to[kBins - 1];
+  const bool by_k = want_k >= 1 && want_k < all;
 
   // ---- the bins that the limits end in
-  if (by_k && to - c < want_k && want_k <= to) {
-    at_k = tid;
-    rank_k = want_k - (to - c);
-    in_k = c;
-    z0 = rank_k == c ? weight_to[tid] : w_before;  // of the first k: exactly, or between these
-    z1 = weight_to[tid];
-  }
+  if (by_k && (tid > 0 ? count_to[tid - 1] : 0) < want_k && want_k <= to) at_k = tid;
   __syncthreads();
-  const double zlo = by_k ? z0 : total, zhi = by_k ? z1 : total;
-  if (by_p && c > 0) {
-    if (w_before < p * zlo) atomicMax(&at_p0, tid);
-    if (w_before < p * zhi) atomicMax(&at_p1, tid);
+  const int rank_k = by_k ? want_k - (at_k > 0 ? count_to[at_k - 1] : 0) : 0;  // of bin at_k the first so many
+  const bool whole_k = by_k && want_k == count_to[at_k];
+  const double total = weight_to[kBins - 1];
+  // the weight of the first k: exactly, or between these
+  const double zlo = !by_k ? total : whole_k ? weight_to[at_k] : at_k > 0 ? weight_to[at_k - 1] : 0.0, zhi = by_k ? weight_to[at_k] : total;
+  const double edge = r.m + T * log(by_m ? minp : 1.0), slack = 1e-9 * (fabs(edge) + T);
+  const int m0 = by_m ? r.bin(edge + slack) : kBins, m1 = by_m ? r.bin(edge - slack) : kBins;
+  if (!few && by_p) {
+    const double w_before = tid > 0 ? weight_to[tid - 1] : 0.0;
+    const bool some = w_to > w_before;
+    raise(&at_p0, some && w_before < p * zlo, tid);
+    raise(&at_p1, some && w_before < p * zhi, tid);
   }
   __syncthreads();
   const int p0 = at_p0, p1 = max(at_p1, at_p0);
-  const double edge = r.m + T * log(minp), slack = 1e-9 * (fabs(edge) + T);
-  const int m0 = by_m ? r.bin(edge + slack) : kBins, m1 = by_m ? r.bin(edge - slack) : kBins;
-  // The cut of top-p lies within the first k: the k-th token is looked for where top-p is off, or its weight matters.
-  const bool use_k = by_k && !(by_p && rank_k == in_k);
-  const bool use_m = m0 < kBins && m0 <= (by_p ? p1 : by_k ? at_k : kBins);
-  auto wanted = [&](int bin) { return (use_k && bin == at_k) || (by_p && bin >= p0 && bin <= p1) || (use_m && bin >= m0 && bin <= m1); };
-  const bool mine = wanted(tid);
-  int n;
-  const int pos = pick_scan(mine ? c : 0, redi, n) - (mine ? c : 0);
-  if (use_k && tid == at_k) pos_k = pos;
-  if (by_p && tid >= p0 && tid <= p1) {
-    if (tid == p0) pos_p = pos;
-    atomicAdd(&n_p, c);
-  }
-  if (use_m && tid >= m0 && tid <= m1) {
-    if (tid == m0) pos_m = pos;
-    atomicAdd(&n_m, c);
-  }
-  __syncthreads();
-
-  // Every token of the row, 8 a thread a pass, the next pass on its way.
-  auto walk = [&](auto&& each) __attribute__((always_inline)) {
-    float x[8], y[8];
-    Loads8<DT>::load(a.logits, row0, 8 * tid, a.V, x);
-    for (int s = 0; s < S; ++s) {
-      const int i0 = s * kSampleSlice + 8 * tid;
-      if (s + 1 < S) Loads8<DT>::load(a.logits, row0, i0 + kSampleSlice, a.V, y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (i0 + e < a.V) each(x[e], i0 + e, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = y[e];
+  // Tokens to collect: with a small k all that may stay; else those of the bins in which a limit ends. The cut of top-p lies
+  // within the first k: the k-th token is looked for where top-p is off, or where the weight of the first k needs it.
+  const bool use_k = few || (by_k && !(by_p && whole_k));
+  const bool use_p = !few && by_p, use_m = !few && m0 < kBins && m0 <= (by_p ? p1 : by_k ? at_k : kBins);
+  float from[3], below[3];  // of logits, [from, below)
+  {
+    // lane i of a wave finds one of their ends
+    float x = 0.0f;
+    const int lane = tid & 63;
+    if (lane < 6) {
+      const int i = lane >> 1, b0 = i == 0 ? (few ? 0 : at_k) : i == 1 ? p0 : m0, b1 = i == 0 ? (by_k ? at_k : kBins - 1) : i == 1 ? p1 : m1;
+      x = r.least(lane & 1 ? b0 - 1 : min(b1, kBins - 1));
     }
-  };
+    const bool used[3] = {use_k, use_p, use_m};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const float lo = __shfl(x, 2 * i, 64), hi = __shfl(x, 2 * i + 1, 64);
+      from[i] = used[i] ? lo : INFINITY;
+      below[i] = used[i] ? hi : -INFINITY;
+    }
+  }
+  const float lowest = fminf(from[0], fminf(from[1], from[2])), highest = fmaxf(below[0], fmaxf(below[1], below[2]));
+  const bool limited = use_k || use_p || use_m;
+
+  if (limited) {
+    // ---- every token of the row, 8 a thread a pass, kAhead passes loaded together
+    auto look = [&](const typename Loads8<DT>::Raw& x, int at8) __attribute__((always_inline)) {
+      float v[8];
+      Loads8<DT>::floats(x, v);
+      unsigned hits = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hits |= static_cast<unsigned>((v[e] >= lowest) & (v[e] < highest)) << e;
+      const int i0 = Loads8<DT>::first(at8, a.V);
+      if (i0 != at8) {  // of the last eight what no other thread has
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hits &= Loads8<DT>::has(at8, a.V, e) ? ~0u : ~(1u << e);
+      }
+      if (__ballot(hits != 0) == 0) return;
+      unsigned in = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float l = v[e];
+        const bool i0 = (l >= from[0]) & (l < below[0]), i1 = (l >= from[1]) & (l < below[1]), i2 = (l >= from[2]) & (l < below[2]);
+        in |= static_cast<unsigned>(i0 | i1 | i2) << e;
+      }
+      in &= hits;
+      if (in == 0) return;
+      int zero;  // to the compiler any number: it would add a wave's lanes up one by one before a single atomic
+      asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+      int to_place = atomicAdd(&found + zero, __popc(in));  // whichever lane comes first: the list is sorted
+      while (in != 0) {
+        const int e = __ffs(in) - 1;
+        in &= in - 1;
+        float l = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) l = j == e ? v[j] : l;
+        if (to_place < kCap) list[to_place] = place(l, i0 + e);
+        ++to_place;
+      }
+    };
+    for (int s0 = 0; s0 < S; s0 += kAhead) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (s0 + j < S) look(ahead[j], (s0 + j) * kSampleSlice + 8 * tid);
+      if (s0 + kAhead < S) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) ahead[j] = Loads8<DT>::raw(a.logits, row0, (s0 + kAhead + j) * kSampleSlice + 8 * tid, a.V);
+      }
+    }
+    __syncthreads();
+  }
+  const int n = found;
 
   unsigned long long cut = 0;  // kept of bin cut_bin: places from here on
   int cut_bin = kBins;         // bins before it are kept whole
@@ -391,39 +585,19 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
       cut_bin = bin;
     }
   };
-  if (n > 0 && n <= kCap) {
-    // ---- collected and sorted
-    walk([&](float l, int i, int) {
-      if (wanted(r.bin(static_cast<double>(l)))) list[min(atomicAdd(&found, 1), kCap - 1)] = place(l, i);
-    });
-    int size = 64;
-    while (size < n) size <<= 1;
-    __syncthreads();
-    for (int i = tid; i < size; i += kPickThreads)
-      if (i >= n) list[i] = 0;
-    __syncthreads();
-    for (int len = 2; len <= size; len <<= 1)
-      for (int half = len >> 1; half > 0; half >>= 1) {
-        for (int i = tid; i < size / 2; i += kPickThreads) {
-          const int lo = 2 * i - (i & (half - 1)), hi = lo + half;
-          const unsigned long long x = list[lo], y = list[hi];
-          if ((x < y) == ((lo & len) == 0)) {
-            list[lo] = y;
-            list[hi] = x;
-          }
-        }
-        __syncthreads();
-      }
-    constexpr int E = kCap / kPickThreads;
-    double e[E], mine_w = 0.0;
+  bool walked = false;  // slices' weights are summed token by token
+  double e[E];
+  if (limited && n <= kCap) {  // the list sorted, its tokens' weights and their sums
+    sort_list((lds_u64_t)list, n);
+    double mine = 0.0, whole;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int i = E * tid + j;
-      e[j] = i < n ? r.weight(place_logit(list[i])) : 0.0;
-      mine_w += e[j];
+      e[j] = 0.0;
+      if (i < n) e[j] = r.weight(place_logit(list[i]));
+      mine += e[j];
     }
-    double all_w;
-    double run = pick_scan(mine_w, redd, all_w) - mine_w;
+    double run = pick_scan(mine, redd, whole) - mine;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       before[E * tid + j] = run;
@@ -431,33 +605,112 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
     if (tid == kPickThreads - 1) before[kCap] = run;
     __syncthreads();
-    double z = total;
-    if (by_k) z = use_k ? (at_k > 0 ? weight_to[at_k - 1] : 0.0) + (before[pos_k + rank_k] - before[pos_k]) : zhi;
-    if (by_p) {  // the last token with less than p z before it
-      const double left = p * z - (p0 > 0 ? weight_to[p0 - 1] : 0.0) + before[pos_p];
-      for (int i = tid; i < n_p; i += kPickThreads)
-        if (i > 0 && !(before[pos_p + i] < left)) atomicMin(&end_p, i - 1);
-    }
-    if (use_m) {  // the first token below min_p
-      for (int i = tid; i < n_m; i += kPickThreads)
-        if (r.weight(place_logit(list[pos_m + i])) < minp) atomicMin(&end_m, i);
+  }
+
+  if (few && n <= kCap) {
+    // ---- all that may stay is in the list: the cut is a length, and the draw is among its tokens, by id
+    const int first_k = min(want_k, n);
+    const double left = p * before[first_k];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = E * tid + j;
+      if (i < first_k && i > 0) {
+        lower(&cut_p, by_p && !(before[i] < left), i);
+        lower(&cut_m, e[j] < minp, i);
+      }
     }
     __syncthreads();
-    auto cut_here = [&](int i, int more) { cut_at(list[i] + more, r.bin(static_cast<double>(place_logit(list[i])))); };
-    if (use_k) cut_here(pos_k + rank_k - 1, 0);
-    if (by_p) cut_here(pos_p + min(end_p, n_p - 1), 0);
-    if (use_m && n_m > 0) {
-      if (end_m < n_m) cut_here(pos_m + end_m, 1);
-      else cut_here(pos_m + n_m - 1, 0);
+    const int stay = min(first_k, min(cut_p, cut_m));
+    unsigned long long mine[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = E * tid + j;
+      mine[j] = i < stay ? (list[i] << 32) | static_cast<unsigned>(i) : 0ull;  // the low word of a place falls as the id grows
     }
-  } else if (n > kCap) {
-    // ---- digit by digit
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      before[E * tid + j] = e[j];
+      list[E * tid + j] = mine[j];
+    }
+    sort_list((lds_u64_t)list, stay);
+    double sum = 0.0, kept;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = E * tid + j;
+      e[j] = i < stay ? before[static_cast<uint32_t>(list[i])] : 0.0;
+      sum += e[j];
+    }
+    double upto = pick_scan(sum, redd, kept) - sum;
+    int first = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      upto += e[j];
+      if (E * tid + j < stay && upto > u * kept) first = min(first, E * tid + j);
+    }
+    lower(&pick, first != 0x7fffffff, first);
+    __syncthreads();
+    if (tid == 0) a.out[b] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(list[min(pick, stay - 1)] >> 32));
+    return;
+  }
+  if (limited && n <= kCap) {
+    // ---- the tokens of the bins that the limits end in
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = E * tid + j;
+      if (i >= n) continue;
+      const float l = place_logit(list[i]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        lower(&begin[k], l < below[k], i);
+        lower(&end[k], l < from[k], i);
+      }
+    }
+    __syncthreads();
+    auto bound = [&](int x) { return min(x, n); };
+    const int k0 = bound(begin[0]), q0 = bound(begin[1]), q1 = bound(end[1]), e0 = bound(begin[2]), e1 = bound(end[2]);
+    double z = total;
+    if (by_k) z = use_k ? (at_k > 0 ? weight_to[at_k - 1] : 0.0) + (before[min(k0 + rank_k, n)] - before[k0]) : zhi;
+    if (use_p) {  // the first token with p z before it
+      const double left = p * z - (p0 > 0 ? weight_to[p0 - 1] : 0.0) + before[q0];
+      for (int i = q0 + tid; i < q1; i += kPickThreads) lower(&cut_p, i > q0 && !(before[i] < left), i);
+    }
+    if (use_m) {  // the first token below min_p
+      for (int i = e0 + tid; i < e1; i += kPickThreads) lower(&cut_m, r.weight(place_logit(list[i])) < minp, i);
+    }
+    __syncthreads();
+    auto bin_at = [&](int i) { return r.bin(static_cast<double>(place_logit(list[i]))); };
+    auto keep_to = [&](int i) { cut_at(list[i], bin_at(i)); };  // the i-th token is the last that stays
+    if (use_k) keep_to(min(k0 + rank_k, n) - 1);
+    if (use_p && q1 > q0) keep_to(min(cut_p, q1) - 1);
+    if (use_m) {
+      if (e1 == e0) cut_at(~0ull, m0);  // no token near the limit
+      else if (cut_m < e1) cut_at(list[cut_m] + 1, bin_at(cut_m));
+      else keep_to(e1 - 1);
+    }
+  } else if (limited) {
+    // ---- too many for the list: the cut digit by digit
     unsigned long long* const digit_w = reinterpret_cast<unsigned long long*>(before);
     unsigned* const digit_c = reinterpret_cast<unsigned*>(before + 256);
-    // The place of the last token of bins b0 .. b1 that is kept: of the first `rank`, or of those with less than `left` before
-    // them, both counted from bin b0.
-    auto select = [&](int b0, int b1, bool by_rank, int rank, double left) {
-      const double unit = ldexp(1.0, r.lift(b0) + 42);  // 2^20 tokens of at most 1 / unit 2^42 fit 64 bits
+    auto walk = [&](auto&& each) {
+      for (int s = 0; s < S; ++s) {
+        const int i0 = s * kSampleSlice + 8 * tid;
+        float v[8];
+        Loads8<DT>::load(a.logits, row0, i0, a.V, v);
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j)
+          if (Loads8<DT>::has(i0, a.V, j)) {
+            float l = v[0];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) l = k == j ? v[k] : l;
+            if (l > -INFINITY) each(l, place(l, Loads8<DT>::first(i0, a.V) + j), s);
+          }
+      }
+    };
+    const double unit = 0x1p42;  // 2^20 tokens of at most 2^42 fit 64 bits
+    auto fix = [&](float l) { return static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5)); };
+    // The place of the last token that is kept, of the first `rank`, or of those with less than `left` before them.
+    auto select = [&](bool by_rank, int rank, double left) {
       if (tid == 0) {
         digit_place = 0;
         digit_rank = rank;
@@ -470,35 +723,33 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         }
         __syncthreads();
         const unsigned long long so_far = digit_place;
-        walk([&](float l, int i, int) {
-          const int bin = r.bin(static_cast<double>(l));
-          const unsigned long long q = place(l, i);
-          if (bin < b0 || bin > b1 || (sh < 56 && (q ^ so_far) >> (sh + 8) != 0)) return;
+        walk([&](float l, unsigned long long q, int) {
+          if (sh < 56 && (q ^ so_far) >> (sh + 8) != 0) return;
           const int d = static_cast<int>(q >> sh) & 255;
-          const unsigned long long f = static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5));
+          const unsigned long long f = by_rank ? 0ull : fix(l);
           const unsigned long long same = __ballot(d == __builtin_amdgcn_readfirstlane(d));
-          if (same == __ballot(true)) {  // equal logits: one addition for the wave's tokens, not one after the other
+          if (same == __ballot(true)) {  // equal digits: one addition for the wave's tokens, not one after the other
             unsigned long long sum = 0;
-            for (unsigned long long left_lanes = same; left_lanes != 0; left_lanes &= left_lanes - 1) {
-              const int lane = __ffsll(left_lanes) - 1;
-              const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(f), lane);
-              const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(f >> 32), lane);
-              sum += (static_cast<unsigned long long>(hi) << 32) | lo;
-            }
+            if (!by_rank)
+              for (unsigned long long lanes = same; lanes != 0; lanes &= lanes - 1) {
+                const int lane = __ffsll(lanes) - 1;
+                const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(f), lane);
+                const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(f >> 32), lane);
+                sum += (static_cast<unsigned long long>(hi) << 32) | lo;
+              }
             if ((threadIdx.x & 63) == __ffsll(same) - 1) {
               atomicAdd(&digit_c[d], static_cast<unsigned>(__popcll(same)));
-              atomicAdd(&digit_w[d], sum);
+              if (!by_rank) atomicAdd(&digit_w[d], sum);
             }
           } else {
             atomicAdd(&digit_c[d], 1u);
-            atomicAdd(&digit_w[d], f);
+            if (!by_rank) atomicAdd(&digit_w[d], f);
           }
         });
         __syncthreads();
         if (tid == 0) {
-          int chosen = -1, rank_at = 0;
+          int chosen = -1, rank_at = 0, c_run = 0;
           double left_at = 0.0, w_run = 0.0;
-          int c_run = 0;
           for (int d = 255; d >= 0; --d) {
             if (digit_c[d] == 0) continue;
             if (chosen < 0 || (by_rank ? c_run < digit_rank : w_run < digit_left)) {
@@ -519,68 +770,49 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
       __syncthreads();
       return q;
     };
-    // The weight of bin b0's tokens up to place q, in units of the row's largest.
-    auto weight_up_to = [&](int b0, unsigned long long q) {
-      double sum = 0.0, all_w;
-      walk([&](float l, int i, int) {
-        if (r.bin(static_cast<double>(l)) == b0 && place(l, i) >= q) sum += r.weight(l);
-      });
-      pick_scan(sum, redd, all_w);
-      return all_w;
-    };
-    double z = total;
-    if (use_k) {
-      const unsigned long long q = select(at_k, at_k, true, rank_k, 0.0);
-      cut_at(q, at_k);
-      if (by_p) z = (at_k > 0 ? weight_to[at_k - 1] : 0.0) + weight_up_to(at_k, q);
-    } else if (by_k) {
-      z = zhi;
-    }
+    if (by_k) cut = select(true, want_k, 0.0);
     if (by_p) {
-      const unsigned long long q = select(p0, p1, false, 0, p * z - (p0 > 0 ? weight_to[p0 - 1] : 0.0));
-      cut_at(q, r.bin(static_cast<double>(place_logit(q))));
+      double mine = 0.0, z;
+      walk([&](float l, unsigned long long q, int) { mine += q >= cut && r.bin(static_cast<double>(l)) < kBins ? r.weight(l) : 0.0; });
+      pick_scan(mine, redd, z);
+      cut = max(cut, select(false, 0, p * z));
     }
-    if (use_m) {
-      walk([&](float l, int i, int) {
-        const int bin = r.bin(static_cast<double>(l));
-        if (bin >= m0 && bin <= m1 && r.weight(l) < minp) atomicMax(&dropped, place(l, i));
+    if (by_m) {
+      walk([&](float l, unsigned long long q, int) {
+        if (r.weight(l) < minp) atomicMax(&dropped, q);
       });
       __syncthreads();
-      if (dropped != 0) cut_at(dropped + 1, r.bin(static_cast<double>(place_logit(dropped))));
-      else cut_at(~0ull, m1 + 1);
+      cut = max(cut, dropped + 1);
     }
+    walk([&](float l, unsigned long long q, int s) {
+      if (q >= cut && r.bin(static_cast<double>(l)) < kBins) atomicAdd(&slice_fix[s], fix(l));
+    });
+    walked = true;
+    __syncthreads();
   }
-  if (use_m && n_m == 0) cut_at(~0ull, m0);  // no token near the limit
 
   // ---- the weight that each slice keeps: whole bins, and the tokens of the cut's bin
-  const double unit = ldexp(kFix / 64, r.lift(cut_bin)), back = 1.0 / unit;  // 8192 tokens of at most 2^42 fit 64 bits
-  if (cut_bin < kBins) {
-    auto add = [&](float l, unsigned long long q, int s) {
+  const double unit = walked ? 0x1p42 : ldexp(0x1p42, r.lift(cut_bin));  // 8192 tokens of at most 2^42 fit 64 bits
+  if (!walked && cut_bin < kBins) {
+    for (int i = tid; i < n; i += kPickThreads) {
+      const unsigned long long q = list[i];
+      const float l = place_logit(q);
       if (q >= cut && r.bin(static_cast<double>(l)) == cut_bin)
-        atomicAdd(&slice_fix[s], static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5)));
-    };
-    if (n <= kCap) {
-      for (int i = tid; i < n; i += kPickThreads)
-        add(place_logit(list[i]), list[i], static_cast<int>((0xffffffffu - static_cast<uint32_t>(list[i])) / kSampleSlice));
-    } else {
-      walk([&](float l, int i, int s) { add(l, place(l, i), s); });
+        atomicAdd(&slice_fix[(0xffffffffu - static_cast<uint32_t>(q)) / kSampleSlice], static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5)));
     }
     __syncthreads();
   }
-  for (int s = tid >> 6; s < S; s += kPickThreads / 64) {
-    double sum = 0.0;
-    for (int i = tid & 63; i < kBins && i + shift[s] < min(cut_bin, kBins); i += 64)
-      sum = fma(static_cast<double>(a.mass[(at + s) * kBins + i]), scale[s], sum);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    if ((tid & 63) == 0) slice_w[s] = fma(static_cast<double>(slice_fix[s]), back, sum);
+  if (tid < S) {
+    const int upto = walked ? -1 : min(cut_bin, kBins) - 1 - shift[tid];
+    const double whole = upto >= 0 ? static_cast<double>(a.mass[(at + tid) * kBins + upto]) * scale[tid] : 0.0;
+    slice_w[tid] = fma(static_cast<double>(slice_fix[tid]), 1.0 / unit, whole);
   }
   __syncthreads();
 
   // ---- the draw: its slice, then its token
   double kept = 0.0;
   for (int s = 0; s < S; ++s) kept += slice_w[s];
-  const double target = static_cast<double>(a.u[b]) * kept;
+  const double target = u * kept;
   int chosen = -1;
   double skipped = 0.0, run = 0.0;
   for (int s = 0; s < S; ++s) {
@@ -592,31 +824,90 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   }
   chosen = max(chosen, 0);
   float x[8];
-  const int i0 = chosen * kSampleSlice + 8 * tid;
-  Loads8<DT>::load(a.logits, row0, i0, a.V, x);
-  double e[8], sum = 0.0;
+  const int at8 = chosen * kSampleSlice + 8 * tid, i0 = Loads8<DT>::first(at8, a.V);
+  Loads8<DT>::load(a.logits, row0, at8, a.V, x);
+  double d[8], sum = 0.0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int bin = r.bin(static_cast<double>(x[j]));
-    const bool in = i0 + j < a.V && bin < kBins && (bin < cut_bin || (bin == cut_bin && place(x[j], i0 + j) >= cut));
-    e[j] = in ? r.weight(x[j]) : 0.0;
-    sum += e[j];
+    const bool above = place(x[j], i0 + j) >= cut;
+    const bool in = Loads8<DT>::has(at8, a.V, j) && bin < kBins && (walked ? above : bin < cut_bin || (bin == cut_bin && above));
+    d[j] = in ? r.weight(x[j]) : 0.0;
+    sum += d[j];
   }
   double all_w;
   double upto = skipped + pick_scan(sum, redd, all_w) - sum;
-  int first = 0x7fffffff, end = -1;
+  int first = 0x7fffffff, least = -1;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    upto += e[j];
-    if (e[j] > 0.0) {
-      end = i0 + j;
+    upto += d[j];
+    if (d[j] > 0.0) {
+      least = i0 + j;
       if (upto > target) first = min(first, i0 + j);
     }
   }
-  if (first != 0x7fffffff) atomicMin(&pick, first);
-  if (end >= 0) atomicMax(&last, end);
+  lower(&pick, first != 0x7fffffff, first);
+  raise(&last, least >= 0, least);
   __syncthreads();
   if (tid == 0) a.out[b] = pick != 0x7fffffff ? pick : last;
+}
+
+// Fewer than eight tokens: a thread a row.
+__global__ __launch_bounds__(256) void sample_short_kernel(const SampleArgs a, int dtype, int B) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int64_t row0 = static_cast<int64_t>(b) * a.V;
+  float l[7];
+  float best = -INFINITY;
+  int arg = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    l[i] = i < a.V ? load_as_f32(a.logits, dtype, row0 + i) : -INFINITY;
+    if (i < a.V && greedy_takes(l[i], i, best, arg)) {
+      best = l[i];
+      arg = i;
+    }
+  }
+  const double T = row_temp(a, b);
+  if (T == 0.0 || !(best < INFINITY) || best == -INFINITY) {
+    a.out[b] = T == 0.0 ? arg : -1;
+    return;
+  }
+  const int k = row_k(a, b);
+  const double p = a.p_t != nullptr ? static_cast<double>(a.p_t[b]) : a.p, u = static_cast<double>(a.u[b]);
+  const double minp = a.minp_t != nullptr ? static_cast<double>(a.minp_t[b]) : a.minp;
+  double w[7], z = 0.0;
+  int rank[7];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    const double d = (static_cast<double>(l[i]) - static_cast<double>(best)) / T;
+    w[i] = i < a.V && d > -32.0 ? exp(d) : 0.0;
+    rank[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 7; ++j) rank[i] += l[j] > l[i] || (l[j] == l[i] && j < i);
+    if (k >= 1 && rank[i] >= k) w[i] = 0.0;
+    z += w[i];
+  }
+  double kept = 0.0, v[7];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    double before = 0.0;
+#pragma unroll
+    for (int j = 0; j < 7; ++j) before += rank[j] < rank[i] ? w[j] : 0.0;
+    v[i] = (p < 1.0 && rank[i] > 0 && !(before < p * z)) || (minp > 0.0 && w[i] < fmin(minp, 1.0)) ? 0.0 : w[i];
+    kept += v[i];
+  }
+  double upto = 0.0;
+  int pick = -1, last = 0;
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    upto += v[i];
+    if (v[i] > 0.0) {
+      last = i;
+      if (pick < 0 && upto > u * kept) pick = i;
+    }
+  }
+  a.out[b] = pick < 0 ? last : pick;
 }
 
 }  // namespace sqx
@@ -660,6 +951,11 @@ extern "C" int sqx_sample(const void* logits, int dtype, const float* u, const f
   a.out = tokens;
   const dim3 grid(static_cast<unsigned>(S), static_cast<unsigned>(B));
   const hipStream_t s = as_stream(stream);
+  if (V < 8) {
+    hipLaunchKernelGGL(sample_short_kernel, dim3(static_cast<unsigned>(ceil_div(B, 256))), dim3(256), 0, s, a, dtype, static_cast<int>(B));
+    SQX_LAUNCH_CHECK(fn);
+    return SQX_OK;
+  }
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     hipLaunchKernelGGL((sample_hist_kernel<DT>), grid, dim3(kHistThreads), 0, s, a);
