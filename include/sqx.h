@@ -952,7 +952,8 @@ int sqx_kvpages_compact(void* k_codes, void* v_codes, float* k_scale, float* v_s
                         int64_t ws_bytes, sqx_stream_t stream);
 
 /* Attention of a batch whose rows share the first pages of their contexts. Rows with the same leaders[b] >= 0 make a group; what
- * they share is the whole blocks in front that all of them name alike and that lie before every one's start. A plan is made
+ * they share is the whole blocks in front that all of them name alike and that lie before every one's start, in multiples of 64
+ * tokens (128 with heads of 64). A plan is made
  * for T tokens a row and these heads (B <= 4096); it holds while the groups' rows and the table entries of their shared blocks
  * stay. A row whose start has fallen behind the shared blocks is attended for itself. sqx_kvshared_attention is
  * sqx_kvblock_attention otherwise, the shared keys read once for a group (with T H / Hkv above 128, or 64 with heads of 256, it is

@@ -51,7 +51,9 @@ __device__ inline int block_scan(int x, int* red, int& total) {
 
 // Copies pages src[i] -> dst[i], i < n, in all layers. A workgroup's piece is kCopyUnits units of one page, or several small
 // pages; pieces are dealt out in a loop, since the count is known on the device only. Pairs that name no page, or the same one
-// twice, are left out.
+// twice, are left out. Stores that pass the caches by leave these to the loads: 500 MB (read and written) of pages of 64 KiB in
+// 99 us, 5.3 TB/s, where plain stores take 115; 2 GiB in 437 and 448; pages of 2 KiB, 250 MB, in 39 and 57. Loads that pass them by
+// too take 112, 434 and 61; twice as many workgroups change nothing.
 __device__ inline void copy_pages(const KvPool& p, const int* src, const int* dst, uint32_t n, uint32_t group, uint32_t groups) {
   const uint32_t units = p.units, per = max(kCopyUnits / units, 1u);      // per: jobs (pair, layer, keys or values) of a piece
   const uint32_t pieces = (units + kCopyUnits - 1) / kCopyUnits;          // of a job
@@ -84,7 +86,7 @@ __device__ inline void copy_pages(const KvPool& p, const int* src, const int* ds
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (to[k] != nullptr) *to[k] = x[k];
+      if (to[k] != nullptr) __builtin_nontemporal_store(x[k], to[k]);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (sc_to[k] != nullptr) *sc_to[k] = *sc_from[k];

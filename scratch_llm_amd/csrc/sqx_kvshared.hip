@@ -17,28 +17,40 @@ namespace sqx {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRows = 4096;      // rows of a batch
-constexpr int kTileFrom = 512;       // query rows of a group from which the prompt kernel takes it
+// The prompt kernel takes groups of so many query rows, and of so many products of these with shared keys: its prologue and the 133
+// KB that each of its workgroups leaves to be joined have to pay. us a call, direct and prompt kernel, 8 kv heads of 128, int8:
+//   512 rows x 8192 keys 57, 63; 1024 x 4096 74, 84; 2048 x 2048 103, 110; 1024 x 16384 124, 108; 2048 x 8192 167, 157
+constexpr int kTileFrom = 512;
+constexpr int64_t kTileWork = int64_t(1) << 23;
 constexpr int kDirectGroups = 512, kTileGroups = 256;
+constexpr int kPartSteps = 40;
 
 // Query rows of a row (T G) up to which the direct kernel takes it; from there on it reads its keys once for many rows by itself.
 constexpr int own_most(int64_t d) { return d == 256 ? 64 : 128; }
 constexpr int direct_rows(int d) { return d == 256 ? 16 : 32; }
 
-// A plan: what it was made for, then its arrays.
-struct KvPlanHead {
-  int direct_items, tile_items, groups, pad[5];
+// A plan's arrays. What a workgroup or a row needs stands together, to be had in one load.
+struct KvItem {  // a workgroup of the shared part
+  int lead;         // a row that names the shared blocks; -1: no item
+  int first, M;     // the group's first row in `order`, its query rows per kv head
+  int keys;         // shared keys
+  int tile, part, parts, pad;
+  int64_t at;       // of the group's first partial result
+  int64_t pad2;
+};
+struct KvRow {  // a row of the batch
+  int shared, parts, M, member;  // shared keys (0: none), the parts they come in, the group's query rows, the row's place among its rows
+  int64_t at;
+  int64_t pad;
 };
 struct KvGroup {
-  int first, rows, keys, parts;  // its first row in `order`, its number of rows, shared keys, parts of the keys
-  int64_t at;                    // of its first partial result
-  int M, pad;                    // query rows per kv head
+  int lead, first, rows, keys, parts, M, item, pad;
+  int64_t at;
 };
-struct KvItem { int group, tile, part, pad; };
 
 struct KvSharedPlan {
-  KvPlanHead* head;
-  int *order, *group, *member, *shared, *same, *lead;
-  KvGroup* groups;
+  int *order, *lead, *same, *member;  // the last three between the plan's two kernels
+  KvRow* rows;
   KvItem *direct, *tile;
 };
 
@@ -57,8 +69,7 @@ inline KvPlanSizes kv_plan_sizes(int64_t B, int64_t T, int64_t H, int64_t Hkv, i
   s.tile = B * s.TG >= kTileFrom ? ceil_div(B * s.TG, tspan) + B / 2 + s.wt : 0;
   s.partials = B * s.TG + s.wd * span + (s.tile ? s.wt * tspan : 0);
   const int64_t r4 = (B + 3) / 4 * 4;
-  s.bytes = static_cast<int64_t>(sizeof(KvPlanHead)) + 6 * r4 * 4 + (B / 2 + 1) * static_cast<int64_t>(sizeof(KvGroup)) +
-            (s.direct + s.tile) * static_cast<int64_t>(sizeof(KvItem));
+  s.bytes = 4 * r4 * 4 + B * static_cast<int64_t>(sizeof(KvRow)) + (s.direct + s.tile) * static_cast<int64_t>(sizeof(KvItem));
   return s;
 }
 inline KvSharedPlan kv_plan_at(void* p, const KvPlanSizes& s) {
@@ -70,30 +81,37 @@ inline KvSharedPlan kv_plan_at(void* p, const KvPlanSizes& s) {
     return at;
   };
   const int64_t r4 = (s.B + 3) / 4 * 4;
-  a.head = reinterpret_cast<KvPlanHead*>(take(sizeof(KvPlanHead)));
-  for (int** x : {&a.order, &a.group, &a.member, &a.shared, &a.same, &a.lead}) *x = reinterpret_cast<int*>(take(4 * r4));
-  a.groups = reinterpret_cast<KvGroup*>(take((s.B / 2 + 1) * sizeof(KvGroup)));
+  for (int** x : {&a.order, &a.lead, &a.same, &a.member}) *x = reinterpret_cast<int*>(take(4 * r4));
+  a.rows = reinterpret_cast<KvRow*>(take(s.B * sizeof(KvRow)));
   a.direct = reinterpret_cast<KvItem*>(take(s.direct * sizeof(KvItem)));
   a.tile = reinterpret_cast<KvItem*>(take(s.tile * sizeof(KvItem)));
   return a;
 }
 
-// Workgroup b: the first row with row b's leader, and how many whole blocks before row b's start name the same pages in both.
+// Workgroup b: the first row with row b's leader, how many such rows stand before b, and how many whole blocks before row b's
+// start name the same pages in both.
 __global__ __launch_bounds__(256) void shared_match_kernel(const int* table, const int* starts, const int* leaders, int B, int width,
                                                            int shift, KvSharedPlan p) {
-  __shared__ int first, differ;
+  __shared__ int first, differ, rank;
   const int b = blockIdx.x, lead = leaders[b];
   if (threadIdx.x == 0) {
     first = b;
     differ = 0x7fffffff;
+    rank = 0;
   }
   __syncthreads();
-  if (lead >= 0)
+  if (lead >= 0) {
+    int mine = 0, least = 0x7fffffff;
     for (int c = threadIdx.x; c < b; c += 256)
       if (leaders[c] == lead) {
-        atomicMin(&first, c);
-        break;
+        least = min(least, c);
+        ++mine;
       }
+    if (mine != 0) {
+      atomicMin(&first, least);
+      atomicAdd(&rank, mine);
+    }
+  }
   __syncthreads();
   const int f = first;
   const int most = lead < 0 ? 0 : min(max(starts[b], 0) >> shift, width);
@@ -115,13 +133,15 @@ __global__ __launch_bounds__(256) void shared_match_kernel(const int* table, con
   if (threadIdx.x == 0) {
     p.same[b] = min(differ, most);
     p.lead[b] = lead < 0 ? -1 : f;
+    p.member[b] = rank;
   }
 }
 
 struct PlanArgs {
   KvSharedPlan p;
   int B, TG, shift, block, span, tspan;
-  int wd, wt;
+  int unit;    // shared keys come in multiples of so many: whole steps of either kernel
+  int wd, wt, direct, tile;  // workgroups per kv head to aim at, and at most
 };
 
 // The sum of `x` over the threads before this one, and of all.
@@ -151,8 +171,7 @@ __device__ inline N plan_scan(N x, N* red, N& total) {
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArgs a) {
   constexpr int E = kPlanRows / kPlanThreads;
   __shared__ int lead[kPlanRows], many[kPlanRows], blocks[kPlanRows], id[kPlanRows];
-  __shared__ int redi[kPlanThreads / 64];
-  __shared__ int64_t redl[kPlanThreads / 64];
+  __shared__ int64_t red[kPlanThreads / 64];
   __shared__ KvGroup group[kPlanRows / 2];
   const int tid = threadIdx.x;
   for (int b = tid; b < a.B; b += kPlanThreads) {
@@ -167,96 +186,91 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArg
       atomicMin(&blocks[lead[b]], a.p.same[b]);
     }
   __syncthreads();
-  // groups in the order of their first rows: E consecutive rows a thread
-  int n = 0, rows = 0;
+  // groups in the order of their first rows: E consecutive rows a thread; rows of groups in the high word, groups in the low
+  int64_t n = 0, sum;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int b = E * tid + e;
-    const bool is = b < a.B && lead[b] == b && many[b] >= 2 && blocks[b] >= 1;
+    const bool is = b < a.B && lead[b] == b && many[b] >= 2 && blocks[b] << a.shift >= a.unit;
     if (b < a.B) id[b] = is ? 0 : -1;
-    n += is;
-    rows += is ? many[b] : 0;
+    n += is ? (static_cast<int64_t>(many[b]) << 32) + 1 : 0;
   }
-  int groups, all;
-  int g = plan_scan(n, redi, groups), at = plan_scan(rows, redi, all);
+  n = plan_scan(n, red, sum);
+  const int groups = static_cast<int>(sum);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int b = E * tid + e;
     if (b < a.B && id[b] == 0) {
+      const int g = static_cast<int>(n);
       id[b] = g;
-      group[g] = KvGroup{at, many[b], blocks[b] << a.shift, 1, 0, many[b] * a.TG, 0};
-      at += many[b];
-      ++g;
+      group[g] = KvGroup{b, static_cast<int>(n >> 32), many[b], (blocks[b] << a.shift) & -a.unit, 1, many[b] * a.TG, 0, 0, 0};
+      n += (static_cast<int64_t>(many[b]) << 32) + 1;
+    }
+  }
+  __syncthreads();
+  // parts: a group's keys in as many as its share of its kernel's workgroups
+  constexpr int F = kPlanRows / 2 / kPlanThreads;  // consecutive groups a thread
+  auto big = [&](const KvGroup& x) { return x.M >= kTileFrom && static_cast<int64_t>(x.M) * x.keys >= kTileWork; };
+  auto tiles_of = [&](const KvGroup& x) { return big(x) ? (x.M + a.tspan - 1) / a.tspan : (x.M + a.span - 1) / a.span; };
+  auto steps_of = [&](const KvGroup& x) { return (x.keys + kStepKeys - 1) / kStepKeys; };
+  int64_t cost[2] = {0, 0}, all[2] = {0, 0};
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int i = F * tid + f;
+    if (i < groups) cost[big(group[i])] += static_cast<int64_t>(tiles_of(group[i])) * steps_of(group[i]);
+  }
+  plan_scan(cost[0], red, all[0]);
+  if (a.tile > 0) plan_scan(cost[1], red, all[1]);  // uniform
+  // The direct kernel's workgroups: one a CU, two where each then still has kPartSteps steps. 64 rows over 8192 keys, a call: 41.8
+  // us with 512, 37.0 with 256; 16 rows over 32768 37, 30; 6 groups of 16 rows over 9000 to 15000 84, 94.
+  const int64_t wd = max(static_cast<int64_t>(a.wd / 2), min(static_cast<int64_t>(a.wd), all[0] / kPartSteps));
+  int64_t items = 0, partials = 0, total;  // items of the prompt kernel in the high word
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int i = F * tid + f;
+    if (i < groups) {
+      KvGroup& x = group[i];
+      const int steps = steps_of(x);
+      // a part has a step for each of the direct kernel's waves, or two tiles of the prompt kernel's
+      const int64_t share = (big(x) ? a.wt : wd) * steps / all[big(x)];
+      x.parts = static_cast<int>(max(static_cast<int64_t>(1), min(share, static_cast<int64_t>(big(x) ? (steps + 1) / 2 : (steps + 3) / 4))));
+      items += static_cast<int64_t>(tiles_of(x) * x.parts) << (big(x) ? 32 : 0);
+      partials += static_cast<int64_t>(x.M) * x.parts;
+    }
+  }
+  int64_t first = plan_scan(items, red, total), every;
+  partials = plan_scan(partials, red, every);
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int i = F * tid + f;
+    if (i < groups) {
+      KvGroup& x = group[i];
+      x.at = partials;
+      x.item = static_cast<int>(big(x) ? first >> 32 : first);
+      partials += static_cast<int64_t>(x.M) * x.parts;
+      first += static_cast<int64_t>(tiles_of(x) * x.parts) << (big(x) ? 32 : 0);
     }
   }
   __syncthreads();
   for (int b = tid; b < a.B; b += kPlanThreads) {
-    const int l = lead[b], to = l >= 0 ? id[l] : -1;
-    int before = 0;
+    const int l = lead[b], to = l >= 0 ? id[l] : -1, member = a.p.member[b];
+    KvRow row{0, 0, 0, 0, 0, 0};
     if (to >= 0) {
-      for (int c = l; c < b; ++c) before += lead[c] == l;
-      a.p.order[group[to].first + before] = b;
+      const KvGroup& x = group[to];
+      a.p.order[x.first + member] = b;
+      row = KvRow{x.keys, x.parts, x.M, member, x.at, 0};
     }
-    a.p.group[b] = to;
-    a.p.member[b] = before;
-    a.p.shared[b] = to >= 0 ? group[to].keys : 0;
+    a.p.rows[b] = row;
   }
-  // parts: a group's keys in as many as its share of its kernel's workgroups
-  constexpr int F = kPlanRows / 2 / kPlanThreads;  // consecutive groups a thread
-  int64_t cost[2] = {0, 0}, sum[2];
-  auto tiles_of = [&](const KvGroup& x, bool big) { return (x.M + (big ? a.tspan : a.span) - 1) / (big ? a.tspan : a.span); };
-  auto steps_of = [&](const KvGroup& x) { return (x.keys + kStepKeys - 1) / kStepKeys; };
-#pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int i = F * tid + f;
-    if (i < groups) {
-      const bool big = group[i].M >= kTileFrom;
-      cost[big] += static_cast<int64_t>(tiles_of(group[i], big)) * steps_of(group[i]);
-    }
-  }
-  plan_scan(cost[0], redl, sum[0]);
-  plan_scan(cost[1], redl, sum[1]);
-  int items[2] = {0, 0}, total[2], first[2];
-  int64_t partials = 0, every;
-#pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int i = F * tid + f;
-    if (i < groups) {
-      KvGroup& x = group[i];
-      const bool big = x.M >= kTileFrom;
-      const int steps = steps_of(x);
-      // a part has a step for each of the direct kernel's waves, or two tiles of the prompt kernel's
-      const int64_t share = static_cast<int64_t>(big ? a.wt : a.wd) * steps / sum[big];
-      x.parts = static_cast<int>(max(static_cast<int64_t>(1), min(share, static_cast<int64_t>(big ? (steps + 1) / 2 : (steps + 3) / 4))));
-      items[big] += tiles_of(x, big) * x.parts;
-      partials += static_cast<int64_t>(x.M) * x.parts;
-    }
-  }
-  first[0] = plan_scan(items[0], redi, total[0]);
-  first[1] = plan_scan(items[1], redi, total[1]);
-  partials = plan_scan(partials, redl, every);
-#pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int i = F * tid + f;
-    if (i < groups) {
-      KvGroup& x = group[i];
-      const bool big = x.M >= kTileFrom;
-      x.at = partials;
-      x.pad = first[big];
-      partials += static_cast<int64_t>(x.M) * x.parts;
-      first[big] += tiles_of(x, big) * x.parts;
-    }
-  }
-  __syncthreads();
   for (int i = tid >> 6; i < groups; i += kPlanThreads / 64) {
     const KvGroup x = group[i];
-    const bool big = x.M >= kTileFrom;
-    const int tiles = tiles_of(x, big);
-    KvItem* const to = (big ? a.p.tile : a.p.direct) + x.pad;
-    for (int j = tid & 63; j < tiles * x.parts; j += 64) to[j] = KvItem{i, j % tiles, j / tiles, 0};
-    if ((tid & 63) == 0) a.p.groups[i] = x;
+    const int tiles = tiles_of(x);
+    KvItem* const to = (big(x) ? a.p.tile : a.p.direct) + x.item;
+    for (int j = tid & 63; j < tiles * x.parts; j += 64) to[j] = KvItem{x.lead, x.first, x.M, x.keys, j % tiles, j / tiles, x.parts, 0, x.at, 0};
   }
-  if (tid == 0) *a.p.head = KvPlanHead{total[0], total[1], groups, {0, 0, 0, 0, 0}};
+  const KvItem none{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  for (int i = static_cast<int>(total & 0xffffffff) + tid; i < a.direct; i += kPlanThreads) a.p.direct[i] = none;
+  for (int i = static_cast<int>(total >> 32) + tid; i < a.tile; i += kPlanThreads) a.p.tile[i] = none;
 }
 
 struct KvSharedArgs {
@@ -268,10 +282,7 @@ struct KvSharedArgs {
 };
 
 // Shared keys of row b: none where its start has fallen behind them since the plan was made.
-__device__ inline int shared_keys(const KvSharedArgs& x, int b) {
-  const int n = x.p.shared[b];
-  return n > 0 && x.a.starts[b] >= n ? n : 0;
-}
+__device__ inline int shared_keys(int shared, int start) { return shared > 0 && start >= shared ? shared : 0; }
 
 template <int D, int DT>
 __device__ inline void put_part(float* po, float* pml, int64_t at, int jd, float M, float sum, const float (&acc)[DT]) {
@@ -284,26 +295,26 @@ __device__ inline void put_part(float* po, float* pml, int64_t at, int jd, float
     *reinterpret_cast<f32x4_t*>(po + at * D + jd + d) = f32x4_t{acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
 }
 
-// The query rows of a group over a part of its shared keys. Every row attends all of them.
+// The query rows of a group over a part of its shared keys. Every row attends all of them, and they are whole steps: so the loops
+// have no masks, which for E4M3 hold 40 registers.
 struct KvGroupRows {
+  static constexpr bool kWhole = true;
   const KvSharedArgs& x;
-  KvGroup g;
+  KvItem g;
   const int* trow;
-  int h, part, row0, TG;
+  int h, row0, TG;
   int base, L, s0, s1, first;
-  __device__ KvGroupRows(const KvSharedArgs& args, const KvItem& item, int span, int keys) : x(args) {
-    g = x.p.groups[item.group];
+  __device__ KvGroupRows(const KvSharedArgs& args, const KvItem& item, int span, int keys) : x(args), g(item) {
     h = blockIdx.x;
-    part = item.part;
     row0 = item.tile * span;
     TG = x.a.T * x.a.G;
     base = 0;
     L = g.keys;
     first = L - 1;
     const int steps = (L + keys - 1) / keys;
-    s0 = static_cast<int>(static_cast<int64_t>(steps) * part / g.parts);
-    s1 = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / g.parts);
-    trow = x.a.table + static_cast<int64_t>(x.p.order[g.first]) * x.a.width;
+    s0 = static_cast<int>(static_cast<int64_t>(steps) * g.part / g.parts);
+    s1 = static_cast<int>(static_cast<int64_t>(steps) * (g.part + 1) / g.parts);
+    trow = x.a.table + static_cast<int64_t>(g.lead) * x.a.width;
   }
   __device__ bool row(int i, int& pos, const uint16_t*& src) const {
     const int row = row0 + i;
@@ -325,7 +336,7 @@ struct KvGroupRows {
   }
   template <int D, bool BF16, int DT>
   __device__ void put(int i, int jd, float M, float sum, const float (&acc)[DT]) const {
-    put_part<D>(x.so, x.sml, h * x.partials + g.at + static_cast<int64_t>(part) * g.M + row0 + i, jd, M, sum, acc);
+    put_part<D>(x.so, x.sml, h * x.partials + g.at + static_cast<int64_t>(g.part) * g.M + row0 + i, jd, M, sum, acc);
   }
 };
 
@@ -334,6 +345,7 @@ __device__ inline int own_parts(int steps, int nsplit) { return min(nsplit, max(
 
 // A row's queries over the keys behind the shared ones.
 struct KvTailRows {
+  static constexpr bool kWhole = false;
   const KvSharedArgs& x;
   KvSpan sp;
   const int* trow;
@@ -350,7 +362,7 @@ struct KvTailRows {
     part = rest / x.own_tiles;
     row0 = (rest - part * x.own_tiles) * span;
     if (!kv_span(a, b, row0, span, sp)) return false;
-    base = shared_keys(x, b);
+    base = shared_keys(x.p.rows[b].shared, sp.start);
     L = sp.keys;
     first = sp.first;
     const int steps = (max(L - base, 0) + kStepKeys - 1) / kStepKeys, parts = own_parts(steps, a.nsplit);
@@ -375,16 +387,19 @@ struct KvTailRows {
   }
 };
 
-// Workgroups (h, i): the i-th item of the small groups, behind them the rows' own keys.
+// Workgroups (h, i): the items of the small groups and the rows' own keys.
 template <int D, int R, bool E4M3, bool BF16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_shared_direct_kernel(const KvSharedArgs x) {
   __shared__ float sm[kAttnWaves][16], sl[kAttnWaves][16];
   __shared__ __attribute__((aligned(16))) float so[kAttnWaves][16][D + 4];
   constexpr int RG = direct_rows(D) / 16;
+  // The shared part first: with one such workgroup a CU, rows of their own fill the other places. (In turn, one and one, the shared
+  // part's would lie on every other CU: 43.7 us where this order takes 34.6.)
   const int i = blockIdx.y;
   if (i < x.direct) {
-    if (i >= x.p.head->direct_items) return;
-    const KvGroupRows rows(x, x.p.direct[i], 16 * RG, kStepKeys);
+    const KvItem item = x.p.direct[i];
+    if (item.lead < 0) return;
+    const KvGroupRows rows(x, item, 16 * RG, kStepKeys);
     kv_attn_body<D, RG, E4M3, BF16>(x.a, rows, sm, sl, so);
   } else {
     KvTailRows rows(x);
@@ -395,8 +410,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_shared_direct_kernel
 template <int D, bool E4M3, bool BF16, bool BIG>
 __global__ __launch_bounds__(64 * tile_waves(D), D == 256 ? 1 : 2) void kv_shared_tile_kernel(const KvSharedArgs x) {
   const int i = blockIdx.y;
-  if (i >= x.p.head->tile_items) return;
-  const KvGroupRows rows(x, x.p.tile[i], tile_rows(D), 64 * tile_steps(D));
+  const KvItem item = x.p.tile[i];
+  if (item.lead < 0) return;
+  const KvGroupRows rows(x, item, tile_rows(D), 64 * tile_steps(D));
   kv_attn_tile_body<D, E4M3, BF16, BIG>(x.a, rows);
 }
 
@@ -413,19 +429,19 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(const KvSharedArgs 
   const int row = static_cast<int>(id % rows);
   const int64_t bh = id / rows;
   const int b = static_cast<int>(bh / a.Hkv), h = static_cast<int>(bh % a.Hkv);
+  const KvRow info = x.p.rows[b];
   KvSpan sp;
   const bool live = kv_span(a, b, row / span * span, span, sp) && row / a.G < sp.count;
   int own = 0, mine = 0;
   const float *so = x.so, *sml = x.sml;
   int64_t shared_at = 0, M = 0;
   if (live) {
-    const int base = shared_keys(x, b);
+    const int base = shared_keys(info.shared, sp.start);
     own = mine = own_parts((max(sp.keys - base, 0) + kStepKeys - 1) / kStepKeys, a.nsplit);
     if (base > 0) {
-      const KvGroup g = x.p.groups[x.p.group[b]];
-      M = g.M;
-      shared_at = h * x.partials + g.at + x.p.member[b] * rows + row;
-      mine += g.parts;
+      M = info.M;
+      shared_at = h * x.partials + info.at + info.member * rows + row;
+      mine += info.parts;
     }
   }
   auto part = [&](int s, const float*& po, const float*& pml) {
@@ -496,7 +512,7 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(const KvSharedArgs 
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += w[e];
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: zeros
   uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D + 4 * c;
   const float o0 = acc[0] * inv, o1 = acc[1] * inv, o2 = acc[2] * inv, o3 = acc[3] * inv;
   *reinterpret_cast<u32x2v_t*>(dst) = BF16 ? u32x2v_t{ActBF16::pack_rne(o0, o1), ActBF16::pack_rne(o2, o3)}
@@ -537,8 +553,9 @@ extern "C" int sqx_kvshared_plan(const int* table, const int* starts, const int*
   PlanArgs a{};
   a.p = kv_plan_at(plan, z);
   a.B = static_cast<int>(B); a.TG = static_cast<int>(z.TG); a.shift = kv_shift(block); a.block = static_cast<int>(block);
+  a.unit = kStepKeys * tile_steps(static_cast<int>(hd));
   a.span = direct_rows(static_cast<int>(hd)); a.tspan = tile_rows(static_cast<int>(hd));
-  a.wd = static_cast<int>(z.wd); a.wt = static_cast<int>(z.wt);
+  a.wd = static_cast<int>(z.wd); a.wt = static_cast<int>(z.wt); a.direct = static_cast<int>(z.direct); a.tile = static_cast<int>(z.tile);
   hipLaunchKernelGGL(shared_match_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, as_stream(stream), table, starts, leaders, a.B,
                      static_cast<int>(width), a.shift, a.p);
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, as_stream(stream), a);
@@ -610,7 +627,7 @@ extern "C" int sqx_kvshared_attention(const void* q, int dtype, int64_t q_sb, in
     constexpr int D = decltype(dd)::value;
     auto go = [&](auto e4, auto bf) {
       constexpr bool E = decltype(e4)::value, BF = decltype(bf)::value;
-      if (z.tile > 0) {
+      if (z.tile > 0 && B * rows * width * block >= kTileWork) {  // else no group is that large
         const dim3 grid(heads, static_cast<unsigned>(z.tile));
         if (block >= kStepKeys) hipLaunchKernelGGL((kv_shared_tile_kernel<D, E, BF, true>), grid, dim3(64 * tile_waves(D)), 0, s, x);
         else hipLaunchKernelGGL((kv_shared_tile_kernel<D, E, BF, false>), grid, dim3(64 * tile_waves(D)), 0, s, x);
@@ -618,10 +635,14 @@ extern "C" int sqx_kvshared_attention(const void* q, int dtype, int64_t q_sb, in
       const dim3 grid(heads, static_cast<unsigned>(items));
       if (own.R == 1) hipLaunchKernelGGL((kv_shared_direct_kernel<D, 1, E, BF>), grid, dim3(256), 0, s, x);
       else if constexpr (D < 256) hipLaunchKernelGGL((kv_shared_direct_kernel<D, 2, E, BF>), grid, dim3(256), 0, s, x);
-      constexpr int PG = D == 256 ? 4 : 8;
       const int64_t total = B * Hkv * rows;
-      hipLaunchKernelGGL((kv_shared_join_kernel<D, BF, PG>), dim3(static_cast<unsigned>(ceil_div(total, 1024 / (PG * D)))), dim3(256), 0, s, x,
-                         16 * own.R, total);
+      auto join = [&](auto pg) {
+        constexpr int PG = decltype(pg)::value;
+        hipLaunchKernelGGL((kv_shared_join_kernel<D, BF, PG>), dim3(static_cast<unsigned>(ceil_div(total, 1024 / (PG * D)))), dim3(256), 0, s, x,
+                           16 * own.R, total);
+      };
+      if (total <= 1024) join(std::integral_constant<int, D == 256 ? 4 : 8>{});
+      else join(std::integral_constant<int, 2>{});
     };
     auto with_type = [&](auto e4) {
       if (dtype == SQX_DTYPE_BF16) go(e4, std::true_type{});
