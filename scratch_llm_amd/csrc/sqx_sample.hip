@@ -526,7 +526,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
   }
   const float lowest = fminf(from[0], fminf(from[1], from[2])), highest = fmaxf(below[0], fmaxf(below[1], below[2]));
-  const bool limited = use_k || use_p || use_m;
+  const bool limited = use_k || use_p || use_m, several = use_k + use_p + use_m > 1;
 
   if (limited) {
     // ---- every token of the row, 8 a thread a pass, kAhead passes loaded together
@@ -542,14 +542,17 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         for (int e = 0; e < 8; ++e) hits &= Loads8<DT>::has(at8, a.V, e) ? ~0u : ~(1u << e);
       }
       if (__ballot(hits != 0) == 0) return;
-      unsigned in = 0;
+      unsigned in = hits;
+      if (several) {
+        in = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float l = v[e];
-        const bool i0 = (l >= from[0]) & (l < below[0]), i1 = (l >= from[1]) & (l < below[1]), i2 = (l >= from[2]) & (l < below[2]);
-        in |= static_cast<unsigned>(i0 | i1 | i2) << e;
+        for (int e = 0; e < 8; ++e) {
+          const float l = v[e];
+          const bool i0 = (l >= from[0]) & (l < below[0]), i1 = (l >= from[1]) & (l < below[1]), i2 = (l >= from[2]) & (l < below[2]);
+          in |= static_cast<unsigned>(i0 | i1 | i2) << e;
+        }
+        in &= hits;
       }
-      in &= hits;
       if (in == 0) return;
       int zero;  // to the compiler any number: it would add a wave's lanes up one by one before a single atomic
       asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
@@ -826,12 +829,17 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   float x[8];
   const int at8 = chosen * kSampleSlice + 8 * tid, i0 = Loads8<DT>::first(at8, a.V);
   Loads8<DT>::load(a.logits, row0, at8, a.V, x);
+  // bins as floats: tokens from `any` on have one, those from `all_from` on one before the cut's
+  const float any = r.least(kBins - 1);
+  const float all_from = walked ? (cut >> 32 == 0 ? any : INFINITY) : r.least(min(cut_bin, kBins) - 1);  // a cut behind all is none
+  const float cut_l = place_logit(cut);  // of no cut a NaN
+  const uint32_t cut_i = 0xffffffffu - static_cast<uint32_t>(cut);
+  const bool has_cut = walked || cut_bin < kBins;
   double d[8], sum = 0.0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int bin = r.bin(static_cast<double>(x[j]));
-    const bool above = place(x[j], i0 + j) >= cut;
-    const bool in = Loads8<DT>::has(at8, a.V, j) && bin < kBins && (walked ? above : bin < cut_bin || (bin == cut_bin && above));
+    const bool above = has_cut & ((x[j] > cut_l) | ((x[j] == cut_l) & (static_cast<uint32_t>(i0 + j) <= cut_i)));
+    const bool in = Loads8<DT>::has(at8, a.V, j) & (x[j] >= any) & ((x[j] >= all_from) | above);
     d[j] = in ? r.weight(x[j]) : 0.0;
     sum += d[j];
   }

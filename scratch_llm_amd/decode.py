@@ -213,7 +213,8 @@ class DecodeState:
     def write_kv(self, layer: int, k: Tensor, v: Tensor, start: int = 0) -> None:
         """Store a block ``[B, Hkv, T, hd]`` of keys and values at positions ``start..start+T`` of every slot
         (a prefill's output, keys rotated): copied for a bf16 cache, quantized with the layer's scales for an fp8 one,
-        block by block for a block-scaled one (whose blocks before ``start`` have to be written first)."""
+        block by block for a block-scaled one (whose blocks before ``start`` have to be written first, and on a pool to have
+        pages: :meth:`reserve`)."""
         t = k.shape[2]
         if k.shape != v.shape or k.shape[0] != self.batch or start < 0 or start + t > self.max_ctx:
             raise ValueError(f"block {tuple(k.shape)} does not fit the cache at {start}")
@@ -295,17 +296,18 @@ class DecodeState:
         if leaders is None:
             self.leaders = self.shared = None
             return
-        old = self.shared if self.shared is not None and self.shared.width == self.block_table.shape[1] else None
-        plan = self._plan(leaders, old)
-        self.leaders, self.shared = leaders, plan
+        same = self.shared is not None and self.shared.width == self.block_table.shape[1]
+        self.shared = self._plan(leaders, self.shared if same else None)
+        self.leaders = leaders
 
     def _plan(self, leaders: Tensor, out: "kv_shared.SharedKV | None") -> "kv_shared.SharedKV":
         return kv_shared.plan_shared_kv(self.block_table, self.lengths, leaders, block=self.k.shape[3], tokens=1, heads=self.n_heads,
                                         kv_heads=self.k.shape[2], head_dim=self.k.shape[4], out=out)
 
     def _replan(self) -> None:
-        if self.shared is not None:
-            self._plan(self.leaders, self.shared)
+        if self.shared is not None:  # written over for a captured step, as long as the table is as wide
+            same = self.shared.width == self.block_table.shape[1]
+            self.shared = self._plan(self.leaders, self.shared if same else None)
 
     def set_sampling(self, sampling: "Sampling | None") -> None:
         """Let steps draw their tokens (:func:`~scratch_llm_amd.sampling.sample_tokens`) with the random numbers in ``u`` (float32 ``[B]``,

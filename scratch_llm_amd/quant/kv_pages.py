@@ -98,7 +98,8 @@ def fork_kv_rows(parents: Tensor, k_codes: Tensor, v_codes: Tensor, k_scale: Ten
     A row that is its own parent stays as it is; a parent outside ``0 .. B - 1`` empties the row. Any other row takes
     its parent's length and shares its full pages; the page that the next token goes to, if the parent has begun it, is
     copied to a free page. (If the parent does not go on from itself, the first row that goes on from it takes that page over
-    instead.) What a row held before is released first, and may be handed out by the same call. Returns int32 ``[1]``: 1, or 0 if
+    instead.) What a row held before is released first, and may be handed out by the same call. A page that further rows
+    held before, after a cut for instance, stays theirs too: :func:`reserve_kv_pages` parts them. Returns int32 ``[1]``: 1, or 0 if
     there are too few free pages; nothing is changed then."""
     fn = "fork_kv_rows"
     layers, hkv, d, block, pages = _check_pool(k_codes, v_codes, k_scale, v_scale, fn)
