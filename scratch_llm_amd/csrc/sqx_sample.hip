@@ -365,6 +365,7 @@ __device__ inline void sort_places(lds_u64_t list, int n) {
 __device__ inline void sort_list(lds_u64_t list, int n) {
   __syncthreads();
   if (n <= kPickThreads) sort_places<1>(list, n);
+  else if (n <= 2 * kPickThreads) sort_places<2>(list, n);
   else sort_places<kCap / kPickThreads>(list, n);
 }
 
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         digit_rank = rank;
         digit_left = left * unit;
       }
-      for (int sh = 56; sh >= 0; sh -= 8) {
+      for (int sh = 56; sh >= 0; sh -= sh == 32 ? 16 : 8) {  // ids have 20 bits: the highest of the low word's bytes is 255
         if (tid < 256) {
           digit_w[tid] = 0;
           digit_c[tid] = 0;
@@ -730,19 +731,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
           if (sh < 56 && (q ^ so_far) >> (sh + 8) != 0) return;
           const int d = static_cast<int>(q >> sh) & 255;
           const unsigned long long f = by_rank ? 0ull : fix(l);
-          const unsigned long long same = __ballot(d == __builtin_amdgcn_readfirstlane(d));
-          if (same == __ballot(true)) {  // equal digits: one addition for the wave's tokens, not one after the other
-            unsigned long long sum = 0;
-            if (!by_rank)
-              for (unsigned long long lanes = same; lanes != 0; lanes &= lanes - 1) {
-                const int lane = __ffsll(lanes) - 1;
-                const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(f), lane);
-                const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(f >> 32), lane);
-                sum += (static_cast<unsigned long long>(hi) << 32) | lo;
-              }
-            if ((threadIdx.x & 63) == __ffsll(same) - 1) {
-              atomicAdd(&digit_c[d], static_cast<unsigned>(__popcll(same)));
-              if (!by_rank) atomicAdd(&digit_w[d], sum);
+          // equal logits: one addition for the wave's tokens, not one after the other
+          const unsigned long long here = __ballot(true), f0 = (static_cast<unsigned long long>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(f >> 32))) << 32) |
+                                                               __builtin_amdgcn_readfirstlane(static_cast<unsigned>(f));
+          if (__ballot(d == __builtin_amdgcn_readfirstlane(d) && f == f0) == here) {
+            if ((threadIdx.x & 63) == __ffsll(here) - 1) {
+              atomicAdd(&digit_c[d], static_cast<unsigned>(__popcll(here)));
+              if (!by_rank) atomicAdd(&digit_w[d], f * __popcll(here));
             }
           } else {
             atomicAdd(&digit_c[d], 1u);
@@ -764,6 +759,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             w_run += static_cast<double>(digit_w[d]);
           }
           digit_place |= static_cast<unsigned long long>(max(chosen, 0)) << sh;
+          if (sh == 32) digit_place |= 0xff000000ull;
           digit_rank = rank_at;
           digit_left = left_at;
         }
