@@ -89,11 +89,12 @@ inline KvSharedPlan kv_plan_at(void* p, const KvPlanSizes& s) {
 }
 
 // Workgroup b: the first row with row b's leader, how many such rows stand before b, and how many whole blocks before row b's
-// start name the same pages in both.
+// start name the same pages in both. Rows that are too short to share anything (emptied ones) belong to no group: they would leave
+// the others nothing.
 __global__ __launch_bounds__(256) void shared_match_kernel(const int* table, const int* starts, const int* leaders, int B, int width,
-                                                           int shift, KvSharedPlan p) {
+                                                           int shift, int unit, KvSharedPlan p) {
   __shared__ int first, differ, rank;
-  const int b = blockIdx.x, lead = leaders[b];
+  const int b = blockIdx.x, lead = starts[b] >= unit ? leaders[b] : -1;
   if (threadIdx.x == 0) {
     first = b;
     differ = 0x7fffffff;
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(256) void shared_match_kernel(const int* table, con
   if (lead >= 0) {
     int mine = 0, least = 0x7fffffff;
     for (int c = threadIdx.x; c < b; c += 256)
-      if (leaders[c] == lead) {
+      if (leaders[c] == lead && starts[c] >= unit) {
         least = min(least, c);
         ++mine;
       }
@@ -557,7 +558,7 @@ extern "C" int sqx_kvshared_plan(const int* table, const int* starts, const int*
   a.span = direct_rows(static_cast<int>(hd)); a.tspan = tile_rows(static_cast<int>(hd));
   a.wd = static_cast<int>(z.wd); a.wt = static_cast<int>(z.wt); a.direct = static_cast<int>(z.direct); a.tile = static_cast<int>(z.tile);
   hipLaunchKernelGGL(shared_match_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, as_stream(stream), table, starts, leaders, a.B,
-                     static_cast<int>(width), a.shift, a.p);
+                     static_cast<int>(width), a.shift, a.unit, a.p);
   hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, as_stream(stream), a);
   SQX_LAUNCH_CHECK(fn);
   return SQX_OK;

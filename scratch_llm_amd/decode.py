@@ -323,6 +323,7 @@ class DecodeState:
         if t.shape != (self.batch,) or bool((t < 0).any()) or bool((t > self.max_ctx).any()):
             raise ValueError(f"lengths must be {self.batch} values in [0, {self.max_ctx}]")
         self.lengths.copy_(t)
+        self._replan()  # a row that is cut goes on with a page of its own where others read
 
     def set_tokens(self, tokens, vocab_size: int) -> None:
         t = torch.as_tensor(tokens, dtype=torch.int64)

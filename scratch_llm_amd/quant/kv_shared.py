@@ -57,8 +57,8 @@ def plan_shared_kv(block_table: Tensor, starts: Tensor, leaders: Tensor, *, bloc
 
     Rows with the same number of 0 or above in ``leaders`` (int32 ``[B]``, for instance the row that each was forked from) make a
     group; -1 stands alone. A group shares the blocks in front that all of its rows name alike, as far as they lie whole before
-    every row's ``starts[b]`` (int32 ``[B]``), in multiples of 64 tokens (128 with heads of 64); rows with less in common are
-    better put into a group of their own.
+    every row's ``starts[b]`` (int32 ``[B]``), in multiples of 64 tokens (128 with heads of 64). Rows shorter than that stand
+    alone (an emptied row stays with its leader's number); longer ones with less in common are better put into a group of their own.
 
     The plan holds while a group's rows and the table's entries of its shared blocks stay, however far the rows
     grow. (A row whose start falls behind the shared blocks is attended for itself.) ``out``: a plan of the same sizes to write

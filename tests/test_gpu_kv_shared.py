@@ -222,6 +222,29 @@ def test_a_long_prefix(ks):
         assert ((x[0, 0, :2] - want).abs() <= lim).all()
 
 
+@pytest.mark.parametrize("empty", [0, 2, 5])
+def test_an_emptied_row_leaves_the_others_their_shared_part(ks, empty):
+    """The first row, one between and the last. That the others still read together shows in their results: their shared part comes
+    through the entries of the first of them, so those of the rest may name a page of NaN scales after the plan is made."""
+    g = np.random.default_rng(empty)
+    block, d, hkv, h, n, rows = 64, 64, 1, 8, 4, 6
+    leaders = [4] * rows
+    table, pages = batch(g, leaders, {4: n}, 1, block, n + 1)
+    starts = [n * block + 3 + i for i in range(rows)]
+    starts[empty] = 0
+    table[empty] = -1
+    cache = fill_valid(make_cache(None, pages, hkv, d, block, "int8", 1), "int8", 2)
+    q = torch.randn(rows, 1, h, d, generator=torch.Generator().manual_seed(4)).half()
+    want, terms = R.attend(q.double().numpy(), *cache, table, starts, [1] * rows, d**-0.5, "int8")
+    plan = ks.plan_shared_kv(i32(table), i32(starts), i32(leaders), block=block, tokens=1, heads=h, kv_heads=hkv, head_dim=d)
+    spare = next(p for p in range(pages) if p not in table)
+    cache[2][spare] = cache[3][spare] = np.nan
+    others = [i for i in range(rows) if i != empty]
+    table[others[1:], :n] = spare
+    got = ks.attend_shared_kv(q.to(DEV), *to_dev(cache, "int8"), i32(table), i32(starts), shared=plan).double().cpu().numpy()
+    assert (np.abs(got - want) <= bound(want, terms, d, "fp16"))[others].all()
+
+
 def test_streams_graphs_and_repetition(ks):
     g = np.random.default_rng(9)
     block, d, hkv, h, n, rows = 64, 128, 2, 8, 5, 40

@@ -145,6 +145,24 @@ def test_a_cut_into_the_shared_part_is_planned_anew(small):
     assert torch.equal(st.logits, other.logits)
 
 
+def test_lengths_set_back_into_the_shared_part(small):
+    """The row through which the group reads is cut and writes on: to a page of its own, which the others do not see."""
+    model, _ = small
+    st, _ = prefilled(model, 3, 70, "int8_block")
+    st.fork(i32([0, 0, 0]))
+    st.share(i32([0, 0, 0]))
+    st.set_lengths([21, 70, 70])
+    alone = own_copies(model, st, [0, 1, 2])
+    for step in range(4):
+        for s in (st, alone):
+            s.tokens.copy_(i32([7, 8, 9]) + step)
+            model.step(s)
+        scale = float(alone.logits.float().abs().max())
+        # as above
+        assert float((st.logits.float() - alone.logits.float()).abs().max()) <= 2.0**-5 * scale
+    assert st.block_table[0, 1] != st.block_table[1, 1] and torch.equal(st.block_table[1, :4], st.block_table[2, :4])
+
+
 @pytest.mark.parametrize("kv_dtype", ["int8_block", "fp8_block"])
 def test_a_pool_that_is_too_small_changes_nothing(small, kv_dtype):
     model, _ = small
@@ -196,14 +214,15 @@ def test_drafts_on_a_pool_equal_drafts_on_own_pages(small, kv_dtype):
         assert torch.equal(st.logits, plain.logits)
 
 
-def test_captured_steps_take_pages_share_and_sample(small):
+@pytest.mark.parametrize("n", [50, 110])
+def test_captured_steps_take_pages_share_and_sample(small, n):
     """One captured step, replayed while rows are forked, cut and freed eagerly between the replays, equal to eager steps."""
     from scratch_llm_amd.sampling import Sampling
 
     model, _ = small
     states = []
     for _ in range(2):
-        st, _ = prefilled(model, 4, 50, "int8_block", pages=40)
+        st, _ = prefilled(model, 4, n, "int8_block", pages=40)
         st.fork(i32([0, 0, 0, -1]))
         st.active.copy_(torch.tensor([1, 1, 1, 0], dtype=torch.uint8))
         st.share(i32([0, 0, 0, 0]))
@@ -211,7 +230,7 @@ def test_captured_steps_take_pages_share_and_sample(small):
         states.append(st)
     a, b = states
     model.step(a)  # loads all code
-    a, _ = prefilled(model, 4, 50, "int8_block", pages=40)
+    a, _ = prefilled(model, 4, n, "int8_block", pages=40)
     a.fork(i32([0, 0, 0, -1]))
     a.active.copy_(torch.tensor([1, 1, 1, 0], dtype=torch.uint8))
     a.share(i32([0, 0, 0, 0]))
