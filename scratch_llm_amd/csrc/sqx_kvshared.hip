@@ -67,6 +67,10 @@ inline KvPlanSizes kv_plan_sizes(int64_t B, int64_t T, int64_t H, int64_t Hkv, i
   KvPlanSizes s{};
   s.B = B;
   s.TG = T * (H / Hkv);
+  if (s.TG > own_most(hd)) {  // the plain kernels: nothing to plan
+    s.bytes = 16;
+    return s;
+  }
   const int64_t span = direct_rows(static_cast<int>(hd)), tspan = tile_rows(static_cast<int>(hd));
   s.wd = std::max<int64_t>(1, kDirectGroups / Hkv);
   s.wt = std::max<int64_t>(1, kTileGroups / Hkv);
@@ -558,6 +562,7 @@ extern "C" int sqx_kvshared_plan(const int* table, const int* starts, const int*
   const KvPlanSizes z = kv_plan_sizes(B, T, H, Hkv, hd);
   SQX_REQUIRE(plan != nullptr && plan_bytes >= z.bytes && al16(plan), SQX_E_SPACE, "%s: %lld bytes of 16-byte aligned plan needed, %lld given",
               fn, (long long)z.bytes, (long long)plan_bytes);
+  if (z.TG > own_most(hd)) return SQX_OK;
   PlanArgs a{};
   a.p = kv_plan_at(plan, z);
   a.B = static_cast<int>(B); a.TG = static_cast<int>(z.TG); a.shift = kv_shift(block); a.block = static_cast<int>(block);

@@ -315,6 +315,8 @@ class DecodeState:
         does not advance."""
         if sampling is not None:
             sampling.check(self.batch, "DecodeState.set_sampling")
+            if any(x is not None for x in sampling.tensors()):
+                _lib.require_device(self.lengths, *sampling.tensors(), fn="DecodeState.set_sampling")
         self.sampling = sampling
 
     def set_lengths(self, lengths) -> None:
@@ -600,7 +602,7 @@ class Int4DecodeLM:
                                  f"{st.block_table.shape[1]}: call share again")
         if st.sampling is not None and (tuple(st.u.shape) != (st.batch,) or st.u.dtype != torch.float32):
             raise ValueError(f"Int4DecodeLM.step: u must be float32 [{st.batch}], got {tuple(st.u.shape)} of {st.u.dtype}")
-        _lib.require_device(st.tokens, self.embed, fn="Int4DecodeLM.step")
+        _lib.require_device(st.tokens, self.embed, None if st.sampling is None else st.u, fn="Int4DecodeLM.step")
         B, d, H, Hkv, hd, T = st.batch, cfg.d_model, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, st.max_ctx
         s = _lib.stream_ptr(self.device)
         ck = _lib.check

@@ -88,4 +88,7 @@ def test_entry_points_refuse():
     assert plan(table=n) == -1 and plan(ptr=n) == -3 and plan(bytes_=nb - 1) == -3 and plan(ptr=ctypes.c_void_p(264)) == -3
     assert attend(dtype=0) == -1 and attend(scale=0.0) == -1 and attend(pages=0) == -1 and attend(q=ctypes.c_void_p(8)) == -1
     assert attend(plan_ptr=n) == -3 and attend(plan_bytes=nb - 1) == -3 and attend(ws=n) == -3 and attend(ws_bytes=wb - 1) == -3
+    # rows that take the plain kernels have no workgroups to list, however many
+    assert lib.sqx_kvshared_plan_bytes(2, (1 << 20) - 1, 8192, 1, 128) == lib.sqx_kvshared_plan_bytes(4096, 33, 4, 1, 128) == 16
+    assert plan(T=(1 << 20) - 1, H=8192, Hkv=1, bytes_=16) == 0 and plan(T=(1 << 20) - 1, H=8192, Hkv=1, bytes_=15) == -3
     assert lib.sqx_kvshared_plan_bytes(0, 1, 4, 2, 64) == 0 and lib.sqx_kvshared_plan_bytes(2, 1, 5, 2, 64) == 0

@@ -53,6 +53,9 @@ def test_sampling_is_checked_when_it_is_set():
         with pytest.raises(ValueError, match=what):
             st.set_sampling(bad)
         assert st.sampling is None
+    with pytest.raises(RuntimeError, match="device tensors"):
+        st.set_sampling(Sampling(temperature=torch.ones(2)))
+    assert st.sampling is None
     st.set_sampling(Sampling(top_k=3))
     st.u = torch.zeros(3)
     with pytest.raises(ValueError, match="u must"):
