@@ -6,9 +6,9 @@
 // calls give equal tables. A call that hands out pages does all of it or, where the pool is too small, nothing.
 //
 // Two kinds of launches: small ones over tables and counts, bound by the latency of a launch and of two or three dependent
-// loads each, and one that copies the pages, bound by HBM. us of the kernels: fork of 8 rows (7 pages of 4 layers copied) 1.9, 3.3,
-// 4.2 and 5.6; of 64 rows of beams (260 MB read and written) 55 for the last, 4.7 TB/s; release and reservation for 96 rows 3.2,
-// 3.5, 4.4 and 4.0, 8.9 with 46 MB copied; a pool of 1100 pages of 32 layers, 128 KiB each, compacted (2.1 GB) 434, 4.9 TB/s, with 5
+// loads each, and one that copies the pages, bound by HBM. us of the kernels: fork of 8 rows (7 pages of 4 layers copied) 5.2
+// and 5.6; of 64 rows of beams (260 MB read and written) 7.4 and 55, 4.7 TB/s; release and reservation for 96 rows 3.2 and 8.4, 8.7
+// for the 46 MB copied; a pool of 1100 pages of 32 layers, 128 KiB each, compacted (2.1 GB) 434, 4.9 TB/s, with 5
 // before it for each of the counts, their sums and the plan.
 //
 // Rows are looked at by many workgroups, but pages are dealt out by one: the place of a page in the list of free ones depends on
@@ -21,6 +21,8 @@ constexpr int kPlan = 1024;      // threads of a workgroup that scans the pool a
 constexpr int kScan = 16;        // pages of a thread, a pass over the pool
 constexpr int kCopyUnits = 1024;  // 16-byte units of a workgroup's piece, four a thread in flight
 constexpr int kCopyGroups = 2048;
+// What one workgroup plans: eight entries of the tables a thread in a fork; at most sixteen in a reservation, which looks at few.
+constexpr int kSmallRows = kPlan, kSmallEntries = 8192, kSmallPages = 8192, kSmallReserve = 16384;
 
 struct KvPool {
   uint8_t *kc, *vc;  // [L, pages, unit16 * 16 bytes]
@@ -222,6 +224,78 @@ __global__ __launch_bounds__(kPlan) void fork_assign_kernel(const ForkArgs a) {
   }
 }
 
+// The three kernels above in one workgroup, the counts in LDS: for up to kSmallRows rows, kSmallEntries entries and kSmallPages pages.
+// 8 rows, 392 entries: 5.2 us, and the call 16.6 where the three take 1.9, 3.3 and 4.2, and it 23.0; 64 rows, 1536 entries: 7.4,
+// 66.5 for 4.7, 4.6, 5.2 and 70.0.
+
+__global__ __launch_bounds__(kPlan) void fork_small_kernel(const ForkArgs a) {
+  __shared__ int refs[kSmallPages], free[kSmallRows], red[kPlan / 64];
+  __shared__ int parent[kSmallRows], taker[kSmallRows];  // taker: the first row that goes on from this one
+  __shared__ int4a todo[kSmallRows];                     // parent (-1: the row stays), blocks, the block without a page of the parent's
+  const int b = threadIdx.x;
+  const int p = b < a.B ? a.parents[b] : -1;
+  parent[b] = p;
+  taker[b] = 0x7fffffff;
+  for (int i = b; i < a.pages; i += kPlan) refs[i] = a.refs[i];
+  __syncthreads();
+  const bool other = b < a.B && p != b, none = p < 0 || p >= a.B;
+  if (other && !none) atomicMin(&taker[p], b);
+  __syncthreads();
+  auto page = [&](int64_t at) {
+    const int x = a.table[at];
+    return x >= 0 && x < a.pages ? x : -1;
+  };
+  int need = -1;
+  if (b < a.B) {
+    const int len = !other ? a.lengths[b] : none ? 0 : min(max(a.lengths[p], 0), a.width << a.shift);
+    int4a x{{-1, 0, -1, 0}};
+    if (other) {
+      const int blocks = (len + a.block - 1) >> a.shift;
+      const int open = (len & (a.block - 1)) != 0 && (parent[p] == p || taker[p] != b) ? blocks - 1 : -1;
+      need = open >= 0 ? page(static_cast<int64_t>(p) * a.width + open) : -1;
+      x = int4a{{none ? 0 : p, blocks, open, 0}};
+    }
+    a.lengths2[b] = len;
+    todo[b] = x;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = b; i < a.B * a.width; i += kPlan) {
+    const int r = i / a.width, j = i - r * a.width;
+    const int4a x = todo[r];
+    const int was = a.table[i];
+    int now = was;
+    if (x.v[0] >= 0) {
+      const int had = was >= 0 && was < a.pages ? was : -1;
+      now = j < x.v[1] && j != x.v[2] ? page(x.v[0] * a.width + j) : -1;
+      if (had != now) {
+        if (had >= 0) atomicAdd(&refs[had], -1);
+        if (now >= 0) atomicAdd(&refs[now], 1);
+      }
+    }
+    a.table2[i] = now;
+  }
+  int n;
+  const int at = block_scan<kPlan / 64>(need >= 0, red, n);  // has a barrier: counts and tables are there behind it
+  const bool ok = free_pages(refs, a.pages, n, free, red) == n;
+  __syncthreads();
+  if (ok) {
+    if (need >= 0) {
+      const int to = free[at];
+      a.src[at] = need;
+      a.dst[at] = to;
+      a.table2[b * a.width + todo[b].v[2]] = to;
+      refs[to] = 1;
+    }
+    __syncthreads();
+    for (int i = b; i < a.pages; i += kPlan) a.refs2[i] = refs[i];
+  }
+  if (b == 0) {
+    *a.count = ok ? n : 0;
+    *a.ok = ok ? 1 : 0;
+  }
+}
+
 // Takes the new tables over and copies.
 __global__ __launch_bounds__(256) void fork_end_kernel(const ForkArgs a, const KvPool p) {
   if (*a.ok == 0) return;
@@ -314,6 +388,64 @@ __global__ __launch_bounds__(256) void reserve_rows_kernel(const ReserveArgs a) 
       a.refs[page] = 1;
     }
     next += total;
+  }
+}
+
+// The three kernels above in one workgroup, for up to kSmallRows rows and kSmallReserve entries: the blocks that tokens lie in stand
+// one behind the other, row after row, a thread for each, kPlan at a time. 96 rows, some 600 blocks: 8.4 us where the three take 3.5,
+// 4.4 and 4.0 and two more launches; with the entries dealt out to the threads in equal runs, looked at or not, 13.8.
+__global__ __launch_bounds__(kPlan) void reserve_small_kernel(const ReserveArgs a) {
+  __shared__ int begin[kSmallRows], from[kSmallRows], red[kPlan / 64], copies;  // begin: blocks of the rows before
+  const int tid = threadIdx.x;
+  int lo = 0, hi = 0, blocks;
+  if (tid < a.B) touched(a, tid, lo, hi);
+  if (tid == 0) copies = 0;
+  begin[tid] = block_scan<kPlan / 64>(hi - lo, red, blocks);
+  from[tid] = lo;
+  __syncthreads();
+  auto entry = [&](int t) {
+    int r = 0;  // the last row that begins at t or before it: it holds t, as rows of no blocks begin where the next does
+#pragma unroll
+    for (int step = kSmallRows / 2; step > 0; step >>= 1) r += begin[r + step] <= t ? step : 0;
+    return r * a.width + from[r] + t - begin[r];
+  };
+  int n = 0;
+  uint32_t fresh = 0, copied = 0;  // bit k: of block kPlan k + tid
+  for (int k = 0; k * kPlan < blocks; ++k) {
+    const int t = k * kPlan + tid;
+    int kind = 0;
+    if (t < blocks) {
+      const int page = a.table[entry(t)];
+      kind = page < 0 || page >= a.pages ? 1 : a.refs[page] > 1 ? 2 : 0;
+      fresh |= (kind == 1 ? 1u : 0u) << k;
+      copied |= (kind == 2 ? 1u : 0u) << k;
+    }
+    n += __syncthreads_count(kind != 0);
+  }
+  const bool ok = n <= a.most && free_pages(a.refs, a.pages, n, a.free, red) == n;
+  __syncthreads();  // the free pages are read by other threads than those that wrote them
+  if (ok) {
+    int next = 0;
+    for (int k = 0; k * kPlan < blocks; ++k) {
+      int total;
+      const int rank = next + block_scan<kPlan / 64>((fresh | copied) >> k & 1u, red, total);
+      next += total;
+      if (((fresh | copied) >> k & 1u) == 0) continue;
+      const int i = entry(k * kPlan + tid), page = a.free[rank];
+      if ((copied >> k) & 1u) {
+        const int had = a.table[i], c = atomicAdd(&copies, 1);  // the copies' order does not show
+        atomicAdd(a.refs + had, -1);
+        a.src[c] = had;
+        a.dst[c] = page;
+      }
+      a.table[i] = page;
+      a.refs[page] = 1;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    *a.count = copies;
+    *a.ok = ok ? 1 : 0;
   }
 }
 
@@ -508,9 +640,13 @@ extern "C" int sqx_kvpages_fork(const int* parents, void* k_codes, void* v_codes
   a.B = static_cast<int>(B); a.width = static_cast<int>(width); a.pages = static_cast<int>(pages);
   a.block = static_cast<int>(block); a.shift = kv_shift(block);
   const hipStream_t s = as_stream(stream);
-  hipLaunchKernelGGL(fork_begin_kernel, dim3(blocks_for(pages)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>(ceil_div(width, 256)), static_cast<unsigned>(B)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(fork_assign_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  if (B <= kSmallRows && B * width <= kSmallEntries && pages <= kSmallPages) {
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(fork_begin_kernel, dim3(blocks_for(pages)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>(ceil_div(width, 256)), static_cast<unsigned>(B)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(fork_assign_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  }
   hipLaunchKernelGGL(fork_end_kernel, dim3(std::max(copy_groups(pool, B), blocks_for(std::max(B * width, pages)))), dim3(256), 0, s, a, pool);
   SQX_LAUNCH_CHECK(fn);
   return SQX_OK;
@@ -546,9 +682,13 @@ extern "C" int sqx_kvpages_reserve(void* k_codes, void* v_codes, float* k_scale,
   a.B = static_cast<int>(B); a.width = static_cast<int>(width); a.pages = static_cast<int>(pages);
   a.block = static_cast<int>(block); a.shift = kv_shift(block); a.most = static_cast<int>(most);
   const hipStream_t s = as_stream(stream);
-  hipLaunchKernelGGL(reserve_count_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(reserve_assign_kernel, dim3(1), dim3(kPlan), 0, s, a);
-  hipLaunchKernelGGL(reserve_rows_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, s, a);
+  if (B <= kSmallRows && B * width <= kSmallReserve) {
+    hipLaunchKernelGGL(reserve_small_kernel, dim3(1), dim3(kPlan), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(reserve_count_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(reserve_assign_kernel, dim3(1), dim3(kPlan), 0, s, a);
+    hipLaunchKernelGGL(reserve_rows_kernel, dim3(static_cast<unsigned>(B)), dim3(256), 0, s, a);
+  }
   hipLaunchKernelGGL(kv_copy_kernel, dim3(copy_groups(pool, most)), dim3(256), 0, s, pool, a.src, a.dst, a.count,
                      static_cast<int>(most));
   SQX_LAUNCH_CHECK(fn);

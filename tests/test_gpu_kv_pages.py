@@ -121,6 +121,28 @@ def test_fork(kp, case):
     same([*there, t, n, r], [*pool, table, lengths, refs], "fork")
 
 
+@pytest.mark.parametrize("width,pages", [(4100, 60), (5, 8200), (1, 8192), (300, 8192)])
+@pytest.mark.parametrize("rows", [4, 1024, 1025])
+def test_fork_at_the_ends_of_its_forms(kp, rows, width, pages):
+    """Few rows, entries and pages are planned by one workgroup, more of any by several."""
+    g = np.random.default_rng(rows + width + pages)
+    block = 16
+    print_case("fork", rows, width, pages)
+    lengths = np.zeros(rows, np.int32)
+    some = g.permutation(rows)[:40]
+    lengths[some] = g.integers(0, min(width * block, 40), len(some))
+    pool = new_pool(g, 1, pages, 1, 64, block)
+    table, refs = owned(g, rows, width, pages, lengths if pages > 200 else lengths * (np.arange(rows) < 4), block)
+    lengths = (table >= 0).sum(1).astype(np.int32) * block - g.integers(0, 2, rows).astype(np.int32) * 5
+    np.maximum(lengths, 0, out=lengths)
+    parents = np.where(g.random(rows) < 0.4, np.arange(rows), g.integers(-1, rows + 1, rows)).astype(np.int32)
+    parents[:4] = [some[0], some[0], 0, 2]
+    there, t, n, r = up(pool), dev(table), dev(lengths), dev(refs)
+    ok = kp.fork_kv_rows(dev(parents), *there, t, n, r)
+    assert int(ok) == R.fork(list(parents), pool, table, lengths, refs, block)
+    same([*there, t, n, r], [*pool, table, lengths, refs], "fork")
+
+
 def test_fork_without_room_changes_nothing(kp):
     g = np.random.default_rng(8)
     pool = new_pool(g, 1, 5, 1, 64, 16)
@@ -176,6 +198,33 @@ def test_reserve_copies_shared_pages(kp):
     assert int(ok) == R.reserve(pool, table, starts, counts, refs, block) == 1
     same([*there, t], [*pool, table], "shared")
     np.testing.assert_array_equal(host(r), refs)
+
+
+@pytest.mark.parametrize("width", [16, 17, 4100])
+@pytest.mark.parametrize("rows", [3, 1024, 1025])
+def test_reserve_at_the_ends_of_its_forms(kp, rows, width):
+    """Few rows and entries are planned by one workgroup, more of either by several. Some pages have two holders."""
+    g = np.random.default_rng(rows + width)
+    block, pages = 16, 4500
+    print_case("reserve", rows, width)
+    lengths = np.zeros(rows, np.int32)
+    some = np.unique(np.r_[g.permutation(rows)[:20], 0, rows - 1])
+    lengths[some] = g.integers(0, min(width, 30) * block, len(some))
+    pool = new_pool(g, 1, pages, 1, 64, block)
+    table, refs = owned(g, rows, width, pages, lengths, block)
+    for a, b in zip(some[:-1], some[1:]):  # a cut row writes into pages that another holds too
+        n = int(min(lengths[a], lengths[b])) // block
+        for j in range(n):
+            refs[table[a, j]] -= 1
+            table[a, j] = table[b, j]
+            refs[table[b, j]] += 1
+    starts = (lengths * g.random(rows)).astype(np.int32)
+    counts = np.where(g.random(rows) < 0.7, g.integers(0, 2 * block, rows), 0).astype(np.int32)
+    counts[0] = 3000  # most of a long row, or past the table
+    there, t, r = up(pool), dev(table), dev(refs)
+    ok = kp.reserve_kv_pages(*there, t, dev(starts), dev(counts), r)
+    assert int(ok) == R.reserve(pool, table, starts, counts, refs, block) == 1
+    same([*there, t, dev(starts), r], [*pool, table, starts, refs], "reserve")
 
 
 def test_reserve_without_room_changes_nothing(kp):
