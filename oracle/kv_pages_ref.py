@@ -1,4 +1,4 @@
-"""Pages of the block-scaled KV cache on the host, in numpy, one entry at a time: the checker of scratch_llm_amd/quant/kv_pages.py.
+"""Pages of the block-scaled KV cache on the host, in numpy, one entry at a time: the oracle of scratch_llm_amd/quant/kv_pages.py.
 
 A pool is [k_codes, v_codes, k_scale, v_scale] with the page as the second axis; tables, lengths and refs are int arrays,
 changed in place."""

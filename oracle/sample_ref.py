@@ -1,4 +1,4 @@
-"""Sampling with temperature, top-k, top-p and min-p in float64, row by row: the checker of scratch_llm_amd/sampling.py."""
+"""Sampling with temperature, top-k, top-p and min-p in float64, row by row: the oracle of scratch_llm_amd/sampling.py."""
 
 from __future__ import annotations
 
