@@ -19,7 +19,7 @@
 // A token 32 T or further behind the maximum (the bins' end lies within 1/32 before that) has less than 2^-45 of its weight and is
 // never drawn; u itself has 24 bits.
 //
-// us of the two launches: 1 row of 32000 in fp32 with top-k 6.6 + 15.2, latency: four dependent rounds in each. 64 rows of 128256 in
+// us of the two launches: 1 row of 32000 in fp32 with top-k 6.6 + 11.1, latency: four dependent rounds in each. 64 rows of 128256 in
 // bf16 with top-p 20.3 + 41.0: the first is bound by its atomics in LDS and its exponentials in double, one of each a token; in the
 // second a row's workgroup, of some 28 us alone, spends 3 on its maximum, 3 on joining the histograms, 8 on collecting, 5 on sorting
 // some 100 tokens (15 for 1000) and 6 on the draw; the longest row counts. 201 rows of 50257 in fp32 with all limits 22.5 + 34.4.
@@ -589,6 +589,43 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     __syncthreads();
   }
   const int n = found;
+
+  if (few && n <= 64) {
+    // ---- all that may stay in the first wave's lanes: no further barrier (1 row of 32000, top-k 40: 11.1 us of the kernel, 15.2
+    // with the way below)
+    if (tid >= 64) return;
+    unsigned long long x[1] = {tid < n ? list[tid] : 0ull};
+    sort_wave<64>(x);
+    const double w = tid < n ? r.weight(place_logit(x[0])) : 0.0;
+    double run = w;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(run, o, 64);
+      run += tid >= o ? y : 0.0;
+    }
+    const int first_k = min(want_k, n);
+    const double left = p * __shfl(run, first_k - 1, 64);
+    const double ahead_of = __shfl_up(run, 1, 64);
+    const unsigned long long ends = __ballot(tid > 0 && tid < first_k && ((by_p && !(ahead_of < left)) || w < minp));
+    const int stay = min(first_k, ends != 0 ? __ffsll(ends) - 1 : 64);
+    // the kept weight of ids up to a lane's, in one order for all lanes
+    const uint32_t id = 0xffffffffu - static_cast<uint32_t>(x[0]);
+    double upto = 0.0, kept = 0.0;
+    for (int i = 0; i < stay; ++i) {
+      const double wi = __shfl(w, i, 64);
+      upto += static_cast<uint32_t>(__shfl(static_cast<int>(id), i, 64)) <= id ? wi : 0.0;
+      kept += wi;
+    }
+    const bool in = tid < stay;
+    uint32_t least = in && upto > u * kept ? id : 0xffffffffu, most = in ? id : 0u;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), o, 64)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64)));
+    }
+    if (tid == 0) a.out[b] = static_cast<int>(least != 0xffffffffu ? least : most);
+    return;
+  }
 
   unsigned long long cut = 0;  // kept of bin cut_bin: places from here on
   int cut_bin = kBins;         // bins before it are kept whole

@@ -98,6 +98,36 @@ def test_ties(draw, v, levels, dtype):
         check(draw, t, x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("v,levels", [(9, 0), (64, 0), (65, 0), (30000, 0), (65, 1), (300, 5), (9000, 500)])
+def test_lists_about_as_long_as_a_wave(draw, v, levels, dtype):
+    """Some 64 tokens that may stay: up to that many one wave decides alone. levels: equal logits, which a bin holds all or none of."""
+    g = np.random.default_rng(v + levels)
+    k = [1, 2, 30, 62, 63, 64, 65, 66, 100]
+    b = len(k)
+    if levels:
+        x = g.integers(0, levels, (b, v)).astype(np.float32) / 16
+        t = torch.from_numpy(x).to(DT[dtype])
+        x = t.float().numpy()
+    else:
+        t, x = logits_of(g, b, v, dtype)
+    x[2, : v // 2] = -math.inf
+    t[2, : v // 2] = -math.inf
+
+    def near(row, kw):  # a token 32 temperatures behind the maximum, in steps of 1/32, is not drawn, which u = 0 would show
+        steps = np.floor(row.astype(np.float64) * (32.0 / kw.get("temperature", 1.0)))
+        return np.where(max(steps) - steps < 1024, row, -math.inf)
+
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.02), dict(min_p=0.2), dict(top_p=0.7, min_p=0.05, temperature=1.7), dict(temperature=0.1)):
+        for u in ([0.0] * b, [LARGEST_U] * b, g.random(b), g.random(b)):
+            got = draw(t.to(DEV), torch.from_numpy(np.float32(u)).to(DEV), top_k=torch.tensor(k, dtype=torch.int32, device=DEV), **kw)
+            assert got.tolist() == [R.sample(near(row, kw), np.float32(ui), top_k=ki, **kw) for row, ui, ki in zip(x, u, k)]
+    got = draw(t[:4].to(DEV), torch.tensor([math.inf, math.nan, 1.0, -1.0], device=DEV), top_k=40)
+    order = np.argsort(-x[:4], axis=1, kind="stable")
+    alive = [[int(i) for i in row[:40] if r[i] > max(r) - 31] for row, r in zip(order, x[:4])]
+    assert got.tolist() == [max(alive[0]), max(alive[1]), max(alive[2]), min(alive[3])]
+
+
 @pytest.mark.parametrize("temperature", [1e-4, 1e-2, 0.3, 20.0, 1e4])
 def test_temperatures(draw, temperature):
     """Rows that are one token, and rows that are flat: more tokens than the sorted list holds end in a bin."""
