@@ -136,6 +136,7 @@ class DecodeState:
         self.k_scale = self.v_scale = self.block_table = self.counts = None
         self.block_kv = kv_dtype in _BLOCK_KV
         self.refs = self.room = self.leaders = self.shared = self.sampling = None
+        self.plans: dict[int, kv_shared.SharedKV] = {}  # by the table's width: kept, since captured steps read them by address
         if kv_pages is not None and (not self.block_kv or kv_pages < 1):
             raise ValueError(f"kv_pages must be positive and belongs to a block-scaled cache, got {kv_pages} for {kv_dtype!r}")
         if self.block_kv:
@@ -289,30 +290,46 @@ class DecodeState:
         """Let steps read what the rows of a group share once (:func:`~scratch_llm_amd.quant.kv_shared.plan_shared_kv`): rows with the
         same number in ``leaders`` (int32 ``[B]``, at least 0; kept, and read again by every :meth:`fork` and :meth:`free`) make
         a group. None: every row for itself. Call it again after other changes of what the table's shared entries name. A step
-        captured while rows share uses the plan as it is when it is replayed; share first, then capture."""
+        captured while rows share uses the plan as it is when it is replayed, after ``share(None)`` every row for itself; a step
+        captured before never shares."""
         if not self.block_kv:
             raise ValueError(f"DecodeState.share needs a block-scaled cache, got {self.kv_dtype!r}")
         self.check_rows("DecodeState.share")
         if leaders is None:
+            self._part()
             self.leaders = self.shared = None
             return
-        same = self.shared is not None and self.shared.width == self.block_table.shape[1]
-        self.shared = self._plan(leaders, self.shared if same else None)
+        self.shared = self._plan(leaders)
         self.leaders = leaders
 
-    def _plan(self, leaders: Tensor, out: "kv_shared.SharedKV | None") -> "kv_shared.SharedKV":
-        return kv_shared.plan_shared_kv(self.block_table, self.lengths, leaders, block=self.k.shape[3], tokens=1, heads=self.n_heads,
+    def _plan(self, leaders: Tensor) -> "kv_shared.SharedKV":
+        """The plan for the table's width, made over the one that captured steps may hold."""
+        width = self.block_table.shape[1]
+        if self.shared is not None and self.shared.width != width:
+            self._part()
+        self.plans[width] = self._plan_table(self.block_table, leaders, self.plans.get(width))
+        return self.plans[width]
+
+    def _plan_table(self, table: Tensor, leaders: Tensor, out: "kv_shared.SharedKV | None") -> "kv_shared.SharedKV":
+        return kv_shared.plan_shared_kv(table, self.lengths, leaders, block=self.k.shape[3], tokens=1, heads=self.n_heads,
                                         kv_heads=self.k.shape[2], head_dim=self.k.shape[4], out=out)
 
+    def _part(self) -> None:
+        """Every row for itself in the plan that is in use: a step that was captured with it must not read as shared what no call
+        plans anew from here on."""
+        if self.shared is not None:
+            table = self.block_table.new_full((self.batch, self.shared.width), -1)
+            self._plan_table(table, table[:, 0].contiguous(), self.shared)
+
     def _replan(self) -> None:
-        if self.shared is not None:  # written over for a captured step, as long as the table is as wide
-            same = self.shared.width == self.block_table.shape[1]
-            self.shared = self._plan(self.leaders, self.shared if same else None)
+        if self.shared is not None:
+            self.shared = self._plan(self.leaders)
 
     def set_sampling(self, sampling: "Sampling | None") -> None:
         """Let steps draw their tokens (:func:`~scratch_llm_amd.sampling.sample_tokens`) with the random numbers in ``u`` (float32 ``[B]``,
         in [0, 1), to be set before every step); None: greedy picks. A row whose logits are no distribution keeps its token and
-        does not advance."""
+        does not advance. A captured step keeps the settings that it was captured with; the values of those that are tensors may
+        change between replays."""
         if sampling is not None:
             sampling.check(self.batch, "DecodeState.set_sampling")
             if any(x is not None for x in sampling.tensors()):
@@ -981,9 +998,12 @@ class Int4DecodeLM:
     def capture(self, st: DecodeState) -> torch.cuda.CUDAGraph:
         """Record one :meth:`step` on ``st`` in a HIP graph. Each ``replay()`` decodes the next token
         from ``st.tokens`` and the cache as they are at that moment. Capturing runs nothing, so ``st``
-        is unchanged."""
+        is unchanged. Replays read the model's and the state's tensors, and those of the settings that
+        :meth:`DecodeState.set_sampling` was given, by their addresses: the graph keeps them, and does not
+        see other tensors or settings that are put in their place later."""
         torch.cuda.synchronize(self.device)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.device(self.device), torch.cuda.graph(g):
             self.step(st)
+        g.reads = (self, dict(vars(st)))
         return g
