@@ -273,10 +273,12 @@ class DecodeState:
 
     def fork(self, parents: Tensor) -> Tensor:
         """Let every row go on from row ``parents[b]`` (int32 ``[B]``): its pages, length and next input token
-        (:func:`~scratch_llm_amd.quant.kv_pages.fork_kv_rows`; the ``active`` flags stay). Returns ``room``: 1, or 0 and nothing changed."""
+        (:func:`~scratch_llm_amd.quant.kv_pages.fork_kv_rows`; the ``active`` flags stay). A row that a parent outside ``0 .. B - 1``
+        empties keeps its own token. Returns ``room``: 1, or 0 and nothing changed."""
         pool = self._pool("DecodeState.fork")
         self.room.copy_(kv_pages.fork_kv_rows(parents, *pool, self.block_table, self.lengths, self.refs))
-        at = torch.where((parents >= 0) & (parents < self.batch), parents, 0).long()
+        own = torch.arange(self.batch, dtype=torch.int32, device=parents.device)
+        at = torch.where((parents >= 0) & (parents < self.batch), parents, own).long()
         self.tokens.copy_(torch.where(self.room > 0, self.tokens[at], self.tokens))
         self._replan()
         return self.room

@@ -280,3 +280,12 @@ def test_sampled_steps_of_every_cache_and_rows_without_a_distribution(small):
     before = st.tokens.clone()
     model.step(st)
     assert bool(st.logits[1].isnan().any()) and int(st.tokens[1]) == int(before[1]) and st.lengths.tolist() == [6, 5, 6]
+
+
+def test_an_emptied_row_keeps_its_token(small):
+    model, _ = small
+    st, _ = prefilled(model, 4, 37, "int8_block")
+    st.tokens.copy_(i32([10, 11, 12, 13]))
+    assert int(st.fork(i32([0, -1, 0, 4]))) == 1
+    assert st.lengths.tolist() == [37, 0, 37, 0] and st.tokens.tolist() == [10, 11, 10, 13]
+    books(st)

@@ -60,3 +60,17 @@ def test_sampling_is_checked_when_it_is_set():
     st.u = torch.zeros(3)
     with pytest.raises(ValueError, match="u must"):
         model().step(st)
+
+
+@pytest.mark.parametrize("ok", [1, 0])
+def test_tokens_of_a_fork(monkeypatch, ok):
+    """A row takes its parent's next token; one that a parent outside the batch empties keeps its own, as do all where pages lack."""
+    from scratch_llm_amd.quant import kv_pages
+
+    monkeypatch.setattr(kv_pages, "fork_kv_rows", lambda *a: ints(ok))
+    monkeypatch.setattr(DecodeState, "check_rows", lambda self, fn: None)
+    st = DecodeState(model(), 5, 64, "int8_block", 16, kv_pages=5)
+    st.tokens.copy_(ints(10, 11, 12, 13, 14))
+    st.fork(ints(2, -1, 2, 5, 0))
+    assert st.tokens.tolist() == ([12, 11, 12, 13, 10] if ok else [10, 11, 12, 13, 14])
+    assert st.room.tolist() == [ok]
