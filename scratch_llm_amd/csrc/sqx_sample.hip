@@ -23,8 +23,9 @@
 // bf16 with top-p 20.3 + 41.0: the first is bound by its atomics in LDS and its exponentials in double, one of each a token; in the
 // second a row's workgroup, of some 28 us alone, spends 3 on its maximum, 3 on joining the histograms, 8 on collecting, 5 on sorting
 // some 100 tokens (15 for 1000) and 6 on the draw; the longest row counts. 201 rows of 50257 in fp32 with all limits 22.5 + 34.4.
-// The way digit by digit takes 64 such rows 0.5 ms (top-k) to 1 ms (top-p; 128256 tokens at T = 20, or all equal): it reads the
-// row for each of seven digits, and most of its time goes to atomics on few addresses.
+// The way digit by digit takes 64 such rows 0.47 ms (top-k) to 0.64 and 0.84 ms (top-p; 128256 tokens at T = 20, and all equal), and
+// 0.88 ms for bf16 logits around 40, whose steps of 1/4 put some 5000 tokens into the bin where top-p 0.95 ends (56 us around 0): it
+// reads the row for each of seven digits, and most of its time goes to atomics on few addresses.
 //
 // Weights are double, from a table of 64 powers and a Taylor polynomial of degree 5 (x^6 / 720 < 4e-17): the decisions fall
 // between neighbours of sums over a vocabulary, which fp32 would move in one row of a hundred.
@@ -405,7 +406,8 @@ struct RowBins {
     const double w = pow2_64th((static_cast<double>(l) - m) * k, pow64);
     return l == -INFINITY ? 0.0 : w;
   }
-  // Weights of tokens from bin c on are at most 2^-lift(c): they are added as whole numbers of 2^-48 2^-lift.
+  // Weights of tokens from bin c on are below 2 2^-lift(c), those of the bin itself above half of that: as whole numbers of 2^-50
+  // 2^-lift they are good to 2^-50 of themselves, and up to 4096 of them add up below 2^63.
   __device__ static int lift(int c) { return static_cast<int>((max(c, 1) - 1) * (1.4426950408889634 / kPerT)); }
 };
 
@@ -421,8 +423,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   __shared__ unsigned long long list[kCap];
   __shared__ double before[kCap + 1];  // weight of the list's tokens before each; where there is no list, of a digit's tokens
   __shared__ int found, at_k, at_p0, at_p1, begin[3], end[3], cut_p, cut_m, pick, last, digit_rank;
-  __shared__ unsigned long long digit_place, dropped;
-  __shared__ double digit_left;
+  __shared__ unsigned long long digit_place, digit_left, dropped;
   const int b = blockIdx.x, tid = threadIdx.x, S = a.S;
   const int64_t at = static_cast<int64_t>(b) * S, row0 = static_cast<int64_t>(b) * a.V;
   // the row's first slices are on their way while the histograms are joined
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     // ---- too many for the list: the cut digit by digit
     unsigned long long* const digit_w = reinterpret_cast<unsigned long long*>(before);
     unsigned* const digit_c = reinterpret_cast<unsigned*>(before + 256);
-    auto walk = [&](auto&& each) {
+    auto walk = [&](auto&& each, auto&& slice_done) {
       for (int s = 0; s < S; ++s) {
         const int i0 = s * kSampleSlice + 8 * tid;
         float v[8];
@@ -753,18 +754,23 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             float l = v[0];
 #pragma unroll
             for (int k = 1; k < 8; ++k) l = k == j ? v[k] : l;
-            if (l > -INFINITY) each(l, place(l, Loads8<DT>::first(i0, a.V) + j), s);
+            if (l > -INFINITY) each(l, place(l, Loads8<DT>::first(i0, a.V) + j));
           }
+        slice_done(s);
       }
     };
-    const double unit = 0x1p42;  // 2^20 tokens of at most 2^42 fit 64 bits
-    auto fix = [&](float l) { return static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5)); };
-    // The place of the last token that is kept, of the first `rank`, or of those with less than `left` before them.
-    auto select = [&](bool by_rank, int rank, double left) {
+    auto go_on = [](int) {};
+    // The place of the last token that is kept: of the first `rank`, or, among those of places from `cut` on, whose weight is z, of
+    // those with less than `left` before them. Their weights are whole numbers of 2^-62 of a power of two above z, so that sums in
+    // any order are equal and below 2^63; 2^17 equal ones are off by 2^-45 of z together, where a sum of doubles may be by 2^-36.
+    auto select = [&](bool by_rank, int rank, double z, double left) {
+      int above = 0;
+      if (!by_rank) frexp(z, &above);
+      const double unit = ldexp(1.0, 62 - above);
       if (tid == 0) {
         digit_place = 0;
         digit_rank = rank;
-        digit_left = left * unit;
+        digit_left = by_rank ? 0ull : static_cast<unsigned long long>(ceil(fmax(left * unit, 0.0)));
       }
       for (int sh = 56; sh >= 0; sh -= sh == 32 ? 16 : 8) {  // ids have 20 bits: the highest of the low word's bytes is 255
         if (tid < 256) {
@@ -773,10 +779,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         }
         __syncthreads();
         const unsigned long long so_far = digit_place;
-        walk([&](float l, unsigned long long q, int) {
-          if (sh < 56 && (q ^ so_far) >> (sh + 8) != 0) return;
+        walk([&](float l, unsigned long long q) {
+          if ((sh < 56 && (q ^ so_far) >> (sh + 8) != 0) || (!by_rank && q < cut)) return;
           const int d = static_cast<int>(q >> sh) & 255;
-          const unsigned long long f = by_rank ? 0ull : fix(l);
+          const unsigned long long f = by_rank ? 0ull : static_cast<unsigned long long>(fma(r.weight(l), unit, 0.5));
           // equal logits: one addition for the wave's tokens, not one after the other
           const unsigned long long here = __ballot(true);
           const unsigned long long f0 = (static_cast<unsigned long long>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(f >> 32))) << 32) |
@@ -790,11 +796,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             atomicAdd(&digit_c[d], 1u);
             if (!by_rank) atomicAdd(&digit_w[d], f);
           }
-        });
+        }, go_on);
         __syncthreads();
         if (tid == 0) {
           int chosen = -1, rank_at = 0, c_run = 0;
-          double left_at = 0.0, w_run = 0.0;
+          unsigned long long left_at = 0, w_run = 0;
           for (int d = 255; d >= 0; --d) {
             if (digit_c[d] == 0) continue;
             if (chosen < 0 || (by_rank ? c_run < digit_rank : w_run < digit_left)) {
@@ -803,7 +809,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
               left_at = digit_left - w_run;
             }
             c_run += digit_c[d];
-            w_run += static_cast<double>(digit_w[d]);
+            w_run += digit_w[d];
           }
           digit_place |= static_cast<unsigned long long>(max(chosen, 0)) << sh;
           if (sh == 32) digit_place |= 0xff000000ull;
@@ -816,29 +822,33 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
       __syncthreads();
       return q;
     };
-    if (by_k) cut = select(true, want_k, 0.0);
+    if (by_k) cut = select(true, want_k, 0.0, 0.0);
     if (by_p) {
       double mine = 0.0, z;
-      walk([&](float l, unsigned long long q, int) { mine += q >= cut && r.bin(static_cast<double>(l)) < kBins ? r.weight(l) : 0.0; });
+      walk([&](float l, unsigned long long q) { mine += q >= cut && r.bin(static_cast<double>(l)) < kBins ? r.weight(l) : 0.0; }, go_on);
       pick_scan(mine, redd, z);
-      cut = max(cut, select(false, 0, p * z));
+      cut = max(cut, select(false, 0, z, p * z));
     }
     if (by_m) {
-      walk([&](float l, unsigned long long q, int) {
+      walk([&](float l, unsigned long long q) {
         if (r.weight(l) < minp) atomicMax(&dropped, q);
-      });
+      }, go_on);
       __syncthreads();
       cut = max(cut, dropped + 1);
     }
-    walk([&](float l, unsigned long long q, int s) {
-      if (q >= cut && r.bin(static_cast<double>(l)) < kBins) atomicAdd(&slice_fix[s], fix(l));
-    });
+    double mine = 0.0;
+    walk([&](float l, unsigned long long q) { mine += q >= cut && r.bin(static_cast<double>(l)) < kBins ? r.weight(l) : 0.0; },
+         [&](int s) {
+           double whole;
+           pick_scan(mine, redd, whole);
+           if (tid == 0) slice_w[s] = whole;
+           mine = 0.0;
+         });
     walked = true;
-    __syncthreads();
   }
 
   // ---- the weight that each slice keeps: whole bins, and the tokens of the cut's bin
-  const double unit = walked ? 0x1p42 : ldexp(0x1p42, r.lift(cut_bin));  // 8192 tokens of at most 2^42 fit 64 bits
+  const double unit = ldexp(0x1p50, r.lift(cut_bin));
   if (!walked && cut_bin < kBins) {
     for (int i = tid; i < n; i += kPickThreads) {
       const unsigned long long q = list[i];
@@ -848,8 +858,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
     __syncthreads();
   }
-  if (tid < S) {
-    const int upto = walked ? -1 : min(cut_bin, kBins) - 1 - shift[tid];
+  if (tid < S && !walked) {
+    const int upto = min(cut_bin, kBins) - 1 - shift[tid];
     const double whole = upto >= 0 ? static_cast<double>(a.mass[(at + tid) * kBins + upto]) * scale[tid] : 0.0;
     slice_w[tid] = fma(static_cast<double>(slice_fix[tid]), 1.0 / unit, whole);
   }
