@@ -9,8 +9,8 @@
 //  1. Workgroup (slice, row) reads its 8192 logits once, keeps them in registers and leaves a histogram of 1024 bins over the
 //     distance from the maximum, 1/32 of the temperature wide: a count and a weight of each bin. Bins lie on a grid that
 //     does not depend on the row (floor(32 l / T)), so slices with different maxima are joined by a shift and a factor,
-//     and the row's maximum need not be known first. Weights are added as whole numbers of 2^-48 of the slice's largest one:
-//     atomics in any order give the same sum.
+//     and the row's maximum need not be known first. Weights are added as whole numbers, of a unit that falls along the bins, so
+//     that atomics in any order give the same sum and every weight counts to 2^-49 of itself.
 //  2. One workgroup a row joins the histograms and finds the bin that each limit ends in. The tokens of these bins, a few
 //     hundred as a rule, are collected and sorted, which gives the cut exactly; slices' weights before the cut come from
 //     the histograms, and one slice is read again for the draw itself. Where more than 4096 tokens lie in these bins
@@ -19,10 +19,11 @@
 // A token 32 T or further behind the maximum (the bins' end lies within 1/32 before that) has less than 2^-45 of its weight and is
 // never drawn; u itself has 24 bits.
 //
-// us of the two launches: 1 row of 32000 in fp32 with top-k 6.6 + 11.1, latency: four dependent rounds in each. 64 rows of 128256 in
-// bf16 with top-p 20.3 + 41.0: the first is bound by its atomics in LDS and its exponentials in double, one of each a token; in the
+// us of the two launches: 1 row of 32000 in fp32 with top-k 6.3 + 10.9, latency: four dependent rounds in each. 64 rows of 128256 in
+// bf16 with top-p 22.2 + 40.9: the first is bound by its atomics in LDS and its exponentials in double, one of each a token; in the
 // second a row's workgroup, of some 28 us alone, spends 3 on its maximum, 3 on joining the histograms, 8 on collecting, 5 on sorting
-// some 100 tokens (15 for 1000) and 6 on the draw; the longest row counts. 201 rows of 50257 in fp32 with all limits 22.5 + 34.4.
+// some 100 tokens (15 for 1000) and 6 on the draw; the longest row counts. 201 rows of 50257 in fp32 with all limits 23.4 + 34.0.
+// The falling unit costs 1.6 of the 22.2: with one unit of 2^-48 a slice of a heavy token and faint ones was up to 0.3 in 100 of these off.
 // The way digit by digit takes 64 such rows 0.47 ms (top-k) to 0.64 and 0.84 ms (top-p; 128256 tokens at T = 20, and all equal), and
 // 0.88 ms for bf16 logits around 40, whose steps of 1/4 put some 5000 tokens into the bin where top-p 0.95 ends (56 us around 0): it
 // reads the row for each of seven digits, and most of its time goes to atomics on few addresses.
@@ -43,7 +44,13 @@ constexpr int kCap = 4096;         // tokens that are sorted
 constexpr int kFew = 1024;         // up to this k all tokens that may stay are collected, and slices leave no weights
 constexpr int kMaxSlices = 128;    // 2^20 tokens
 constexpr int kHistThreads = 512, kPickThreads = 1024;
-constexpr double kFix = 0x1p48;
+constexpr double kFix = 0x1p50;
+
+// Weights of bin c are between 0.46 and 1.001 times 2^-lift: as whole numbers of 2^-50 2^-lift they are good to 2^-49 of themselves,
+// and 8192 of them add up below 2^64.
+__host__ __device__ constexpr int bin_lift20(int c) { return (c - 1) * 47274; }  // 2^20 (c - 1) log2 e / kPerT
+__host__ __device__ constexpr int bin_lift(int c) { return bin_lift20(c) >> 20; }
+constexpr int kMostLift = bin_lift(kBins - 1);
 
 struct SampleArgs {
   const void* logits;  // [B, V]
@@ -54,13 +61,13 @@ struct SampleArgs {
   int k, V, S;
   float* smax;                // [B, S]
   int* sarg;                  // [B, S]
-  unsigned long long* mass;   // [B, S, kBins], summed from bin 0 on
+  double* mass;               // [B, S, kBins], of the slice's maximum's weight, summed from bin 0 on
   unsigned* count;            // [B, S, kBins], likewise
   int* out;
 };
 
-// 2^(y / 64), y <= 0.
-__device__ inline double pow2_64th(double y, const double* pow64) {
+// 2^(y / 64 + floor(lift20 / 2^20)), y <= 0.
+__device__ inline double pow2_64th(double y, const double* pow64, int lift20 = 0) {
   y = fmax(y, -64000.0);
   const double t = y + 0x1.8p52;
   const int n = __double2loint(t);
@@ -71,10 +78,10 @@ __device__ inline double pow2_64th(double y, const double* pow64) {
   q = fma(q, x, 1.0);
   q = fma(q, x, 1.0);
   const double w = pow64[n & 63];
-  return q * __hiloint2double(__double2hiint(w) + ((n & ~63) << 14), __double2loint(w));
+  return q * __hiloint2double(__double2hiint(w) + ((n & ~63) << 14) + (lift20 & ~0xfffff), __double2loint(w));  // to its exponent
 }
 
-// The whole number nearest to w 2^48, 0 <= w <= 1.
+// The whole number nearest to w 2^50, 0 <= w < 2.
 __device__ inline unsigned long long to_fix(double w) {
   return __builtin_bit_cast(unsigned long long, fma(w, kFix, 0x1p52)) & 0xfffffffffffffull;
 }
@@ -121,6 +128,29 @@ __device__ inline bool greedy_takes(float ov, int oi, float cv, int ci) {
   return ov > cv || (ov == cv && oi < ci);
 }
 
+// Sums over a wave's lanes up to each one's own, by moves between lanes' registers: within rows of 16, then a row's last lane to the
+// next row (of rows 1 and 3), then lane 31 to the upper half. (As shuffles, through LDS, 0.7 us more of 22.)
+template <int CTRL, int ROWS, typename N>
+__device__ inline void add_moved(N& x) {
+  constexpr int W = sizeof(N) / 4;
+  uint32_t w[W];
+  __builtin_memcpy(w, &x, sizeof(N));
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = __builtin_amdgcn_update_dpp(0u, w[i], CTRL, ROWS, 0xf, false);  // 0 where no lane sends
+  N y;
+  __builtin_memcpy(&y, w, sizeof(N));
+  x += y;
+}
+template <typename N>
+__device__ inline void wave_sums(N& x) {
+  add_moved<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
+  add_moved<0x112, 0xf>(x);
+  add_moved<0x114, 0xf>(x);
+  add_moved<0x118, 0xf>(x);
+  add_moved<0x142, 0xa>(x);  // row_bcast:15
+  add_moved<0x143, 0xc>(x);  // row_bcast:31
+}
+
 // 8192 tokens a workgroup: 16 a thread stay in registers between the maximum and the bins, and a row of 128256 leaves 16 histograms
 // to be joined.
 template <int DT>
@@ -131,7 +161,7 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(const SampleA
   __shared__ unsigned count[kBins];
   __shared__ float redv[W];
   __shared__ int redi[W];
-  __shared__ unsigned long long redm[W];
+  __shared__ unsigned __int128 redm[W];
   __shared__ unsigned redc[W];
   static_assert(kBins == 2 * kHistThreads, "two bins a thread");
   const int s = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -198,44 +228,46 @@ __global__ __launch_bounds__(kHistThreads) void sample_hist_kernel(const SampleA
       if (Loads8<DT>::has(base + g * 8 * kHistThreads, a.V, e) && d < kBins) {  // false of a NaN: a masked token of a slice that is all masked
         const int bin = static_cast<int>(d);
         if (want_k >= 1) atomicAdd(&count[bin], 1u);
-        if (!few) atomicAdd(&mass[bin], to_fix(pow2_64th((l - m) * k, pow64)));
+        if (!few) atomicAdd(&mass[bin], to_fix(pow2_64th((l - m) * k, pow64, __mul24(bin - 1, 47274))));
       }
     }
   __syncthreads();
-  // sums from bin 0 on: two bins a thread, then over the workgroup
+  // sums from bin 0 on: two bins a thread, then over the workgroup. Weights are whole numbers of 2^-50 2^-kMostLift, below 2^110:
+  // exact, and so no sum is less than the one before it, rounded to double too
+  using u128 = unsigned __int128;
   const int lane = tid & 63, wave = tid >> 6;
-  const unsigned long long m0 = mass[2 * tid], m1 = m0 + mass[2 * tid + 1];
+  const bool counts = want_k >= 1;  // as `few` of the whole workgroup
+  auto of = [&](int bin) { return static_cast<u128>(mass[bin]) << (kMostLift - bin_lift(bin)); };
+  const u128 m0 = of(2 * tid), m1 = m0 + of(2 * tid + 1);
   const unsigned c0 = count[2 * tid], c1 = c0 + count[2 * tid + 1];
-  unsigned long long ms = m1;
+  u128 ms = m1;
   unsigned cs = c1;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long y = __shfl_up(ms, o, 64);
-    const unsigned z = __shfl_up(cs, o, 64);
-    if (lane >= o) {
-      ms += y;
-      cs += z;
-    }
+  if (!few) {
+    wave_sums(ms);
+    if (lane == 63) redm[wave] = ms;
   }
-  if (lane == 63) {
-    redm[wave] = ms;
-    redc[wave] = cs;
+  if (counts) {
+    wave_sums(cs);
+    if (lane == 63) redc[wave] = cs;
   }
   __syncthreads();
-  ms -= m1;
-  cs -= c1;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    ms += w < wave ? redm[w] : 0ull;
-    cs += w < wave ? redc[w] : 0u;
-  }
   if (!few) {
-    ulonglong2 mo;
-    mo.x = ms + m0;
-    mo.y = ms + m1;
-    reinterpret_cast<ulonglong2*>(a.mass + at * kBins)[tid] = mo;
+    ms -= m1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) ms += w < wave ? redm[w] : u128{0};
+    auto weight = [](u128 x) {
+      const double hi = static_cast<double>(static_cast<unsigned long long>(x >> 64));
+      return fma(hi, 0x1p64, static_cast<double>(static_cast<unsigned long long>(x))) * (1.0 / kFix) * ldexp(1.0, -kMostLift);
+    };
+    double2 mo;
+    mo.x = weight(ms + m0);
+    mo.y = weight(ms + m1);
+    reinterpret_cast<double2*>(a.mass + at * kBins)[tid] = mo;
   }
-  if (want_k >= 1) {
+  if (counts) {
+    cs -= c1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) cs += w < wave ? redc[w] : 0u;
     uint2 co;
     co.x = cs + c0;
     co.y = cs + c1;
@@ -406,9 +438,6 @@ struct RowBins {
     const double w = pow2_64th((static_cast<double>(l) - m) * k, pow64);
     return l == -INFINITY ? 0.0 : w;
   }
-  // Weights of tokens from bin c on are below 2 2^-lift(c), those of the bin itself above half of that: as whole numbers of 2^-50
-  // 2^-lift they are good to 2^-50 of themselves, and up to 4096 of them add up below 2^63.
-  __device__ static int lift(int c) { return static_cast<int>((max(c, 1) - 1) * (1.4426950408889634 / kPerT)); }
 };
 
 // One workgroup a row.
@@ -468,7 +497,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   // ---- the row's histogram: thread i is bin i
   if (tid < S) {
     shift[tid] = r.bin(static_cast<double>(smax[tid]));
-    scale[tid] = smax[tid] == -INFINITY ? 0.0 : r.weight(smax[tid]) * (1.0 / kFix);
+    scale[tid] = smax[tid] == -INFINITY ? 0.0 : r.weight(smax[tid]);
   }
   __syncthreads();
   int to = 0;
@@ -483,8 +512,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         to += from >= 0 ? cs : 0u;
       }
       if constexpr (decltype(weights)::value) {
-        const unsigned long long ws = a.mass[h];
-        w_to = fma(from >= 0 ? static_cast<double>(ws) : 0.0, scale[s], w_to);
+        const double ws = a.mass[h];
+        w_to = fma(from >= 0 ? ws : 0.0, scale[s], w_to);
       }
     }
   };
@@ -848,7 +877,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   }
 
   // ---- the weight that each slice keeps: whole bins, and the tokens of the cut's bin
-  const double unit = ldexp(0x1p50, r.lift(cut_bin));
+  const double unit = ldexp(kFix, bin_lift(cut_bin));
   if (!walked && cut_bin < kBins) {
     for (int i = tid; i < n; i += kPickThreads) {
       const unsigned long long q = list[i];
@@ -860,7 +889,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
   }
   if (tid < S && !walked) {
     const int upto = min(cut_bin, kBins) - 1 - shift[tid];
-    const double whole = upto >= 0 ? static_cast<double>(a.mass[(at + tid) * kBins + upto]) * scale[tid] : 0.0;
+    const double whole = upto >= 0 ? a.mass[(at + tid) * kBins + upto] * scale[tid] : 0.0;
     slice_w[tid] = fma(static_cast<double>(slice_fix[tid]), 1.0 / unit, whole);
   }
   __syncthreads();
@@ -1005,7 +1034,7 @@ extern "C" int sqx_sample(const void* logits, int dtype, const float* u, const f
   a.temp_t = temperature_t; a.p_t = top_p_t; a.minp_t = min_p_t; a.k_t = top_k_t;
   a.temp = temperature; a.p = top_p; a.minp = min_p;
   a.k = static_cast<int>(std::min<int64_t>(top_k, 0x7fffffff)); a.V = static_cast<int>(V); a.S = static_cast<int>(S);
-  a.mass = static_cast<unsigned long long*>(ws);
+  a.mass = static_cast<double*>(ws);
   a.count = reinterpret_cast<unsigned*>(a.mass + B * S * kBins);
   a.smax = reinterpret_cast<float*>(a.count + B * S * kBins);
   a.sarg = reinterpret_cast<int*>(a.smax + B * S);

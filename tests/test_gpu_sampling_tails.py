@@ -1,10 +1,10 @@
 """Draws that fall into a tail of many light tokens, against sums of whole numbers (oracle/sample_ref.py, Exact): weights and their sums
 hold what float64 holds, also where more tokens than the sorted list has share the bin that a limit ends in.
 
-A decision may fall otherwise within 2^-44 of the whole weight: weights are good to 2^-47 of themselves and the heavy ones to more,
-some hundred float64 roundings of sums make 2^-46, and where a limit is looked for digit by digit, 2^17 tokens of equal weight are each
-off by up to 2^-62 of the whole, 2^-45. Draws nearer to a border than that are left out, a few in a hundred at most; a float64 sum of that
-many equal terms, one after the other, may be off by 2^-36."""
+A decision may fall otherwise within 2^-44 of the whole weight: weights are good to 2^-47 of themselves and the heavy ones to more, each
+is rounded to 2^-49 of itself before 8192 of them are added up exactly, some hundred float64 roundings of sums make 2^-46, and where a
+limit is looked for digit by digit, 2^17 tokens of equal weight are each off by up to 2^-62 of the whole, 2^-45. Draws nearer to a border
+than that are left out, a few in a hundred at most; a float64 sum of that many equal terms, one after the other, may be off by 2^-36."""
 
 from __future__ import annotations
 
@@ -44,6 +44,7 @@ ROWS = {
     "equal -18, min_p": lambda g: (one_high(g, -18.0), dict(min_p=1.5e-8)),
     "equal -26": lambda g: (one_high(g, -26.0), dict(top_p=1 - 3e-7)),
     "equal -27, no limit": lambda g: (one_high(g, -27.0), dict()),
+    "equal -28, no limit": lambda g: (one_high(g, -28.0), dict()),
     "spread -22": lambda g: (one_high(g, -22.0, 1.0), dict(top_p=1 - 2e-5)),
     "spread -22, by k too": lambda g: (one_high(g, -22.0, 1.0), dict(top_p=1 - 1e-5, top_k=100000)),
     "spread -22, min_p": lambda g: (one_high(g, -22.0, 1.0), dict(min_p=math.exp(-22.7))),
@@ -79,3 +80,22 @@ def test_tails(name):
     assert sum(sure) >= 0.9 * len(u)
     off = [(float(v), a, b) for v, a, (b, _), s in zip(u, got, want, sure) if s and a != b]
     assert not off, f"{len(off)} of {sum(sure)}: {off[:5]}"
+
+
+@pytest.mark.parametrize("first", [0, 5000])
+def test_the_last_draw_in_a_faint_tail(first):
+    """The largest random number falls among equal tokens of 2^-41 of the heavy one's weight, in the same 8192 tokens as it or soon behind
+    them: what these hold in all decides which."""
+    from scratch_llm_amd.sampling import sample_tokens
+
+    u = 1.0 - 2.0**-24
+    sure = 0
+    for at in np.float32(np.log(2.0**-24 * (1.0 + np.linspace(0.005, 0.055, 12) + first / V) / (V - 1))):
+        x = torch.full((V,), float(at))
+        x[first] = 0.0
+        want, margin = R.Exact(x.numpy()).draw(u)
+        got = sample_tokens(x.to(DEV)[None], torch.tensor([u], device=DEV))
+        if margin > 2.0**-44:
+            sure += 1
+            assert first < want and got.tolist() == [want], at
+    assert sure >= 6
