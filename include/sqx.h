@@ -973,8 +973,8 @@ int sqx_kvshared_attention(const void* q, int dtype, int64_t q_sb, int64_t q_st,
  * exp((l_i - m) / temperature), tokens stand in the order of their logits, equal ones by their id. Kept of these: the first top_k
  * (0: all); of these those with less than top_p of these's weight before them (1: all; always the first); of these those with
  * w_i >= min_p. tokens[b] is the least i whose cumulative kept weight, ids ascending, exceeds u[b] times the whole. Weights and sums
- * in double, or in whole numbers that hold as much; a token with (m - l_i) / temperature of about 32 or more is not drawn. temperature 0: the first maximum, a NaN counts as one; else
- * a row with a NaN or +inf, or of -inf only, gives -1. Each setting is a number, or per row where its pointer is not NULL
+ * in double, or in whole numbers that hold as much; a token with (m - l_i) / temperature of about 32 or more is not drawn.
+ * temperature 0: the first maximum, a NaN counts as one; else a row with a NaN or +inf, or of -inf only, gives -1. Each setting is a number, or per row where its pointer is not NULL
  * (temperature not above 0: 0, else within 1e-4 .. 1e4; top_k below 1: 0; top_p not above 0: the first token; min_p above 1:
  * 1; a limit of NaN: none). ws: 16-byte aligned. */
 int64_t sqx_sample_workspace_bytes(int64_t B, int64_t V);

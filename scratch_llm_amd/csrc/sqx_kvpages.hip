@@ -6,9 +6,9 @@
 // calls give equal tables. A call that hands out pages does all of it or, where the pool is too small, nothing.
 //
 // Two kinds of launches: small ones over tables and counts, bound by the latency of a launch and of two or three dependent
-// loads each, and one that copies the pages, bound by HBM. us of the kernels: fork of 8 rows (7 pages of 4 layers copied) 5.2
-// and 5.6; of 64 rows of beams (260 MB read and written) 7.4 and 55, 4.7 TB/s; release and reservation for 96 rows 3.2 and 8.4, 8.7
-// for the 46 MB copied; a pool of 1100 pages of 32 layers, 128 KiB each, compacted (2.1 GB) 434, 4.9 TB/s, with 5
+// loads each, and one that copies the pages, bound by HBM. us of the kernels: fork of 8 rows (7 pages of 4 layers copied) 5.4
+// and 5.5; of 64 rows of beams (260 MB read and written) 7.4 to 8.4 and 54 to 60, 4.3 to 4.8 TB/s; release and reservation for 96 rows 3.2 and
+// 8.9, 8.9 for the 46 MB copied; a pool of 1100 pages of 32 layers, 128 KiB each, compacted (2.1 GB) 434, 4.9 TB/s, with 5
 // before it for each of the counts, their sums and the plan.
 //
 // Rows are looked at by many workgroups, but pages are dealt out by one: the place of a page in the list of free ones depends on

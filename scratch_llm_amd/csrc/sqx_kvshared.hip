@@ -13,8 +13,8 @@
 // small groups' and every row's own keys in one (the direct kernel, 32 rows, straight from memory); the join.
 //
 // us a call in a graph, beside the attention that reads all keys for each row (32 heads over 8 of 128, int8 unless stated): 8 rows
-// behind 2000 keys 13 (13); 64 behind 8192 34 (101); 32 behind 8192 27 (57); 128 behind 8192 57 (189); 256 behind 4096 74 (200); 16
-// behind 32768 29 (101); 2 groups of 32 behind 16384 52 (186); 6 of 16 behind some 15000, E4M3, 80 (251); 24 pairs behind 4000 48
+// behind 2000 keys 13 (13); 64 behind 8192 33 (106); 32 behind 8192 26 (59); 128 behind 8192 55 (189); 256 behind 4096 73 (201); 16
+// behind 32768 28 (101); 2 groups of 32 behind 16384 50 (186); 6 of 16 behind some 15000, E4M3, 78 (251); 24 pairs behind 4000 47
 // (59). Few rows are bound by launches and dependent loads, the others by the products over the shared keys, whose conversion
 // from 8 bits is repeated for every 32 query rows, and by the rows' own keys, from HBM.
 #include "sqx_kvattn.h"
@@ -24,8 +24,12 @@ namespace sqx {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanRows = 4096;      // rows of a batch
 // The prompt kernel takes groups of so many query rows, and of so many products of these with shared keys: its prologue and the 133
-// KB that each of its workgroups leaves to be joined have to pay. us a call, direct and prompt kernel, 8 kv heads of 128, int8:
-//   512 rows x 8192 keys 57, 63; 1024 x 4096 74, 84; 2048 x 2048 103, 110; 1024 x 16384 124, 108; 2048 x 8192 167, 157
+// KB that each of its workgroups leaves to be joined have to pay. us a call, direct and prompt kernel, 8 kv heads of 128, int8, at half
+// the products, at the border and at twice as many:
+//   512 rows x 8192 keys 51, 56; 16384 75, 72; 32768 122, 110
+//   1024 x 4096 57, 66; 8192 86, 84; 16384 132, 120 (E4M3: 8192 83, 84; 16384 126, 120; heads of 64: 49, 57; 78, 75)
+//   2048 x 2048 85, 94; 4096 111, 112; 8192 160, 149
+// Heads of 256 gain more (4 kv heads: 512 x 16384 125, 90). The rule does not look at the kv heads: one alone at 1024 x 8192 24, 38.
 constexpr int kTileFrom = 512;
 constexpr int64_t kTileWork = int64_t(1) << 23;
 constexpr int kDirectGroups = 512, kTileGroups = 256;
@@ -640,7 +644,7 @@ extern "C" int sqx_kvshared_attention(const void* q, int dtype, int64_t q_sb, in
     constexpr int D = decltype(dd)::value;
     auto go = [&](auto e4, auto bf) {
       constexpr bool E = decltype(e4)::value, BF = decltype(bf)::value;
-      if (z.tile > 0 && B * rows * width * block >= kTileWork) {  // else no group is that large
+      if (z.tile > 0 && B * rows * width * block >= kTileWork) {  // else no group is that large; a wide table alone gives no items
         const dim3 grid(heads, static_cast<unsigned>(z.tile));
         if (block >= kStepKeys) hipLaunchKernelGGL((kv_shared_tile_kernel<D, E, BF, true>), grid, dim3(64 * tile_waves(D)), 0, s, x);
         else hipLaunchKernelGGL((kv_shared_tile_kernel<D, E, BF, false>), grid, dim3(64 * tile_waves(D)), 0, s, x);

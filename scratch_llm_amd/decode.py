@@ -11,9 +11,10 @@ is ``w4a16_linear`` (int4_group.py:148-164). This module is that step on the lib
 * everything between them from sqx_decode.hip: residual add + RMSNorm, split-key GQA attention
   with RoPE and the cache write folded in, SiLU-gate, embedding rows, greedy pick, ``advance``.
 
-A step allocates nothing: :class:`DecodeState` holds the cache and every buffer for one batch
-size, so :meth:`Int4DecodeLM.capture` can record the whole step in a HIP graph whose replays
-decode token after token (the pick of one replay is the input of the next).
+A greedy step on pages of its own allocates nothing: :class:`DecodeState` holds the cache and every buffer for one
+batch size (sampling, a pool and shared reading take workspaces from torch's allocator). :meth:`Int4DecodeLM.capture`
+records the whole step in a HIP graph whose replays decode token after token (the pick of one replay is the input of
+the next).
 
 On the block-scaled 8-bit cache (``kv_dtype="int8_block"`` or ``"fp8_block"``,
 :mod:`scratch_llm_amd.quant.kv_block`) the model also takes several tokens a row: a chunk of a prompt
@@ -291,7 +292,7 @@ class DecodeState:
     def share(self, leaders: Tensor | None) -> None:
         """Let steps read what the rows of a group share once (:func:`~scratch_llm_amd.quant.kv_shared.plan_shared_kv`): rows with the
         same number in ``leaders`` (int32 ``[B]``, at least 0; kept, and read again by every :meth:`fork` and :meth:`free`) make
-        a group. None: every row for itself. Call it again after other changes of what the table's shared entries name. A step
+        a group. None: every row for itself. :meth:`Int4DecodeLM.extend` and ``verify`` read every row's keys for itself. Call it again after other changes of what the table's shared entries name. A step
         captured while rows share uses the plan as it is when it is replayed, after ``share(None)`` every row for itself; a step
         captured before never shares."""
         if not self.block_kv:
@@ -329,7 +330,8 @@ class DecodeState:
 
     def set_sampling(self, sampling: "Sampling | None") -> None:
         """Let steps draw their tokens (:func:`~scratch_llm_amd.sampling.sample_tokens`) with the random numbers in ``u`` (float32 ``[B]``,
-        in [0, 1), to be set before every step); None: greedy picks. A row whose logits are no distribution keeps its token and
+        in [0, 1), to be set before every step); None: greedy picks. :meth:`Int4DecodeLM.verify` does not look at it: it draws with
+        its own temperature and no limits, so only settings of that temperature alone draw the same way in both. A row whose logits are no distribution keeps its token and
         does not advance. A captured step keeps the settings that it was captured with; the values of those that are tensors may
         change between replays."""
         if sampling is not None:

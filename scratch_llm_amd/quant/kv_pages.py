@@ -120,9 +120,9 @@ def reserve_kv_pages(k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale:
     """Make positions ``starts[b] .. starts[b] + counts[b] - 1`` of every row (int32 ``[B]`` both) writable by that row alone.
 
     Blocks of these positions that have no page get a free one, whose codes and scales are what its last owner left; blocks
-    whose page others hold too get a copy of it (all who write to it do, if several do). Blocks before them are left as they
-    are. Rows with a negative start or no tokens get nothing, nor do positions past the table. Returns int32 ``[1]``: 1, or
-    0 if there are too few free pages; nothing is changed then."""
+    whose page others hold too get a copy of it (all who write to it do, if several do; if nobody else holds it, it goes free).
+    Blocks before them are left as they are. Rows with a negative start or no tokens get nothing, nor do positions past the table.
+    Returns int32 ``[1]``: 1, or 0 if there are too few free pages; nothing is changed then."""
     fn = "reserve_kv_pages"
     layers, hkv, d, block, pages = _check_pool(k_codes, v_codes, k_scale, v_scale, fn)
     b, width = _check_table(block_table, refs, pages, fn)

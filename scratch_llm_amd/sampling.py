@@ -68,7 +68,8 @@ def sample_tokens(logits: Tensor, u: Tensor, *, temperature: float | Tensor = 1.
     equal ones by their id. Of these the limits keep, one after the other: the first ``top_k`` (0: all); those with less than
     ``top_p`` of the kept tokens' weight before them (1: all; the first always stays); those with ``w_i >= min_p``. The draw is the
     least id whose cumulative kept weight, ids ascending, exceeds ``u[b]`` times the whole (``u`` float32 ``[B]`` in [0, 1)).
-    Weights and sums are float64, or whole numbers that hold as much; a token about 32 temperatures or more below the maximum, whose weight is below 2^-45, is not drawn.
+    Weights and sums are float64, or whole numbers that hold as much; a token about 32 temperatures or more below the maximum,
+    whose weight is below 2^-45, is not drawn. The call's workspace is 12 KB for every 8192 tokens of a row.
 
     ``temperature`` 0 takes the maximum (the first of equals; a NaN counts as the maximum). At others a row that is no
     distribution (NaN, +inf, or -inf everywhere) gives -1. -inf masks a token.
